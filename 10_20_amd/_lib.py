@@ -157,6 +157,11 @@ _SIGNATURES = {
     "v1_union_map_topk": (_c_i32, [_vp, _c_i32, _vp, _vp, _c_i64, _c_i32, _vp, _vp, _vp, _vp, _vp, _c_i64, _vp,
                                    _c_i32, _vp, _vp,
                                    _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _vp]),
+    "v1_latent_store": (_c_i32, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i32, _vp, _c_i64, _c_i64, _vp]),
+    "v1_latent_attend": (_c_i32, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i32, _vp, _c_i64,
+                                  _vp, _c_i32, _c_i32, _c_i32, ctypes.c_float, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64,
+                                  _vp]),
+    "v1_latent_attend_workspace": (_c_i64, [_c_i32, _c_i32, _c_i32, _c_i32]),
 }
 
 _lock = threading.Lock()

@@ -1,0 +1,277 @@
+// What the attention kernels over 8-bit and latent caches share: fragments of
+// v_mfma_f32_16x16x32_bf16, copies from memory to LDS, and the join of the
+// parts that a row's keys were split into.
+#pragma once
+#include "common.h"
+
+namespace v1 {
+namespace attn {
+
+using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+using f32x2 = __attribute__((ext_vector_type(2))) float;
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+using i32x2 = __attribute__((ext_vector_type(2))) int;
+using u32x2 = __attribute__((ext_vector_type(2))) uint32_t;
+using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+
+union Frag {
+    u32x4 u;
+    uint32_t w[4];
+    bf16x8 v;
+};
+
+__device__ __forceinline__ f32x4 mfma16(const Frag& a, const Frag& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0);
+}
+
+// Two fp32 -> two bf16, round to nearest even.
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
+
+// 8 e4m3 codes -> 8 bf16, exact (4 significant bits, exponents -9 .. 8).
+__device__ __forceinline__ Frag bf16_of_codes(uint32_t lo, uint32_t hi) {
+    Frag f;
+    f.w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false));
+    f.w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true));
+    f.w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false));
+    f.w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true));
+    return f;
+}
+
+// Exponent e of the scale 2^e of codes whose largest magnitude is `amax`
+// (finite): the smallest with amax <= 448 * 2^e, at least -126.
+__device__ __forceinline__ int scale_exponent(float amax) {
+    const uint32_t u = __float_as_uint(amax);
+    const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return e < -126 ? -126 : e;
+}
+
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// Four values, scaled, -> e4m3 codes: round to nearest even, past +-448 and
+// infinities to +-448, NaN stays NaN.
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+    auto clip = [](float x) { return x != x ? x : __builtin_amdgcn_fmed3f(x, -448.f, 448.f); };
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(clip(a), clip(b), 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(clip(c), clip(d), r, true);
+}
+
+__device__ __forceinline__ float finite_abs(float x) {
+    const float a = fabsf(x);
+    return a < __builtin_inff() ? a : 0.f;  // (NaN compares false)
+}
+
+__device__ __forceinline__ uint32_t lds_offset(const void* p) {
+    return (uint32_t)reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)p);
+}
+
+// 16 bytes per lane, memory -> LDS at `lds` + 16 * lane (`lds` the same for the
+// wave).  Written as asm so that the compiler puts no waits of its own before
+// LDS reads; they are counted by the caller (vm_wait).  There is no output
+// register that could be reused while the copy is in flight.
+__device__ __forceinline__ void copy_to_lds(const void* src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+                 :: "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory", "m0");
+}
+
+// Waits until at most N vector memory operations of this wave are in flight
+// and its LDS operations are done, then joins the work-group's barrier.
+template <int N>
+__device__ __forceinline__ void wait_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// The work-group's barrier for LDS data alone: copies stay in flight.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// ------------------------------------------------ parts of a row's keys
+// A row's keys, in tiles of 64, are split over several work-groups where the
+// rows alone would not fill the GPU.  Each part leaves its unnormalised sums
+// with their maximum (base 2) and total in a workspace, and join_kernel adds
+// them.  Two rules, both functions of the call's shapes and lengths alone:
+//   chunk > 0  every row in the same number of parts (rows of one capacity);
+//   chunk == 0 rows of different lengths (`lens` on the device, at most
+//              kPlanRows of them): parts of about sum(tiles) / target tiles,
+//              found by every work-group from the lengths.
+constexpr int kTileKeys = 64;
+constexpr int kPlanRows = 256;
+
+struct Plan {
+    const int32_t* lens;  // NULL: `keys` keys in every row
+    int32_t rows, keys, chunk, target;
+};
+
+struct Item {
+    int32_t row, keys;           // keys: of the row
+    int32_t first, tiles, parts; // tiles [first, first + tiles) of the row; parts of the row
+    int32_t part;
+};
+
+__device__ __forceinline__ int32_t tiles_of(int32_t keys) { return (keys + kTileKeys - 1) / kTileKeys; }
+__device__ __forceinline__ int32_t keys_of(const Plan& p, int32_t row) {
+    return p.lens ? min(max(p.lens[row], 0), p.keys) : p.keys;
+}
+
+__device__ __forceinline__ void cut(Item& it) {
+    const int32_t tiles = tiles_of(it.keys), each = (tiles + it.parts - 1) / it.parts;
+    it.first = min(it.part * each, tiles);
+    it.tiles = min(each, tiles - it.first);
+}
+
+// The planned parts of up to kPlanRows rows, four rows a lane (row 4 lane + i);
+// returns the number of parts before the lane's first row.
+__device__ __forceinline__ int32_t plan_parts(const Plan& p, int32_t (&keys)[4], int32_t (&parts)[4]) {
+    const int32_t lane = (int32_t)threadIdx.x % kWave;
+    int32_t tiles = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int32_t r = 4 * lane + i;
+        keys[i] = min(max(p.lens[min(r, p.rows - 1)], 0), p.keys);
+        if (r >= p.rows) keys[i] = 0;
+        tiles += tiles_of(keys[i]);
+    }
+    const int32_t all = __shfl((int32_t)wave_inclusive_sum((uint32_t)tiles), kWave - 1, kWave);
+    const int32_t chunk = max(1, (all + p.target - 1) / p.target);
+    int32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        parts[i] = 4 * lane + i < p.rows ? max(1, (tiles_of(keys[i]) + chunk - 1) / chunk) : 0;
+        mine += parts[i];
+    }
+    return (int32_t)wave_inclusive_sum((uint32_t)mine) - mine;
+}
+
+// Work item `index`; false: there is none.  (Every wave finds it by itself.)
+__device__ __forceinline__ bool find_item(const Plan& p, int32_t index, Item& it) {
+    if (p.chunk > 0) {
+        it.parts = max(1, (tiles_of(p.keys) + p.chunk - 1) / p.chunk);
+        it.row = index / it.parts;
+        it.part = index - it.row * it.parts;
+        if (it.row >= p.rows) return false;
+        it.keys = keys_of(p, it.row);
+    } else {
+        int32_t keys[4], parts[4];
+        const int32_t lane = (int32_t)threadIdx.x % kWave;
+        int32_t at = plan_parts(p, keys, parts);
+        int32_t row = -1, part = 0, n = 0, of = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (index >= at && index < at + parts[i]) {
+                row = 4 * lane + i;
+                part = index - at;
+                n = keys[i];
+                of = parts[i];
+            }
+            at += parts[i];
+        }
+        const uint64_t who = __ballot(row >= 0);
+        if (who == 0) return false;
+        const int src = __ffsll((unsigned long long)who) - 1;
+        it.row = __shfl(row, src, kWave);
+        it.part = __shfl(part, src, kWave);
+        it.keys = __shfl(n, src, kWave);
+        it.parts = __shfl(of, src, kWave);
+    }
+    it.row = __builtin_amdgcn_readfirstlane(it.row);
+    it.part = __builtin_amdgcn_readfirstlane(it.part);
+    it.keys = __builtin_amdgcn_readfirstlane(it.keys);
+    it.parts = __builtin_amdgcn_readfirstlane(it.parts);
+    cut(it);
+    return true;
+}
+
+// First work item and number of parts of a row.
+__device__ __forceinline__ void items_of(const Plan& p, int32_t row, int32_t& first, int32_t& parts) {
+    if (p.chunk > 0) {
+        parts = max(1, (tiles_of(p.keys) + p.chunk - 1) / p.chunk);
+        first = row * parts;
+        return;
+    }
+    int32_t keys[4], of[4];
+    int32_t at = plan_parts(p, keys, of), mine_at = 0, mine = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if ((row & 3) == i) {
+            mine_at = at;
+            mine = of[i];
+        }
+        at += of[i];
+    }
+    first = __shfl(mine_at, row >> 2, kWave);
+    parts = __shfl(mine, row >> 2, kWave);
+}
+
+// Most work items that a call can have.
+inline int64_t items_at_most(const Plan& p) {
+    if (p.chunk > 0) return (int64_t)p.rows * std::max<int64_t>(1, cdiv(cdiv(p.keys, kTileKeys), p.chunk));
+    return (int64_t)p.rows + p.target;
+}
+
+// Workspace: sums [items][heads][dims], then maxima and totals [items][heads].
+struct Parts {
+    float* sums;
+    f32x2* stats;
+};
+
+inline int64_t parts_bytes(int64_t items, int32_t heads, int32_t dims) {
+    return items * heads * (dims + 2) * (int64_t)sizeof(float);
+}
+
+inline Parts parts_at(void* ws, int64_t items, int32_t heads, int32_t dims) {
+    float* sums = static_cast<float*>(ws);
+    return {sums, reinterpret_cast<f32x2*>(sums + items * heads * dims)};
+}
+
+struct JoinParams {
+    Plan plan;
+    Parts parts;
+    uint16_t* out;
+    int64_t o_row, o_head;
+    float* lse;
+    int32_t heads;
+};
+
+// One wave per (row, head): lane l adds dims 2l, 2l + 1 (+ 128 i) of the parts,
+// scaled to the largest of their maxima.  Rows of one part have been written.
+template <int D>
+__global__ __launch_bounds__(256) void join_kernel(JoinParams p) {
+    const int32_t row = (int32_t)blockIdx.x, lane = (int32_t)threadIdx.x % kWave;
+    const int32_t h = (int32_t)blockIdx.y * 4 + (int32_t)threadIdx.x / kWave;
+    int32_t first, parts;
+    items_of(p.plan, row, first, parts);
+    if (parts <= 1 || h >= p.heads) return;
+    float top = -__builtin_inff(), total = 0.f;
+    for (int32_t i = lane; i < parts; i += kWave) top = fmaxf(top, p.parts.stats[(int64_t)(first + i) * p.heads + h][0]);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
+    const float sub = top == -__builtin_inff() ? 0.f : top;
+    f32x2 o[D / 128];
+#pragma unroll
+    for (int k = 0; k < D / 128; ++k) o[k] = f32x2{0.f, 0.f};
+    for (int32_t i = 0; i < parts; ++i) {
+        const int64_t at = (int64_t)(first + i) * p.heads + h;
+        const f32x2 st = p.parts.stats[at];
+        const float f = __builtin_amdgcn_exp2f(st[0] - sub);
+        total = fmaf(f, st[1], total);
+#pragma unroll
+        for (int k = 0; k < D / 128; ++k) {
+            const f32x2 x = *reinterpret_cast<const f32x2*>(p.parts.sums + at * D + 128 * k + 2 * lane);
+            o[k][0] = fmaf(f, x[0], o[k][0]);
+            o[k][1] = fmaf(f, x[1], o[k][1]);
+        }
+    }
+    const bool none = total == 0.f;  // no key attended
+    const float inv = none ? 0.f : 1.0f / total;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + row * p.o_row + h * p.o_head);
+#pragma unroll
+    for (int k = 0; k < D / 128; ++k) dst[64 * k + lane] = none ? 0u : pack_bf16(o[k][0] * inv, o[k][1] * inv);
+    if (p.lse && lane == 0)
+        p.lse[(int64_t)row * p.heads + h] = none ? -__builtin_inff() : (top + __builtin_amdgcn_logf(total)) * kLn2;
+}
+
+}  // namespace attn
+}  // namespace v1

@@ -1,0 +1,443 @@
+// Latent K/V cache rows of 656 bytes (512 e4m3 codes, 64 bf16 rope numbers, 4
+// fp32 scales, one for 128 codes) and attention over them with queries that
+// already carry the key projection ("absorbed" form): one shared row of 512 + 64
+// numbers is every head's key, its first 512 every head's value,
+//   S[h, j] = scale * (q[h, 0:512] . c_j + q[h, 512:576] . r_j),
+//   O[h] = sum_j softmax_j(S[h, :]) c_j,  c_j[d] = code_j[d] * s_j[d / 128].
+#include "attn.h"
+
+namespace v1 {
+namespace {
+
+using namespace attn;
+
+constexpr int kLatent = 512, kRope = 64, kRowBytes = 656, kScaleBlocks = 4;
+constexpr int kRopeAt = kLatent, kScaleAt = kLatent + 2 * kRope;
+constexpr int kChunks = kRowBytes / 16;  // 41, odd: 16-byte reads of 8 rows at one offset meet 8 different banks
+constexpr int kTileBytes = kTileKeys * kRowBytes;
+
+// ------------------------------------------------------------------ store
+// One wave per token: lane l holds numbers 8l .. 8l + 7; the 16 lanes of a
+// block of 128 find its largest magnitude.  Bound by memory: 1152 bytes read and
+// 656 written a token.
+struct StoreParams {
+    const uint16_t* latent;
+    int64_t latent_stride;
+    const uint16_t* rope;
+    int64_t rope_stride;
+    const int32_t* slots;
+    int32_t tokens;
+    uint8_t* pool;
+    int64_t pool_rows, pool_stride;
+};
+
+__global__ __launch_bounds__(256) void latent_store_kernel(StoreParams p) {
+    const int32_t t = (int32_t)(blockIdx.x * 4 + threadIdx.x / kWave), lane = (int32_t)threadIdx.x % kWave;
+    if (t >= p.tokens) return;
+    const int32_t slot = p.slots[t];
+    const u32x4 x = *reinterpret_cast<const u32x4*>(p.latent + t * p.latent_stride + 8 * lane);
+    u32x4 r = {0, 0, 0, 0};
+    if (lane < 8) r = *reinterpret_cast<const u32x4*>(p.rope + t * p.rope_stride + 8 * lane);
+    if (slot < 0 || slot >= p.pool_rows) return;
+    float v[8], amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(x[i] << 16);
+        v[2 * i + 1] = __uint_as_float(x[i] & 0xffff0000u);
+        amax = fmaxf(amax, fmaxf(finite_abs(v[2 * i]), finite_abs(v[2 * i + 1])));
+    }
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off, kWave));
+    const int e = scale_exponent(amax);
+    const float inv = exp2i(-e);  // (e is -126 .. 120)
+    uint8_t* row = p.pool + slot * p.pool_stride;
+    const u32x2 codes = {codes4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
+                         codes4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv)};
+    *reinterpret_cast<u32x2*>(row + 8 * lane) = codes;
+    if (lane < 8) *reinterpret_cast<u32x4*>(row + kRopeAt + 16 * lane) = r;
+    if (lane % 16 == 0) *reinterpret_cast<float*>(row + kScaleAt + lane / 4) = exp2i(e);
+}
+
+// --------------------------------------------------------------- absorbed
+struct AbsorbedParams {
+    const uint16_t* q;
+    int64_t q_row, q_head;
+    const uint8_t* pool;
+    int64_t pool_rows, pool_stride;
+    const int32_t* map;  // NULL: ids are rows of the pool
+    int64_t map_len, map_stride;
+    int32_t map_shift;
+    const int32_t* ids;  // NULL: positions 0, 1, ...
+    int64_t ids_stride;
+    Plan plan;
+    int32_t heads, splits, spread;  // splits: work-groups of a row's heads; spread: items on an XCD
+    float scale2;
+    uint16_t* out;
+    int64_t o_row, o_head;
+    float* lse;
+    Parts parts;
+};
+
+// The row of keys that are not attended (their scores are -inf).
+__device__ const u32x4 zero_latent[kChunks] = {};
+
+constexpr int kPRow = kTileKeys * 2 + 16;  // bytes of a head's probabilities of a tile; 9 chunks of 16: 8 heads meet 8 different banks
+constexpr float kLag = 6.f;  // the subtracted maximum may lag the true one by 2^6
+
+template <int HT, int HG, int NB>
+struct AbsorbedLds {
+    static constexpr int kHeads = 16 * HT * HG;
+    uint8_t tile[NB][kTileBytes];
+    uint8_t prob[kScaleBlocks][kHeads][kPRow];
+    float hidden[NB][kTileKeys];  // 0, or -inf: not attended
+    float top[4][kHeads];
+    float keep[kHeads];
+    float total[4][kHeads];
+};
+
+// A work-group of 4 * HG waves attends 16 * HT * HG heads of one row over one
+// part of its keys, tile by tile of 64 keys that come memory -> LDS as they are
+// stored (NB buffers).
+//   scores  S^T = K Q^T: wave (hg, kq) takes heads 16 HT hg .. and keys 16 kq ..;
+//           codes become bf16 (exact) as they are read, one accumulator per block
+//           of 128 numbers, joined with the block's scales in fp32.
+//   softmax the four key quarters exchange their maxima through LDS; each
+//           probability is multiplied by its key's four scales and rounded to
+//           bf16 once (2^-9 relative, as in the output), the sum stays fp32.
+//   output  O^T = C^T P^T: wave w takes 512 / waves columns of all heads, its
+//           codes transposed by the LDS read (ds_read_b64_tr_b8), exact in bf16.
+template <int HT, int HG, int NB>
+__global__ __launch_bounds__(256 * HG) void absorbed_kernel(AbsorbedParams p) {
+    constexpr int NW = 4 * HG, HB = 16 * HT * HG, RPW = kTileKeys / NW, GT = kWave / RPW;
+    constexpr int COPIES = (RPW * kChunks + kWave - 1) / kWave;
+    constexpr int DV = kLatent / NW, DT = DV / 16, PT = HB / 16;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
+    auto& lds = *reinterpret_cast<AbsorbedLds<HT, HG, NB>*>(lds_raw);
+    const int32_t wave = __builtin_amdgcn_readfirstlane((int32_t)threadIdx.x / kWave);
+    const int32_t lane = (int32_t)threadIdx.x % kWave, g = lane >> 4, c = lane & 15;
+    const int32_t hg = wave >> 2, kq = wave & 3;
+
+    // work-groups reach the XCDs in turn: the splits of an item follow each other on one of them
+    const int32_t xcd = (int32_t)blockIdx.x % 8, turn = (int32_t)blockIdx.x / 8;
+    const int32_t index = xcd * p.spread + turn / p.splits, split = turn % p.splits;
+    Item it;
+    if (!find_item(p.plan, index, it)) return;
+    const int32_t head0 = split * HB;
+
+    // rows of this wave's part of a tile, GT tiles at a time: lane = tile * RPW + row
+    const int32_t* ids = p.ids ? p.ids + it.row * p.ids_stride : nullptr;
+    const int32_t* map = p.map ? p.map + it.row * p.map_stride : nullptr;
+    auto key_of = [&](int32_t group) __attribute__((always_inline)) {
+        return (it.first + group * GT + lane / RPW) * kTileKeys + wave * RPW + lane % RPW;
+    };
+    auto fetch_id = [&](int32_t group) __attribute__((always_inline)) -> int32_t {
+        const int32_t j = key_of(group);
+        if (j >= it.keys) return -1;
+        return ids ? ids[j] : j;
+    };
+    auto fetch_row = [&](int32_t id) __attribute__((always_inline)) -> int32_t {
+        if (id < 0) return -1;
+        int64_t row = id;
+        if (map) {
+            const int64_t e = (int64_t)id >> p.map_shift;
+            if (e >= p.map_len) return -1;
+            const int32_t m = map[e];
+            if (m < 0) return -1;
+            row = ((int64_t)m << p.map_shift) | (id & ((1 << p.map_shift) - 1));
+        }
+        return row < p.pool_rows ? (int32_t)row : -1;
+    };
+    int32_t rows_now = fetch_row(fetch_id(0)), rows_next = fetch_row(fetch_id(1)), ids_after = fetch_id(2);
+
+    // copies of tile t into buffer t % NB, asked for in the order of the tiles
+    auto copy_tile = [&](int32_t t) __attribute__((always_inline)) {
+        if (t > 0 && t % GT == 0) {
+            rows_now = rows_next;
+            rows_next = fetch_row(ids_after);
+            ids_after = fetch_id(t / GT + 2);
+        }
+        const int32_t buf = t % NB;
+        if (lane / RPW == t % GT) lds.hidden[buf][wave * RPW + lane % RPW] = rows_now < 0 ? -__builtin_inff() : 0.f;
+        const uint32_t to = lds_offset(&lds.tile[buf][wave * RPW * kRowBytes]);
+#pragma unroll
+        for (int j = 0; j < COPIES; ++j) {
+            const uint32_t i = 64 * j + lane, r = (i * 1599u) >> 16, chunk = i - r * kChunks;  // i / 41, exact below 2009
+            const int32_t row = __shfl(rows_now, (t % GT) * RPW + (int)(r < RPW ? r : RPW - 1), kWave);
+            const uint8_t* src = row < 0 ? reinterpret_cast<const uint8_t*>(zero_latent) : p.pool + row * p.pool_stride;
+            if (r < RPW) copy_to_lds(src + 16 * chunk, to + 1024 * j);
+        }
+    };
+    const int32_t tiles = it.tiles;
+    for (int t = 0; t < NB - 1; ++t)
+        if (t < tiles) copy_tile(t);
+
+    // B fragments of Q^T: column c = head c of 16; 64 numbers in two steps: lane
+    // group g takes 16g .. 16g + 7 of them, then 16g + 8 .. 16g + 15 (the order in which the codes are read)
+    Frag q[HT][18];
+#pragma unroll
+    for (int ht = 0; ht < HT; ++ht) {
+        const int32_t h = min(head0 + hg * 16 * HT + 16 * ht + c, p.heads - 1);
+        const uint16_t* src = p.q + it.row * p.q_row + h * p.q_head;
+#pragma unroll
+        for (int s = 0; s < 16; ++s) q[ht][s].u = *reinterpret_cast<const u32x4*>(src + 64 * (s / 2) + 16 * g + 8 * (s % 2));
+#pragma unroll
+        for (int s = 0; s < 2; ++s) q[ht][16 + s].u = *reinterpret_cast<const u32x4*>(src + kLatent + 32 * s + 8 * g);
+    }
+    f32x4 acc[DT][PT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int h = 0; h < PT; ++h) acc[d][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float mx[HT], total[HT];
+#pragma unroll
+    for (int ht = 0; ht < HT; ++ht) mx[ht] = -__builtin_inff(), total[ht] = 0.f;
+
+#pragma unroll 1
+    for (int32_t t = 0; t < tiles; ++t) {
+        // tile t has landed, and every wave has left the buffer that comes next
+        if (NB > 2 && t + 1 < tiles) wait_barrier<(NB - 2) * COPIES>();
+        else wait_barrier<0>();
+        if (t + NB - 1 < tiles) copy_tile(t + NB - 1);
+        const uint8_t* tile = lds.tile[t % NB];
+        // scores of keys 16 kq + 4g + i, heads c
+        float s[HT][4];
+        f32x4 sc[4];
+        {
+            const uint8_t* key = tile + (16 * kq + c) * kRowBytes;
+            f32x4 d[HT];
+#pragma unroll
+            for (int ht = 0; ht < HT; ++ht) d[ht] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                Frag k;
+                k.u = *reinterpret_cast<const u32x4*>(key + kRopeAt + 64 * r + 16 * g);
+#pragma unroll
+                for (int ht = 0; ht < HT; ++ht) d[ht] = mfma16(k, q[ht][16 + r], d[ht]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                sc[i] = *reinterpret_cast<const f32x4*>(tile + (16 * kq + 4 * g + i) * kRowBytes + kScaleAt);
+#pragma unroll
+            for (int ht = 0; ht < HT; ++ht)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[ht][i] = d[ht][i];
+#pragma unroll
+            for (int b = 0; b < kScaleBlocks; ++b) {
+#pragma unroll
+                for (int ht = 0; ht < HT; ++ht) d[ht] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const u32x4 w = *reinterpret_cast<const u32x4*>(key + 128 * b + 64 * half + 16 * g);
+                    const Frag k0 = bf16_of_codes(w[0], w[1]), k1 = bf16_of_codes(w[2], w[3]);
+#pragma unroll
+                    for (int ht = 0; ht < HT; ++ht) d[ht] = mfma16(k0, q[ht][4 * b + 2 * half], d[ht]);
+#pragma unroll
+                    for (int ht = 0; ht < HT; ++ht) d[ht] = mfma16(k1, q[ht][4 * b + 2 * half + 1], d[ht]);
+                }
+#pragma unroll
+                for (int ht = 0; ht < HT; ++ht)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[ht][i] = fmaf(sc[i][b], d[ht][i], s[ht][i]);
+            }
+        }
+        const f32x4 hidden = *reinterpret_cast<const f32x4*>(&lds.hidden[t % NB][16 * kq + 4 * g]);
+#pragma unroll
+        for (int ht = 0; ht < HT; ++ht) {
+            float top = -__builtin_inff();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[ht][i] = hidden[i] < 0.f ? -__builtin_inff() : s[ht][i] * p.scale2;
+                top = fmaxf(top, s[ht][i]);
+            }
+            top = fmaxf(top, __shfl_xor(top, 16, kWave));
+            top = fmaxf(top, __shfl_xor(top, 32, kWave));
+            if (g == 0) lds.top[kq][16 * (HT * hg + ht) + c] = top;
+        }
+        lds_barrier();
+#pragma unroll
+        for (int ht = 0; ht < HT; ++ht) {
+            const int32_t h = 16 * (HT * hg + ht) + c;
+            const float top = fmaxf(fmaxf(lds.top[0][h], lds.top[1][h]), fmaxf(lds.top[2][h], lds.top[3][h]));
+            float keep = 1.f;
+            if (top > mx[ht] + kLag) {  // (-inf + kLag is -inf)
+                keep = mx[ht] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mx[ht] - top);
+                mx[ht] = top;
+            }
+            const float sub = mx[ht] == -__builtin_inff() ? 0.f : mx[ht];
+            total[ht] *= keep;
+            if (kq == 0 && g == 0) lds.keep[h] = keep;
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = __builtin_amdgcn_exp2f(s[ht][i] - sub);
+                total[ht] += x[i];
+            }
+#pragma unroll
+            for (int b = 0; b < kScaleBlocks; ++b)
+                *reinterpret_cast<u32x2*>(&lds.prob[b][h][2 * (16 * kq + 4 * g)]) =
+                    u32x2{pack_bf16(x[0] * sc[0][b], x[1] * sc[1][b]), pack_bf16(x[2] * sc[2][b], x[3] * sc[3][b])};
+        }
+        lds_barrier();
+        // output columns DV wave .. of all heads
+        {
+            float keep[PT];
+            bool any = false;
+#pragma unroll
+            for (int h = 0; h < PT; ++h) {
+                keep[h] = lds.keep[16 * h + c];
+                any |= keep[h] != 1.f;
+            }
+            if (__ballot(any))
+#pragma unroll
+                for (int h = 0; h < PT; ++h)
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) acc[d][h] *= keep[h];
+            const int32_t b = wave * DV / 128;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                Frag pf[PT];
+#pragma unroll
+                for (int h = 0; h < PT; ++h)
+                    pf[h].u = *reinterpret_cast<const u32x4*>(&lds.prob[b][16 * h + c][64 * ks + 16 * g]);
+                // lanes 2r, 2r + 1 of a group hand in 16 columns of key 8g + r; lane c gets column c of its eight keys
+                const uint8_t* v = tile + (32 * ks + 8 * g + c / 2) * kRowBytes + wave * DV + 8 * (c & 1);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                        (__attribute__((address_space(3))) i32x2*)(v + 16 * d));
+                    const Frag a = bf16_of_codes((uint32_t)w[0], (uint32_t)w[1]);
+#pragma unroll
+                    for (int h = 0; h < PT; ++h) acc[d][h] = mfma16(a, pf[h], acc[d][h]);
+                }
+            }
+        }
+    }
+    // totals of the four key quarters
+#pragma unroll
+    for (int ht = 0; ht < HT; ++ht) {
+        const int32_t h = 16 * (HT * hg + ht) + c;
+        float x = total[ht];
+        x += __shfl_xor(x, 16, kWave);
+        x += __shfl_xor(x, 32, kWave);
+        if (g == 0) lds.total[kq][h] = x;
+        if (g == 0 && kq == 0) lds.top[0][h] = mx[ht];
+    }
+    __syncthreads();
+    const bool whole = it.parts == 1;
+#pragma unroll
+    for (int ht = 0; ht < PT; ++ht) {
+        const int32_t h = 16 * ht + c, head = head0 + h;
+        if (head >= p.heads) continue;
+        const float sum = (lds.total[0][h] + lds.total[1][h]) + (lds.total[2][h] + lds.total[3][h]);
+        const float top = lds.top[0][h];
+        const bool none = sum == 0.f;  // no key attended
+        if (whole) {
+            const float inv = none ? 0.f : 1.0f / sum;
+            uint16_t* out = p.out + it.row * p.o_row + head * p.o_head + wave * DV + 4 * g;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+                *reinterpret_cast<u32x2*>(out + 16 * d) =
+                    none ? u32x2{0, 0} : u32x2{pack_bf16(acc[d][ht][0] * inv, acc[d][ht][1] * inv),
+                                               pack_bf16(acc[d][ht][2] * inv, acc[d][ht][3] * inv)};
+            if (p.lse && wave == 0 && g == 0)
+                p.lse[(int64_t)it.row * p.heads + head] =
+                    none ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+        } else {
+            const int64_t at = (int64_t)index * p.heads + head;
+            float* o = p.parts.sums + at * kLatent + wave * DV + 4 * g;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(o + 16 * d) = acc[d][ht];
+            if (wave == 0 && g == 0) p.parts.stats[at] = f32x2{top, sum};
+        }
+    }
+}
+
+// Heads of a work-group: 16, 32 or 64 (more: several work-groups a row).
+inline int32_t absorbed_heads(int32_t heads) { return heads <= 16 ? 16 : heads <= 32 ? 32 : 64; }
+
+inline Plan absorbed_plan(const int32_t* lens, int32_t rows, int32_t heads, int32_t keys, bool ragged) {
+    const int64_t splits = cdiv(heads, absorbed_heads(heads)), tiles = cdiv(keys, kTileKeys);
+    const int64_t groups = std::max<int64_t>(1, device_cus() / splits);  // items that fill the GPU once
+    Plan p{lens, rows, keys, (int32_t)std::max<int64_t>(1, tiles), (int32_t)groups};
+    if (rows >= groups) return p;
+    if (ragged && rows <= kPlanRows) {
+        p.chunk = 0;
+        return p;
+    }
+    p.chunk = (int32_t)std::max<int64_t>(1, cdiv(tiles * rows, groups));
+    return p;
+}
+
+template <int HT, int HG, int NB>
+int launch_absorbed(const AbsorbedParams& p, int64_t blocks, hipStream_t st) {
+    static OncePerDevice once;
+    constexpr size_t bytes = sizeof(AbsorbedLds<HT, HG, NB>);
+    static_assert(bytes <= 160 * 1024, "LDS of a CU");
+    const int rc = allow_lds(once, reinterpret_cast<const void*>(absorbed_kernel<HT, HG, NB>), bytes, "latent_attend: LDS");
+    if (rc != V1_OK) return rc;
+    hipLaunchKernelGGL((absorbed_kernel<HT, HG, NB>), dim3((uint32_t)blocks), dim3(256 * HG), bytes, st, p);
+    return V1_LAUNCHED("latent_attend");
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+}  // namespace v1
+
+using namespace v1;
+
+extern "C" int v1_latent_store(const void* latent, int64_t latent_stride, const void* rope, int64_t rope_stride,
+                               const int32_t* slots, int32_t tokens, void* pool, int64_t pool_rows,
+                               int64_t pool_stride_bytes, void* stream) {
+    V1_REQUIRE(tokens >= 0 && pool_rows >= 0 && pool_rows < 1ll << 31, "latent_store: bad shape");
+    V1_REQUIRE(aligned16(latent) && aligned16(rope) && aligned16(pool) && latent_stride % 8 == 0 && rope_stride % 8 == 0,
+               "latent_store: inputs and pool must be 16-byte aligned, strides multiples of 8");
+    V1_REQUIRE(pool_stride_bytes % 16 == 0 && pool_stride_bytes >= kRowBytes,
+               "latent_store: pool stride must be a multiple of 16 and >= %d", kRowBytes);
+    if (tokens == 0) return V1_OK;
+    StoreParams p{static_cast<const uint16_t*>(latent), latent_stride, static_cast<const uint16_t*>(rope), rope_stride,
+                  slots, tokens, static_cast<uint8_t*>(pool), pool_rows, pool_stride_bytes};
+    hipLaunchKernelGGL(latent_store_kernel, dim3((uint32_t)cdiv(tokens, 4)), dim3(256), 0, as_stream(stream), p);
+    return V1_LAUNCHED("latent_store");
+}
+
+extern "C" int64_t v1_latent_attend_workspace(int32_t rows, int32_t heads, int32_t keys, int32_t ragged) {
+    if (rows <= 0 || heads <= 0 || keys <= 0) return 0;
+    const attn::Plan plan = absorbed_plan(nullptr, rows, heads, keys, ragged != 0);
+    const int64_t items = attn::items_at_most(plan);
+    return plan.chunk > 0 && items == rows ? 0 : attn::parts_bytes(items, heads, kLatent);
+}
+
+extern "C" int v1_latent_attend(const void* q, int64_t q_row, int64_t q_head, const void* pool, int64_t pool_rows,
+                                int64_t pool_stride_bytes, const int32_t* map, int64_t map_len, int64_t map_stride,
+                                int32_t map_shift, const int32_t* ids, int64_t ids_stride, const int32_t* lens,
+                                int32_t rows, int32_t heads, int32_t keys, float scale, void* out, int64_t o_row,
+                                int64_t o_head, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+    V1_REQUIRE(rows >= 0 && heads > 0 && keys >= 0 && pool_rows >= 0 && pool_rows < 1ll << 31, "latent_attend: bad shape");
+    V1_REQUIRE(map_shift >= 0 && map_shift < 31 && map_len >= 0, "latent_attend: bad page map");
+    V1_REQUIRE(aligned16(q) && aligned16(pool) && reinterpret_cast<uintptr_t>(out) % 8 == 0 && q_row % 8 == 0 &&
+                   q_head % 8 == 0 && o_row % 4 == 0 && o_head % 4 == 0,
+               "latent_attend: q and pool must be 16-byte aligned, out 8-byte, q strides multiples of 8, out strides of 4");
+    V1_REQUIRE(pool_stride_bytes % 16 == 0 && pool_stride_bytes >= kRowBytes,
+               "latent_attend: pool stride must be a multiple of 16 and >= %d", kRowBytes);
+    if (rows == 0) return V1_OK;
+    const Plan plan = absorbed_plan(lens, rows, heads, keys, lens != nullptr);
+    const int64_t items = items_at_most(plan), need = v1_latent_attend_workspace(rows, heads, keys, lens != nullptr);
+    V1_REQUIRE(workspace_bytes >= need && (need == 0 || workspace != nullptr),
+               "latent_attend: workspace of %lld bytes needed", (long long)need);
+    const int32_t hb = absorbed_heads(heads);
+    const int64_t splits = cdiv(heads, hb), spread = cdiv(items, 8), blocks = 8 * spread * splits;
+    V1_REQUIRE(blocks < 1ll << 31, "latent_attend: too many rows");
+    AbsorbedParams p{static_cast<const uint16_t*>(q), q_row, q_head, static_cast<const uint8_t*>(pool), pool_rows,
+                     pool_stride_bytes, map, map_len, map_stride, map_shift, ids, ids_stride, plan, heads,
+                     (int32_t)splits, (int32_t)spread, scale * kLog2e, static_cast<uint16_t*>(out), o_row, o_head, lse,
+                     parts_at(workspace, items, heads, kLatent)};
+    const hipStream_t st = as_stream(stream);
+    const int rc = hb == 16   ? launch_absorbed<1, 1, 3>(p, blocks, st)
+                   : hb == 32 ? launch_absorbed<2, 1, 3>(p, blocks, st)
+                              : launch_absorbed<2, 2, 2>(p, blocks, st);
+    if (rc != V1_OK || need == 0) return rc;
+    JoinParams j{plan, p.parts, p.out, o_row, o_head, lse, heads};
+    hipLaunchKernelGGL(join_kernel<kLatent>, dim3((uint32_t)rows, (uint32_t)cdiv(heads, 4)), dim3(256), 0, st, j);
+    return V1_LAUNCHED("latent_attend: join");
+}

@@ -1,0 +1,119 @@
+"""Latent K/V cache and its attention: the consumer of the indexer's Top-K slots
+where one latent vector per token serves every head.
+
+A cache row is 656 bytes: 512 OCP e4m3fn codes, 64 bf16 rope-key numbers, 4 fp32
+scales (code j stands for code * scale[j // 128]); the row that
+native_kernels.gather_rows, the page manager and the tail staging move as opaque
+bytes.  `store_rows` writes rows, `attend` reads them with queries that already
+carry the key projection ("absorbed": one key of 512 + 64 numbers for all heads,
+its first 512 the value), `attend_expanded` is the prompt's form over keys and
+values expanded per head from the latent.
+
+Every call launches on the current stream of its tensors' device, never
+synchronises, and raises ValueError for arguments that do not fit.
+"""
+import math
+
+import torch
+
+from . import _lib
+
+LATENT, ROPE, ROW_BYTES = 512, 64, 656
+HEAD = 128  # key numbers of a head beside the rope's, and value numbers, in the expanded form
+
+
+def _int32(name, t, shape):
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {list(shape)}")
+
+
+def _pool(pool):
+    if pool.dtype != torch.uint8 or pool.dim() != 2 or pool.shape[1] != ROW_BYTES or pool.stride(1) != 1:
+        raise ValueError(f"pool must be a uint8 [rows, {ROW_BYTES}] tensor with unit inner stride")
+
+
+def _output(out, like, shape):
+    if out is None:
+        return torch.empty(shape, device=like.device, dtype=torch.bfloat16)
+    if out.dtype != torch.bfloat16 or tuple(out.shape) != shape or out.stride(-1) != 1:
+        raise ValueError(f"out must be bfloat16 {list(shape)} with a contiguous last dimension")
+    return out
+
+
+def store_rows(latent, rope, pool, slots):
+    """Writes token t's row into pool[slots[t]] (a slot below zero or past the
+    pool: the token is skipped; slots of one call are distinct, or which token's
+    bytes a row holds is undefined).
+
+    latent: [tokens, 512] bf16, rope: [tokens, 64] bf16, pool: [rows, 656] uint8
+    (row strides free), slots: [tokens] int32.  A block's scale is the smallest
+    power of two s (2^-126 at least) with |x| <= 448 s for its finite numbers, a
+    code the nearest e4m3 value of x / s (ties to even); infinities are stored as
+    +-448 s, NaN as NaN."""
+    _lib.require_gpu(latent, rope, pool, slots)
+    tokens = latent.shape[0]
+    for name, t, n in (("latent", latent, LATENT), ("rope", rope, ROPE)):
+        if t.dtype != torch.bfloat16 or t.dim() != 2 or tuple(t.shape) != (tokens, n) or t.stride(1) != 1:
+            raise ValueError(f"{name} must be bfloat16 [tokens, {n}] with a contiguous last dimension")
+    _pool(pool)
+    _int32("slots", slots, (tokens,))
+    _lib.call("v1_latent_store", _lib.ptr(latent), latent.stride(0), _lib.ptr(rope), rope.stride(0), _lib.ptr(slots),
+              tokens, _lib.ptr(pool), pool.shape[0], pool.stride(0), _lib.stream_of(pool))
+    return pool
+
+
+def attend(q, pool, ids=None, table=None, page_bits=0, lens=None, softmax_scale=None, out=None, return_lse=False):
+    """out[r, h] = sum_j softmax_j(scale * (q[r, h, :512] . c_j + q[r, h, 512:] . rope_j)) c_j
+    over the keys of row r, c_j the dequantised latent vector.
+
+    q:     [rows, heads, 576] bf16
+    pool:  [slots, 656] uint8 (row stride free)
+    ids:   [rows, keys] int32 positions (the Top-K's output), or None: positions 0, 1, ...
+    table: None (positions are pool rows), a 1-D page table shared by all rows, or
+           [rows, entries]; row = (table[r, id >> page_bits] << page_bits) | (id & (2**page_bits - 1)),
+           as in native_kernels.gather_rows
+    lens:  [rows] int32: the first lens[r] entries of ids (or positions) are row r's; None: all.
+           Without ids and lens every position of the table (or pool) is attended.
+
+    Ids below zero, past the table or outside the pool are not attended.  A row
+    without keys gives zeros and a log-sum-exp of -inf.  softmax_scale: default
+    1 / sqrt(192), that of the expanded form.  Returns out [rows, heads, 512] bf16,
+    and with return_lse the natural log of the sum of exponentials, [rows, heads] fp32."""
+    _lib.require_gpu(q, pool, ids, table, lens, out)
+    if q.dim() != 3 or q.shape[2] != LATENT + ROPE or q.dtype != torch.bfloat16 or q.stride(2) != 1 or not q.shape[1]:
+        raise ValueError(f"q must be bfloat16 [rows, heads, {LATENT + ROPE}] with a contiguous last dimension")
+    _pool(pool)
+    rows, heads, _ = q.shape
+    page_bits = int(page_bits)
+    if not 0 <= page_bits < 31:
+        raise ValueError("page_bits must be in [0, 31)")
+    map_len, map_stride = 0, 0
+    if table is not None:
+        if table.dtype != torch.int32 or table.dim() not in (1, 2) or (table.dim() == 2 and table.shape[0] != rows):
+            raise ValueError("table must be int32 [entries] or [rows, entries]")
+        map_len, map_stride = table.shape[-1], table.stride(0) if table.dim() == 2 else 0
+        if map_len and table.stride(-1) != 1:
+            raise ValueError("table must have unit inner stride")
+    if ids is not None:
+        if ids.dtype != torch.int32 or ids.dim() != 2 or ids.shape[0] != rows or (ids.shape[1] and ids.stride(1) != 1):
+            raise ValueError("ids must be int32 [rows, keys] with unit inner stride")
+        keys = ids.shape[1]
+    else:
+        keys = map_len << page_bits if table is not None else pool.shape[0]
+        if keys >= 1 << 31:
+            raise ValueError("positions must stay below 2**31")
+    if table is not None and map_len == 0:
+        keys = 0
+    if lens is not None:
+        _int32("lens", lens, (rows,))
+    out = _output(out, q, (rows, heads, LATENT))
+    lse = torch.empty((rows, heads), device=q.device, dtype=torch.float32) if return_lse else None
+    scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(HEAD + ROPE)
+    # (the sums of a row's parts are the call's own, as in attention.attend_slots)
+    ws_bytes = _lib.lib().v1_latent_attend_workspace(rows, heads, keys, lens is not None)
+    ws = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8) if ws_bytes else None
+    _lib.call("v1_latent_attend", _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(pool), pool.shape[0], pool.stride(0),
+              _lib.ptr(table), map_len, map_stride, page_bits, _lib.ptr(ids), ids.stride(0) if ids is not None else 0,
+              _lib.ptr(lens), rows, heads, keys, scale, _lib.ptr(out), out.stride(0), out.stride(1), _lib.ptr(lse),
+              _lib.ptr(ws), ws_bytes, _lib.stream_of(q))
+    return (out, lse) if return_lse else out

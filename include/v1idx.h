@@ -579,6 +579,36 @@ int v1_decode_attention_slots_ws(const void* q, int64_t q_batch, int64_t q_head,
                               float scale, void* workspace, int64_t workspace_bytes,
                               void* stream);
 int64_t v1_decode_attention_slots_workspace(int32_t rows, int32_t heads_q, int32_t keys);
+/* ------------------------------------------------------------------------
+ * Latent K/V cache rows of 656 bytes: 512 OCP e4m3fn codes, 64 bf16 rope
+ * numbers, 4 fp32 scales (one for 128 codes).  No counterpart in the reference,
+ * whose backends leave this attention to an external library.
+ *
+ * v1_latent_store: row pool[slots[t]] from latent [tokens, 512] and rope
+ * [tokens, 64] bf16; a block's scale is the smallest power of two s >= 2^-126
+ * with |x| <= 448 s for its finite numbers, codes round to nearest even,
+ * infinities become +-448 s.  Slots outside [0, pool_rows) are skipped; slots of
+ * one call are distinct.
+ * ---------------------------------------------------------------------- */
+int v1_latent_store(const void* latent, int64_t latent_stride, const void* rope, int64_t rope_stride,
+                    const int32_t* slots, int32_t tokens, void* pool, int64_t pool_rows,
+                    int64_t pool_stride_bytes, void* stream);
+/* Attention over latent rows: q [rows, heads, 576] bf16, out[r, h] (bf16, 512)
+ * = softmax over the row's keys of scale * q . (c_j, rope_j), times c_j (the
+ * dequantised codes).  Key j of row r is id = ids[r * ids_stride + j] (j when ids
+ * is NULL), j < lens[r] clamped to [0, keys] (keys when lens is NULL), at pool
+ * row (map[r * map_stride + (id >> map_shift)] << map_shift) | low bits (id when
+ * map is NULL).  An id < 0, past map_len or outside the pool is not attended; a
+ * row without keys gives zeros.  lse (may be NULL): [rows, heads] natural log of
+ * the sum of exponentials, -inf without keys.  workspace:
+ * v1_latent_attend_workspace(rows, heads, keys, lens != NULL) bytes, 256-byte
+ * aligned, the call's own until the stream has passed it. */
+int v1_latent_attend(const void* q, int64_t q_row, int64_t q_head, const void* pool, int64_t pool_rows,
+                     int64_t pool_stride_bytes, const int32_t* map, int64_t map_len, int64_t map_stride,
+                     int32_t map_shift, const int32_t* ids, int64_t ids_stride, const int32_t* lens,
+                     int32_t rows, int32_t heads, int32_t keys, float scale, void* out, int64_t o_row,
+                     int64_t o_head, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t v1_latent_attend_workspace(int32_t rows, int32_t heads, int32_t keys, int32_t ragged);
 #ifdef __cplusplus
 }
 #endif
