@@ -162,6 +162,10 @@ _SIGNATURES = {
                                   _vp, _c_i32, _c_i32, _c_i32, ctypes.c_float, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64,
                                   _vp]),
     "v1_latent_attend_workspace": (_c_i64, [_c_i32, _c_i32, _c_i32, _c_i32]),
+    "v1_latent_expanded": (_c_i32, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp, _c_i32, _c_i32,
+                                    _c_i32, _c_i32, _c_i32, _c_i32, ctypes.c_float, _vp, _c_i64, _c_i64, _vp, _vp,
+                                    _c_i64, _vp]),
+    "v1_latent_expanded_workspace": (_c_i64, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32]),
 }
 
 _lock = threading.Lock()

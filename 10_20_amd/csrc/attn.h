@@ -233,6 +233,8 @@ struct JoinParams {
     int64_t o_row, o_head;
     float* lse;
     int32_t heads;
+    const int32_t* cu;  // not NULL: rows outside [cu[0], cu[batch]) are left as they are
+    int32_t batch;
 };
 
 // One wave per (row, head): lane l adds dims 2l, 2l + 1 (+ 128 i) of the parts,
@@ -241,6 +243,7 @@ template <int D>
 __global__ __launch_bounds__(256) void join_kernel(JoinParams p) {
     const int32_t row = (int32_t)blockIdx.x, lane = (int32_t)threadIdx.x % kWave;
     const int32_t h = (int32_t)blockIdx.y * 4 + (int32_t)threadIdx.x / kWave;
+    if (p.cu && (row < p.cu[0] || row >= p.cu[p.batch])) return;
     int32_t first, parts;
     items_of(p.plan, row, first, parts);
     if (parts <= 1 || h >= p.heads) return;

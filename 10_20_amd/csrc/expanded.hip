@@ -1,0 +1,385 @@
+// Attention of ragged sequences over keys and values expanded per head from the
+// latent: q [tokens, heads, 128 + 64], kv [keys, heads, 128 key | 128 value]
+// numbers, one rope key [keys, 64] for all heads, bf16:
+//   S[i, j] = scale * (q[i, 0:128] . k_j + q[i, 128:192] . rope_j),  O[i] = sum_j softmax_j(S[i, :]) v_j,
+// query i of a sequence of nq queries and nk keys sees keys j <= nk - nq + i
+// (causal) or all.
+//
+// A work-group of NW waves takes 32 * NW queries of one head; each wave its own
+// 32, as columns of v_mfma_f32_32x32x16_bf16:
+//   scores  S^T = K Q^T, a tile of 64 keys at a time from LDS;
+//   output  O^T = V^T P^T: a lane's scores are already the probabilities of its
+//           B fragment (the key order inside 16 keys is chosen so), rounded to
+//           bf16 once; V comes transposed from LDS (ds_read_b64_tr_b16).
+// Scores, maxima and sums stay fp32, exponentials are base 2.  Tiles come memory
+// -> LDS two deep; rows are laid with their 16-byte chunks XORed by the row so
+// that the fragments' reads meet different banks.
+#include "attn.h"
+
+namespace v1 {
+namespace {
+
+using namespace attn;
+
+constexpr int kKey = 128, kValue = 128, kRopeDims = 64;
+constexpr int kRows = 32;  // queries of a wave
+constexpr float kLag = 6.f;  // the subtracted maximum may lag the true one by 2^6
+
+using f32x16 = __attribute__((ext_vector_type(16))) float;
+using i16x4 = __attribute__((ext_vector_type(4))) short;
+
+struct ExpandedParams {
+    const uint16_t* q;
+    int64_t q_row, q_head;
+    const uint16_t* kv;
+    int64_t kv_row, kv_head;
+    const uint16_t* rope;
+    int64_t rope_row;
+    const int32_t* cu_q;
+    const int32_t* cu_k;
+    int32_t tokens, keys, batch, heads, blocks;  // blocks: of queries, of the longest sequence
+    int32_t causal, parts, spread;
+    float scale2;
+    uint16_t* out;
+    int64_t o_row, o_head;
+    float* lse;
+    Parts partial;
+};
+
+struct ExpandedTile {
+    uint8_t key[kTileKeys][2 * kKey];
+    uint8_t value[kTileKeys][2 * kValue];
+    uint8_t rope[kTileKeys][2 * kRopeDims];
+};
+
+__device__ __forceinline__ f32x16 mfma32(const Frag& a, const Frag& b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, c, 0, 0, 0);
+}
+
+// A fragment of V^T, rows 32 d .., of 16 keys 16 kk ..: lanes 4r .. 4r + 3 of a
+// group of 16 hand in 16 columns of a key, lane n gets column n of four keys.
+__device__ __forceinline__ Frag values(const ExpandedTile& tile, int kk, int d) {
+    const int32_t lane = (int32_t)threadIdx.x % kWave;
+    const int32_t r = 16 * kk + 4 * (lane >> 5) + ((lane & 15) >> 2);
+    const int32_t chunk = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    Frag v;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const uint8_t* at = &tile.value[r + 8 * e][16 * (chunk ^ (4 * (r & 3))) + 8 * (lane & 1)];
+        const u32x2 w = __builtin_bit_cast(
+            u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)at));
+        v.w[2 * e] = w[0];
+        v.w[2 * e + 1] = w[1];
+    }
+    return v;
+}
+
+// bf16 pairs without their infinities and NaN (zeros there), and with 1.0 where
+// the number is +inf or NaN, or -inf or NaN.
+__device__ __forceinline__ void split_odd(uint32_t w, uint32_t& plain, uint32_t& pos, uint32_t& neg) {
+    plain = pos = neg = 0;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const uint32_t x = (w >> (16 * half)) & 0xffffu;
+        const bool odd = (x & 0x7f80u) == 0x7f80u, nan = odd && (x & 0x7fu) != 0;
+        plain |= (odd ? 0u : x) << (16 * half);
+        pos |= (odd && (nan || x == 0x7f80u) ? 0x3f80u : 0u) << (16 * half);
+        neg |= (odd && (nan || x == 0xff80u) ? 0x3f80u : 0u) << (16 * half);
+    }
+}
+
+// The product of a tile with masked keys where a value may be infinite or NaN:
+// the finite values as they are, and counts of the +inf and -inf (NaN: both)
+// that each query sees.
+__device__ __forceinline__ void careful_product(f32x16 (&sums)[4], const Frag (&p)[4], const ExpandedTile& tile,
+                                                int32_t left) {
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        f32x16 up, down;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) up[i] = down[i] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            const Frag v = values(tile, kk, d);
+            Frag plain, pos, neg, see;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                split_odd(v.w[i], plain.w[i], pos.w[i], neg.w[i]);
+                const int32_t key = 16 * kk + 8 * (i / 2) + 2 * (i & 1);  // (of the lane's numbers 2i, 2i + 1)
+                see.w[i] = (key < left ? 0x3f80u : 0u) | (key + 1 < left ? 0x3f800000u : 0u);
+            }
+            sums[d] = mfma32(plain, p[kk], sums[d]);
+            up = mfma32(pos, see, up);
+            down = mfma32(neg, see, down);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            sums[d][i] += (up[i] > 0.f ? __builtin_inff() : 0.f) - (down[i] > 0.f ? __builtin_inff() : 0.f);
+    }
+}
+
+// The work-group's part of the attention.  A masked key's probability is zero,
+// which an infinite or NaN value would turn into NaN in the product: sums that
+// end up not finite (true is returned, nothing written) are found again by the
+// CAREFUL form.
+template <int NW, int NB, bool CAREFUL>
+__device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedTile* lds) {
+    constexpr int COPIES = (int)(sizeof(ExpandedTile) / 1024) / NW;
+    const int32_t wave = __builtin_amdgcn_readfirstlane((int32_t)threadIdx.x / kWave);
+    const int32_t lane = (int32_t)threadIdx.x % kWave, c = lane & 31, h = lane >> 5;
+
+    // work-groups reach the XCDs in turn: each XCD takes whole heads, their
+    // blocks side by side (they read the same keys), the longest first
+    int32_t index = ((int32_t)blockIdx.x % 8) * p.spread + (int32_t)blockIdx.x / 8;
+    const int32_t part = index % p.parts;
+    index /= p.parts;
+    const int32_t block = p.blocks - 1 - index % p.blocks;
+    index /= p.blocks;
+    const int32_t head = index % p.heads, b = index / p.heads;
+    if (b >= p.batch) return false;
+    const int32_t q_lo = min(max(p.cu_q[b], 0), p.tokens), q_hi = min(max(p.cu_q[b + 1], q_lo), p.tokens);
+    const int32_t k_lo = min(max(p.cu_k[b], 0), p.keys), k_hi = min(max(p.cu_k[b + 1], k_lo), p.keys);
+    const int32_t nq = q_hi - q_lo, nk = k_hi - k_lo;
+    const int32_t q0 = block * kRows * NW;
+    if (q0 >= nq) return false;
+
+    // keys that query i sees: the first seen(i)
+    auto seen = [&](int32_t i) __attribute__((always_inline)) { return p.causal ? min(max(nk - nq + i + 1, 0), nk) : nk; };
+    const int32_t i0 = q0 + wave * kRows;                                // this wave's first query
+    const int32_t my_seen = seen(min(i0 + c, nq - 1));
+    const int32_t wave_least = i0 < nq ? seen(i0) : 0, wave_most = i0 < nq ? seen(min(i0 + kRows, nq) - 1) : 0;
+    const int32_t all_tiles = tiles_of(seen(min(q0 + kRows * NW, nq) - 1));
+    const int32_t each = (all_tiles + p.parts - 1) / p.parts;
+    const int32_t first = min(part * each, all_tiles), tiles = min(each, all_tiles - first);
+
+    auto copy_tile = [&](int32_t t) __attribute__((always_inline)) {
+        ExpandedTile& to = lds[t % NB];
+        const int32_t k0 = (first + t) * kTileKeys;
+#pragma unroll
+        for (int j = 0; j < COPIES; ++j) {
+            const int32_t i = j * NW + wave;
+            if (i < 32) {  // keys (16 copies of 4 rows), then values
+                const int32_t r = 4 * (i & 15) + (lane >> 4), at = lane & 15;
+                const int32_t chunk = i < 16 ? at ^ (r & 15) : 16 + (at ^ (4 * (r & 3)));
+                const int64_t key = k_lo + min(k0 + r, nk - 1);
+                copy_to_lds(p.kv + key * p.kv_row + head * p.kv_head + 8 * chunk,
+                            lds_offset(i < 16 ? &to.key[4 * i][0] : &to.value[4 * (i - 16)][0]));
+            } else {
+                const int32_t r = 8 * (i - 32) + (lane >> 3);
+                const int64_t key = k_lo + min(k0 + r, nk - 1);
+                copy_to_lds(p.rope + key * p.rope_row + 8 * ((lane & 7) ^ (r & 7)), lds_offset(&to.rope[8 * (i - 32)][0]));
+            }
+        }
+    };
+    for (int t = 0; t < NB - 1; ++t)
+        if (t < tiles) copy_tile(t);
+
+    // B fragments of Q^T: column c = query i0 + c
+    Frag q[12];
+    {
+        const uint16_t* src = p.q + (q_lo + (int64_t)min(i0 + c, nq - 1)) * p.q_row + head * p.q_head + 8 * h;
+#pragma unroll
+        for (int s = 0; s < 12; ++s) q[s].u = *reinterpret_cast<const u32x4*>(src + 16 * s);
+    }
+    f32x16 acc[4];
+    float mx = -__builtin_inff(), total = 0.f;
+
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+#pragma unroll 1
+    for (int32_t t = 0; t < tiles; ++t) {
+        if (NB > 2 && t + 1 < tiles) wait_barrier<(NB - 2) * COPIES>();
+        else wait_barrier<0>();
+        if (t + NB - 1 < tiles) copy_tile(t + NB - 1);
+        const int32_t k0 = (first + t) * kTileKeys;
+        if (k0 >= wave_most) continue;
+        const ExpandedTile& tile = lds[t % NB];
+        // scores: register i of half u is key 32u + 8 (i / 4) + 4h + i % 4
+        f32x16 s[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
+            const int32_t r = 32 * u + c;
+#pragma unroll
+            for (int st = 0; st < 8; ++st) {
+                Frag k;
+                k.u = *reinterpret_cast<const u32x4*>(&tile.key[r][16 * ((2 * st + h) ^ (r & 15))]);
+                s[u] = mfma32(k, q[st], s[u]);
+            }
+#pragma unroll
+            for (int st = 0; st < 4; ++st) {
+                Frag k;
+                k.u = *reinterpret_cast<const u32x4*>(&tile.rope[r][16 * ((2 * st + h) ^ (r & 7))]);
+                s[u] = mfma32(k, q[8 + st], s[u]);
+            }
+        }
+        const bool masked = k0 + kTileKeys > wave_least;  // a key of the tile that a query of the wave does not see
+        if (masked) {
+            const int32_t left = my_seen - k0 - 4 * h;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (32 * u + 8 * (i / 4) + i % 4 >= left) s[u][i] = -__builtin_inff();
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
+        top = fmaxf(top, __shfl_xor(top, 32, kWave)) * p.scale2;
+        if (__ballot(top > mx + kLag)) {
+            const float next = top > mx + kLag ? top : mx;
+            const float keep = mx == -__builtin_inff() ? (next == mx ? 1.f : 0.f) : __builtin_amdgcn_exp2f(mx - next);
+            mx = next;
+            total *= keep;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) acc[d] *= keep;
+        }
+        const float sub = mx == -__builtin_inff() ? 0.f : mx;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], p.scale2, -sub));
+                total += s[u][i];
+            }
+        Frag pf[4];
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                pf[kk].w[i] = pack_bf16(s[kk / 2][8 * (kk & 1) + 2 * i], s[kk / 2][8 * (kk & 1) + 2 * i + 1]);
+        if (CAREFUL && masked) {
+            careful_product(acc, pf, tile, my_seen - k0 - 4 * h);
+        } else {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) acc[d] = mfma32(values(tile, kk, d), pf[kk], acc[d]);
+        }
+    }
+    if constexpr (!CAREFUL) {
+        float odd = 0.f;  // NaN if a sum is not finite
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) odd = fmaf(acc[d][i], 0.f, odd);
+        if (__syncthreads_or(odd != odd)) return true;
+    }
+    total += __shfl_xor(total, 32, kWave);
+    const int32_t i = i0 + c;
+    if (i >= nq) return false;
+    const bool none = total == 0.f;  // no key seen
+    const int64_t row = q_lo + i;
+    if (p.parts == 1) {
+        const float inv = none ? 0.f : 1.0f / total;
+        uint16_t* out = p.out + row * p.o_row + head * p.o_head + 4 * h;
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int a = 0; a < 4; ++a)
+                *reinterpret_cast<u32x2*>(out + 32 * d + 8 * a) =
+                    none ? u32x2{0, 0} : u32x2{pack_bf16(acc[d][4 * a] * inv, acc[d][4 * a + 1] * inv),
+                                               pack_bf16(acc[d][4 * a + 2] * inv, acc[d][4 * a + 3] * inv)};
+        if (p.lse && h == 0)
+            p.lse[row * p.heads + head] = none ? -__builtin_inff() : (mx + __builtin_amdgcn_logf(total)) * kLn2;
+    } else {
+        const int64_t at = (row * p.parts + part) * p.heads + head;
+        float* o = p.partial.sums + at * kValue + 4 * h;
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int a = 0; a < 4; ++a)
+                *reinterpret_cast<f32x4*>(o + 32 * d + 8 * a) =
+                    f32x4{acc[d][4 * a], acc[d][4 * a + 1], acc[d][4 * a + 2], acc[d][4 * a + 3]};
+        if (h == 0) p.partial.stats[at] = f32x2{mx, total};
+    }
+    return false;
+}
+
+// (A call, so that its registers are not the common form's.)
+template <int NW, int NB>
+__device__ __attribute__((noinline)) void careful_part(ExpandedParams p, ExpandedTile* lds) {
+    expanded_part<NW, NB, true>(p, lds);
+}
+
+template <int NW, int NB>
+__global__ __launch_bounds__(64 * NW, 2) void expanded_kernel(ExpandedParams p) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
+    ExpandedTile* const lds = reinterpret_cast<ExpandedTile*>(lds_raw);
+    if (__builtin_expect(expanded_part<NW, NB, false>(p, lds), 0)) careful_part<NW, NB>(p, lds);
+}
+
+// Waves of a work-group and parts of the keys: 256 queries where that gives
+// every CU a work-group, else 128; parts where 128 do not either.
+struct ExpandedShape {
+    int32_t waves, blocks, parts;
+};
+
+inline ExpandedShape expanded_shape(int32_t tokens, int32_t keys, int32_t batch, int32_t heads, int32_t max_q) {
+    const int64_t cus = device_cus();
+    ExpandedShape s;
+    s.waves = (int64_t)heads * (tokens / (8 * kRows)) >= cus ? 8 : 4;
+    s.blocks = (int32_t)cdiv(max_q, s.waves * kRows);
+    const int64_t groups = std::min((int64_t)batch * s.blocks, batch + cdiv(tokens, s.waves * kRows)) * heads;
+    const int64_t tiles = cdiv(keys, kTileKeys);
+    s.parts = (int32_t)std::max<int64_t>(1, std::min(2 * cus / std::max<int64_t>(1, groups), tiles / (4 * batch)));
+    return s;
+}
+
+template <int NW, int NB>
+int launch_expanded(const ExpandedParams& p, int64_t blocks, hipStream_t st) {
+    static OncePerDevice once;
+    constexpr size_t bytes = NB * sizeof(ExpandedTile);
+    const int rc = allow_lds(once, reinterpret_cast<const void*>(expanded_kernel<NW, NB>), bytes, "latent_expanded: LDS");
+    if (rc != V1_OK) return rc;
+    hipLaunchKernelGGL((expanded_kernel<NW, NB>), dim3((uint32_t)blocks), dim3(64 * NW), bytes, st, p);
+    return V1_LAUNCHED("latent_expanded");
+}
+
+}  // namespace
+}  // namespace v1
+
+using namespace v1;
+
+extern "C" int64_t v1_latent_expanded_workspace(int32_t tokens, int32_t keys, int32_t batch, int32_t heads,
+                                                int32_t max_q) {
+    if (tokens <= 0 || keys <= 0 || batch <= 0 || heads <= 0 || max_q <= 0) return 0;
+    const ExpandedShape s = expanded_shape(tokens, keys, batch, heads, max_q);
+    return s.parts == 1 ? 0 : attn::parts_bytes((int64_t)tokens * s.parts, heads, kValue);
+}
+
+extern "C" int v1_latent_expanded(const void* q, int64_t q_row, int64_t q_head, const void* kv, int64_t kv_row,
+                                  int64_t kv_head, const void* rope, int64_t rope_row, const int32_t* cu_q,
+                                  const int32_t* cu_k, int32_t tokens, int32_t keys, int32_t batch, int32_t heads,
+                                  int32_t max_q, int32_t causal, float scale, void* out, int64_t o_row, int64_t o_head,
+                                  float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+    V1_REQUIRE(tokens >= 0 && keys >= 0 && batch >= 0 && heads > 0 && max_q >= 0, "latent_expanded: bad shape");
+    V1_REQUIRE(scale > 0.f && scale < __builtin_inff(), "latent_expanded: scale must be positive and finite");
+    const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kv) | reinterpret_cast<uintptr_t>(rope);
+    V1_REQUIRE(all % 16 == 0 && (q_row | q_head | kv_row | kv_head | rope_row) % 8 == 0 &&
+                   reinterpret_cast<uintptr_t>(out) % 8 == 0 && (o_row | o_head) % 4 == 0,
+               "latent_expanded: q, kv and rope must be 16-byte aligned with strides in multiples of 8, out 8-byte and 4");
+    if (tokens == 0 || batch == 0 || max_q == 0) return V1_OK;
+    const ExpandedShape s = expanded_shape(tokens, std::max(keys, 1), batch, heads, max_q);
+    const int64_t need = v1_latent_expanded_workspace(tokens, keys, batch, heads, max_q);
+    V1_REQUIRE(workspace_bytes >= need && (need == 0 || workspace != nullptr),
+               "latent_expanded: workspace of %lld bytes needed", (long long)need);
+    const int64_t items = (int64_t)batch * heads * s.blocks * s.parts, spread = cdiv(items, 8);
+    V1_REQUIRE(items < 1ll << 30, "latent_expanded: too many work items");
+    ExpandedParams p{static_cast<const uint16_t*>(q), q_row, q_head, static_cast<const uint16_t*>(kv), kv_row, kv_head,
+                     static_cast<const uint16_t*>(rope), rope_row, cu_q, cu_k, tokens, keys, batch, heads, s.blocks,
+                     causal, s.parts, (int32_t)spread, scale * kLog2e, static_cast<uint16_t*>(out), o_row, o_head, lse,
+                     parts_at(workspace, (int64_t)tokens * s.parts, heads, kValue)};
+    const hipStream_t st = as_stream(stream);
+    const int rc = s.waves == 8 ? launch_expanded<8, 3>(p, 8 * spread, st) : launch_expanded<4, 2>(p, 8 * spread, st);
+    if (rc != V1_OK || s.parts == 1) return rc;
+    // (as rows of s.parts one-tile parts)
+    JoinParams j{Plan{nullptr, tokens, s.parts * kTileKeys, 1, 0}, p.partial, p.out, o_row, o_head, lse, heads, cu_q, batch};
+    hipLaunchKernelGGL(join_kernel<kValue>, dim3((uint32_t)tokens, (uint32_t)cdiv(heads, 4)), dim3(256), 0, st, j);
+    return V1_LAUNCHED("latent_expanded: join");
+}

@@ -414,6 +414,7 @@ extern "C" int v1_latent_attend(const void* q, int64_t q_row, int64_t q_head, co
                                 int32_t rows, int32_t heads, int32_t keys, float scale, void* out, int64_t o_row,
                                 int64_t o_head, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
     V1_REQUIRE(rows >= 0 && heads > 0 && keys >= 0 && pool_rows >= 0 && pool_rows < 1ll << 31, "latent_attend: bad shape");
+    V1_REQUIRE(scale > 0.f && scale < __builtin_inff(), "latent_attend: scale must be positive and finite");
     V1_REQUIRE(map_shift >= 0 && map_shift < 31 && map_len >= 0, "latent_attend: bad page map");
     V1_REQUIRE(aligned16(q) && aligned16(pool) && reinterpret_cast<uintptr_t>(out) % 8 == 0 && q_row % 8 == 0 &&
                    q_head % 8 == 0 && o_row % 4 == 0 && o_head % 4 == 0,
@@ -437,7 +438,7 @@ extern "C" int v1_latent_attend(const void* q, int64_t q_row, int64_t q_head, co
                    : hb == 32 ? launch_absorbed<2, 1, 3>(p, blocks, st)
                               : launch_absorbed<2, 2, 2>(p, blocks, st);
     if (rc != V1_OK || need == 0) return rc;
-    JoinParams j{plan, p.parts, p.out, o_row, o_head, lse, heads};
+    JoinParams j{plan, p.parts, p.out, o_row, o_head, lse, heads, nullptr, 0};
     hipLaunchKernelGGL(join_kernel<kLatent>, dim3((uint32_t)rows, (uint32_t)cdiv(heads, 4)), dim3(256), 0, st, j);
     return V1_LAUNCHED("latent_attend: join");
 }

@@ -40,6 +40,13 @@ def _output(out, like, shape):
     return out
 
 
+def _scale(softmax_scale):
+    scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(HEAD + ROPE)
+    if not 0.0 < scale < math.inf:
+        raise ValueError("softmax_scale must be positive and finite")
+    return scale
+
+
 def store_rows(latent, rope, pool, slots):
     """Writes token t's row into pool[slots[t]] (a slot below zero or past the
     pool: the token is skipped; slots of one call are distinct, or which token's
@@ -76,7 +83,7 @@ def attend(q, pool, ids=None, table=None, page_bits=0, lens=None, softmax_scale=
            Without ids and lens every position of the table (or pool) is attended.
 
     Ids below zero, past the table or outside the pool are not attended.  A row
-    without keys gives zeros and a log-sum-exp of -inf.  softmax_scale: default
+    without keys gives zeros and a log-sum-exp of -inf.  softmax_scale > 0: default
     1 / sqrt(192), that of the expanded form.  Returns out [rows, heads, 512] bf16,
     and with return_lse the natural log of the sum of exponentials, [rows, heads] fp32."""
     _lib.require_gpu(q, pool, ids, table, lens, out)
@@ -108,7 +115,7 @@ def attend(q, pool, ids=None, table=None, page_bits=0, lens=None, softmax_scale=
         _int32("lens", lens, (rows,))
     out = _output(out, q, (rows, heads, LATENT))
     lse = torch.empty((rows, heads), device=q.device, dtype=torch.float32) if return_lse else None
-    scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(HEAD + ROPE)
+    scale = _scale(softmax_scale)
     # (the sums of a row's parts are the call's own, as in attention.attend_slots)
     ws_bytes = _lib.lib().v1_latent_attend_workspace(rows, heads, keys, lens is not None)
     ws = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8) if ws_bytes else None
@@ -116,4 +123,56 @@ def attend(q, pool, ids=None, table=None, page_bits=0, lens=None, softmax_scale=
               _lib.ptr(table), map_len, map_stride, page_bits, _lib.ptr(ids), ids.stride(0) if ids is not None else 0,
               _lib.ptr(lens), rows, heads, keys, scale, _lib.ptr(out), out.stride(0), out.stride(1), _lib.ptr(lse),
               _lib.ptr(ws), ws_bytes, _lib.stream_of(q))
+    return (out, lse) if return_lse else out
+
+
+def attend_expanded(q, kv, k_rope, cu_q, cu_k=None, max_q=None, softmax_scale=None, causal=True, out=None,
+                    return_lse=False):
+    """Attention of a batch of sequences laid end to end, over keys and values
+    expanded per head from the latent:
+    S[i, j] = scale * (q[i, h, :128] . kv[j, h, :128] + q[i, h, 128:] . k_rope[j]),
+    out[i, h] = sum_j softmax_j(S[i, j]) kv[j, h, 128:].
+
+    q:      [tokens, heads, 192] bf16
+    kv:     [keys, heads, 256] bf16 (128 key numbers, then 128 value numbers: the
+            up-projection's output as it is)
+    k_rope: [keys, 64] bf16, every head's
+    cu_q, cu_k: [batch + 1] int32, where each sequence's queries and keys begin and
+            end (cu_k None: cu_q).  With `causal`, query i of nq sees keys
+            j <= nk - nq + i of its nk (a chunk at the end of its context), else all.
+    max_q:  at least the longest sequence's queries (queries past it are not
+            computed); None: tokens.
+
+    A query without keys gives zeros and -inf; rows outside [cu_q[0], cu_q[-1]) of
+    `out` are left as they are.  softmax_scale > 0, default 1 / sqrt(192).  Returns
+    out [tokens, heads, 128] bf16, and with return_lse the natural log of the sum
+    of exponentials, [tokens, heads] fp32."""
+    cu_k = cu_q if cu_k is None else cu_k
+    _lib.require_gpu(q, kv, k_rope, cu_q, cu_k, out)
+    if q.dim() != 3 or q.shape[2] != HEAD + ROPE or q.dtype != torch.bfloat16 or q.stride(2) != 1 or not q.shape[1]:
+        raise ValueError(f"q must be bfloat16 [tokens, heads, {HEAD + ROPE}] with a contiguous last dimension")
+    tokens, heads, _ = q.shape
+    if kv.dtype != torch.bfloat16 or kv.dim() != 3 or tuple(kv.shape[1:]) != (heads, 2 * HEAD) or kv.stride(2) != 1:
+        raise ValueError(f"kv must be bfloat16 [keys, heads, {2 * HEAD}] with a contiguous last dimension")
+    keys = kv.shape[0]
+    if k_rope.dtype != torch.bfloat16 or tuple(k_rope.shape) != (keys, ROPE) or k_rope.stride(1) != 1:
+        raise ValueError(f"k_rope must be bfloat16 [keys, {ROPE}] with a contiguous last dimension")
+    if cu_q.dim() != 1 or cu_q.numel() < 1:
+        raise ValueError("cu_q must be a contiguous int32 [batch + 1] tensor")
+    _int32("cu_q", cu_q, (cu_q.numel(),))
+    _int32("cu_k", cu_k, (cu_q.numel(),))
+    max_q = tokens if max_q is None else int(max_q)
+    if max_q < 0:
+        raise ValueError("max_q must not be negative")
+    max_q = min(max_q, tokens)
+    scale = _scale(softmax_scale)
+    out = _output(out, q, (tokens, heads, HEAD))
+    lse = torch.empty((tokens, heads), device=q.device, dtype=torch.float32) if return_lse else None
+    batch = cu_q.numel() - 1
+    ws_bytes = _lib.lib().v1_latent_expanded_workspace(tokens, keys, batch, heads, max_q)
+    ws = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8) if ws_bytes else None
+    _lib.call("v1_latent_expanded", _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(kv), kv.stride(0), kv.stride(1),
+              _lib.ptr(k_rope), k_rope.stride(0), _lib.ptr(cu_q), _lib.ptr(cu_k), tokens, keys, batch, heads, max_q,
+              int(bool(causal)), scale, _lib.ptr(out), out.stride(0), out.stride(1), _lib.ptr(lse), _lib.ptr(ws),
+              ws_bytes, _lib.stream_of(q))
     return (out, lse) if return_lse else out

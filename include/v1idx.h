@@ -609,6 +609,21 @@ int v1_latent_attend(const void* q, int64_t q_row, int64_t q_head, const void* p
                      int32_t rows, int32_t heads, int32_t keys, float scale, void* out, int64_t o_row,
                      int64_t o_head, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
 int64_t v1_latent_attend_workspace(int32_t rows, int32_t heads, int32_t keys, int32_t ragged);
+/* Attention of ragged sequences over keys and values expanded per head: q
+ * [tokens, heads, 192], kv [keys, heads, 128 key | 128 value], rope [keys, 64]
+ * (every head's), all bf16; sequence b holds queries cu_q[b] .. cu_q[b + 1] and
+ * keys cu_k[b] .. cu_k[b + 1] (clamped to the tensors).  out[i, h] (bf16, 128) =
+ * softmax over the keys that query i sees of scale * q . (k_j, rope_j), times
+ * v_j; causal: query i of nq sees keys j <= nk - nq + i, else all.  No key: zeros
+ * and an lse of -inf.  max_q: at least the longest sequence's queries.  lse (may
+ * be NULL): [tokens, heads].  Rows outside the sequences are not written.
+ * workspace: v1_latent_expanded_workspace bytes, as above.  scale > 0. */
+int v1_latent_expanded(const void* q, int64_t q_row, int64_t q_head, const void* kv, int64_t kv_row,
+                       int64_t kv_head, const void* rope, int64_t rope_row, const int32_t* cu_q,
+                       const int32_t* cu_k, int32_t tokens, int32_t keys, int32_t batch, int32_t heads,
+                       int32_t max_q, int32_t causal, float scale, void* out, int64_t o_row, int64_t o_head,
+                       float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t v1_latent_expanded_workspace(int32_t tokens, int32_t keys, int32_t batch, int32_t heads, int32_t max_q);
 #ifdef __cplusplus
 }
 #endif
