@@ -165,6 +165,13 @@ _SIGNATURES = {
     "v1_latent_expanded": (_c_i32, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp, _c_i32, _c_i32,
                                     _c_i32, _c_i32, _c_i32, _c_i32, ctypes.c_float, _vp, _c_i64, _c_i64, _vp, _vp,
                                     _c_i64, _vp]),
+    "v1_kv8_store": (_c_i32, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64,
+                              _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i32, _vp, _vp, _c_i32, _c_i32,
+                              _c_i32, _vp]),
+    "v1_kv8_attend": (_c_i32, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64,
+                               _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i32, _vp, _c_i64, _vp, _c_i32, _c_i32, _c_i32, _c_i32,
+                               ctypes.c_float, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64, _vp]),
+    "v1_kv8_attend_workspace": (_c_i64, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32]),
     "v1_latent_expanded_workspace": (_c_i64, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32]),
 }
 

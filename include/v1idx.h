@@ -624,6 +624,43 @@ int v1_latent_expanded(const void* q, int64_t q_row, int64_t q_head, const void*
                        int32_t max_q, int32_t causal, float scale, void* out, int64_t o_row, int64_t o_head,
                        float* lse, void* workspace, int64_t workspace_bytes, void* stream);
 int64_t v1_latent_expanded_workspace(int32_t tokens, int32_t keys, int32_t batch, int32_t heads, int32_t max_q);
+/* ------------------------------------------------------------------------
+ * K / V pages of 64 tokens in OCP e4m3fn codes, [pages, 64, kv_heads, 128] with
+ * any strides (bytes: page, token, head), and one fp32 scale for each page and
+ * head, [pages, kv_heads] (K and V their own; *_page: row strides).  No
+ * counterpart in the reference, whose K / V pools are bf16.
+ *
+ * v1_kv8_store appends cu_tokens[r + 1] - cu_tokens[r] tokens of k, v [tokens,
+ * kv_heads, 128] bf16 to request r at positions starts[r] .. of its page table
+ * row.  A page written from its first token gets the smallest power of two s >=
+ * 2^-126 with |x| <= 448 s for the new tokens' finite numbers; one that holds
+ * older tokens the larger of that and its scale, its older codes rounded again
+ * where the scale grew.  Codes round to nearest even, infinities become +-448 s.
+ * Positions past the table, pages outside the pool and negative starts are
+ * skipped; a page is appended to by one request of a call.
+ * ---------------------------------------------------------------------- */
+int v1_kv8_store(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                 void* k_pool, int64_t kp_page, int64_t kp_token, int64_t kp_head, void* v_pool,
+                 int64_t vp_page, int64_t vp_token, int64_t vp_head, float* k_scale, int64_t ks_page,
+                 float* v_scale, int64_t vs_page, int64_t pages, const int32_t* table, int64_t table_stride,
+                 int32_t table_len, const int32_t* starts, const int32_t* cu_tokens, int32_t tokens,
+                 int32_t requests, int32_t kv_heads, void* stream);
+/* Attention of one query position per row: q [rows, kv_heads * group, 128] bf16
+ * (group <= 16), key j of row r at position id = ids[r * ids_stride + j] (j when
+ * ids is NULL), j < lens[r] clamped to [0, keys] (keys when lens is NULL), in
+ * page table[r * table_stride + id / 64].  An id < 0, past the table or in a page
+ * outside the pool is not attended; a row without keys gives zeros and an lse of
+ * -inf.  out [rows, heads, 128] bf16, lse [rows, heads] (may be NULL).  workspace:
+ * v1_kv8_attend_workspace(rows, kv_heads, group, keys, lens != NULL) bytes, the
+ * call's own until the stream has passed it.  scale > 0. */
+int v1_kv8_attend(const void* q, int64_t q_row, int64_t q_head, const void* k_pool, int64_t kp_page,
+                  int64_t kp_token, int64_t kp_head, const void* v_pool, int64_t vp_page, int64_t vp_token,
+                  int64_t vp_head, const float* k_scale, int64_t ks_page, const float* v_scale, int64_t vs_page,
+                  int64_t pages, const int32_t* table, int64_t table_stride, int32_t table_len,
+                  const int32_t* ids, int64_t ids_stride, const int32_t* lens, int32_t rows, int32_t kv_heads,
+                  int32_t group, int32_t keys, float scale, void* out, int64_t o_row, int64_t o_head,
+                  float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t v1_kv8_attend_workspace(int32_t rows, int32_t kv_heads, int32_t group, int32_t keys, int32_t ragged);
 #ifdef __cplusplus
 }
 #endif
