@@ -81,57 +81,198 @@ struct AbsorbedParams {
 // The row of keys that are not attended (their scores are -inf).
 __device__ const u32x4 zero_latent[kChunks] = {};
 
-constexpr int kPRow = kTileKeys * 2 + 16;  // bytes of a head's probabilities of a tile; 9 chunks of 16: 8 heads meet 8 different banks
 constexpr float kLag = 6.f;  // the subtracted maximum may lag the true one by 2^6
 
-template <int HT, int HG, int NB>
+template <int HT, int HG>
 struct AbsorbedLds {
-    static constexpr int kHeads = 16 * HT * HG;
-    uint8_t tile[NB][kTileBytes];
-    uint8_t prob[kScaleBlocks][kHeads][kPRow];
-    float hidden[NB][kTileKeys];  // 0, or -inf: not attended
-    float top[4][kHeads];
+    static constexpr int kHeads = 16 * HT * HG, kQuarters = 4 / HG;
+    uint8_t tile[3][kTileBytes];
+    uint16_t prob[kScaleBlocks][kHeads][kTileKeys];  // 16-byte chunk n of head h at n ^ (h % 8)
+    float hidden[3][kTileKeys];                      // 0, or -inf: not attended
+    float top[kQuarters][kHeads];
     float keep[kHeads];
-    float total[4][kHeads];
+    float total[kQuarters][kHeads];
 };
 
-// A work-group of 4 * HG waves attends 16 * HT * HG heads of one row over one
+// A work-group of eight waves attends HB = 16 * HT * HG heads of one row over one
 // part of its keys, tile by tile of 64 keys that come memory -> LDS as they are
-// stored (NB buffers).
-//   scores  S^T = K Q^T: wave (hg, kq) takes heads 16 HT hg .. and keys 16 kq ..;
+// stored.  Four waves make the probabilities of tile t while the other four, one
+// on each SIMD beside them, multiply those of tile t - 1 with the latents and
+// bring in tile t + 1: the products keep the matrix cores busy through the
+// others' softmax, and neither kind holds both Q and the output (144 and 128
+// registers at 64 heads: two waves per SIMD have 256 each).
+//   scores  S^T = K Q^T: wave (hg, kq) takes heads 16 HT hg .. and 16 HG keys;
 //           codes become bf16 (exact) as they are read, one accumulator per block
 //           of 128 numbers, joined with the block's scales in fp32.
-//   softmax the four key quarters exchange their maxima through LDS; each
-//           probability is multiplied by its key's four scales and rounded to
-//           bf16 once (2^-9 relative, as in the output), the sum stays fp32.
-//   output  O^T = C^T P^T: wave w takes 512 / waves columns of all heads, its
+//   softmax the key groups exchange their maxima through LDS; each probability is
+//           multiplied by its key's four scales and rounded to bf16 once (2^-9
+//           of it at most, as the output), the sum stays fp32.
+//   output  O^T = C^T P^T: a wave takes a block of 128 columns of all heads, its
 //           codes transposed by the LDS read (ds_read_b64_tr_b8), exact in bf16.
-template <int HT, int HG, int NB>
-__global__ __launch_bounds__(256 * HG) void absorbed_kernel(AbsorbedParams p) {
-    constexpr int NW = 4 * HG, HB = 16 * HT * HG, RPW = kTileKeys / NW, GT = kWave / RPW;
+template <int HT, int HG>
+__global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
+    constexpr int HB = 16 * HT * HG, KT = HG, KQ = 4 / HG, RPW = kTileKeys / 4, GT = kWave / RPW;
     constexpr int COPIES = (RPW * kChunks + kWave - 1) / kWave;
-    constexpr int DV = kLatent / NW, DT = DV / 16, PT = HB / 16;
+    constexpr int DT = 8, PT = HB / 16;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
-    auto& lds = *reinterpret_cast<AbsorbedLds<HT, HG, NB>*>(lds_raw);
-    const int32_t wave = __builtin_amdgcn_readfirstlane((int32_t)threadIdx.x / kWave);
+    auto& lds = *reinterpret_cast<AbsorbedLds<HT, HG>*>(lds_raw);
+    const int32_t wave = __builtin_amdgcn_readfirstlane((int32_t)threadIdx.x / kWave) & 3;
+    const bool scorer = __builtin_amdgcn_readfirstlane((int32_t)threadIdx.x / kWave) < 4;
     const int32_t lane = (int32_t)threadIdx.x % kWave, g = lane >> 4, c = lane & 15;
-    const int32_t hg = wave >> 2, kq = wave & 3;
 
     // work-groups reach the XCDs in turn: the splits of an item follow each other on one of them
     const int32_t xcd = (int32_t)blockIdx.x % 8, turn = (int32_t)blockIdx.x / 8;
     const int32_t index = xcd * p.spread + turn / p.splits, split = turn % p.splits;
     Item it;
     if (!find_item(p.plan, index, it)) return;
-    const int32_t head0 = split * HB;
+    const int32_t head0 = split * HB, tiles = it.tiles;
+
+    if (scorer) {
+        const int32_t hg = wave / KQ, kq = wave % KQ;
+        // B fragments of Q^T: column c = head c of 16; 64 numbers in two steps: lane
+        // group g takes 16g .. 16g + 7 of them, then 16g + 8 .. 16g + 15 (the order in which the codes are read)
+        Frag q[HT][18];
+#pragma unroll
+        for (int ht = 0; ht < HT; ++ht) {
+            const int32_t h = min(head0 + hg * 16 * HT + 16 * ht + c, p.heads - 1);
+            const uint16_t* src = p.q + it.row * p.q_row + h * p.q_head;
+#pragma unroll
+            for (int s = 0; s < 16; ++s)
+                q[ht][s].u = *reinterpret_cast<const u32x4*>(src + 64 * (s / 2) + 16 * g + 8 * (s % 2));
+#pragma unroll
+            for (int s = 0; s < 2; ++s) q[ht][16 + s].u = *reinterpret_cast<const u32x4*>(src + kLatent + 32 * s + 8 * g);
+        }
+        float mx[HT], total[HT];
+#pragma unroll
+        for (int ht = 0; ht < HT; ++ht) mx[ht] = -__builtin_inff(), total[ht] = 0.f;
+
+#pragma unroll 1
+        for (int32_t t = 0; t <= tiles; ++t) {
+            lds_barrier();  // tile t has landed; probabilities of tile t - 1 are written
+            const uint8_t* tile = lds.tile[t % 3];
+            float s[KT][HT][4];  // of keys 16 (KT kq + kt) + 4g + i, heads c
+            if (t < tiles) {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    const int32_t k0 = 16 * (KT * kq + kt);
+                    const uint8_t* key = tile + (k0 + c) * kRowBytes;
+                    f32x4 d[HT];
+#pragma unroll
+                    for (int ht = 0; ht < HT; ++ht) d[ht] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        Frag k;
+                        k.u = *reinterpret_cast<const u32x4*>(key + kRopeAt + 64 * r + 16 * g);
+#pragma unroll
+                        for (int ht = 0; ht < HT; ++ht) d[ht] = mfma16(k, q[ht][16 + r], d[ht]);
+                    }
+                    f32x4 sc[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        sc[i] = *reinterpret_cast<const f32x4*>(tile + (k0 + 4 * g + i) * kRowBytes + kScaleAt);
+#pragma unroll
+                    for (int ht = 0; ht < HT; ++ht)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[kt][ht][i] = d[ht][i];
+#pragma unroll
+                    for (int b = 0; b < kScaleBlocks; ++b) {
+#pragma unroll
+                        for (int ht = 0; ht < HT; ++ht) d[ht] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const u32x4 w = *reinterpret_cast<const u32x4*>(key + 128 * b + 64 * half + 16 * g);
+                            const Frag k0f = bf16_of_codes(w[0], w[1]), k1f = bf16_of_codes(w[2], w[3]);
+#pragma unroll
+                            for (int ht = 0; ht < HT; ++ht) d[ht] = mfma16(k0f, q[ht][4 * b + 2 * half], d[ht]);
+#pragma unroll
+                            for (int ht = 0; ht < HT; ++ht) d[ht] = mfma16(k1f, q[ht][4 * b + 2 * half + 1], d[ht]);
+                        }
+#pragma unroll
+                        for (int ht = 0; ht < HT; ++ht)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s[kt][ht][i] = fmaf(sc[i][b], d[ht][i], s[kt][ht][i]);
+                    }
+                    const f32x4 hidden = *reinterpret_cast<const f32x4*>(&lds.hidden[t % 3][k0 + 4 * g]);
+#pragma unroll
+                    for (int ht = 0; ht < HT; ++ht)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            s[kt][ht][i] = hidden[i] < 0.f ? -__builtin_inff() : s[kt][ht][i] * p.scale2;
+                }
+#pragma unroll
+                for (int ht = 0; ht < HT; ++ht) {
+                    float top = -__builtin_inff();
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[kt][ht][i]);
+                    top = fmaxf(top, __shfl_xor(top, 16, kWave));
+                    top = fmaxf(top, __shfl_xor(top, 32, kWave));
+                    if (g == 0) lds.top[kq][16 * (HT * hg + ht) + c] = top;
+                }
+            }
+            lds_barrier();  // maxima of tile t are there; probabilities of tile t - 1 have been read
+            if (t < tiles) {
+                float sub[HT];
+#pragma unroll
+                for (int ht = 0; ht < HT; ++ht) {
+                    const int32_t h = 16 * (HT * hg + ht) + c;
+                    float top = lds.top[0][h];
+#pragma unroll
+                    for (int k = 1; k < KQ; ++k) top = fmaxf(top, lds.top[k][h]);
+                    float keep = 1.f;
+                    if (top > mx[ht] + kLag) {  // (-inf + kLag is -inf)
+                        keep = mx[ht] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mx[ht] - top);
+                        mx[ht] = top;
+                    }
+                    sub[ht] = mx[ht] == -__builtin_inff() ? 0.f : mx[ht];
+                    total[ht] *= keep;
+                    if (kq == 0 && g == 0) lds.keep[h] = keep;
+                }
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    const int32_t k0 = 16 * (KT * kq + kt);
+                    f32x4 sc[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        sc[i] = *reinterpret_cast<const f32x4*>(tile + (k0 + 4 * g + i) * kRowBytes + kScaleAt);
+#pragma unroll
+                    for (int ht = 0; ht < HT; ++ht) {
+                        const int32_t h = 16 * (HT * hg + ht) + c;
+                        float x[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            x[i] = __builtin_amdgcn_exp2f(s[kt][ht][i] - sub[ht]);
+                            total[ht] += x[i];
+                        }
+                        uint16_t* at = &lds.prob[0][h][8 * ((k0 / 8 + (g >> 1)) ^ (h & 7)) + 4 * (g & 1)];
+#pragma unroll
+                        for (int b = 0; b < kScaleBlocks; ++b)
+                            *reinterpret_cast<u32x2*>(at + b * HB * kTileKeys) =
+                                u32x2{pack_bf16(x[0] * sc[0][b], x[1] * sc[1][b]), pack_bf16(x[2] * sc[2][b], x[3] * sc[3][b])};
+                    }
+                }
+            }
+        }
+        // totals of the key groups
+#pragma unroll
+        for (int ht = 0; ht < HT; ++ht) {
+            const int32_t h = 16 * (HT * hg + ht) + c;
+            float x = total[ht];
+            x += __shfl_xor(x, 16, kWave);
+            x += __shfl_xor(x, 32, kWave);
+            if (g == 0) lds.total[kq][h] = x;
+            if (g == 0 && kq == 0) lds.top[0][h] = mx[ht];
+        }
+        __syncthreads();
+        return;
+    }
 
     // rows of this wave's part of a tile, GT tiles at a time: lane = tile * RPW + row
     const int32_t* ids = p.ids ? p.ids + it.row * p.ids_stride : nullptr;
     const int32_t* map = p.map ? p.map + it.row * p.map_stride : nullptr;
-    auto key_of = [&](int32_t group) __attribute__((always_inline)) {
-        return (it.first + group * GT + lane / RPW) * kTileKeys + wave * RPW + lane % RPW;
-    };
     auto fetch_id = [&](int32_t group) __attribute__((always_inline)) -> int32_t {
-        const int32_t j = key_of(group);
+        const int32_t j = (it.first + group * GT + lane / RPW) * kTileKeys + wave * RPW + lane % RPW;
         if (j >= it.keys) return -1;
         return ids ? ids[j] : j;
     };
@@ -148,15 +289,14 @@ __global__ __launch_bounds__(256 * HG) void absorbed_kernel(AbsorbedParams p) {
         return row < p.pool_rows ? (int32_t)row : -1;
     };
     int32_t rows_now = fetch_row(fetch_id(0)), rows_next = fetch_row(fetch_id(1)), ids_after = fetch_id(2);
-
-    // copies of tile t into buffer t % NB, asked for in the order of the tiles
+    // copies of tile t into buffer t % 3, asked for in the order of the tiles
     auto copy_tile = [&](int32_t t) __attribute__((always_inline)) {
         if (t > 0 && t % GT == 0) {
             rows_now = rows_next;
             rows_next = fetch_row(ids_after);
             ids_after = fetch_id(t / GT + 2);
         }
-        const int32_t buf = t % NB;
+        const int32_t buf = t % 3;
         if (lane / RPW == t % GT) lds.hidden[buf][wave * RPW + lane % RPW] = rows_now < 0 ? -__builtin_inff() : 0.f;
         const uint32_t to = lds_offset(&lds.tile[buf][wave * RPW * kRowBytes]);
 #pragma unroll
@@ -167,160 +307,49 @@ __global__ __launch_bounds__(256 * HG) void absorbed_kernel(AbsorbedParams p) {
             if (r < RPW) copy_to_lds(src + 16 * chunk, to + 1024 * j);
         }
     };
-    const int32_t tiles = it.tiles;
-    for (int t = 0; t < NB - 1; ++t)
-        if (t < tiles) copy_tile(t);
-
-    // B fragments of Q^T: column c = head c of 16; 64 numbers in two steps: lane
-    // group g takes 16g .. 16g + 7 of them, then 16g + 8 .. 16g + 15 (the order in which the codes are read)
-    Frag q[HT][18];
-#pragma unroll
-    for (int ht = 0; ht < HT; ++ht) {
-        const int32_t h = min(head0 + hg * 16 * HT + 16 * ht + c, p.heads - 1);
-        const uint16_t* src = p.q + it.row * p.q_row + h * p.q_head;
-#pragma unroll
-        for (int s = 0; s < 16; ++s) q[ht][s].u = *reinterpret_cast<const u32x4*>(src + 64 * (s / 2) + 16 * g + 8 * (s % 2));
-#pragma unroll
-        for (int s = 0; s < 2; ++s) q[ht][16 + s].u = *reinterpret_cast<const u32x4*>(src + kLatent + 32 * s + 8 * g);
-    }
     f32x4 acc[DT][PT];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int h = 0; h < PT; ++h) acc[d][h] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float mx[HT], total[HT];
-#pragma unroll
-    for (int ht = 0; ht < HT; ++ht) mx[ht] = -__builtin_inff(), total[ht] = 0.f;
-
+    if (tiles > 0) copy_tile(0);
 #pragma unroll 1
-    for (int32_t t = 0; t < tiles; ++t) {
-        // tile t has landed, and every wave has left the buffer that comes next
-        if (NB > 2 && t + 1 < tiles) wait_barrier<(NB - 2) * COPIES>();
-        else wait_barrier<0>();
-        if (t + NB - 1 < tiles) copy_tile(t + NB - 1);
-        const uint8_t* tile = lds.tile[t % NB];
-        // scores of keys 16 kq + 4g + i, heads c
-        float s[HT][4];
-        f32x4 sc[4];
-        {
-            const uint8_t* key = tile + (16 * kq + c) * kRowBytes;
-            f32x4 d[HT];
+    for (int32_t t = 0; t <= tiles; ++t) {
+        wait_barrier<0>();
+        if (t + 1 < tiles) copy_tile(t + 1);
+        Frag pf[2][PT];
+        // lanes 2r, 2r + 1 of a group hand in 16 columns of key 8g + r; lane c gets column c of its eight keys
+        const uint8_t* v = lds.tile[(t + 2) % 3] + (8 * g + c / 2) * kRowBytes + wave * 128 + 8 * (c & 1);
+        auto product = [&](int ks) __attribute__((always_inline)) {
 #pragma unroll
-            for (int ht = 0; ht < HT; ++ht) d[ht] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int d = 0; d < DT; ++d) {
+                const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                    (__attribute__((address_space(3))) i32x2*)(v + 32 * ks * kRowBytes + 16 * d));
+                const Frag a = bf16_of_codes((uint32_t)w[0], (uint32_t)w[1]);
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                Frag k;
-                k.u = *reinterpret_cast<const u32x4*>(key + kRopeAt + 64 * r + 16 * g);
-#pragma unroll
-                for (int ht = 0; ht < HT; ++ht) d[ht] = mfma16(k, q[ht][16 + r], d[ht]);
+                for (int h = 0; h < PT; ++h) acc[d][h] = mfma16(a, pf[ks][h], acc[d][h]);
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                sc[i] = *reinterpret_cast<const f32x4*>(tile + (16 * kq + 4 * g + i) * kRowBytes + kScaleAt);
-#pragma unroll
-            for (int ht = 0; ht < HT; ++ht)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[ht][i] = d[ht][i];
-#pragma unroll
-            for (int b = 0; b < kScaleBlocks; ++b) {
-#pragma unroll
-                for (int ht = 0; ht < HT; ++ht) d[ht] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const u32x4 w = *reinterpret_cast<const u32x4*>(key + 128 * b + 64 * half + 16 * g);
-                    const Frag k0 = bf16_of_codes(w[0], w[1]), k1 = bf16_of_codes(w[2], w[3]);
-#pragma unroll
-                    for (int ht = 0; ht < HT; ++ht) d[ht] = mfma16(k0, q[ht][4 * b + 2 * half], d[ht]);
-#pragma unroll
-                    for (int ht = 0; ht < HT; ++ht) d[ht] = mfma16(k1, q[ht][4 * b + 2 * half + 1], d[ht]);
-                }
-#pragma unroll
-                for (int ht = 0; ht < HT; ++ht)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[ht][i] = fmaf(sc[i][b], d[ht][i], s[ht][i]);
-            }
-        }
-        const f32x4 hidden = *reinterpret_cast<const f32x4*>(&lds.hidden[t % NB][16 * kq + 4 * g]);
-#pragma unroll
-        for (int ht = 0; ht < HT; ++ht) {
-            float top = -__builtin_inff();
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s[ht][i] = hidden[i] < 0.f ? -__builtin_inff() : s[ht][i] * p.scale2;
-                top = fmaxf(top, s[ht][i]);
-            }
-            top = fmaxf(top, __shfl_xor(top, 16, kWave));
-            top = fmaxf(top, __shfl_xor(top, 32, kWave));
-            if (g == 0) lds.top[kq][16 * (HT * hg + ht) + c] = top;
-        }
-        lds_barrier();
-#pragma unroll
-        for (int ht = 0; ht < HT; ++ht) {
-            const int32_t h = 16 * (HT * hg + ht) + c;
-            const float top = fmaxf(fmaxf(lds.top[0][h], lds.top[1][h]), fmaxf(lds.top[2][h], lds.top[3][h]));
-            float keep = 1.f;
-            if (top > mx[ht] + kLag) {  // (-inf + kLag is -inf)
-                keep = mx[ht] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mx[ht] - top);
-                mx[ht] = top;
-            }
-            const float sub = mx[ht] == -__builtin_inff() ? 0.f : mx[ht];
-            total[ht] *= keep;
-            if (kq == 0 && g == 0) lds.keep[h] = keep;
-            float x[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[i] = __builtin_amdgcn_exp2f(s[ht][i] - sub);
-                total[ht] += x[i];
-            }
-#pragma unroll
-            for (int b = 0; b < kScaleBlocks; ++b)
-                *reinterpret_cast<u32x2*>(&lds.prob[b][h][2 * (16 * kq + 4 * g)]) =
-                    u32x2{pack_bf16(x[0] * sc[0][b], x[1] * sc[1][b]), pack_bf16(x[2] * sc[2][b], x[3] * sc[3][b])};
-        }
-        lds_barrier();
-        // output columns DV wave .. of all heads
-        {
+        };
+        if (t > 0) {
             float keep[PT];
             bool any = false;
 #pragma unroll
             for (int h = 0; h < PT; ++h) {
                 keep[h] = lds.keep[16 * h + c];
                 any |= keep[h] != 1.f;
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks)
+                    pf[ks][h].u = *reinterpret_cast<const u32x4*>(&lds.prob[wave][16 * h + c][8 * ((4 * ks + g) ^ (c & 7))]);
             }
             if (__ballot(any))
 #pragma unroll
                 for (int h = 0; h < PT; ++h)
 #pragma unroll
                     for (int d = 0; d < DT; ++d) acc[d][h] *= keep[h];
-            const int32_t b = wave * DV / 128;
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                Frag pf[PT];
-#pragma unroll
-                for (int h = 0; h < PT; ++h)
-                    pf[h].u = *reinterpret_cast<const u32x4*>(&lds.prob[b][16 * h + c][64 * ks + 16 * g]);
-                // lanes 2r, 2r + 1 of a group hand in 16 columns of key 8g + r; lane c gets column c of its eight keys
-                const uint8_t* v = tile + (32 * ks + 8 * g + c / 2) * kRowBytes + wave * DV + 8 * (c & 1);
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                        (__attribute__((address_space(3))) i32x2*)(v + 16 * d));
-                    const Frag a = bf16_of_codes((uint32_t)w[0], (uint32_t)w[1]);
-#pragma unroll
-                    for (int h = 0; h < PT; ++h) acc[d][h] = mfma16(a, pf[h], acc[d][h]);
-                }
-            }
+            product(0);
         }
-    }
-    // totals of the four key quarters
-#pragma unroll
-    for (int ht = 0; ht < HT; ++ht) {
-        const int32_t h = 16 * (HT * hg + ht) + c;
-        float x = total[ht];
-        x += __shfl_xor(x, 16, kWave);
-        x += __shfl_xor(x, 32, kWave);
-        if (g == 0) lds.total[kq][h] = x;
-        if (g == 0 && kq == 0) lds.top[0][h] = mx[ht];
+        lds_barrier();
+        if (t > 0) product(1);
     }
     __syncthreads();
     const bool whole = it.parts == 1;
@@ -328,12 +357,14 @@ __global__ __launch_bounds__(256 * HG) void absorbed_kernel(AbsorbedParams p) {
     for (int ht = 0; ht < PT; ++ht) {
         const int32_t h = 16 * ht + c, head = head0 + h;
         if (head >= p.heads) continue;
-        const float sum = (lds.total[0][h] + lds.total[1][h]) + (lds.total[2][h] + lds.total[3][h]);
+        float sum = lds.total[0][h];
+#pragma unroll
+        for (int k = 1; k < KQ; ++k) sum += lds.total[k][h];
         const float top = lds.top[0][h];
         const bool none = sum == 0.f;  // no key attended
         if (whole) {
             const float inv = none ? 0.f : 1.0f / sum;
-            uint16_t* out = p.out + it.row * p.o_row + head * p.o_head + wave * DV + 4 * g;
+            uint16_t* out = p.out + it.row * p.o_row + head * p.o_head + wave * 128 + 4 * g;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
                 *reinterpret_cast<u32x2*>(out + 16 * d) =
@@ -344,7 +375,7 @@ __global__ __launch_bounds__(256 * HG) void absorbed_kernel(AbsorbedParams p) {
                     none ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * kLn2;
         } else {
             const int64_t at = (int64_t)index * p.heads + head;
-            float* o = p.parts.sums + at * kLatent + wave * DV + 4 * g;
+            float* o = p.parts.sums + at * kLatent + wave * 128 + 4 * g;
 #pragma unroll
             for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(o + 16 * d) = acc[d][ht];
             if (wave == 0 && g == 0) p.parts.stats[at] = f32x2{top, sum};
@@ -368,14 +399,14 @@ inline Plan absorbed_plan(const int32_t* lens, int32_t rows, int32_t heads, int3
     return p;
 }
 
-template <int HT, int HG, int NB>
+template <int HT, int HG>
 int launch_absorbed(const AbsorbedParams& p, int64_t blocks, hipStream_t st) {
     static OncePerDevice once;
-    constexpr size_t bytes = sizeof(AbsorbedLds<HT, HG, NB>);
+    constexpr size_t bytes = sizeof(AbsorbedLds<HT, HG>);
     static_assert(bytes <= 160 * 1024, "LDS of a CU");
-    const int rc = allow_lds(once, reinterpret_cast<const void*>(absorbed_kernel<HT, HG, NB>), bytes, "latent_attend: LDS");
+    const int rc = allow_lds(once, reinterpret_cast<const void*>(absorbed_kernel<HT, HG>), bytes, "latent_attend: LDS");
     if (rc != V1_OK) return rc;
-    hipLaunchKernelGGL((absorbed_kernel<HT, HG, NB>), dim3((uint32_t)blocks), dim3(256 * HG), bytes, st, p);
+    hipLaunchKernelGGL((absorbed_kernel<HT, HG>), dim3((uint32_t)blocks), dim3(512), bytes, st, p);
     return V1_LAUNCHED("latent_attend");
 }
 
@@ -434,9 +465,9 @@ extern "C" int v1_latent_attend(const void* q, int64_t q_row, int64_t q_head, co
                      (int32_t)splits, (int32_t)spread, scale * kLog2e, static_cast<uint16_t*>(out), o_row, o_head, lse,
                      parts_at(workspace, items, heads, kLatent)};
     const hipStream_t st = as_stream(stream);
-    const int rc = hb == 16   ? launch_absorbed<1, 1, 3>(p, blocks, st)
-                   : hb == 32 ? launch_absorbed<2, 1, 3>(p, blocks, st)
-                              : launch_absorbed<2, 2, 2>(p, blocks, st);
+    const int rc = hb == 16   ? launch_absorbed<1, 1>(p, blocks, st)
+                   : hb == 32 ? launch_absorbed<2, 1>(p, blocks, st)
+                              : launch_absorbed<2, 2>(p, blocks, st);
     if (rc != V1_OK || need == 0) return rc;
     JoinParams j{plan, p.parts, p.out, o_row, o_head, lse, heads, nullptr, 0};
     hipLaunchKernelGGL(join_kernel<kLatent>, dim3((uint32_t)rows, (uint32_t)cdiv(heads, 4)), dim3(256), 0, st, j);
