@@ -97,8 +97,8 @@ struct AbsorbedLds {
 // A work-group of eight waves attends HB = 16 * HT * HG heads of one row over one
 // part of its keys, tile by tile of 64 keys that come memory -> LDS as they are
 // stored.  Four waves make the probabilities of tile t while the other four, one
-// on each SIMD beside them, multiply those of tile t - 1 with the latents and
-// bring in tile t + 1: the products keep the matrix cores busy through the
+// on each SIMD beside them, multiply those of tile t - 1 with its latents (held in
+// registers, so that their buffer is free) and bring in tile t + 2: the products keep the matrix cores busy through the
 // others' softmax, and neither kind holds both Q and the output (144 and 128
 // registers at 64 heads: two waves per SIMD have 256 each).
 //   scores  S^T = K Q^T: wave (hg, kq) takes heads 16 HT hg .. and 16 HG keys;
@@ -152,47 +152,71 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
             const uint8_t* tile = lds.tile[t % 3];
             float s[KT][HT][4];  // of keys 16 (KT kq + kt) + 4g + i, heads c
             if (t < tiles) {
+                // Steps of one block of one key tile (the rope numbers are a fifth
+                // block of scale 1): the next step's codes and scales are read, this
+                // one's codes converted and multiplied, the last one's products folded.
+                constexpr int STEPS = KT * 5;
+                const uint8_t* const key0 = tile + (16 * KT * kq + c) * kRowBytes + 16 * g;
+                const uint8_t* const scale0 = tile + (16 * KT * kq + 4 * g) * kRowBytes + kScaleAt;
+                u32x4 raw[2][2];
+                float sc[2][4];
+                f32x4 d[2][HT];
+                auto fetch = [&](int n) __attribute__((always_inline)) {
+                    const int at = (n / 5) * 16 * kRowBytes, b = n % 5;
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    const int32_t k0 = 16 * (KT * kq + kt);
-                    const uint8_t* key = tile + (k0 + c) * kRowBytes;
-                    f32x4 d[HT];
+                    for (int half = 0; half < 2; ++half)
+                        raw[n & 1][half] = *reinterpret_cast<const u32x4*>(key0 + at + 128 * b + 64 * half);
+                    if (b < kScaleBlocks)
 #pragma unroll
-                    for (int ht = 0; ht < HT; ++ht) d[ht] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        Frag k;
-                        k.u = *reinterpret_cast<const u32x4*>(key + kRopeAt + 64 * r + 16 * g);
-#pragma unroll
-                        for (int ht = 0; ht < HT; ++ht) d[ht] = mfma16(k, q[ht][16 + r], d[ht]);
-                    }
-                    f32x4 sc[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        sc[i] = *reinterpret_cast<const f32x4*>(tile + (k0 + 4 * g + i) * kRowBytes + kScaleAt);
+                        for (int i = 0; i < 4; ++i)
+                            sc[n & 1][i] = *reinterpret_cast<const float*>(scale0 + at + i * kRowBytes + 4 * b);
+                };
+                auto fold = [&](int n, float (&f)[4]) __attribute__((always_inline)) {
 #pragma unroll
                     for (int ht = 0; ht < HT; ++ht)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) s[kt][ht][i] = d[ht][i];
-#pragma unroll
-                    for (int b = 0; b < kScaleBlocks; ++b) {
-#pragma unroll
-                        for (int ht = 0; ht < HT; ++ht) d[ht] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            const u32x4 w = *reinterpret_cast<const u32x4*>(key + 128 * b + 64 * half + 16 * g);
-                            const Frag k0f = bf16_of_codes(w[0], w[1]), k1f = bf16_of_codes(w[2], w[3]);
-#pragma unroll
-                            for (int ht = 0; ht < HT; ++ht) d[ht] = mfma16(k0f, q[ht][4 * b + 2 * half], d[ht]);
-#pragma unroll
-                            for (int ht = 0; ht < HT; ++ht) d[ht] = mfma16(k1f, q[ht][4 * b + 2 * half + 1], d[ht]);
+                        for (int i = 0; i < 4; ++i) {
+                            float& x = s[n / 5][ht][i];
+                            x = n % 5 == kScaleBlocks ? x + d[n & 1][ht][i]
+                                : n % 5 == 0          ? f[i] * d[n & 1][ht][i]
+                                                      : fmaf(f[i], d[n & 1][ht][i], x);
                         }
+                };
+                fetch(0);
+                float last[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int ht = 0; ht < HT; ++ht)
+                for (int n = 0; n < STEPS; ++n) {
+                    const int b = n % 5;
+                    float now[4];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) s[kt][ht][i] = fmaf(sc[i][b], d[ht][i], s[kt][ht][i]);
+                    for (int i = 0; i < 4; ++i) now[i] = sc[n & 1][i];
+                    if (n + 1 < STEPS) fetch(n + 1);
+                    Frag k[4];
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const u32x4 w = raw[n & 1][half];
+                        if (b < kScaleBlocks) {
+                            k[2 * half] = bf16_of_codes(w[0], w[1]);
+                            k[2 * half + 1] = bf16_of_codes(w[2], w[3]);
+                        } else {
+                            k[half].u = w;
+                        }
                     }
-                    const f32x4 hidden = *reinterpret_cast<const f32x4*>(&lds.hidden[t % 3][k0 + 4 * g]);
+#pragma unroll
+                    for (int ht = 0; ht < HT; ++ht) d[n & 1][ht] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int j = 0; j < (b < kScaleBlocks ? 4 : 2); ++j)
+#pragma unroll
+                        for (int ht = 0; ht < HT; ++ht) d[n & 1][ht] = mfma16(k[j], q[ht][4 * b + j], d[n & 1][ht]);
+                    if (n > 0) fold(n - 1, last);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) last[i] = now[i];
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                fold(STEPS - 1, last);
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    const f32x4 hidden = *reinterpret_cast<const f32x4*>(&lds.hidden[t % 3][16 * (KT * kq + kt) + 4 * g]);
 #pragma unroll
                     for (int ht = 0; ht < HT; ++ht)
 #pragma unroll
@@ -313,22 +337,29 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
 #pragma unroll
         for (int h = 0; h < PT; ++h) acc[d][h] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (tiles > 0) copy_tile(0);
+    if (tiles > 1) copy_tile(1);
+    i32x2 v[2][DT];  // this wave's codes of the last tile, transposed: its buffer is free for the next copies
 #pragma unroll 1
     for (int32_t t = 0; t <= tiles; ++t) {
-        wait_barrier<0>();
-        if (t + 1 < tiles) copy_tile(t + 1);
+        if (t + 1 < tiles) wait_barrier<COPIES>();
+        else wait_barrier<0>();
+        if (t + 2 < tiles) copy_tile(t + 2);
         Frag pf[2][PT];
         // lanes 2r, 2r + 1 of a group hand in 16 columns of key 8g + r; lane c gets column c of its eight keys
-        const uint8_t* v = lds.tile[(t + 2) % 3] + (8 * g + c / 2) * kRowBytes + wave * 128 + 8 * (c & 1);
+        const uint8_t* const next = lds.tile[t % 3] + (8 * g + c / 2) * kRowBytes + wave * 128 + 8 * (c & 1);
         auto product = [&](int ks) __attribute__((always_inline)) {
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                    (__attribute__((address_space(3))) i32x2*)(v + 32 * ks * kRowBytes + 16 * d));
-                const Frag a = bf16_of_codes((uint32_t)w[0], (uint32_t)w[1]);
+                const Frag a = bf16_of_codes((uint32_t)v[ks][d][0], (uint32_t)v[ks][d][1]);
 #pragma unroll
                 for (int h = 0; h < PT; ++h) acc[d][h] = mfma16(a, pf[ks][h], acc[d][h]);
             }
+        };
+        auto fetch = [&](int ks) __attribute__((always_inline)) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+                v[ks][d] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                    (__attribute__((address_space(3))) i32x2*)(next + 32 * ks * kRowBytes + 16 * d));
         };
         if (t > 0) {
             float keep[PT];
@@ -348,8 +379,10 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
                     for (int d = 0; d < DT; ++d) acc[d][h] *= keep[h];
             product(0);
         }
+        if (t < tiles) fetch(0);
         lds_barrier();
         if (t > 0) product(1);
+        if (t < tiles) fetch(1);
     }
     __syncthreads();
     const bool whole = it.parts == 1;
