@@ -95,8 +95,9 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 // them.  Two rules, both functions of the call's shapes and lengths alone:
 //   chunk > 0  every row in the same number of parts (rows of one capacity);
 //   chunk == 0 rows of different lengths (`lens` on the device, at most
-//              kPlanRows of them): parts of about sum(tiles) / target tiles,
-//              found by every work-group from the lengths.
+//              kPlanRows of them): parts of at most about sum(tiles) / target
+//              tiles, at most target + rows of them, found by every work-group
+//              from the lengths.
 constexpr int kTileKeys = 64;
 constexpr int kPlanRows = 256;
 
@@ -211,6 +212,19 @@ inline int64_t items_at_most(const Plan& p) {
     return (int64_t)p.rows + p.target;
 }
 
+// Tiles of a part of rows of `tiles` tiles: the number of parts whose work-groups
+// end first, `slots` of them running at a time, where a part costs `start` tiles'
+// time beside its own and each part of several another `leave` (its sums, written
+// and joined).
+inline int32_t chunk_for(int64_t rows, int64_t tiles, int64_t slots, int64_t start, int64_t leave) {
+    int64_t best = tiles, least = cdiv(rows, slots) * (tiles + start);
+    for (int64_t parts = 2; parts <= tiles && rows * (parts - 1) < slots; ++parts) {
+        const int64_t chunk = cdiv(tiles, parts), cost = cdiv(rows * cdiv(tiles, chunk), slots) * (chunk + start + leave);
+        if (cost < least) least = cost, best = chunk;
+    }
+    return (int32_t)std::max<int64_t>(1, best);
+}
+
 // Workspace: sums [items][heads][dims], then maxima and totals [items][heads].
 struct Parts {
     float* sums;
@@ -237,42 +251,51 @@ struct JoinParams {
     int32_t batch;
 };
 
-// One wave per (row, head): lane l adds dims 2l, 2l + 1 (+ 128 i) of the parts,
-// scaled to the largest of their maxima.  Rows of one part have been written.
+// One work-group per (row, head): D / 4 threads add four dims of every (1024 / D)-th
+// part, scaled to the largest of the parts' maxima, and the groups meet in LDS (one
+// thread per two dims over all parts took 30 us for 37 parts of 7 rows x 64 heads x
+// 512: a chain of memory latencies).  Rows of one part have been written.
 template <int D>
 __global__ __launch_bounds__(256) void join_kernel(JoinParams p) {
-    const int32_t row = (int32_t)blockIdx.x, lane = (int32_t)threadIdx.x % kWave;
-    const int32_t h = (int32_t)blockIdx.y * 4 + (int32_t)threadIdx.x / kWave;
+    constexpr int T = D / 4, G = 256 / T;
+    __shared__ f32x4 sums[G][T];
+    __shared__ float totals[G];
+    const int32_t row = (int32_t)blockIdx.x, h = (int32_t)blockIdx.y, lane = (int32_t)threadIdx.x % kWave;
+    const int32_t group = (int32_t)threadIdx.x / T, at4 = (int32_t)threadIdx.x % T;
     if (p.cu && (row < p.cu[0] || row >= p.cu[p.batch])) return;
     int32_t first, parts;
     items_of(p.plan, row, first, parts);
-    if (parts <= 1 || h >= p.heads) return;
+    if (parts <= 1) return;
     float top = -__builtin_inff(), total = 0.f;
     for (int32_t i = lane; i < parts; i += kWave) top = fmaxf(top, p.parts.stats[(int64_t)(first + i) * p.heads + h][0]);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
     const float sub = top == -__builtin_inff() ? 0.f : top;
-    f32x2 o[D / 128];
-#pragma unroll
-    for (int k = 0; k < D / 128; ++k) o[k] = f32x2{0.f, 0.f};
-    for (int32_t i = 0; i < parts; ++i) {
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int32_t i = group; i < parts; i += G) {
         const int64_t at = (int64_t)(first + i) * p.heads + h;
         const f32x2 st = p.parts.stats[at];
+        const f32x4 x = *reinterpret_cast<const f32x4*>(p.parts.sums + at * D + 4 * at4);
         const float f = __builtin_amdgcn_exp2f(st[0] - sub);
         total = fmaf(f, st[1], total);
 #pragma unroll
-        for (int k = 0; k < D / 128; ++k) {
-            const f32x2 x = *reinterpret_cast<const f32x2*>(p.parts.sums + at * D + 128 * k + 2 * lane);
-            o[k][0] = fmaf(f, x[0], o[k][0]);
-            o[k][1] = fmaf(f, x[1], o[k][1]);
-        }
+        for (int k = 0; k < 4; ++k) o[k] = fmaf(f, x[k], o[k]);
+    }
+    sums[group][at4] = o;
+    if (at4 == 0) totals[group] = total;
+    __syncthreads();
+    if (group != 0) return;
+#pragma unroll
+    for (int k = 1; k < G; ++k) {
+        o += sums[k][at4];
+        total += totals[k];
     }
     const bool none = total == 0.f;  // no key attended
     const float inv = none ? 0.f : 1.0f / total;
-    uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + row * p.o_row + h * p.o_head);
-#pragma unroll
-    for (int k = 0; k < D / 128; ++k) dst[64 * k + lane] = none ? 0u : pack_bf16(o[k][0] * inv, o[k][1] * inv);
-    if (p.lse && lane == 0)
+    *reinterpret_cast<u32x2*>(p.out + row * p.o_row + h * p.o_head + 4 * at4) =
+        none ? u32x2{0, 0} : u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
+    if (p.lse && at4 == 0)
         p.lse[(int64_t)row * p.heads + h] = none ? -__builtin_inff() : (top + __builtin_amdgcn_logf(total)) * kLn2;
 }
 

@@ -380,6 +380,6 @@ extern "C" int v1_latent_expanded(const void* q, int64_t q_row, int64_t q_head, 
     if (rc != V1_OK || s.parts == 1) return rc;
     // (as rows of s.parts one-tile parts)
     JoinParams j{Plan{nullptr, tokens, s.parts * kTileKeys, 1, 0}, p.partial, p.out, o_row, o_head, lse, heads, cu_q, batch};
-    hipLaunchKernelGGL(join_kernel<kValue>, dim3((uint32_t)tokens, (uint32_t)cdiv(heads, 4)), dim3(256), 0, st, j);
+    hipLaunchKernelGGL(join_kernel<kValue>, dim3((uint32_t)tokens, (uint32_t)heads), dim3(256), 0, st, j);
     return V1_LAUNCHED("latent_expanded: join");
 }

@@ -372,15 +372,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_attend_kernel(Kv8Params p)
     }
 }
 
+// (Two work-groups a CU, a tile of each wave at a time.)
 inline Plan kv8_plan(const int32_t* lens, int32_t rows, int32_t kv_heads, int32_t keys, bool ragged) {
-    const int64_t tiles = cdiv(keys, kTileKeys), groups = std::max<int64_t>(1, 2 * device_cus() / kv_heads);
-    Plan p{lens, rows, keys, (int32_t)std::max<int64_t>(1, tiles), (int32_t)groups};
-    if (rows >= groups) return p;
-    if (ragged && rows <= kPlanRows) {
-        p.chunk = 0;
-        return p;
-    }
-    p.chunk = (int32_t)std::max<int64_t>(kWaves, cdiv(tiles * rows, groups));
+    const int64_t steps = cdiv(cdiv(keys, kTileKeys), kWaves), slots = std::max<int64_t>(1, 2 * device_cus() / kv_heads);
+    Plan p{lens, rows, keys, 0, 0};
+    if (ragged && rows <= kPlanRows && rows < slots) p.target = (int32_t)std::max(slots - rows, (slots + 1) / 2);
+    else p.chunk = kWaves * chunk_for(rows, steps, slots, 2, 1);
     return p;
 }
 
@@ -436,9 +433,9 @@ extern "C" int v1_kv8_attend(const void* q, int64_t q_row, int64_t q_head, const
                    (int64_t)kv_heads * group < 1ll << 31, "kv8_attend: bad shape");
     V1_REQUIRE(group <= kMaxGroup, "kv8_attend: at most %d query heads per KV head", kMaxGroup);
     V1_REQUIRE(scale > 0.f && scale < __builtin_inff(), "kv8_attend: scale must be positive and finite");
-    V1_REQUIRE(aligned16(q) && (q_row | q_head) % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0 &&
-                   (o_row | o_head) % 2 == 0,
-               "kv8_attend: q must be 16-byte aligned with strides in multiples of 8, out 4-byte and 2");
+    V1_REQUIRE(aligned16(q) && (q_row | q_head) % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0 &&
+                   (o_row | o_head) % 4 == 0,
+               "kv8_attend: q must be 16-byte aligned with strides in multiples of 8, out 8-byte and 4");
     V1_REQUIRE(aligned16(k_pool) && aligned16(v_pool) &&
                    (kp_page | kp_token | kp_head | vp_page | vp_token | vp_head) % 16 == 0,
                "kv8_attend: pools must be 16-byte aligned with strides in multiples of 16");
@@ -465,6 +462,6 @@ extern "C" int v1_kv8_attend(const void* q, int64_t q_row, int64_t q_head, const
     rc = V1_LAUNCHED("kv8_attend");
     if (rc != V1_OK || need == 0) return rc;
     JoinParams j{plan, p.parts, p.out, o_row, o_head, lse, heads, nullptr, 0};
-    hipLaunchKernelGGL(join_kernel<kDim>, dim3((uint32_t)rows, (uint32_t)cdiv(heads, 4)), dim3(256), 0, st, j);
+    hipLaunchKernelGGL(join_kernel<kDim>, dim3((uint32_t)rows, (uint32_t)heads), dim3(256), 0, st, j);
     return V1_LAUNCHED("kv8_attend: join");
 }

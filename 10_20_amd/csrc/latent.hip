@@ -419,16 +419,14 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
 // Heads of a work-group: 16, 32 or 64 (more: several work-groups a row).
 inline int32_t absorbed_heads(int32_t heads) { return heads <= 16 ? 16 : heads <= 32 ? 32 : 64; }
 
+// (One work-group a CU.  A part's start is two to four dependent loads, its sums
+// are three tiles' bytes at 64 heads and less than one at 16.)
 inline Plan absorbed_plan(const int32_t* lens, int32_t rows, int32_t heads, int32_t keys, bool ragged) {
-    const int64_t splits = cdiv(heads, absorbed_heads(heads)), tiles = cdiv(keys, kTileKeys);
-    const int64_t groups = std::max<int64_t>(1, device_cus() / splits);  // items that fill the GPU once
-    Plan p{lens, rows, keys, (int32_t)std::max<int64_t>(1, tiles), (int32_t)groups};
-    if (rows >= groups) return p;
-    if (ragged && rows <= kPlanRows) {
-        p.chunk = 0;
-        return p;
-    }
-    p.chunk = (int32_t)std::max<int64_t>(1, cdiv(tiles * rows, groups));
+    const int32_t hb = absorbed_heads(heads);
+    const int64_t splits = cdiv(heads, hb), tiles = cdiv(keys, kTileKeys), slots = std::max<int64_t>(1, device_cus() / splits);
+    Plan p{lens, rows, keys, 0, 0};
+    if (ragged && rows <= kPlanRows && rows < slots) p.target = (int32_t)std::max(slots - rows, (slots + 1) / 2);
+    else p.chunk = chunk_for(rows, tiles, slots, 3, hb / 16);
     return p;
 }
 
@@ -503,6 +501,6 @@ extern "C" int v1_latent_attend(const void* q, int64_t q_row, int64_t q_head, co
                               : launch_absorbed<2, 2>(p, blocks, st);
     if (rc != V1_OK || need == 0) return rc;
     JoinParams j{plan, p.parts, p.out, o_row, o_head, lse, heads, nullptr, 0};
-    hipLaunchKernelGGL(join_kernel<kLatent>, dim3((uint32_t)rows, (uint32_t)cdiv(heads, 4)), dim3(256), 0, st, j);
+    hipLaunchKernelGGL(join_kernel<kLatent>, dim3((uint32_t)rows, (uint32_t)heads), dim3(256), 0, st, j);
     return V1_LAUNCHED("latent_attend: join");
 }

@@ -142,10 +142,10 @@ def test_strides_outputs_and_far_pages():
     ids = torch.randint(0, 40 * 64, (5, 1000), device=DEV, generator=g, dtype=torch.int32)[:, 7:]
     k = kp[table.long()[ids[0].long() // 64], ids[0].long() % 64, 0].double() * scales[table.long()[ids[0].long() // 64], :1].double()
     ids[0] = ids[0][torch.argsort(k @ q[0, 0].double())].clone()
-    space = torch.full((5, 4, 132), 7.0, device=DEV, dtype=torch.bfloat16)
-    out, lse = K8.attend(q, *pools, table, ids=ids, out=space[..., 2:130], return_lse=True)
+    space = torch.full((5, 4, 136), 7.0, device=DEV, dtype=torch.bfloat16)
+    out, lse = K8.attend(q, *pools, table, ids=ids, out=space[..., 4:132], return_lse=True)
     check(out, lse, q, pools, [keys_of(table, ids[r], 2000, pages) for r in range(5)])
-    assert bool((space[..., :2] == 7).all()) and bool((space[..., 130:] == 7).all())
+    assert bool((space[..., :4] == 7).all()) and bool((space[..., 132:] == 7).all())
 
 
 def plain_store(k, v, pools, table, starts, cu):
@@ -282,8 +282,8 @@ def test_library_refusals():
     base = dict(q=256, qr=1024, qh=128, kp=256, kpp=8192, kpt=128, kph=128, vp=256, vpp=8192, vpt=128, vph=128, ks=256, ksp=1, vs=256,
                 vsp=1, pages=4, table=256, ts=9, tl=9, ids=0, ids_s=0, lens=0, rows=4096, kv_heads=1, group=4, keys=100, scale=0.1, out=256,
                 o_row=512, o_head=128, lse=0, ws=0, wsb=0, stream=0)
-    for bad in (dict(q=8), dict(qh=100), dict(kp=8), dict(vpt=120), dict(kph=8), dict(out=2), dict(o_row=511), dict(group=17), dict(group=0),
-                dict(kv_heads=0), dict(rows=-1), dict(scale=0.0), dict(rows=1, keys=4096)):
+    for bad in (dict(q=8), dict(qh=100), dict(kp=8), dict(vpt=120), dict(kph=8), dict(out=4), dict(o_row=510), dict(group=17), dict(group=0),
+                dict(kv_heads=0), dict(rows=-1), dict(scale=0.0), dict(rows=1, keys=8192)):
         assert h.v1_kv8_attend(*{**base, **bad}.values()) == L.V1_ERR_INVALID, bad
         assert b"kv8_attend" in h.v1_last_error()
     assert h.v1_kv8_attend(*{**base, "rows": 0}.values()) == 0
