@@ -5,6 +5,7 @@ no fallback: if the library is missing every operator raises, so a run can
 never silently compute on another path.
 """
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -157,22 +158,25 @@ _SIGNATURES = {
     "v1_union_map_topk": (_c_i32, [_vp, _c_i32, _vp, _vp, _c_i64, _c_i32, _vp, _vp, _vp, _vp, _vp, _c_i64, _vp,
                                    _c_i32, _vp, _vp,
                                    _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _vp]),
-    "v1_latent_store": (_c_i32, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i32, _vp, _c_i64, _c_i64, _vp]),
-    "v1_latent_attend": (_c_i32, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i32, _vp, _c_i64,
-                                  _vp, _c_i32, _c_i32, _c_i32, ctypes.c_float, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64,
-                                  _vp]),
+    "v1_latent_store": (_c_i32, [ctypes.c_char_p, _vp]),
+    "v1_latent_attend": (_c_i32, [ctypes.c_char_p, _vp]),
     "v1_latent_attend_workspace": (_c_i64, [_c_i32, _c_i32, _c_i32, _c_i32]),
-    "v1_latent_expanded": (_c_i32, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp, _c_i32, _c_i32,
-                                    _c_i32, _c_i32, _c_i32, _c_i32, ctypes.c_float, _vp, _c_i64, _c_i64, _vp, _vp,
-                                    _c_i64, _vp]),
-    "v1_kv8_store": (_c_i32, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64,
-                              _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i32, _vp, _vp, _c_i32, _c_i32,
-                              _c_i32, _vp]),
-    "v1_kv8_attend": (_c_i32, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64,
-                               _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i32, _vp, _c_i64, _vp, _c_i32, _c_i32, _c_i32, _c_i32,
-                               ctypes.c_float, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64, _vp]),
+    "v1_latent_expanded": (_c_i32, [ctypes.c_char_p, _vp]),
+    "v1_kv8_store": (_c_i32, [ctypes.c_char_p, _vp]),
+    "v1_kv8_attend": (_c_i32, [ctypes.c_char_p, _vp]),
     "v1_kv8_attend_workspace": (_c_i64, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32]),
     "v1_latent_expanded_workspace": (_c_i64, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32]),
+}
+
+# Arguments of the entry points that take them in a structure, packed by
+# struct.Struct in the header's field order (a ctypes structure or a call of
+# 20 and more arguments costs 2-4 us, this 0.5).
+PACKED = {
+    "v1_latent_store": struct.Struct("8qi4x"),
+    "v1_latent_attend": struct.Struct("18q4if4x"),
+    "v1_latent_expanded": struct.Struct("16q6if4x"),
+    "v1_kv8_store": struct.Struct("23q4i"),
+    "v1_kv8_attend": struct.Struct("27q5if"),
 }
 
 _lock = threading.Lock()
@@ -213,6 +217,20 @@ def check(rc, what):
 
 def call(name, *args):
     check(getattr(lib(), name)(*args), name)
+
+
+def call_packed(name, t, *fields):
+    """An entry point of PACKED, with its structure's fields in order, on the
+    current stream of t's device (which need not be the current one)."""
+    index = t.get_device()
+    entry, args = getattr(_lib or lib(), name), PACKED[name].pack(*fields)
+    if index == torch._C._cuda_getDevice():
+        rc = entry(args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = entry(args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != V1_OK:
+        check(rc, name)
 
 
 def ptr(t):

@@ -38,7 +38,7 @@ struct ExpandedParams {
     const int32_t* cu_q;
     const int32_t* cu_k;
     int32_t tokens, keys, batch, heads, blocks;  // blocks: of queries, of the longest sequence
-    int32_t causal, parts, spread;
+    int32_t causal, parts, by_pair;
     float scale2;
     uint16_t* out;
     int64_t o_row, o_head;
@@ -128,13 +128,19 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedT
     const int32_t wave = __builtin_amdgcn_readfirstlane((int32_t)threadIdx.x / kWave);
     const int32_t lane = (int32_t)threadIdx.x % kWave, c = lane & 31, h = lane >> 5;
 
-    // work-groups reach the XCDs in turn: each XCD takes whole heads, their
-    // blocks side by side (they read the same keys), the longest first
-    int32_t index = ((int32_t)blockIdx.x % 8) * p.spread + (int32_t)blockIdx.x / 8;
-    const int32_t part = index % p.parts;
-    index /= p.parts;
-    const int32_t block = p.blocks - 1 - index % p.blocks;
-    index /= p.blocks;
+    // Work-groups reach the XCDs in turn.  Each takes whole (sequence, head) pairs
+    // where they divide evenly, so that blocks of the same keys meet in one L2;
+    // longest blocks first.
+    const int32_t per = p.blocks * p.parts;
+    int32_t index = (int32_t)blockIdx.x, at = index % per;
+    if (p.by_pair) {
+        const int32_t turn = index / 8;
+        at = turn % per;
+        index = turn / per * 8 + index % 8;
+    } else {
+        index /= per;
+    }
+    const int32_t part = at % p.parts, block = p.blocks - 1 - at / p.parts;
     const int32_t head = index % p.heads, b = index / p.heads;
     if (b >= p.batch) return false;
     const int32_t q_lo = min(max(p.cu_q[b], 0), p.tokens), q_hi = min(max(p.cu_q[b + 1], q_lo), p.tokens);
@@ -353,12 +359,12 @@ extern "C" int64_t v1_latent_expanded_workspace(int32_t tokens, int32_t keys, in
     return s.parts == 1 ? 0 : attn::parts_bytes((int64_t)tokens * s.parts, heads, kValue);
 }
 
-extern "C" int v1_latent_expanded(const void* q, int64_t q_row, int64_t q_head, const void* kv, int64_t kv_row,
-                                  int64_t kv_head, const void* rope, int64_t rope_row, const int32_t* cu_q,
-                                  const int32_t* cu_k, int32_t tokens, int32_t keys, int32_t batch, int32_t heads,
-                                  int32_t max_q, int32_t causal, float scale, void* out, int64_t o_row, int64_t o_head,
-                                  float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+extern "C" int v1_latent_expanded(const v1_latent_expanded_args* a, void* stream) {
+    V1_REQUIRE(a != nullptr, "latent_expanded: null arguments");
+    auto [q, q_row, q_head, kv, kv_row, kv_head, rope, rope_row, cu_q, cu_k, out, o_row, o_head, lse, workspace,
+          workspace_bytes, tokens, keys, batch, heads, max_q, causal, scale] = *a;
     V1_REQUIRE(tokens >= 0 && keys >= 0 && batch >= 0 && heads > 0 && max_q >= 0, "latent_expanded: bad shape");
+    V1_REQUIRE(heads < 1 << 16, "latent_expanded: too many heads");
     V1_REQUIRE(scale > 0.f && scale < __builtin_inff(), "latent_expanded: scale must be positive and finite");
     const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kv) | reinterpret_cast<uintptr_t>(rope);
     V1_REQUIRE(all % 16 == 0 && (q_row | q_head | kv_row | kv_head | rope_row) % 8 == 0 &&
@@ -369,14 +375,15 @@ extern "C" int v1_latent_expanded(const void* q, int64_t q_row, int64_t q_head, 
     const int64_t need = v1_latent_expanded_workspace(tokens, keys, batch, heads, max_q);
     V1_REQUIRE(workspace_bytes >= need && (need == 0 || workspace != nullptr),
                "latent_expanded: workspace of %lld bytes needed", (long long)need);
-    const int64_t items = (int64_t)batch * heads * s.blocks * s.parts, spread = cdiv(items, 8);
+    const int64_t pairs = (int64_t)batch * heads, by_pair = pairs % 8 == 0 || pairs >= 64;
+    const int64_t items = (by_pair ? 8 * cdiv(pairs, 8) : pairs) * s.blocks * s.parts;
     V1_REQUIRE(items < 1ll << 30, "latent_expanded: too many work items");
     ExpandedParams p{static_cast<const uint16_t*>(q), q_row, q_head, static_cast<const uint16_t*>(kv), kv_row, kv_head,
                      static_cast<const uint16_t*>(rope), rope_row, cu_q, cu_k, tokens, keys, batch, heads, s.blocks,
-                     causal, s.parts, (int32_t)spread, scale * kLog2e, static_cast<uint16_t*>(out), o_row, o_head, lse,
+                     causal, s.parts, (int32_t)by_pair, scale * kLog2e, static_cast<uint16_t*>(out), o_row, o_head, lse,
                      parts_at(workspace, (int64_t)tokens * s.parts, heads, kValue)};
     const hipStream_t st = as_stream(stream);
-    const int rc = s.waves == 8 ? launch_expanded<8, 3>(p, 8 * spread, st) : launch_expanded<4, 2>(p, 8 * spread, st);
+    const int rc = s.waves == 8 ? launch_expanded<8, 3>(p, items, st) : launch_expanded<4, 2>(p, items, st);
     if (rc != V1_OK || s.parts == 1) return rc;
     // (as rows of s.parts one-tile parts)
     JoinParams j{Plan{nullptr, tokens, s.parts * kTileKeys, 1, 0}, p.partial, p.out, o_row, o_head, lse, heads, cu_q, batch};

@@ -388,12 +388,11 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 using namespace v1;
 
-extern "C" int v1_kv8_store(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token,
-                            int64_t v_head, void* k_pool, int64_t kp_page, int64_t kp_token, int64_t kp_head,
-                            void* v_pool, int64_t vp_page, int64_t vp_token, int64_t vp_head, float* k_scale,
-                            int64_t ks_page, float* v_scale, int64_t vs_page, int64_t pages, const int32_t* table,
-                            int64_t table_stride, int32_t table_len, const int32_t* starts, const int32_t* cu_tokens,
-                            int32_t tokens, int32_t requests, int32_t kv_heads, void* stream) {
+extern "C" int v1_kv8_store(const v1_kv8_store_args* a, void* stream) {
+    V1_REQUIRE(a != nullptr, "kv8_store: null arguments");
+    auto [k, k_token, k_head, v, v_token, v_head, k_pool, kp_page, kp_token, kp_head, v_pool, vp_page, vp_token,
+          vp_head, k_scale, ks_page, v_scale, vs_page, pages, table, table_stride, starts, cu_tokens, table_len,
+          tokens, requests, kv_heads] = *a;
     V1_REQUIRE(tokens >= 0 && requests >= 0 && kv_heads > 0 && pages >= 0 && table_len >= 0, "kv8_store: bad shape");
     V1_REQUIRE(kv_heads <= 32767, "kv8_store: too many heads");
     V1_REQUIRE(aligned16(k) && aligned16(v) && (k_token | k_head | v_token | v_head) % 8 == 0,
@@ -421,16 +420,14 @@ extern "C" int64_t v1_kv8_attend_workspace(int32_t rows, int32_t kv_heads, int32
     return plan.chunk > 0 && items == rows ? 0 : attn::parts_bytes(items, kv_heads * group, kDim);
 }
 
-extern "C" int v1_kv8_attend(const void* q, int64_t q_row, int64_t q_head, const void* k_pool, int64_t kp_page,
-                             int64_t kp_token, int64_t kp_head, const void* v_pool, int64_t vp_page, int64_t vp_token,
-                             int64_t vp_head, const float* k_scale, int64_t ks_page, const float* v_scale,
-                             int64_t vs_page, int64_t pages, const int32_t* table, int64_t table_stride,
-                             int32_t table_len, const int32_t* ids, int64_t ids_stride, const int32_t* lens,
-                             int32_t rows, int32_t kv_heads, int32_t group, int32_t keys, float scale, void* out,
-                             int64_t o_row, int64_t o_head, float* lse, void* workspace, int64_t workspace_bytes,
-                             void* stream) {
+extern "C" int v1_kv8_attend(const v1_kv8_attend_args* a, void* stream) {
+    V1_REQUIRE(a != nullptr, "kv8_attend: null arguments");
+    auto [q, q_row, q_head, k_pool, kp_page, kp_token, kp_head, v_pool, vp_page, vp_token, vp_head, k_scale,
+          ks_page, v_scale, vs_page, pages, table, table_stride, ids, ids_stride, lens, out, o_row, o_head, lse,
+          workspace, workspace_bytes, table_len, rows, kv_heads, group, keys, scale] = *a;
     V1_REQUIRE(rows >= 0 && kv_heads > 0 && group > 0 && keys >= 0 && pages >= 0 && table_len >= 0 &&
-                   (int64_t)kv_heads * group < 1ll << 31, "kv8_attend: bad shape");
+                   (int64_t)kv_heads * group < 1ll << 16,
+               "kv8_attend: bad shape");
     V1_REQUIRE(group <= kMaxGroup, "kv8_attend: at most %d query heads per KV head", kMaxGroup);
     V1_REQUIRE(scale > 0.f && scale < __builtin_inff(), "kv8_attend: scale must be positive and finite");
     V1_REQUIRE(aligned16(q) && (q_row | q_head) % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0 &&

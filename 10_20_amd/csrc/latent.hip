@@ -448,9 +448,9 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 using namespace v1;
 
-extern "C" int v1_latent_store(const void* latent, int64_t latent_stride, const void* rope, int64_t rope_stride,
-                               const int32_t* slots, int32_t tokens, void* pool, int64_t pool_rows,
-                               int64_t pool_stride_bytes, void* stream) {
+extern "C" int v1_latent_store(const v1_latent_store_args* a, void* stream) {
+    V1_REQUIRE(a != nullptr, "latent_store: null arguments");
+    auto [latent, latent_stride, rope, rope_stride, slots, pool, pool_rows, pool_stride_bytes, tokens] = *a;
     V1_REQUIRE(tokens >= 0 && pool_rows >= 0 && pool_rows < 1ll << 31, "latent_store: bad shape");
     V1_REQUIRE(aligned16(latent) && aligned16(rope) && aligned16(pool) && latent_stride % 8 == 0 && rope_stride % 8 == 0,
                "latent_store: inputs and pool must be 16-byte aligned, strides multiples of 8");
@@ -470,12 +470,12 @@ extern "C" int64_t v1_latent_attend_workspace(int32_t rows, int32_t heads, int32
     return plan.chunk > 0 && items == rows ? 0 : attn::parts_bytes(items, heads, kLatent);
 }
 
-extern "C" int v1_latent_attend(const void* q, int64_t q_row, int64_t q_head, const void* pool, int64_t pool_rows,
-                                int64_t pool_stride_bytes, const int32_t* map, int64_t map_len, int64_t map_stride,
-                                int32_t map_shift, const int32_t* ids, int64_t ids_stride, const int32_t* lens,
-                                int32_t rows, int32_t heads, int32_t keys, float scale, void* out, int64_t o_row,
-                                int64_t o_head, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+extern "C" int v1_latent_attend(const v1_latent_attend_args* a, void* stream) {
+    V1_REQUIRE(a != nullptr, "latent_attend: null arguments");
+    auto [q, q_row, q_head, pool, pool_rows, pool_stride_bytes, map, map_len, map_stride, ids, ids_stride, lens,
+          out, o_row, o_head, lse, workspace, workspace_bytes, map_shift, rows, heads, keys, scale] = *a;
     V1_REQUIRE(rows >= 0 && heads > 0 && keys >= 0 && pool_rows >= 0 && pool_rows < 1ll << 31, "latent_attend: bad shape");
+    V1_REQUIRE(heads < 1 << 16, "latent_attend: too many heads");
     V1_REQUIRE(scale > 0.f && scale < __builtin_inff(), "latent_attend: scale must be positive and finite");
     V1_REQUIRE(map_shift >= 0 && map_shift < 31 && map_len >= 0, "latent_attend: bad page map");
     V1_REQUIRE(aligned16(q) && aligned16(pool) && reinterpret_cast<uintptr_t>(out) % 8 == 0 && q_row % 8 == 0 &&

@@ -12,6 +12,7 @@ values expanded per head from the latent.
 Every call launches on the current stream of its tensors' device, never
 synchronises, and raises ValueError for arguments that do not fit.
 """
+import functools
 import math
 
 import torch
@@ -22,9 +23,12 @@ LATENT, ROPE, ROW_BYTES = 512, 64, 656
 HEAD = 128  # key numbers of a head beside the rope's, and value numbers, in the expanded form
 
 
-def _int32(name, t, shape):
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {list(shape)}")
+_BF16, _I32 = torch.bfloat16, torch.int32
+
+
+def _int32(name, t, n):
+    if t.dtype != _I32 or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape [{n}]")
 
 
 def _pool(pool):
@@ -32,19 +36,29 @@ def _pool(pool):
         raise ValueError(f"pool must be a uint8 [rows, {ROW_BYTES}] tensor with unit inner stride")
 
 
-def _output(out, like, shape):
+def _output(out, q, shape):
     if out is None:
-        return torch.empty(shape, device=like.device, dtype=torch.bfloat16)
-    if out.dtype != torch.bfloat16 or tuple(out.shape) != shape or out.stride(-1) != 1:
+        return q.new_empty(shape)
+    if out.dtype != _BF16 or out.shape != shape or out.stride(2) != 1:
         raise ValueError(f"out must be bfloat16 {list(shape)} with a contiguous last dimension")
     return out
 
 
+_DEFAULT_SCALE = 1.0 / math.sqrt(HEAD + ROPE)
+
+
 def _scale(softmax_scale):
-    scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(HEAD + ROPE)
+    scale = _DEFAULT_SCALE if softmax_scale is None else float(softmax_scale)
     if not 0.0 < scale < math.inf:
         raise ValueError("softmax_scale must be positive and finite")
     return scale
+
+
+# (sizes alone decide: asked of the library once for each)
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(entry, index, *sizes):
+    with torch.cuda.device(index):
+        return getattr(_lib.lib(), entry)(*sizes)
 
 
 def store_rows(latent, rope, pool, slots):
@@ -60,12 +74,12 @@ def store_rows(latent, rope, pool, slots):
     _lib.require_gpu(latent, rope, pool, slots)
     tokens = latent.shape[0]
     for name, t, n in (("latent", latent, LATENT), ("rope", rope, ROPE)):
-        if t.dtype != torch.bfloat16 or t.dim() != 2 or tuple(t.shape) != (tokens, n) or t.stride(1) != 1:
+        if t.dtype != _BF16 or t.shape != (tokens, n) or t.stride(1) != 1:
             raise ValueError(f"{name} must be bfloat16 [tokens, {n}] with a contiguous last dimension")
     _pool(pool)
-    _int32("slots", slots, (tokens,))
-    _lib.call("v1_latent_store", _lib.ptr(latent), latent.stride(0), _lib.ptr(rope), rope.stride(0), _lib.ptr(slots),
-              tokens, _lib.ptr(pool), pool.shape[0], pool.stride(0), _lib.stream_of(pool))
+    _int32("slots", slots, tokens)
+    _lib.call_packed("v1_latent_store", pool, latent.data_ptr(), latent.stride(0), rope.data_ptr(),
+                     rope.stride(0), slots.data_ptr(), pool.data_ptr(), pool.shape[0], pool.stride(0), tokens)
     return pool
 
 
@@ -87,24 +101,25 @@ def attend(q, pool, ids=None, table=None, page_bits=0, lens=None, softmax_scale=
     1 / sqrt(192), that of the expanded form.  Returns out [rows, heads, 512] bf16,
     and with return_lse the natural log of the sum of exponentials, [rows, heads] fp32."""
     _lib.require_gpu(q, pool, ids, table, lens, out)
-    if q.dim() != 3 or q.shape[2] != LATENT + ROPE or q.dtype != torch.bfloat16 or q.stride(2) != 1 or not q.shape[1]:
+    if q.dim() != 3 or q.shape[2] != LATENT + ROPE or q.dtype != _BF16 or q.stride(2) != 1 or not q.shape[1]:
         raise ValueError(f"q must be bfloat16 [rows, heads, {LATENT + ROPE}] with a contiguous last dimension")
     _pool(pool)
     rows, heads, _ = q.shape
     page_bits = int(page_bits)
     if not 0 <= page_bits < 31:
         raise ValueError("page_bits must be in [0, 31)")
-    map_len, map_stride = 0, 0
+    map_ptr = map_len = map_stride = ids_ptr = ids_stride = lens_ptr = 0
     if table is not None:
-        if table.dtype != torch.int32 or table.dim() not in (1, 2) or (table.dim() == 2 and table.shape[0] != rows):
+        dims = table.dim()
+        if table.dtype != _I32 or not (dims == 1 or (dims == 2 and table.shape[0] == rows)):
             raise ValueError("table must be int32 [entries] or [rows, entries]")
-        map_len, map_stride = table.shape[-1], table.stride(0) if table.dim() == 2 else 0
+        map_ptr, map_len, map_stride = table.data_ptr(), table.shape[-1], table.stride(0) if dims == 2 else 0
         if map_len and table.stride(-1) != 1:
             raise ValueError("table must have unit inner stride")
     if ids is not None:
-        if ids.dtype != torch.int32 or ids.dim() != 2 or ids.shape[0] != rows or (ids.shape[1] and ids.stride(1) != 1):
+        if ids.dtype != _I32 or ids.dim() != 2 or ids.shape[0] != rows or (ids.shape[1] and ids.stride(1) != 1):
             raise ValueError("ids must be int32 [rows, keys] with unit inner stride")
-        keys = ids.shape[1]
+        keys, ids_ptr, ids_stride = ids.shape[1], ids.data_ptr(), ids.stride(0)
     else:
         keys = map_len << page_bits if table is not None else pool.shape[0]
         if keys >= 1 << 31:
@@ -112,17 +127,19 @@ def attend(q, pool, ids=None, table=None, page_bits=0, lens=None, softmax_scale=
     if table is not None and map_len == 0:
         keys = 0
     if lens is not None:
-        _int32("lens", lens, (rows,))
-    out = _output(out, q, (rows, heads, LATENT))
-    lse = torch.empty((rows, heads), device=q.device, dtype=torch.float32) if return_lse else None
+        _int32("lens", lens, rows)
+        lens_ptr = lens.data_ptr()
     scale = _scale(softmax_scale)
+    out = _output(out, q, (rows, heads, LATENT))
+    lse = q.new_empty((rows, heads), dtype=torch.float32) if return_lse else None
     # (the sums of a row's parts are the call's own, as in attention.attend_slots)
-    ws_bytes = _lib.lib().v1_latent_attend_workspace(rows, heads, keys, lens is not None)
-    ws = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8) if ws_bytes else None
-    _lib.call("v1_latent_attend", _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(pool), pool.shape[0], pool.stride(0),
-              _lib.ptr(table), map_len, map_stride, page_bits, _lib.ptr(ids), ids.stride(0) if ids is not None else 0,
-              _lib.ptr(lens), rows, heads, keys, scale, _lib.ptr(out), out.stride(0), out.stride(1), _lib.ptr(lse),
-              _lib.ptr(ws), ws_bytes, _lib.stream_of(q))
+    ws_bytes = _workspace_bytes("v1_latent_attend_workspace", q.get_device(), rows, heads, keys, lens is not None)
+    ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
+    o_row, o_head, _ = out.stride()
+    q_row, q_head, _ = q.stride()
+    _lib.call_packed("v1_latent_attend", q, q.data_ptr(), q_row, q_head, pool.data_ptr(), pool.shape[0],
+                     pool.stride(0), map_ptr, map_len, map_stride, ids_ptr, ids_stride, lens_ptr, out.data_ptr(), o_row,
+                     o_head, _lib.ptr(lse), _lib.ptr(ws), ws_bytes, page_bits, rows, heads, keys, scale)
     return (out, lse) if return_lse else out
 
 
@@ -149,30 +166,31 @@ def attend_expanded(q, kv, k_rope, cu_q, cu_k=None, max_q=None, softmax_scale=No
     of exponentials, [tokens, heads] fp32."""
     cu_k = cu_q if cu_k is None else cu_k
     _lib.require_gpu(q, kv, k_rope, cu_q, cu_k, out)
-    if q.dim() != 3 or q.shape[2] != HEAD + ROPE or q.dtype != torch.bfloat16 or q.stride(2) != 1 or not q.shape[1]:
+    if q.dim() != 3 or q.shape[2] != HEAD + ROPE or q.dtype != _BF16 or q.stride(2) != 1 or not q.shape[1]:
         raise ValueError(f"q must be bfloat16 [tokens, heads, {HEAD + ROPE}] with a contiguous last dimension")
     tokens, heads, _ = q.shape
-    if kv.dtype != torch.bfloat16 or kv.dim() != 3 or tuple(kv.shape[1:]) != (heads, 2 * HEAD) or kv.stride(2) != 1:
-        raise ValueError(f"kv must be bfloat16 [keys, heads, {2 * HEAD}] with a contiguous last dimension")
     keys = kv.shape[0]
-    if k_rope.dtype != torch.bfloat16 or tuple(k_rope.shape) != (keys, ROPE) or k_rope.stride(1) != 1:
+    if kv.dtype != _BF16 or kv.shape != (keys, heads, 2 * HEAD) or kv.stride(2) != 1:
+        raise ValueError(f"kv must be bfloat16 [keys, heads, {2 * HEAD}] with a contiguous last dimension")
+    if k_rope.dtype != _BF16 or k_rope.shape != (keys, ROPE) or k_rope.stride(1) != 1:
         raise ValueError(f"k_rope must be bfloat16 [keys, {ROPE}] with a contiguous last dimension")
-    if cu_q.dim() != 1 or cu_q.numel() < 1:
+    batch = cu_q.numel() - 1
+    if cu_q.dim() != 1 or batch < 0:
         raise ValueError("cu_q must be a contiguous int32 [batch + 1] tensor")
-    _int32("cu_q", cu_q, (cu_q.numel(),))
-    _int32("cu_k", cu_k, (cu_q.numel(),))
-    max_q = tokens if max_q is None else int(max_q)
+    _int32("cu_q", cu_q, batch + 1)
+    _int32("cu_k", cu_k, batch + 1)
+    max_q = tokens if max_q is None else min(int(max_q), tokens)
     if max_q < 0:
         raise ValueError("max_q must not be negative")
-    max_q = min(max_q, tokens)
     scale = _scale(softmax_scale)
     out = _output(out, q, (tokens, heads, HEAD))
-    lse = torch.empty((tokens, heads), device=q.device, dtype=torch.float32) if return_lse else None
-    batch = cu_q.numel() - 1
-    ws_bytes = _lib.lib().v1_latent_expanded_workspace(tokens, keys, batch, heads, max_q)
-    ws = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8) if ws_bytes else None
-    _lib.call("v1_latent_expanded", _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(kv), kv.stride(0), kv.stride(1),
-              _lib.ptr(k_rope), k_rope.stride(0), _lib.ptr(cu_q), _lib.ptr(cu_k), tokens, keys, batch, heads, max_q,
-              int(bool(causal)), scale, _lib.ptr(out), out.stride(0), out.stride(1), _lib.ptr(lse), _lib.ptr(ws),
-              ws_bytes, _lib.stream_of(q))
+    lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
+    ws_bytes = _workspace_bytes("v1_latent_expanded_workspace", q.get_device(), tokens, keys, batch, heads, max_q)
+    ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
+    o_row, o_head, _ = out.stride()
+    q_row, q_head, _ = q.stride()
+    _lib.call_packed("v1_latent_expanded", q, q.data_ptr(), q_row, q_head, kv.data_ptr(), kv.stride(0),
+                     kv.stride(1), k_rope.data_ptr(), k_rope.stride(0), cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(),
+                     o_row, o_head, _lib.ptr(lse), _lib.ptr(ws), ws_bytes, tokens, keys, batch, heads, max_q,
+                     1 if causal else 0, scale)
     return (out, lse) if return_lse else out

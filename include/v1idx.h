@@ -590,9 +590,17 @@ int64_t v1_decode_attention_slots_workspace(int32_t rows, int32_t heads_q, int32
  * infinities become +-448 s.  Slots outside [0, pool_rows) are skipped; slots of
  * one call are distinct.
  * ---------------------------------------------------------------------- */
-int v1_latent_store(const void* latent, int64_t latent_stride, const void* rope, int64_t rope_stride,
-                    const int32_t* slots, int32_t tokens, void* pool, int64_t pool_rows,
-                    int64_t pool_stride_bytes, void* stream);
+typedef struct {
+    const void* latent;
+    int64_t latent_stride;
+    const void* rope;
+    int64_t rope_stride;
+    const int32_t* slots;
+    void* pool;
+    int64_t pool_rows, pool_stride_bytes;
+    int32_t tokens;
+} v1_latent_store_args;
+int v1_latent_store(const v1_latent_store_args* a, void* stream);
 /* Attention over latent rows: q [rows, heads, 576] bf16, out[r, h] (bf16, 512)
  * = softmax over the row's keys of scale * q . (c_j, rope_j), times c_j (the
  * dequantised codes).  Key j of row r is id = ids[r * ids_stride + j] (j when ids
@@ -603,11 +611,25 @@ int v1_latent_store(const void* latent, int64_t latent_stride, const void* rope,
  * the sum of exponentials, -inf without keys.  workspace:
  * v1_latent_attend_workspace(rows, heads, keys, lens != NULL) bytes, 256-byte
  * aligned, the call's own until the stream has passed it. */
-int v1_latent_attend(const void* q, int64_t q_row, int64_t q_head, const void* pool, int64_t pool_rows,
-                     int64_t pool_stride_bytes, const int32_t* map, int64_t map_len, int64_t map_stride,
-                     int32_t map_shift, const int32_t* ids, int64_t ids_stride, const int32_t* lens,
-                     int32_t rows, int32_t heads, int32_t keys, float scale, void* out, int64_t o_row,
-                     int64_t o_head, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+typedef struct {
+    const void* q;
+    int64_t q_row, q_head;
+    const void* pool;
+    int64_t pool_rows, pool_stride_bytes;
+    const int32_t* map;
+    int64_t map_len, map_stride;
+    const int32_t* ids;
+    int64_t ids_stride;
+    const int32_t* lens;
+    void* out;
+    int64_t o_row, o_head;
+    float* lse;
+    void* workspace;
+    int64_t workspace_bytes;
+    int32_t map_shift, rows, heads, keys;
+    float scale;
+} v1_latent_attend_args;
+int v1_latent_attend(const v1_latent_attend_args* a, void* stream);
 int64_t v1_latent_attend_workspace(int32_t rows, int32_t heads, int32_t keys, int32_t ragged);
 /* Attention of ragged sequences over keys and values expanded per head: q
  * [tokens, heads, 192], kv [keys, heads, 128 key | 128 value], rope [keys, 64]
@@ -618,11 +640,24 @@ int64_t v1_latent_attend_workspace(int32_t rows, int32_t heads, int32_t keys, in
  * and an lse of -inf.  max_q: at least the longest sequence's queries.  lse (may
  * be NULL): [tokens, heads].  Rows outside the sequences are not written.
  * workspace: v1_latent_expanded_workspace bytes, as above.  scale > 0. */
-int v1_latent_expanded(const void* q, int64_t q_row, int64_t q_head, const void* kv, int64_t kv_row,
-                       int64_t kv_head, const void* rope, int64_t rope_row, const int32_t* cu_q,
-                       const int32_t* cu_k, int32_t tokens, int32_t keys, int32_t batch, int32_t heads,
-                       int32_t max_q, int32_t causal, float scale, void* out, int64_t o_row, int64_t o_head,
-                       float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+typedef struct {
+    const void* q;
+    int64_t q_row, q_head;
+    const void* kv;
+    int64_t kv_row, kv_head;
+    const void* rope;
+    int64_t rope_row;
+    const int32_t* cu_q;
+    const int32_t* cu_k;
+    void* out;
+    int64_t o_row, o_head;
+    float* lse;
+    void* workspace;
+    int64_t workspace_bytes;
+    int32_t tokens, keys, batch, heads, max_q, causal;
+    float scale;
+} v1_latent_expanded_args;
+int v1_latent_expanded(const v1_latent_expanded_args* a, void* stream);
 int64_t v1_latent_expanded_workspace(int32_t tokens, int32_t keys, int32_t batch, int32_t heads, int32_t max_q);
 /* ------------------------------------------------------------------------
  * K / V pages of 64 tokens in OCP e4m3fn codes, [pages, 64, kv_heads, 128] with
@@ -639,12 +674,27 @@ int64_t v1_latent_expanded_workspace(int32_t tokens, int32_t keys, int32_t batch
  * Positions past the table, pages outside the pool and negative starts are
  * skipped; a page is appended to by one request of a call.
  * ---------------------------------------------------------------------- */
-int v1_kv8_store(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
-                 void* k_pool, int64_t kp_page, int64_t kp_token, int64_t kp_head, void* v_pool,
-                 int64_t vp_page, int64_t vp_token, int64_t vp_head, float* k_scale, int64_t ks_page,
-                 float* v_scale, int64_t vs_page, int64_t pages, const int32_t* table, int64_t table_stride,
-                 int32_t table_len, const int32_t* starts, const int32_t* cu_tokens, int32_t tokens,
-                 int32_t requests, int32_t kv_heads, void* stream);
+typedef struct {
+    const void* k;
+    int64_t k_token, k_head;
+    const void* v;
+    int64_t v_token, v_head;
+    void* k_pool;
+    int64_t kp_page, kp_token, kp_head; /* bytes */
+    void* v_pool;
+    int64_t vp_page, vp_token, vp_head; /* bytes */
+    float* k_scale;
+    int64_t ks_page;
+    float* v_scale;
+    int64_t vs_page;
+    int64_t pages;
+    const int32_t* table;
+    int64_t table_stride;
+    const int32_t* starts;
+    const int32_t* cu_tokens;
+    int32_t table_len, tokens, requests, kv_heads;
+} v1_kv8_store_args;
+int v1_kv8_store(const v1_kv8_store_args* a, void* stream);
 /* Attention of one query position per row: q [rows, kv_heads * group, 128] bf16
  * (group <= 16), key j of row r at position id = ids[r * ids_stride + j] (j when
  * ids is NULL), j < lens[r] clamped to [0, keys] (keys when lens is NULL), in
@@ -653,13 +703,32 @@ int v1_kv8_store(const void* k, int64_t k_token, int64_t k_head, const void* v, 
  * -inf.  out [rows, heads, 128] bf16, lse [rows, heads] (may be NULL).  workspace:
  * v1_kv8_attend_workspace(rows, kv_heads, group, keys, lens != NULL) bytes, the
  * call's own until the stream has passed it.  scale > 0. */
-int v1_kv8_attend(const void* q, int64_t q_row, int64_t q_head, const void* k_pool, int64_t kp_page,
-                  int64_t kp_token, int64_t kp_head, const void* v_pool, int64_t vp_page, int64_t vp_token,
-                  int64_t vp_head, const float* k_scale, int64_t ks_page, const float* v_scale, int64_t vs_page,
-                  int64_t pages, const int32_t* table, int64_t table_stride, int32_t table_len,
-                  const int32_t* ids, int64_t ids_stride, const int32_t* lens, int32_t rows, int32_t kv_heads,
-                  int32_t group, int32_t keys, float scale, void* out, int64_t o_row, int64_t o_head,
-                  float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+typedef struct {
+    const void* q;
+    int64_t q_row, q_head;
+    const void* k_pool;
+    int64_t kp_page, kp_token, kp_head; /* bytes */
+    const void* v_pool;
+    int64_t vp_page, vp_token, vp_head; /* bytes */
+    const float* k_scale;
+    int64_t ks_page;
+    const float* v_scale;
+    int64_t vs_page;
+    int64_t pages;
+    const int32_t* table;
+    int64_t table_stride;
+    const int32_t* ids;
+    int64_t ids_stride;
+    const int32_t* lens;
+    void* out;
+    int64_t o_row, o_head;
+    float* lse;
+    void* workspace;
+    int64_t workspace_bytes;
+    int32_t table_len, rows, kv_heads, group, keys;
+    float scale;
+} v1_kv8_attend_args;
+int v1_kv8_attend(const v1_kv8_attend_args* a, void* stream);
 int64_t v1_kv8_attend_workspace(int32_t rows, int32_t kv_heads, int32_t group, int32_t keys, int32_t ragged);
 #ifdef __cplusplus
 }

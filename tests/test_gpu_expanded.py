@@ -202,11 +202,15 @@ def test_library_refusals():
     if not L.LIB_PATH.exists():
         pkg("build").build()
     h = L.lib()
-    base = dict(q=256, qr=384, qh=192, kv=256, kr=512, kh=256, rope=256, rr=64, cu_q=256, cu_k=256, tokens=4096, keys=4096,
-                batch=1, heads=16, max_q=4096, causal=1, scale=0.1, out=256, o_row=256, o_head=128, lse=0, ws=0, wsb=0, stream=0)
+    def call(fields):
+        return h.v1_latent_expanded(L.PACKED["v1_latent_expanded"].pack(*fields.values()), None)
+
+    base = dict(q=256, qr=384, qh=192, kv=256, kr=512, kh=256, rope=256, rr=64, cu_q=256, cu_k=256, out=256, o_row=256, o_head=128,
+                lse=0, ws=0, wsb=0, tokens=4096, keys=4096, batch=1, heads=16, max_q=4096, causal=1, scale=0.1)
     for bad in (dict(q=8), dict(kv=8), dict(rope=4), dict(qr=380), dict(kh=252), dict(out=4), dict(o_row=254), dict(heads=0),
-                dict(tokens=-1), dict(scale=0.0), dict(scale=-1.0), dict(tokens=1, max_q=1, heads=1)):
-        assert h.v1_latent_expanded(*{**base, **bad}.values()) == L.V1_ERR_INVALID, bad
+                dict(tokens=-1), dict(scale=0.0), dict(scale=-1.0), dict(heads=1 << 16), dict(tokens=1, max_q=1, heads=1)):
+        assert call({**base, **bad}) == L.V1_ERR_INVALID, bad
         assert b"latent_expanded" in h.v1_last_error()
     for none in (dict(tokens=0), dict(batch=0), dict(max_q=0)):
-        assert h.v1_latent_expanded(*{**base, **none}.values()) == 0
+        assert call({**base, **none}) == 0
+    assert h.v1_latent_expanded(None, None) == L.V1_ERR_INVALID

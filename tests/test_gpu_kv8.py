@@ -279,18 +279,22 @@ def test_library_refusals():
     if not L.LIB_PATH.exists():
         pkg("build").build()
     h = L.lib()
+    def call(name, fields):
+        return getattr(h, name)(L.PACKED[name].pack(*fields.values()), None)
+
     base = dict(q=256, qr=1024, qh=128, kp=256, kpp=8192, kpt=128, kph=128, vp=256, vpp=8192, vpt=128, vph=128, ks=256, ksp=1, vs=256,
-                vsp=1, pages=4, table=256, ts=9, tl=9, ids=0, ids_s=0, lens=0, rows=4096, kv_heads=1, group=4, keys=100, scale=0.1, out=256,
-                o_row=512, o_head=128, lse=0, ws=0, wsb=0, stream=0)
+                vsp=1, pages=4, table=256, ts=9, ids=0, ids_s=0, lens=0, out=256, o_row=512, o_head=128, lse=0, ws=0, wsb=0, tl=9,
+                rows=4096, kv_heads=1, group=4, keys=100, scale=0.1)
     for bad in (dict(q=8), dict(qh=100), dict(kp=8), dict(vpt=120), dict(kph=8), dict(out=4), dict(o_row=510), dict(group=17), dict(group=0),
-                dict(kv_heads=0), dict(rows=-1), dict(scale=0.0), dict(rows=1, keys=8192)):
-        assert h.v1_kv8_attend(*{**base, **bad}.values()) == L.V1_ERR_INVALID, bad
+                dict(kv_heads=0), dict(rows=-1), dict(scale=0.0), dict(kv_heads=1 << 14), dict(rows=1, keys=8192)):
+        assert call("v1_kv8_attend", {**base, **bad}) == L.V1_ERR_INVALID, bad
         assert b"kv8_attend" in h.v1_last_error()
-    assert h.v1_kv8_attend(*{**base, "rows": 0}.values()) == 0
+    assert call("v1_kv8_attend", {**base, "rows": 0}) == 0
+    assert h.v1_kv8_attend(None, None) == h.v1_kv8_store(None, None) == L.V1_ERR_INVALID
     base = dict(k=256, kt=128, kh=128, v=256, vt=128, vh=128, kp=256, kpp=8192, kpt=128, kph=128, vp=256, vpp=8192, vpt=128, vph=128, ks=256,
-                ksp=1, vs=256, vsp=1, pages=4, table=256, ts=9, tl=9, starts=256, cu=256, tokens=5, requests=2, kv_heads=1, stream=0)
+                ksp=1, vs=256, vsp=1, pages=4, table=256, ts=9, starts=256, cu=256, tl=9, tokens=5, requests=2, kv_heads=1)
     for bad in (dict(k=8), dict(vh=100), dict(kp=4), dict(vpp=8196), dict(tokens=-1), dict(requests=-1), dict(kv_heads=0), dict(pages=-1)):
-        assert h.v1_kv8_store(*{**base, **bad}.values()) == L.V1_ERR_INVALID, bad
+        assert call("v1_kv8_store", {**base, **bad}) == L.V1_ERR_INVALID, bad
         assert b"kv8_store" in h.v1_last_error()
     for none in (dict(tokens=0), dict(requests=0), dict(pages=0), dict(tl=0)):
-        assert h.v1_kv8_store(*{**base, **none}.values()) == 0
+        assert call("v1_kv8_store", {**base, **none}) == 0

@@ -261,19 +261,23 @@ def test_library_refusals():
     if not L.LIB_PATH.exists():
         pkg("build").build()
     h = L.lib()
-    base = dict(q=256, q_row=576, q_head=576, pool=256, pool_rows=8, stride=656, map=0, map_len=0, map_stride=0, shift=0,
-                ids=256, ids_stride=3, lens=0, rows=1000, heads=1, keys=3, scale=1.0, out=256, o_row=512, o_head=512, lse=0,
-                ws=0, ws_bytes=0, stream=0)
+    def call(name, fields):
+        return getattr(h, name)(L.PACKED[name].pack(*fields.values()), None)
+
+    base = dict(q=256, q_row=576, q_head=576, pool=256, pool_rows=8, stride=656, map=0, map_len=0, map_stride=0, ids=256, ids_stride=3,
+                lens=0, out=256, o_row=512, o_head=512, lse=0, ws=0, ws_bytes=0, shift=0, rows=1000, heads=1, keys=3, scale=1.0)
     for bad in (dict(q=8), dict(pool=24), dict(q_row=572), dict(stride=640), dict(stride=664), dict(heads=0), dict(rows=-1),
                 dict(keys=-1), dict(out=4), dict(o_head=510), dict(shift=31), dict(map_len=-1), dict(pool_rows=1 << 31),
+                dict(scale=0.0), dict(scale=math.nan), dict(heads=1 << 16),
                 dict(rows=1, keys=2048)):  # (the last: parts without a workspace)
-        assert h.v1_latent_attend(*{**base, **bad}.values()) == L.V1_ERR_INVALID, bad
+        assert call("v1_latent_attend", {**base, **bad}) == L.V1_ERR_INVALID, bad
         assert b"latent_attend" in h.v1_last_error()
-    assert h.v1_latent_attend(*{**base, "rows": 0}.values()) == 0
-    store = dict(latent=256, ls=512, rope=256, rs=64, slots=256, tokens=3, pool=256, rows=8, stride=656, stream=0)
+    assert call("v1_latent_attend", {**base, "rows": 0}) == 0
+    assert h.v1_latent_attend(None, None) == h.v1_latent_store(None, None) == L.V1_ERR_INVALID
+    store = dict(latent=256, ls=512, rope=256, rs=64, slots=256, pool=256, rows=8, stride=656, tokens=3)
     for bad in (dict(latent=8), dict(rope=8), dict(ls=510), dict(pool=8), dict(stride=640), dict(tokens=-1), dict(rows=-1)):
-        assert h.v1_latent_store(*{**store, **bad}.values()) == L.V1_ERR_INVALID, bad
-    assert h.v1_latent_store(*{**store, "tokens": 0}.values()) == 0
+        assert call("v1_latent_store", {**store, **bad}) == L.V1_ERR_INVALID, bad
+    assert call("v1_latent_store", {**store, "tokens": 0}) == 0
     # 8 rows of 2048 keys, 16 heads: 32 parts a row
     assert h.v1_latent_attend_workspace(8, 16, 2048, 0) == 8 * 32 * 16 * 514 * 4
     assert h.v1_latent_attend_workspace(4096, 16, 2048, 0) == 0 == h.v1_latent_attend_workspace(0, 16, 2048, 0)
