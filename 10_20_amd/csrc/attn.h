@@ -32,13 +32,19 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
 }
 
-// 8 e4m3 codes -> 8 bf16, exact (4 significant bits, exponents -9 .. 8).
+// Two e4m3 codes (the low or the high pair of four) -> two bf16, exact: 4
+// significant bits, exponents -9 .. 8.
+template <int HIGH>
+__device__ __forceinline__ uint32_t codes_pair(uint32_t four) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(four, 1.0f, HIGH != 0));
+}
+
 __device__ __forceinline__ Frag bf16_of_codes(uint32_t lo, uint32_t hi) {
     Frag f;
-    f.w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false));
-    f.w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true));
-    f.w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false));
-    f.w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true));
+    f.w[0] = codes_pair<0>(lo);
+    f.w[1] = codes_pair<1>(lo);
+    f.w[2] = codes_pair<0>(hi);
+    f.w[3] = codes_pair<1>(hi);
     return f;
 }
 
@@ -76,6 +82,12 @@ __device__ __forceinline__ uint32_t lds_offset(const void* p) {
 __device__ __forceinline__ void copy_to_lds(const void* src, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
                  :: "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory", "m0");
+}
+
+// The same from `base` (the same for the wave) + `offset`.
+__device__ __forceinline__ void copy_to_lds(uint64_t base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :: "v"(offset), "s"(base), "s"(lds) : "memory", "m0");
 }
 
 // Waits until at most N vector memory operations of this wave are in flight

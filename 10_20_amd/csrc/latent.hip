@@ -83,12 +83,22 @@ __device__ const u32x4 zero_latent[kChunks] = {};
 
 constexpr float kLag = 6.f;  // the subtracted maximum may lag the true one by 2^6
 
+// (opaque: offsets of the three buffers kept apart for every read of the loop
+// take the registers that Q and the sums need)
+__device__ __forceinline__ int32_t buffer_of(int32_t t) {
+    int32_t b = t % 3;
+    asm volatile("" : "+s"(b));
+    return b;
+}
+
 template <int HT, int HG>
 struct AbsorbedLds {
     static constexpr int kHeads = 16 * HT * HG, kQuarters = 4 / HG;
     uint8_t tile[3][kTileBytes];
-    uint16_t prob[kScaleBlocks][kHeads][kTileKeys];  // 16-byte chunk n of head h at n ^ (h % 8)
-    float hidden[3][kTileKeys];                      // 0, or -inf: not attended
+    float prob[kHeads][kTileKeys];         // 16-byte chunk n of head h at n ^ (h % 16)
+    float scale[kScaleBlocks][kTileKeys];  // of the tile whose probabilities these are
+    u32x4 q_rope[HG][HT][2][kWave];        // fragments of the queries' rope numbers
+    float hidden[3][kTileKeys];            // 0, or -inf: not attended
     float top[kQuarters][kHeads];
     float keep[kHeads];
     float total[kQuarters][kHeads];
@@ -104,11 +114,12 @@ struct AbsorbedLds {
 //   scores  S^T = K Q^T: wave (hg, kq) takes heads 16 HT hg .. and 16 HG keys;
 //           codes become bf16 (exact) as they are read, one accumulator per block
 //           of 128 numbers, joined with the block's scales in fp32.
-//   softmax the key groups exchange their maxima through LDS; each probability is
-//           multiplied by its key's four scales and rounded to bf16 once (2^-9
-//           of it at most, as the output), the sum stays fp32.
-//   output  O^T = C^T P^T: a wave takes a block of 128 columns of all heads, its
-//           codes transposed by the LDS read (ds_read_b64_tr_b8), exact in bf16.
+//   softmax the key groups exchange their maxima through LDS; probabilities and
+//           their sums stay fp32.
+//   output  O^T = C^T P^T: a wave takes a block of 128 columns of all heads: the
+//           probabilities times their keys' scale of that block, rounded to bf16
+//           once (2^-8 of each at most, as the output's rounding), and its codes
+//           transposed by the LDS read (ds_read_b64_tr_b8), exact in bf16.
 template <int HT, int HG>
 __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
     constexpr int HB = 16 * HT * HG, KT = HG, KQ = 4 / HG, RPW = kTileKeys / 4, GT = kWave / RPW;
@@ -118,7 +129,8 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
     auto& lds = *reinterpret_cast<AbsorbedLds<HT, HG>*>(lds_raw);
     const int32_t wave = __builtin_amdgcn_readfirstlane((int32_t)threadIdx.x / kWave) & 3;
     const bool scorer = __builtin_amdgcn_readfirstlane((int32_t)threadIdx.x / kWave) < 4;
-    const int32_t lane = (int32_t)threadIdx.x % kWave, g = lane >> 4, c = lane & 15;
+    const int32_t lane = (int32_t)threadIdx.x % kWave;
+    int32_t g = lane >> 4, c = lane & 15;  // (opaque in the loops, as buffer_of)
 
     // work-groups reach the XCDs in turn: the splits of an item follow each other on one of them
     const int32_t xcd = (int32_t)blockIdx.x % 8, turn = (int32_t)blockIdx.x / 8;
@@ -131,7 +143,7 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
         const int32_t hg = wave / KQ, kq = wave % KQ;
         // B fragments of Q^T: column c = head c of 16; 64 numbers in two steps: lane
         // group g takes 16g .. 16g + 7 of them, then 16g + 8 .. 16g + 15 (the order in which the codes are read)
-        Frag q[HT][18];
+        Frag q[HT][16];
 #pragma unroll
         for (int ht = 0; ht < HT; ++ht) {
             const int32_t h = min(head0 + hg * 16 * HT + 16 * ht + c, p.heads - 1);
@@ -139,84 +151,88 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
 #pragma unroll
             for (int s = 0; s < 16; ++s)
                 q[ht][s].u = *reinterpret_cast<const u32x4*>(src + 64 * (s / 2) + 16 * g + 8 * (s % 2));
+            if (kq == 0)  // (read before the first tile's products, behind its barrier)
 #pragma unroll
-            for (int s = 0; s < 2; ++s) q[ht][16 + s].u = *reinterpret_cast<const u32x4*>(src + kLatent + 32 * s + 8 * g);
+                for (int s = 0; s < 2; ++s)
+                    lds.q_rope[hg][ht][s][lane] = *reinterpret_cast<const u32x4*>(src + kLatent + 32 * s + 8 * g);
         }
         float mx[HT], total[HT];
 #pragma unroll
         for (int ht = 0; ht < HT; ++ht) mx[ht] = -__builtin_inff(), total[ht] = 0.f;
 
 #pragma unroll 1
-        for (int32_t t = 0; t <= tiles; ++t) {
+        for (int32_t t = 0; t < tiles; ++t) {
+            asm volatile("" : "+v"(g), "+v"(c));
             lds_barrier();  // tile t has landed; probabilities of tile t - 1 are written
-            const uint8_t* tile = lds.tile[t % 3];
-            float s[KT][HT][4];  // of keys 16 (KT kq + kt) + 4g + i, heads c
-            if (t < tiles) {
+            const uint8_t* tile = lds.tile[buffer_of(t)];
+            f32x4 s[KT][HT];  // of keys 16 (KT kq + kt) + 4g + i, heads c
+            {
                 // Steps of one block of one key tile (the rope numbers are a fifth
-                // block of scale 1): the next step's codes and scales are read, this
-                // one's codes converted and multiplied, the last one's products folded.
+                // block, of scale 1).  A step's products are issued between the
+                // conversions of the next one's codes, the reads of those after it
+                // and the folding of the last one's products: 16 cycles of the
+                // matrix core cover three vector operations.
                 constexpr int STEPS = KT * 5;
                 const uint8_t* const key0 = tile + (16 * KT * kq + c) * kRowBytes + 16 * g;
                 const uint8_t* const scale0 = tile + (16 * KT * kq + 4 * g) * kRowBytes + kScaleAt;
-                u32x4 raw[2][2];
-                float sc[2][4];
-                f32x4 d[2][HT];
-                auto fetch = [&](int n) __attribute__((always_inline)) {
-                    const int at = (n / 5) * 16 * kRowBytes, b = n % 5;
-#pragma unroll
-                    for (int half = 0; half < 2; ++half)
-                        raw[n & 1][half] = *reinterpret_cast<const u32x4*>(key0 + at + 128 * b + 64 * half);
-                    if (b < kScaleBlocks)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            sc[n & 1][i] = *reinterpret_cast<const float*>(scale0 + at + i * kRowBytes + 4 * b);
+                u32x4 raw[2];
+                Frag k[4], qr[HT][2];
+                f32x4 sc, d[2][HT];
+                auto fetch = [&](int n, int half) __attribute__((always_inline)) {
+                    if (n < STEPS) raw[half] = *reinterpret_cast<const u32x4*>(key0 + (n / 5) * 16 * kRowBytes + 128 * (n % 5) + 64 * half);
                 };
-                auto fold = [&](int n, float (&f)[4]) __attribute__((always_inline)) {
-#pragma unroll
-                    for (int ht = 0; ht < HT; ++ht)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            float& x = s[n / 5][ht][i];
-                            x = n % 5 == kScaleBlocks ? x + d[n & 1][ht][i]
-                                : n % 5 == 0          ? f[i] * d[n & 1][ht][i]
-                                                      : fmaf(f[i], d[n & 1][ht][i], x);
-                        }
+                auto fetch_scale = [&](int n, int i) __attribute__((always_inline)) {
+                    if (n < STEPS && n % 5 < kScaleBlocks)
+                        sc[i] = *reinterpret_cast<const float*>(scale0 + (n / 5 * 16 + i) * kRowBytes + 4 * (n % 5));
                 };
-                fetch(0);
-                float last[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int n = 0; n < STEPS; ++n) {
-                    const int b = n % 5;
-                    float now[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) now[i] = sc[n & 1][i];
-                    if (n + 1 < STEPS) fetch(n + 1);
-                    Frag k[4];
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const u32x4 w = raw[n & 1][half];
-                        if (b < kScaleBlocks) {
-                            k[2 * half] = bf16_of_codes(w[0], w[1]);
-                            k[2 * half + 1] = bf16_of_codes(w[2], w[3]);
-                        } else {
-                            k[half].u = w;
-                        }
+                // quarter m % 4 of step m / 4 (of the rope's step the first two): its fragment, words lo .. hi
+                auto convert = [&](int m, int part) __attribute__((always_inline)) {
+                    const int n = m / 4, j = m % 4;
+                    if (n >= STEPS) return;
+                    const u32x4 w = raw[j / 2];
+                    if (n % 5 < kScaleBlocks) {
+                        k[j].w[2 * part] = codes_pair<0>(w[2 * (j & 1) + part]);
+                        k[j].w[2 * part + 1] = codes_pair<1>(w[2 * (j & 1) + part]);
+                    } else if (j < 2 && part == 1) {
+                        k[j].u = raw[j];
                     }
+                    if (part == 1 && (j & 1)) fetch(n + 1, j / 2);
+                };
+                auto fold = [&](int n, int ht, int i) __attribute__((always_inline)) {
+                    if (n < 0) return;
+                    const float x = s[n / 5][ht][i], y = d[n & 1][ht][i];
+                    s[n / 5][ht][i] = n % 5 == 0 ? sc[i] * y : n % 5 < kScaleBlocks ? fmaf(sc[i], y, x) : x + y;
+                };
 #pragma unroll
-                    for (int ht = 0; ht < HT; ++ht) d[n & 1][ht] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int half = 0; half < 2; ++half) fetch(0, half);
+                convert(0, 0), convert(0, 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int j = 0; j < (b < kScaleBlocks ? 4 : 2); ++j)
+                for (int m = 0; m < 4 * STEPS; ++m) {
+                    const int n = m / 4, b = n % 5, j = m % 4;
+                    if (b == kScaleBlocks - 1 && j == 3)
 #pragma unroll
-                        for (int ht = 0; ht < HT; ++ht) d[n & 1][ht] = mfma16(k[j], q[ht][4 * b + j], d[n & 1][ht]);
-                    if (n > 0) fold(n - 1, last);
+                        for (int ht = 0; ht < HT; ++ht)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) last[i] = now[i];
-                    __builtin_amdgcn_sched_barrier(0);
+                            for (int i = 0; i < 2; ++i) qr[ht][i].u = lds.q_rope[hg][ht][i][16 * g + c];
+#pragma unroll
+                    for (int ht = 0; ht < HT; ++ht) {
+                        if (j < (b < kScaleBlocks ? 4 : 2))
+                            d[n & 1][ht] = mfma16(k[j], b < kScaleBlocks ? q[ht][4 * (b % 4) + j] : qr[ht][j % 2], j == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : d[n & 1][ht]);
+                        if (HT == 1) convert(m + 1, 0);
+                        convert(m + 1, HT == 1 ? 1 : ht);
+                        fold(n - 1, ht, j);
+                        if (ht == HT - 1) fetch_scale(n, j);  // (after the last step's use)
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
-                fold(STEPS - 1, last);
+#pragma unroll
+                for (int ht = 0; ht < HT; ++ht)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) fold(STEPS - 1, ht, i);
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) {
-                    const f32x4 hidden = *reinterpret_cast<const f32x4*>(&lds.hidden[t % 3][16 * (KT * kq + kt) + 4 * g]);
+                    const f32x4 hidden = *reinterpret_cast<const f32x4*>(&lds.hidden[buffer_of(t)][16 * (KT * kq + kt) + 4 * g]);
 #pragma unroll
                     for (int ht = 0; ht < HT; ++ht)
 #pragma unroll
@@ -236,7 +252,8 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
                 }
             }
             lds_barrier();  // maxima of tile t are there; probabilities of tile t - 1 have been read
-            if (t < tiles) {
+            {
+                lds.scale[g][16 * wave + c] = *reinterpret_cast<const float*>(tile + (16 * wave + c) * kRowBytes + kScaleAt + 4 * g);
                 float sub[HT];
 #pragma unroll
                 for (int ht = 0; ht < HT; ++ht) {
@@ -256,28 +273,23 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) {
                     const int32_t k0 = 16 * (KT * kq + kt);
-                    f32x4 sc[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        sc[i] = *reinterpret_cast<const f32x4*>(tile + (k0 + 4 * g + i) * kRowBytes + kScaleAt);
 #pragma unroll
                     for (int ht = 0; ht < HT; ++ht) {
                         const int32_t h = 16 * (HT * hg + ht) + c;
-                        float x[4];
+                        f32x4 x;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             x[i] = __builtin_amdgcn_exp2f(s[kt][ht][i] - sub[ht]);
                             total[ht] += x[i];
                         }
-                        uint16_t* at = &lds.prob[0][h][8 * ((k0 / 8 + (g >> 1)) ^ (h & 7)) + 4 * (g & 1)];
-#pragma unroll
-                        for (int b = 0; b < kScaleBlocks; ++b)
-                            *reinterpret_cast<u32x2*>(at + b * HB * kTileKeys) =
-                                u32x2{pack_bf16(x[0] * sc[0][b], x[1] * sc[1][b]), pack_bf16(x[2] * sc[2][b], x[3] * sc[3][b])};
+                        *reinterpret_cast<f32x4*>(&lds.prob[h][4 * ((k0 / 4 + g) ^ c)]) = x;
+                        __builtin_amdgcn_sched_barrier(0);  // (mixed, the two tiles' values take Q's registers)
                     }
                 }
             }
         }
+        lds_barrier();  // (the multipliers' last round)
+        lds_barrier();
         // totals of the key groups
 #pragma unroll
         for (int ht = 0; ht < HT; ++ht) {
@@ -296,8 +308,8 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
     const int32_t* ids = p.ids ? p.ids + it.row * p.ids_stride : nullptr;
     const int32_t* map = p.map ? p.map + it.row * p.map_stride : nullptr;
     auto fetch_id = [&](int32_t group) __attribute__((always_inline)) -> int32_t {
-        const int32_t j = (it.first + group * GT + lane / RPW) * kTileKeys + wave * RPW + lane % RPW;
-        if (j >= it.keys) return -1;
+        const int32_t lane = 16 * g + c, tile = group * GT + lane / RPW, j = (it.first + tile) * kTileKeys + wave * RPW + lane % RPW;
+        if (tile >= tiles || j >= it.keys) return -1;
         return ids ? ids[j] : j;
     };
     auto fetch_row = [&](int32_t id) __attribute__((always_inline)) -> int32_t {
@@ -312,78 +324,120 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
         }
         return row < p.pool_rows ? (int32_t)row : -1;
     };
-    int32_t rows_now = fetch_row(fetch_id(0)), rows_next = fetch_row(fetch_id(1)), ids_after = fetch_id(2);
+    const uint64_t nowhere = reinterpret_cast<uint64_t>(zero_latent);
+    auto address = [&](int32_t row) __attribute__((always_inline)) -> uint64_t {
+        return row < 0 ? nowhere : reinterpret_cast<uint64_t>(p.pool) + (uint64_t)((int64_t)row * p.pool_stride);
+    };
+    uint64_t at_now = address(fetch_row(fetch_id(0)));
+    int32_t row_next = fetch_row(fetch_id(1)), id_after = fetch_id(2);
     // copies of tile t into buffer t % 3, asked for in the order of the tiles
-    auto copy_tile = [&](int32_t t) __attribute__((always_inline)) {
+    int32_t from, chunk;  // of the next copy: its row's lane in at_now (times 4, for the shuffle), its chunk of the row
+    auto begin_tile = [&](int32_t t) __attribute__((always_inline)) {
         if (t > 0 && t % GT == 0) {
-            rows_now = rows_next;
-            rows_next = fetch_row(ids_after);
-            ids_after = fetch_id(t / GT + 2);
+            at_now = address(row_next);
+            row_next = fetch_row(id_after);
+            id_after = fetch_id(t / GT + 2);
         }
-        const int32_t buf = t % 3;
-        if (lane / RPW == t % GT) lds.hidden[buf][wave * RPW + lane % RPW] = rows_now < 0 ? -__builtin_inff() : 0.f;
-        const uint32_t to = lds_offset(&lds.tile[buf][wave * RPW * kRowBytes]);
+        const int32_t lane = 16 * g + c;
+        if (lane / RPW == t % GT) lds.hidden[buffer_of(t)][wave * RPW + lane % RPW] = at_now == nowhere ? -__builtin_inff() : 0.f;
+        from = 4 * (t % GT) * RPW + (lane < kChunks ? 0 : 4);
+        chunk = lane < kChunks ? lane : lane - kChunks;
+        asm volatile("" : "+v"(chunk));  // (found anew for every tile: kept for all copies, they spill)
+    };
+    auto copy = [&](int32_t t, int j) __attribute__((always_inline)) {  // j = 0, 1, ... in order
+        const uint32_t to = lds_offset(&lds.tile[buffer_of(t)][wave * RPW * kRowBytes]);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)(uint32_t)at_now);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)(at_now >> 32));
+        const uint64_t a = (((uint64_t)hi << 32) | lo) + (uint32_t)(16 * chunk);
+        if (64 * j + 63 < RPW * kChunks || 16 * g + c < RPW * kChunks % kWave)
+            copy_to_lds(reinterpret_cast<const void*>(a), to + 1024 * j);
+        const bool wrap = chunk >= 2 * kChunks - kWave;  // 64 chunks on: one row and 23 chunks, or two and 18 less
+        from += wrap ? 8 : 4;
+        chunk += wrap ? kWave - 2 * kChunks : kWave - kChunks;
+    };
+    auto copy_tile = [&](int32_t t) __attribute__((always_inline)) {
+        begin_tile(t);
 #pragma unroll
-        for (int j = 0; j < COPIES; ++j) {
-            const uint32_t i = 64 * j + lane, r = (i * 1599u) >> 16, chunk = i - r * kChunks;  // i / 41, exact below 2009
-            const int32_t row = __shfl(rows_now, (t % GT) * RPW + (int)(r < RPW ? r : RPW - 1), kWave);
-            const uint8_t* src = row < 0 ? reinterpret_cast<const uint8_t*>(zero_latent) : p.pool + row * p.pool_stride;
-            if (r < RPW) copy_to_lds(src + 16 * chunk, to + 1024 * j);
-        }
+        for (int j = 0; j < COPIES; ++j) copy(t, j);
     };
     f32x4 acc[DT][PT];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int h = 0; h < PT; ++h) acc[d][h] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (tiles > 0) copy_tile(0);
-    if (tiles > 1) copy_tile(1);
+    // (tiles past the last are copies of the row of zeros: no copy is conditional,
+    // and the waits count the same for every tile)
+    copy_tile(0);
+    copy_tile(1);
+    copy_tile(2);
     i32x2 v[2][DT];  // this wave's codes of the last tile, transposed: its buffer is free for the next copies
+    // lanes 2r, 2r + 1 of a group hand in 16 columns of key 8g + r; lane c gets column c of its eight keys
+    auto fetch = [&](int32_t t, int ks) __attribute__((always_inline)) {
+        const uint8_t* const at = lds.tile[buffer_of(t)] + (32 * ks + 8 * g + c / 2) * kRowBytes + wave * 128 + 8 * (c & 1);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+            v[ks][d] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(at + 16 * d));
+    };
+    wait_barrier<2 * COPIES>();
+    fetch(0, 0);
+    lds_barrier();
+    fetch(0, 1);
 #pragma unroll 1
-    for (int32_t t = 0; t <= tiles; ++t) {
-        if (t + 1 < tiles) wait_barrier<COPIES>();
-        else wait_barrier<0>();
-        if (t + 2 < tiles) copy_tile(t + 2);
+    for (int32_t t = 1; t <= tiles; ++t) {
+        asm volatile("" : "+v"(g), "+v"(c));
+        wait_barrier<COPIES>();
+        begin_tile(t + 2);
         Frag pf[2][PT];
-        // lanes 2r, 2r + 1 of a group hand in 16 columns of key 8g + r; lane c gets column c of its eight keys
-        const uint8_t* const next = lds.tile[t % 3] + (8 * g + c / 2) * kRowBytes + wave * 128 + 8 * (c & 1);
+        // (a copy is held up at the memory's rate: they are spread over the products)
         auto product = [&](int ks) __attribute__((always_inline)) {
+            Frag a[2];
+            a[0] = bf16_of_codes((uint32_t)v[ks][0][0], (uint32_t)v[ks][0][1]);
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const Frag a = bf16_of_codes((uint32_t)v[ks][d][0], (uint32_t)v[ks][d][1]);
 #pragma unroll
-                for (int h = 0; h < PT; ++h) acc[d][h] = mfma16(a, pf[ks][h], acc[d][h]);
+                for (int h = 0; h < PT; ++h) {
+                    acc[d][h] = mfma16(a[d & 1], pf[ks][h], acc[d][h]);
+                    if (h == 0 && d + 1 < DT)
+                        a[(d + 1) & 1] = bf16_of_codes((uint32_t)v[ks][d + 1][0], (uint32_t)v[ks][d + 1][1]);
+                }
+                if (DT * ks + d < COPIES) copy(t + 2, DT * ks + d);
+                __builtin_amdgcn_sched_barrier(0);
             }
         };
-        auto fetch = [&](int ks) __attribute__((always_inline)) {
+        float keep[PT];
+        bool any = false;
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
-                v[ks][d] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                    (__attribute__((address_space(3))) i32x2*)(next + 32 * ks * kRowBytes + 16 * d));
-        };
-        if (t > 0) {
-            float keep[PT];
-            bool any = false;
+        for (int h = 0; h < PT; ++h) {
+            keep[h] = lds.keep[16 * h + c];
+            any |= keep[h] != 1.f;
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(&lds.scale[wave][32 * ks + 8 * g]);
+            const f32x4 b = *reinterpret_cast<const f32x4*>(&lds.scale[wave][32 * ks + 8 * g + 4]);
 #pragma unroll
             for (int h = 0; h < PT; ++h) {
-                keep[h] = lds.keep[16 * h + c];
-                any |= keep[h] != 1.f;
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks)
-                    pf[ks][h].u = *reinterpret_cast<const u32x4*>(&lds.prob[wave][16 * h + c][8 * ((4 * ks + g) ^ (c & 7))]);
+                const f32x4 x = *reinterpret_cast<const f32x4*>(&lds.prob[16 * h + c][4 * ((8 * ks + 2 * g) ^ c)]);
+                const f32x4 y = *reinterpret_cast<const f32x4*>(&lds.prob[16 * h + c][4 * ((8 * ks + 2 * g + 1) ^ c)]);
+                pf[ks][h].w[0] = pack_bf16(x[0] * a[0], x[1] * a[1]);
+                pf[ks][h].w[1] = pack_bf16(x[2] * a[2], x[3] * a[3]);
+                pf[ks][h].w[2] = pack_bf16(y[0] * b[0], y[1] * b[1]);
+                pf[ks][h].w[3] = pack_bf16(y[2] * b[2], y[3] * b[3]);
             }
-            if (__ballot(any))
-#pragma unroll
-                for (int h = 0; h < PT; ++h)
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) acc[d][h] *= keep[h];
-            product(0);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if (t < tiles) fetch(0);
+        if (__ballot(any))
+#pragma unroll
+            for (int h = 0; h < PT; ++h)
+#pragma unroll
+                for (int d = 0; d < DT; ++d) acc[d][h] *= keep[h];
+        product(0);
+        fetch(t, 0);
         lds_barrier();
-        if (t > 0) product(1);
-        if (t < tiles) fetch(1);
+        product(1);
+        fetch(t, 1);
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy is left in flight
     __syncthreads();
     const bool whole = it.parts == 1;
 #pragma unroll
