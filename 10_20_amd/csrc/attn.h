@@ -84,11 +84,18 @@ __device__ __forceinline__ void copy_to_lds(const void* src, uint32_t lds) {
                  :: "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory", "m0");
 }
 
-// The same from `base` (the same for the wave) + `offset`.
-__device__ __forceinline__ void copy_to_lds(uint64_t base, uint32_t offset, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-                 :: "v"(offset), "s"(base), "s"(lds) : "memory", "m0");
+// 4 bytes per lane.
+__device__ __forceinline__ void copy4_to_lds(const void* src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
+                 :: "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory", "m0");
 }
+
+// Waits until at most N vector memory operations of this wave are in flight and
+// its LDS operations are done.
+template <int N>
+__device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 // Waits until at most N vector memory operations of this wave are in flight
 // and its LDS operations are done, then joins the work-group's barrier.

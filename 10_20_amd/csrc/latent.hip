@@ -102,6 +102,7 @@ struct AbsorbedLds {
     float top[kQuarters][kHeads];
     float keep[kHeads];
     float total[kQuarters][kHeads];
+    int32_t ids[4][kWave], pages[4][kWave];
 };
 
 // A work-group of eight waves attends HB = 16 * HT * HG heads of one row over one
@@ -307,19 +308,32 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
     // rows of this wave's part of a tile, GT tiles at a time: lane = tile * RPW + row
     const int32_t* ids = p.ids ? p.ids + it.row * p.ids_stride : nullptr;
     const int32_t* map = p.map ? p.map + it.row * p.map_stride : nullptr;
-    auto fetch_id = [&](int32_t group) __attribute__((always_inline)) -> int32_t {
-        const int32_t lane = 16 * g + c, tile = group * GT + lane / RPW, j = (it.first + tile) * kTileKeys + wave * RPW + lane % RPW;
-        if (tile >= tiles || j >= it.keys) return -1;
-        return ids ? ids[j] : j;
+    // Positions and page entries of the groups to come are copied to LDS like the
+    // rows: loads into registers would have the compiler wait for every copy in flight.
+    auto position = [&](int32_t group) __attribute__((always_inline)) -> int32_t {  // in ids; -1: none
+        const int32_t lane = 16 * g + c, tile = group * GT + lane / RPW;
+        const int32_t j = (it.first + tile) * kTileKeys + wave * RPW + lane % RPW;
+        return tile < tiles && j < it.keys ? j : -1;
     };
-    auto fetch_row = [&](int32_t id) __attribute__((always_inline)) -> int32_t {
+    auto ask_id = [&](int32_t group) __attribute__((always_inline)) {
+        const int32_t j = position(group);
+        if (ids) copy4_to_lds(j < 0 ? reinterpret_cast<const int32_t*>(zero_latent) : ids + j, lds_offset(&lds.ids[wave][0]));
+    };
+    auto take_id = [&](int32_t group) __attribute__((always_inline)) -> int32_t {
+        const int32_t j = position(group);
+        return j < 0 ? -1 : ids ? lds.ids[wave][16 * g + c] : j;
+    };
+    auto ask_page = [&](int32_t id) __attribute__((always_inline)) {
+        const int64_t e = (int64_t)id >> p.map_shift;
+        if (map) copy4_to_lds(id < 0 || e >= p.map_len ? reinterpret_cast<const int32_t*>(zero_latent) : map + e,
+                              lds_offset(&lds.pages[wave][0]));
+    };
+    auto take_row = [&](int32_t id) __attribute__((always_inline)) -> int32_t {
         if (id < 0) return -1;
         int64_t row = id;
         if (map) {
-            const int64_t e = (int64_t)id >> p.map_shift;
-            if (e >= p.map_len) return -1;
-            const int32_t m = map[e];
-            if (m < 0) return -1;
+            const int32_t m = lds.pages[wave][16 * g + c];
+            if (((int64_t)id >> p.map_shift) >= p.map_len || m < 0) return -1;
             row = ((int64_t)m << p.map_shift) | (id & ((1 << p.map_shift) - 1));
         }
         return row < p.pool_rows ? (int32_t)row : -1;
@@ -328,15 +342,27 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
     auto address = [&](int32_t row) __attribute__((always_inline)) -> uint64_t {
         return row < 0 ? nowhere : reinterpret_cast<uint64_t>(p.pool) + (uint64_t)((int64_t)row * p.pool_stride);
     };
-    uint64_t at_now = address(fetch_row(fetch_id(0)));
-    int32_t row_next = fetch_row(fetch_id(1)), id_after = fetch_id(2);
+    ask_id(0);
+    wait_copies<0>();
+    int32_t id_next = take_id(0);
+    wait_copies<0>();
+    ask_page(id_next);
+    ask_id(1);
+    wait_copies<0>();
+    uint64_t at_now = address(take_row(id_next));
+    id_next = take_id(1);
+    wait_copies<0>();
+    ask_page(id_next);  // of the next group; its rows are taken, and the group after it asked for, when its first tile begins
+    ask_id(2);
     // copies of tile t into buffer t % 3, asked for in the order of the tiles
     int32_t from, chunk;  // of the next copy: its row's lane in at_now (times 4, for the shuffle), its chunk of the row
     auto begin_tile = [&](int32_t t) __attribute__((always_inline)) {
         if (t > 0 && t % GT == 0) {
-            at_now = address(row_next);
-            row_next = fetch_row(id_after);
-            id_after = fetch_id(t / GT + 2);
+            at_now = address(take_row(id_next));
+            id_next = take_id(t / GT + 1);
+            wait_lds();
+            ask_page(id_next);
+            ask_id(t / GT + 2);
         }
         const int32_t lane = 16 * g + c;
         if (lane / RPW == t % GT) lds.hidden[buffer_of(t)][wave * RPW + lane % RPW] = at_now == nowhere ? -__builtin_inff() : 0.f;
