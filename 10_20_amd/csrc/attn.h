@@ -71,6 +71,20 @@ __device__ __forceinline__ float finite_abs(float x) {
     return a < __builtin_inff() ? a : 0.f;  // (NaN compares false)
 }
 
+// f(Number<0>{}), .., f(Number<N - 1>{})
+template <int I>
+struct Number {
+    static constexpr int value = I;
+};
+
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void each_of(F&& f) {
+    if constexpr (I < N) {
+        f(Number<I>{});
+        each_of<N, I + 1>(f);
+    }
+}
+
 __device__ __forceinline__ uint32_t lds_offset(const void* p) {
     return (uint32_t)reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)p);
 }

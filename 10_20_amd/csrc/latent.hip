@@ -13,7 +13,7 @@ using namespace attn;
 
 constexpr int kLatent = 512, kRope = 64, kRowBytes = 656, kScaleBlocks = 4;
 constexpr int kRopeAt = kLatent, kScaleAt = kLatent + 2 * kRope;
-constexpr int kChunks = kRowBytes / 16;  // 41, odd: 16-byte reads of 8 rows at one offset meet 8 different banks
+constexpr int kChunks = kRowBytes / 16;
 constexpr int kTileBytes = kTileKeys * kRowBytes;
 
 // ------------------------------------------------------------------ store
@@ -83,13 +83,14 @@ __device__ const u32x4 zero_latent[kChunks] = {};
 
 constexpr float kLag = 6.f;  // the subtracted maximum may lag the true one by 2^6
 
-// (opaque: offsets of the three buffers kept apart for every read of the loop
-// take the registers that Q and the sums need)
-__device__ __forceinline__ int32_t buffer_of(int32_t t) {
-    int32_t b = t % 3;
-    asm volatile("" : "+s"(b));
-    return b;
-}
+// A tile in LDS: 16-row regions; in a region the rows' chunks of 16 bytes in
+// blocks of four, chunk 4j + q of row r at 1024 j + 64 r + 16 (q ^ (r / 4)), then
+// the scales, [block][row].  A copy is then 64 bytes of each of 16 rows: its
+// address differs from the last one's by a constant (whole rows end to end need
+// ten operations a copy for theirs), reads of 16 rows at one place are 1 KB in a
+// piece, and the transposing reads of eight rows meet different banks.
+constexpr int kRegionRows = 16, kRegion = kRegionRows * kRowBytes, kCopies = 11;
+constexpr int kScales = kRegion - kRegionRows * 4 * kScaleBlocks;
 
 template <int HT, int HG>
 struct AbsorbedLds {
@@ -103,15 +104,33 @@ struct AbsorbedLds {
     float keep[kHeads];
     float total[kQuarters][kHeads];
     int32_t ids[4][kWave], pages[4][kWave];
+    int32_t seen[4];
 };
+
+// (opaque: offsets of the three buffers kept apart for every read of the loop
+// take the registers that Q and the sums need)
+__device__ __forceinline__ int32_t buffer_of(int32_t t) {
+    int32_t b = t % 3;
+    asm volatile("" : "+s"(b));
+    return b;
+}
+
+// Copy j of a tile's region: 16 bytes per lane from `src` + 64 j.  (The
+// instruction adds its offset to the address in LDS as well.)
+template <int J>
+__device__ __forceinline__ void copy_block(uint64_t src, uint32_t region) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off offset:%2"
+                 :: "v"(src), "s"(__builtin_amdgcn_readfirstlane(region + (1024 - 64) * J)), "n"(64 * J) : "memory", "m0");
+}
 
 // A work-group of eight waves attends HB = 16 * HT * HG heads of one row over one
 // part of its keys, tile by tile of 64 keys that come memory -> LDS as they are
 // stored.  Four waves make the probabilities of tile t while the other four, one
 // on each SIMD beside them, multiply those of tile t - 1 with its latents (held in
-// registers, so that their buffer is free) and bring in tile t + 2: the products keep the matrix cores busy through the
-// others' softmax, and neither kind holds both Q and the output (144 and 128
-// registers at 64 heads: two waves per SIMD have 256 each).
+// registers, so that their buffer is free) and bring in tile t + 2: the products
+// keep the matrix cores busy through the others' softmax, and neither kind holds
+// both Q and the output (128 registers each at 64 heads; two waves per SIMD have
+// 256 each).
 //   scores  S^T = K Q^T: wave (hg, kq) takes heads 16 HT hg .. and 16 HG keys;
 //           codes become bf16 (exact) as they are read, one accumulator per block
 //           of 128 numbers, joined with the block's scales in fp32.
@@ -123,8 +142,7 @@ struct AbsorbedLds {
 //           transposed by the LDS read (ds_read_b64_tr_b8), exact in bf16.
 template <int HT, int HG>
 __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
-    constexpr int HB = 16 * HT * HG, KT = HG, KQ = 4 / HG, RPW = kTileKeys / 4, GT = kWave / RPW;
-    constexpr int COPIES = (RPW * kChunks + kWave - 1) / kWave;
+    constexpr int HB = 16 * HT * HG, KT = HG, KQ = 4 / HG, RPW = kRegionRows, GT = kWave / RPW;
     constexpr int DT = 8, PT = HB / 16;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
     auto& lds = *reinterpret_cast<AbsorbedLds<HT, HG>*>(lds_raw);
@@ -165,26 +183,28 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
         for (int32_t t = 0; t < tiles; ++t) {
             asm volatile("" : "+v"(g), "+v"(c));
             lds_barrier();  // tile t has landed; probabilities of tile t - 1 are written
-            const uint8_t* tile = lds.tile[buffer_of(t)];
+            const int32_t buf = buffer_of(t);
+            const uint8_t* const region = lds.tile[buf] + kRegion * KT * kq;
             f32x4 s[KT][HT];  // of keys 16 (KT kq + kt) + 4g + i, heads c
             {
                 // Steps of one block of one key tile (the rope numbers are a fifth
-                // block, of scale 1).  A step's products are issued between the
-                // conversions of the next one's codes, the reads of those after it
-                // and the folding of the last one's products: 16 cycles of the
-                // matrix core cover three vector operations.
+                // block, of scale 1, which starts from -inf at the hidden keys).  A
+                // step's products are issued between the conversions of the next
+                // one's codes, the reads of those after it and the folding of the
+                // last one's products: 16 cycles of the matrix core cover three
+                // vector operations.
                 constexpr int STEPS = KT * 5;
-                const uint8_t* const key0 = tile + (16 * KT * kq + c) * kRowBytes + 16 * g;
-                const uint8_t* const scale0 = tile + (16 * KT * kq + 4 * g) * kRowBytes + kScaleAt;
+                const uint8_t* const key0 = region + 64 * c + 16 * (g ^ (c >> 2));
+                const uint8_t* const scale0 = region + kScales + 16 * g;
                 u32x4 raw[2];
                 Frag k[4], qr[HT][2];
-                f32x4 sc, d[2][HT];
+                f32x4 sc[2], d[2][HT], hidden;
                 auto fetch = [&](int n, int half) __attribute__((always_inline)) {
-                    if (n < STEPS) raw[half] = *reinterpret_cast<const u32x4*>(key0 + (n / 5) * 16 * kRowBytes + 128 * (n % 5) + 64 * half);
+                    if (n < STEPS) raw[half] = *reinterpret_cast<const u32x4*>(key0 + n / 5 * kRegion + 1024 * (2 * (n % 5) + half));
                 };
-                auto fetch_scale = [&](int n, int i) __attribute__((always_inline)) {
+                auto fetch_scale = [&](int n) __attribute__((always_inline)) {
                     if (n < STEPS && n % 5 < kScaleBlocks)
-                        sc[i] = *reinterpret_cast<const float*>(scale0 + (n / 5 * 16 + i) * kRowBytes + 4 * (n % 5));
+                        sc[n & 1] = *reinterpret_cast<const f32x4*>(scale0 + n / 5 * kRegion + 4 * kRegionRows * (n % 5));
                 };
                 // quarter m % 4 of step m / 4 (of the rope's step the first two): its fragment, words lo .. hi
                 auto convert = [&](int m, int part) __attribute__((always_inline)) {
@@ -202,28 +222,32 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
                 auto fold = [&](int n, int ht, int i) __attribute__((always_inline)) {
                     if (n < 0) return;
                     const float x = s[n / 5][ht][i], y = d[n & 1][ht][i];
-                    s[n / 5][ht][i] = n % 5 == 0 ? sc[i] * y : n % 5 < kScaleBlocks ? fmaf(sc[i], y, x) : x + y;
+                    s[n / 5][ht][i] = n % 5 == 0 ? sc[n & 1][i] * y : n % 5 < kScaleBlocks ? fmaf(sc[n & 1][i], y, x) : x + y;
                 };
 #pragma unroll
                 for (int half = 0; half < 2; ++half) fetch(0, half);
+                fetch_scale(0);
                 convert(0, 0), convert(0, 1);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int m = 0; m < 4 * STEPS; ++m) {
                     const int n = m / 4, b = n % 5, j = m % 4;
-                    if (b == kScaleBlocks - 1 && j == 3)
+                    if (b == kScaleBlocks - 1 && j == 3) {
+                        hidden = *reinterpret_cast<const f32x4*>(&lds.hidden[buf][16 * (KT * kq + n / 5) + 4 * g]);
 #pragma unroll
                         for (int ht = 0; ht < HT; ++ht)
 #pragma unroll
                             for (int i = 0; i < 2; ++i) qr[ht][i].u = lds.q_rope[hg][ht][i][16 * g + c];
+                    }
 #pragma unroll
                     for (int ht = 0; ht < HT; ++ht) {
                         if (j < (b < kScaleBlocks ? 4 : 2))
-                            d[n & 1][ht] = mfma16(k[j], b < kScaleBlocks ? q[ht][4 * (b % 4) + j] : qr[ht][j % 2], j == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : d[n & 1][ht]);
+                            d[n & 1][ht] = mfma16(k[j], b < kScaleBlocks ? q[ht][4 * (b % 4) + j] : qr[ht][j % 2],
+                                                  j > 0 ? d[n & 1][ht] : b < kScaleBlocks ? f32x4{0.f, 0.f, 0.f, 0.f} : hidden);
                         if (HT == 1) convert(m + 1, 0);
                         convert(m + 1, HT == 1 ? 1 : ht);
                         fold(n - 1, ht, j);
-                        if (ht == HT - 1) fetch_scale(n, j);  // (after the last step's use)
+                        if (ht == HT - 1 && j == 3) fetch_scale(n + 1);  // (after the last use of these registers)
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
@@ -231,15 +255,6 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
                 for (int ht = 0; ht < HT; ++ht)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) fold(STEPS - 1, ht, i);
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    const f32x4 hidden = *reinterpret_cast<const f32x4*>(&lds.hidden[buffer_of(t)][16 * (KT * kq + kt) + 4 * g]);
-#pragma unroll
-                    for (int ht = 0; ht < HT; ++ht)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            s[kt][ht][i] = hidden[i] < 0.f ? -__builtin_inff() : s[kt][ht][i] * p.scale2;
-                }
 #pragma unroll
                 for (int ht = 0; ht < HT; ++ht) {
                     float top = -__builtin_inff();
@@ -249,13 +264,13 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
                         for (int i = 0; i < 4; ++i) top = fmaxf(top, s[kt][ht][i]);
                     top = fmaxf(top, __shfl_xor(top, 16, kWave));
                     top = fmaxf(top, __shfl_xor(top, 32, kWave));
-                    if (g == 0) lds.top[kq][16 * (HT * hg + ht) + c] = top;
+                    if (g == 0) lds.top[kq][16 * (HT * hg + ht) + c] = top * p.scale2;
                 }
             }
             lds_barrier();  // maxima of tile t are there; probabilities of tile t - 1 have been read
             {
-                lds.scale[g][16 * wave + c] = *reinterpret_cast<const float*>(tile + (16 * wave + c) * kRowBytes + kScaleAt + 4 * g);
                 float sub[HT];
+                lds.scale[g][16 * wave + c] = *reinterpret_cast<const float*>(lds.tile[buf] + kRegion * wave + kScales + 64 * g + 4 * c);
 #pragma unroll
                 for (int ht = 0; ht < HT; ++ht) {
                     const int32_t h = 16 * (HT * hg + ht) + c;
@@ -280,7 +295,7 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
                         f32x4 x;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            x[i] = __builtin_amdgcn_exp2f(s[kt][ht][i] - sub[ht]);
+                            x[i] = __builtin_amdgcn_exp2f(fmaf(s[kt][ht][i], p.scale2, -sub[ht]));
                             total[ht] += x[i];
                         }
                         *reinterpret_cast<f32x4*>(&lds.prob[h][4 * ((k0 / 4 + g) ^ c)]) = x;
@@ -305,14 +320,13 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
         return;
     }
 
-    // rows of this wave's part of a tile, GT tiles at a time: lane = tile * RPW + row
+    // rows of this wave's region of a tile, GT tiles at a time: lane = 16 * tile + row
     const int32_t* ids = p.ids ? p.ids + it.row * p.ids_stride : nullptr;
     const int32_t* map = p.map ? p.map + it.row * p.map_stride : nullptr;
     // Positions and page entries of the groups to come are copied to LDS like the
     // rows: loads into registers would have the compiler wait for every copy in flight.
     auto position = [&](int32_t group) __attribute__((always_inline)) -> int32_t {  // in ids; -1: none
-        const int32_t lane = 16 * g + c, tile = group * GT + lane / RPW;
-        const int32_t j = (it.first + tile) * kTileKeys + wave * RPW + lane % RPW;
+        const int32_t tile = group * GT + g, j = (it.first + tile) * kTileKeys + RPW * wave + c;
         return tile < tiles && j < it.keys ? j : -1;
     };
     auto ask_id = [&](int32_t group) __attribute__((always_inline)) {
@@ -339,7 +353,9 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
         return row < p.pool_rows ? (int32_t)row : -1;
     };
     const uint64_t nowhere = reinterpret_cast<uint64_t>(zero_latent);
+    bool seen = false;  // a key that is attended
     auto address = [&](int32_t row) __attribute__((always_inline)) -> uint64_t {
+        seen |= __ballot(row >= 0) != 0;
         return row < 0 ? nowhere : reinterpret_cast<uint64_t>(p.pool) + (uint64_t)((int64_t)row * p.pool_stride);
     };
     ask_id(0);
@@ -354,8 +370,10 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
     wait_copies<0>();
     ask_page(id_next);  // of the next group; its rows are taken, and the group after it asked for, when its first tile begins
     ask_id(2);
-    // copies of tile t into buffer t % 3, asked for in the order of the tiles
-    int32_t from, chunk;  // of the next copy: its row's lane in at_now (times 4, for the shuffle), its chunk of the row
+    // Copies of tile t into buffer t % 3, asked for in the order of the tiles:
+    // lane 4r + q takes chunks 4j + (q ^ (r / 4)) of row r, at last four scales of 16 rows.
+    uint64_t from, from_scale;
+    uint32_t to;
     auto begin_tile = [&](int32_t t) __attribute__((always_inline)) {
         if (t > 0 && t % GT == 0) {
             at_now = address(take_row(id_next));
@@ -364,27 +382,25 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
             ask_page(id_next);
             ask_id(t / GT + 2);
         }
-        const int32_t lane = 16 * g + c;
-        if (lane / RPW == t % GT) lds.hidden[buffer_of(t)][wave * RPW + lane % RPW] = at_now == nowhere ? -__builtin_inff() : 0.f;
-        from = 4 * (t % GT) * RPW + (lane < kChunks ? 0 : 4);
-        chunk = lane < kChunks ? lane : lane - kChunks;
-        asm volatile("" : "+v"(chunk));  // (found anew for every tile: kept for all copies, they spill)
+        const int32_t buf = buffer_of(t);
+        to = __builtin_amdgcn_readfirstlane(lds_offset(&lds.tile[buf][kRegion * wave]));
+        if (g == t % GT) lds.hidden[buf][RPW * wave + c] = at_now == nowhere ? -__builtin_inff() : 0.f;
+        auto of_row = [&](int32_t r) __attribute__((always_inline)) -> uint64_t {
+            const int at = 4 * (RPW * (t % GT) + r);
+            const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(at, (int)(uint32_t)at_now);
+            const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_bpermute(at, (int)(at_now >> 32));
+            return ((uint64_t)hi << 32) | lo;
+        };
+        from = of_row(4 * g + (c >> 2)) + (uint32_t)(16 * ((c & 3) ^ g));
+        from_scale = of_row(c) + (uint32_t)(kScaleAt + 4 * g);
     };
-    auto copy = [&](int32_t t, int j) __attribute__((always_inline)) {  // j = 0, 1, ... in order
-        const uint32_t to = lds_offset(&lds.tile[buffer_of(t)][wave * RPW * kRowBytes]);
-        const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)(uint32_t)at_now);
-        const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)(at_now >> 32));
-        const uint64_t a = (((uint64_t)hi << 32) | lo) + (uint32_t)(16 * chunk);
-        if (64 * j + 63 < RPW * kChunks || 16 * g + c < RPW * kChunks % kWave)
-            copy_to_lds(reinterpret_cast<const void*>(a), to + 1024 * j);
-        const bool wrap = chunk >= 2 * kChunks - kWave;  // 64 chunks on: one row and 23 chunks, or two and 18 less
-        from += wrap ? 8 : 4;
-        chunk += wrap ? kWave - 2 * kChunks : kWave - kChunks;
+    auto copy = [&](auto j) __attribute__((always_inline)) {
+        if constexpr (j.value < kCopies - 1) copy_block<j.value>(from, to);
+        else copy4_to_lds(reinterpret_cast<const void*>(from_scale), to + kScales);
     };
     auto copy_tile = [&](int32_t t) __attribute__((always_inline)) {
         begin_tile(t);
-#pragma unroll
-        for (int j = 0; j < COPIES; ++j) copy(t, j);
+        each_of<kCopies>(copy);
     };
     f32x4 acc[DT][PT];
 #pragma unroll
@@ -399,37 +415,26 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
     i32x2 v[2][DT];  // this wave's codes of the last tile, transposed: its buffer is free for the next copies
     // lanes 2r, 2r + 1 of a group hand in 16 columns of key 8g + r; lane c gets column c of its eight keys
     auto fetch = [&](int32_t t, int ks) __attribute__((always_inline)) {
-        const uint8_t* const at = lds.tile[buffer_of(t)] + (32 * ks + 8 * g + c / 2) * kRowBytes + wave * 128 + 8 * (c & 1);
+        const int32_t r = 8 * (g & 1) + (c >> 1);
+        const uint32_t at = lds_offset(lds.tile[buffer_of(t)]) + kRegion * (2 * ks + (g >> 1)) + 1024 * 2 * wave + 64 * r +
+                            16 * (r >> 2) + 8 * (c & 1);
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-            v[ks][d] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(at + 16 * d));
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int d = q; d < DT; d += 4)
+                v[ks][d] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                    (__attribute__((address_space(3))) i32x2*)((at ^ (16 * q)) + 1024 * (d / 4)));
     };
-    wait_barrier<2 * COPIES>();
+    wait_barrier<2 * kCopies>();
     fetch(0, 0);
     lds_barrier();
     fetch(0, 1);
 #pragma unroll 1
     for (int32_t t = 1; t <= tiles; ++t) {
         asm volatile("" : "+v"(g), "+v"(c));
-        wait_barrier<COPIES>();
+        wait_barrier<kCopies>();
         begin_tile(t + 2);
         Frag pf[2][PT];
-        // (a copy is held up at the memory's rate: they are spread over the products)
-        auto product = [&](int ks) __attribute__((always_inline)) {
-            Frag a[2];
-            a[0] = bf16_of_codes((uint32_t)v[ks][0][0], (uint32_t)v[ks][0][1]);
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-#pragma unroll
-                for (int h = 0; h < PT; ++h) {
-                    acc[d][h] = mfma16(a[d & 1], pf[ks][h], acc[d][h]);
-                    if (h == 0 && d + 1 < DT)
-                        a[(d + 1) & 1] = bf16_of_codes((uint32_t)v[ks][d + 1][0], (uint32_t)v[ks][d + 1][1]);
-                }
-                if (DT * ks + d < COPIES) copy(t + 2, DT * ks + d);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        };
         float keep[PT];
         bool any = false;
 #pragma unroll
@@ -449,6 +454,7 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
                 pf[ks][h].w[1] = pack_bf16(x[2] * a[2], x[3] * a[3]);
                 pf[ks][h].w[2] = pack_bf16(y[0] * b[0], y[1] * b[1]);
                 pf[ks][h].w[3] = pack_bf16(y[2] * b[2], y[3] * b[3]);
+                asm volatile("" : "+v"(pf[ks][h].u));  // (here, not where they are used)
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -457,15 +463,34 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
             for (int h = 0; h < PT; ++h)
 #pragma unroll
                 for (int d = 0; d < DT; ++d) acc[d][h] *= keep[h];
-        product(0);
+        // (a copy is held up at the memory's rate: they are spread over the products)
+        auto product = [&](auto ks) __attribute__((always_inline)) {
+            Frag a[2];
+            a[0] = bf16_of_codes((uint32_t)v[ks.value][0][0], (uint32_t)v[ks.value][0][1]);
+            each_of<DT>([&](auto d) __attribute__((always_inline)) {
+#pragma unroll
+                for (int h = 0; h < PT; ++h) {
+                    acc[d.value][h] = mfma16(a[d.value & 1], pf[ks.value][h], acc[d.value][h]);
+                    if (h == 0 && d.value + 1 < DT)
+                        a[(d.value + 1) & 1] = bf16_of_codes((uint32_t)v[ks.value][(d.value + 1) % DT][0],
+                                                             (uint32_t)v[ks.value][(d.value + 1) % DT][1]);
+                }
+                constexpr int j = DT * ks.value + d.value;
+                if constexpr (j < kCopies) copy(Number<j>{});
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        };
+        product(Number<0>{});
         fetch(t, 0);
         lds_barrier();
-        product(1);
+        product(Number<1>{});
         fetch(t, 1);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy is left in flight
+    wait_copies<0>();  // no copy is left in flight
+    if (lane == 0) lds.seen[wave] = seen;
     __syncthreads();
     const bool whole = it.parts == 1;
+    const bool none = !(lds.seen[0] | lds.seen[1] | lds.seen[2] | lds.seen[3]);  // no key attended
 #pragma unroll
     for (int ht = 0; ht < PT; ++ht) {
         const int32_t h = 16 * ht + c, head = head0 + h;
@@ -473,10 +498,9 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
         float sum = lds.total[0][h];
 #pragma unroll
         for (int k = 1; k < KQ; ++k) sum += lds.total[k][h];
-        const float top = lds.top[0][h];
-        const bool none = sum == 0.f;  // no key attended
+        const float top = none ? -__builtin_inff() : lds.top[0][h];
         if (whole) {
-            const float inv = none ? 0.f : 1.0f / sum;
+            const float inv = 1.0f / sum;
             uint16_t* out = p.out + it.row * p.o_row + head * p.o_head + wave * 128 + 4 * g;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
@@ -484,14 +508,14 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
                     none ? u32x2{0, 0} : u32x2{pack_bf16(acc[d][ht][0] * inv, acc[d][ht][1] * inv),
                                                pack_bf16(acc[d][ht][2] * inv, acc[d][ht][3] * inv)};
             if (p.lse && wave == 0 && g == 0)
-                p.lse[(int64_t)it.row * p.heads + head] =
-                    none ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+                p.lse[(int64_t)it.row * p.heads + head] = none ? top : (top + __builtin_amdgcn_logf(sum)) * kLn2;
         } else {
             const int64_t at = (int64_t)index * p.heads + head;
             float* o = p.parts.sums + at * kLatent + wave * 128 + 4 * g;
 #pragma unroll
-            for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(o + 16 * d) = acc[d][ht];
-            if (wave == 0 && g == 0) p.parts.stats[at] = f32x2{top, sum};
+            for (int d = 0; d < DT; ++d)
+                *reinterpret_cast<f32x4*>(o + 16 * d) = none ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[d][ht];
+            if (wave == 0 && g == 0) p.parts.stats[at] = f32x2{top, none ? 0.f : sum};
         }
     }
 }
