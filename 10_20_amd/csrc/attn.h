@@ -15,6 +15,10 @@ using i32x2 = __attribute__((ext_vector_type(2))) int;
 using u32x2 = __attribute__((ext_vector_type(2))) uint32_t;
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 
+// The maximum that is subtracted may lag the true one by 2^kLag: sums are
+// rescaled only past that (probabilities keep their relative precision; at 2^6
+// every third tile of 64 heads had a head to rescale, 4% of the time).
+constexpr float kLag = 16.f;
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 
 union Frag {

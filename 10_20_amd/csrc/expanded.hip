@@ -23,7 +23,6 @@ using namespace attn;
 
 constexpr int kKey = 128, kValue = 128, kRopeDims = 64;
 constexpr int kRows = 32;  // queries of a wave
-constexpr float kLag = 6.f;  // the subtracted maximum may lag the true one by 2^6
 
 using f32x16 = __attribute__((ext_vector_type(16))) float;
 using i16x4 = __attribute__((ext_vector_type(4))) short;

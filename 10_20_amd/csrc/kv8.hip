@@ -11,7 +11,6 @@ using namespace attn;
 
 constexpr int kDim = 128;
 constexpr int kMaxGroup = 16;  // query heads of a KV head: the columns of a fragment
-constexpr float kLag = 6.f;    // the subtracted maximum may lag the true one by 2^6
 
 // ------------------------------------------------------------------ store
 // A work-group appends the tokens of one request that fall into one page, for

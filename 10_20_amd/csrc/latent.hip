@@ -81,7 +81,6 @@ struct AbsorbedParams {
 // The row of keys that are not attended (their scores are -inf).
 __device__ const u32x4 zero_latent[kChunks] = {};
 
-constexpr float kLag = 6.f;  // the subtracted maximum may lag the true one by 2^6
 
 // A tile in LDS: 16-row regions; in a region the rows' chunks of 16 bytes in
 // blocks of four, chunk 4j + q of row r at 1024 j + 64 r + 16 (q ^ (r / 4)), then
