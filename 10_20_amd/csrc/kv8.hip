@@ -139,6 +139,7 @@ struct Kv8Params {
     int64_t ids_stride;
     Plan plan;
     int32_t kv_heads, group, spread;
+    int32_t together;  // KV heads of a work-group: 1, 2 or 4
     float scale2;
     uint16_t* out;
     int64_t o_row, o_head;
@@ -161,9 +162,10 @@ struct Kv8Lds {
     float top[kWaves][kMaxGroup], total[kWaves][kMaxGroup];
 };
 
-// A work-group attends one KV head of a row over one part of its keys; its waves
-// take the part's tiles of 64 keys in turn, each with its own running maximum,
-// and join through LDS.
+// A work-group attends one, two or four KV heads of a row over one part of its
+// keys, a wave each; waves of one head take the part's tiles of 64 keys in turn,
+// each with its own running maximum, and join through LDS.  (The rows of a
+// token's heads lie side by side: four heads in step read them in one go.)
 //   scores  S^T = K Q^T (v_mfma_f32_16x16x32_bf16): K codes come straight into
 //           registers (lane = key % 16, 32 of its 128 codes), exact in bf16; column
 //           c is query head c of the group.
@@ -176,11 +178,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_attend_kernel(Kv8Params p)
     const int32_t wave = __builtin_amdgcn_readfirstlane((int32_t)threadIdx.x / kWave);
     const int32_t lane = (int32_t)threadIdx.x % kWave, g = lane >> 4, c = lane & 15;
     int32_t index = ((int32_t)blockIdx.x % 8) * p.spread + (int32_t)blockIdx.x / 8;
-    const int32_t kvh = index % p.kv_heads;
-    index /= p.kv_heads;
+    const int32_t sets = p.kv_heads / p.together, set = index % sets;
+    index /= sets;
     Item it;
     if (!find_item(p.plan, index, it)) return;
-    const int32_t mine = (it.tiles - wave + kWaves - 1) / kWaves;  // this wave's tiles: wave, wave + 4, ...
+    const int32_t streams = kWaves / p.together, stream = wave / p.together, kvh = set * p.together + wave % p.together;
+    const int32_t mine = (it.tiles - stream + streams - 1) / streams;  // this wave's tiles: stream, stream + streams, ...
     const int32_t* ids = p.ids ? p.ids + it.row * p.ids_stride : nullptr;
     const int32_t* table = p.table + it.row * p.table_stride;
     const uint8_t* kb = p.pool[0] + kvh * p.head[0];
@@ -188,7 +191,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_attend_kernel(Kv8Params p)
 
     // the lane's key of the wave's tile t: its id, then its page
     auto fetch_id = [&](int32_t t) __attribute__((always_inline)) -> int32_t {
-        const int32_t j = (it.first + wave + kWaves * t) * kTileKeys + lane;
+        const int32_t j = (it.first + stream + streams * t) * kTileKeys + lane;
         if (t >= mine || j >= it.keys) return -1;
         return ids ? ids[j] : j;
     };
@@ -341,15 +344,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_attend_kernel(Kv8Params p)
         lds.total[wave][c] = total;
     }
     __syncthreads();
-    for (int32_t i = (int32_t)threadIdx.x; i < p.group * (kDim / 2); i += 64 * kWaves) {
-        const int32_t h = i / (kDim / 2), dim = 2 * (i % (kDim / 2)), head = kvh * p.group + h;
-        float top = lds.top[0][h];
-#pragma unroll
-        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, lds.top[w][h]);
+    for (int32_t i = (int32_t)threadIdx.x; i < p.together * p.group * (kDim / 2); i += 64 * kWaves) {
+        const int32_t row = i / (kDim / 2), dim = 2 * (i % (kDim / 2)), sub_head = row / p.group, h = row % p.group;
+        const int32_t head = set * p.together * p.group + row;
+        float top = -__builtin_inff();
+        for (int32_t w = sub_head; w < kWaves; w += p.together) top = fmaxf(top, lds.top[w][h]);
         const float sub = top == -__builtin_inff() ? 0.f : top;
         float sum = 0.f, o0 = 0.f, o1 = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int32_t w = sub_head; w < kWaves; w += p.together) {
             const float f = __builtin_amdgcn_exp2f(lds.top[w][h] - sub);
             sum = fmaf(f, lds.total[w][h], sum);
             o0 = fmaf(f, lds.u[w].out[h][dim], o0);
@@ -371,12 +373,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_attend_kernel(Kv8Params p)
     }
 }
 
+// KV heads of a work-group.
+inline int32_t kv8_together(int32_t kv_heads) { return kv_heads % 4 == 0 ? 4 : kv_heads % 2 == 0 ? 2 : 1; }
+
 // (Two work-groups a CU, a tile of each wave at a time.)
 inline Plan kv8_plan(const int32_t* lens, int32_t rows, int32_t kv_heads, int32_t keys, bool ragged) {
-    const int64_t steps = cdiv(cdiv(keys, kTileKeys), kWaves), slots = std::max<int64_t>(1, 2 * device_cus() / kv_heads);
+    const int64_t together = kv8_together(kv_heads), streams = kWaves / together, steps = cdiv(cdiv(keys, kTileKeys), streams);
+    const int64_t slots = std::max<int64_t>(1, 2 * device_cus() * together / kv_heads);
     Plan p{lens, rows, keys, 0, 0};
     if (ragged && rows <= kPlanRows && rows < slots) p.target = (int32_t)std::max(slots - rows, (slots + 1) / 2);
-    else p.chunk = kWaves * chunk_for(rows, steps, slots, 2, 1);
+    else p.chunk = (int32_t)streams * chunk_for(rows, steps, slots, 2, 1);
     return p;
 }
 
@@ -438,7 +444,8 @@ extern "C" int v1_kv8_attend(const v1_kv8_attend_args* a, void* stream) {
     if (rows == 0) return V1_OK;
     if (pages == 0 || table_len == 0) keys = 0;
     const Plan plan = kv8_plan(lens, rows, kv_heads, keys, lens != nullptr);
-    const int64_t items = items_at_most(plan), spread = cdiv(items * kv_heads, 8);
+    const int32_t together = kv8_together(kv_heads);
+    const int64_t items = items_at_most(plan), spread = cdiv(items * (kv_heads / together), 8);
     const int64_t need = v1_kv8_attend_workspace(rows, kv_heads, group, keys, lens != nullptr);
     V1_REQUIRE(workspace_bytes >= need && (need == 0 || workspace != nullptr),
                "kv8_attend: workspace of %lld bytes needed", (long long)need);
@@ -448,7 +455,7 @@ extern "C" int v1_kv8_attend(const v1_kv8_attend_args* a, void* stream) {
                 {static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool)},
                 {kp_page, vp_page}, {kp_token, vp_token}, {kp_head, vp_head},
                 {k_scale, v_scale}, {ks_page, vs_page}, pages, table, table_stride, table_len, ids, ids_stride, plan,
-                kv_heads, group, (int32_t)spread, scale * kLog2e, static_cast<uint16_t*>(out), o_row, o_head, lse,
+                kv_heads, group, (int32_t)spread, together, scale * kLog2e, static_cast<uint16_t*>(out), o_row, o_head, lse,
                 parts_at(workspace, items, heads, kDim)};
     static OncePerDevice once;
     int rc = allow_lds(once, reinterpret_cast<const void*>(kv8_attend_kernel), sizeof(Kv8Lds), "kv8_attend: LDS");
