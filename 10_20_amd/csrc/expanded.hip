@@ -5,15 +5,22 @@
 // query i of a sequence of nq queries and nk keys sees keys j <= nk - nq + i
 // (causal) or all.
 //
-// A work-group of NW waves takes 32 * NW queries of one head; each wave its own
-// 32, as columns of v_mfma_f32_32x32x16_bf16:
+// A work-group of 8 waves takes 256 queries of one head; each wave its own 32, as
+// columns of v_mfma_f32_32x32x16_bf16:
 //   scores  S^T = K Q^T, a tile of 64 keys at a time from LDS;
 //   output  O^T = V^T P^T: a lane's scores are already the probabilities of its
 //           B fragment (the key order inside 16 keys is chosen so), rounded to
 //           bf16 once; V comes transposed from LDS (ds_read_b64_tr_b16).
 // Scores, maxima and sums stay fp32, exponentials are base 2.  Tiles come memory
-// -> LDS two deep; rows are laid with their 16-byte chunks XORed by the row so
+// -> LDS two ahead; rows are laid with their 16-byte chunks XORed by the row so
 // that the fragments' reads meet different banks.
+//
+// Bound by the matrix units: 16 heads of 4096 queries over 32768 keys take 1232 us,
+// 1046 TFLOP/s (an 8192^3 library product: 1210).  With both waves of a SIMD in
+// the same step, matrix products and exponentials took turns: 1336 us.  Work-groups
+// of 128 queries, two to a CU: 1800 us there, 326 against 312 us for 32 sequences
+// of 100 queries and 4096 keys, and ahead only below some 300 keys a sequence
+// (64 sequences of 300, 8 heads: 70 against 78 us).
 #include "attn.h"
 
 namespace v1 {
@@ -23,6 +30,8 @@ using namespace attn;
 
 constexpr int kKey = 128, kValue = 128, kRopeDims = 64;
 constexpr int kRows = 32;  // queries of a wave
+constexpr int kWaves = 8, kBlock = kWaves * kRows;  // of a work-group
+constexpr int kBuffers = 4;  // tiles in LDS: all of its 160 KB
 
 using f32x16 = __attribute__((ext_vector_type(16))) float;
 using i16x4 = __attribute__((ext_vector_type(4))) short;
@@ -37,7 +46,7 @@ struct ExpandedParams {
     const int32_t* cu_q;
     const int32_t* cu_k;
     int32_t tokens, keys, batch, heads, blocks;  // blocks: of queries, of the longest sequence
-    int32_t causal, parts, by_pair;
+    int32_t causal, parts, xcds, group;
     float scale2;
     uint16_t* out;
     int64_t o_row, o_head;
@@ -121,31 +130,28 @@ __device__ __forceinline__ void careful_product(f32x16 (&sums)[4], const Frag (&
 // which an infinite or NaN value would turn into NaN in the product: sums that
 // end up not finite (true is returned, nothing written) are found again by the
 // CAREFUL form.
-template <int NW, int NB, bool CAREFUL>
+template <bool CAREFUL>
 __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedTile* lds) {
-    constexpr int COPIES = (int)(sizeof(ExpandedTile) / 1024) / NW;
+    constexpr int COPIES = (int)(sizeof(ExpandedTile) / 1024) / kWaves;
     const int32_t wave = __builtin_amdgcn_readfirstlane((int32_t)threadIdx.x / kWave);
     const int32_t lane = (int32_t)threadIdx.x % kWave, c = lane & 31, h = lane >> 5;
 
-    // Work-groups reach the XCDs in turn.  Each takes whole (sequence, head) pairs
-    // where they divide evenly, so that blocks of the same keys meet in one L2;
-    // longest blocks first.
-    const int32_t per = p.blocks * p.parts;
-    int32_t index = (int32_t)blockIdx.x, at = index % per;
-    if (p.by_pair) {
-        const int32_t turn = index / 8;
-        at = turn % per;
-        index = turn / per * 8 + index % 8;
-    } else {
-        index /= per;
-    }
+    // Work-groups reach the XCDs in turn.  An XCD takes whole (sequence, head)
+    // pairs, `group` of them at a time: the group's blocks longest first, so that
+    // the last ones to end are short and blocks of the same keys meet in one L2.
+    // Of 4 sequences of 4096, 32 heads: a pair at a time 803 us, so 740; of 2 times
+    // 4096 queries, 16384 keys, 128 heads: all pairs at a time 10290 us, so 9200.
+    const int32_t per = p.blocks * p.parts, pairs = ((int32_t)p.batch * p.heads + p.xcds - 1) / p.xcds;
+    const int32_t turn = (int32_t)blockIdx.x / p.xcds, before = turn / (p.group * per) * p.group;
+    const int32_t size = min(p.group, pairs - before), within = turn - before * per, at = within / size;
+    const int32_t index = (before + within % size) * p.xcds + (int32_t)blockIdx.x % p.xcds;
     const int32_t part = at % p.parts, block = p.blocks - 1 - at / p.parts;
     const int32_t head = index % p.heads, b = index / p.heads;
     if (b >= p.batch) return false;
     const int32_t q_lo = min(max(p.cu_q[b], 0), p.tokens), q_hi = min(max(p.cu_q[b + 1], q_lo), p.tokens);
     const int32_t k_lo = min(max(p.cu_k[b], 0), p.keys), k_hi = min(max(p.cu_k[b + 1], k_lo), p.keys);
     const int32_t nq = q_hi - q_lo, nk = k_hi - k_lo;
-    const int32_t q0 = block * kRows * NW;
+    const int32_t q0 = block * kBlock;
     if (q0 >= nq) return false;
 
     // keys that query i sees: the first seen(i)
@@ -153,16 +159,16 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedT
     const int32_t i0 = q0 + wave * kRows;                                // this wave's first query
     const int32_t my_seen = seen(min(i0 + c, nq - 1));
     const int32_t wave_least = i0 < nq ? seen(i0) : 0, wave_most = i0 < nq ? seen(min(i0 + kRows, nq) - 1) : 0;
-    const int32_t all_tiles = tiles_of(seen(min(q0 + kRows * NW, nq) - 1));
+    const int32_t all_tiles = tiles_of(seen(min(q0 + kBlock, nq) - 1));
     const int32_t each = (all_tiles + p.parts - 1) / p.parts;
     const int32_t first = min(part * each, all_tiles), tiles = min(each, all_tiles - first);
 
     auto copy_tile = [&](int32_t t) __attribute__((always_inline)) {
-        ExpandedTile& to = lds[t % NB];
+        ExpandedTile& to = lds[t % kBuffers];
         const int32_t k0 = (first + t) * kTileKeys;
 #pragma unroll
         for (int j = 0; j < COPIES; ++j) {
-            const int32_t i = j * NW + wave;
+            const int32_t i = j * kWaves + wave;
             if (i < 32) {  // keys (16 copies of 4 rows), then values
                 const int32_t r = 4 * (i & 15) + (lane >> 4), at = lane & 15;
                 const int32_t chunk = i < 16 ? at ^ (r & 15) : 16 + (at ^ (4 * (r & 3)));
@@ -176,7 +182,7 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedT
             }
         }
     };
-    for (int t = 0; t < NB - 1; ++t)
+    for (int t = 0; t < 2; ++t)
         if (t < tiles) copy_tile(t);
 
     // B fragments of Q^T: column c = query i0 + c
@@ -186,23 +192,19 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedT
 #pragma unroll
         for (int s = 0; s < 12; ++s) q[s].u = *reinterpret_cast<const u32x4*>(src + 16 * s);
     }
-    f32x16 acc[4];
+    f32x16 acc[4], s[2];
+    Frag pf[4];
     float mx = -__builtin_inff(), total = 0.f;
-
 #pragma unroll
     for (int d = 0; d < 4; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
-#pragma unroll 1
-    for (int32_t t = 0; t < tiles; ++t) {
-        if (NB > 2 && t + 1 < tiles) wait_barrier<(NB - 2) * COPIES>();
-        else wait_barrier<0>();
-        if (t + NB - 1 < tiles) copy_tile(t + NB - 1);
-        const int32_t k0 = (first + t) * kTileKeys;
-        if (k0 >= wave_most) continue;
-        const ExpandedTile& tile = lds[t % NB];
-        // scores: register i of half u is key 32u + 8 (i / 4) + 4h + i % 4
-        f32x16 s[2];
+    auto first_key = [&](int32_t t) __attribute__((always_inline)) { return (first + t) * kTileKeys; };
+    // a key of the tile that a query of the wave does not see
+    auto is_masked = [&](int32_t t) __attribute__((always_inline)) { return first_key(t) + kTileKeys > wave_least; };
+    // scores: register i of half u is key 32u + 8 (i / 4) + 4h + i % 4
+    auto scores = [&](int32_t t) __attribute__((always_inline)) {
+        const ExpandedTile& tile = lds[t % kBuffers];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
@@ -221,9 +223,10 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedT
                 s[u] = mfma32(k, q[8 + st], s[u]);
             }
         }
-        const bool masked = k0 + kTileKeys > wave_least;  // a key of the tile that a query of the wave does not see
-        if (masked) {
-            const int32_t left = my_seen - k0 - 4 * h;
+    };
+    auto softmax = [&](int32_t t) __attribute__((always_inline)) {
+        if (is_masked(t)) {
+            const int32_t left = my_seen - first_key(t) - 4 * h;
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -252,28 +255,64 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedT
                 s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], p.scale2, -sub));
                 total += s[u][i];
             }
-        Frag pf[4];
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 pf[kk].w[i] = pack_bf16(s[kk / 2][8 * (kk & 1) + 2 * i], s[kk / 2][8 * (kk & 1) + 2 * i + 1]);
-        if (CAREFUL && masked) {
-            careful_product(acc, pf, tile, my_seen - k0 - 4 * h);
+    };
+    auto products = [&](int32_t t) __attribute__((always_inline)) {
+        const ExpandedTile& tile = lds[t % kBuffers];
+        if (CAREFUL && is_masked(t)) {
+            careful_product(acc, pf, tile, my_seen - first_key(t) - 4 * h);
         } else {
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
                 for (int d = 0; d < 4; ++d) acc[d] = mfma32(values(tile, kk, d), pf[kk], acc[d]);
         }
+    };
+    const int32_t mine = min(tiles, max(tiles_of(wave_most) - first, 0));  // tiles that the wave sees something of
+    // The two waves of a SIMD half a tile apart: one multiplies (the last tile's
+    // values, this one's keys) while the other makes probabilities.  Half-steps
+    // are divided by barriers; the even ones begin with tile `to_come` in LDS and
+    // the one after the next asked for, whose buffer was read until the last.
+    const bool second = wave >= kWaves / 2;
+    auto sync = [&](bool even, int32_t to_come) __attribute__((always_inline)) {
+        if (even) {
+            if (to_come + 1 < tiles) wait_barrier<COPIES>();
+            else wait_barrier<0>();
+            if (to_come + 2 < tiles) copy_tile(to_come + 2);
+        } else {
+            lds_barrier();
+        }
+    };
+    if (second) sync(true, 0);
+#pragma unroll 1
+    for (int32_t t = 0; t <= tiles; ++t) {
+        sync(!second, t);
+        if (t > 0 && t <= mine) products(t - 1);
+        if (t < mine) scores(t);
+        sync(second, t + 1);
+        if (t < mine) softmax(t);
     }
+    if (!second) lds_barrier();
     if constexpr (!CAREFUL) {
         float odd = 0.f;  // NaN if a sum is not finite
 #pragma unroll
         for (int d = 0; d < 4; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) odd = fmaf(acc[d][i], 0.f, odd);
-        if (__syncthreads_or(odd != odd)) return true;
+        int32_t* const flag = reinterpret_cast<int32_t*>(lds);
+        __syncthreads();
+        if (threadIdx.x == 0) *flag = 0;
+        __syncthreads();
+        if (odd != odd) *flag = 1;
+        __syncthreads();
+        if (*flag != 0) {
+            __syncthreads();
+            return true;
+        }
     }
     total += __shfl_xor(total, 32, kWave);
     const int32_t i = i0 + c;
@@ -307,43 +346,29 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedT
 }
 
 // (A call, so that its registers are not the common form's.)
-template <int NW, int NB>
 __device__ __attribute__((noinline)) void careful_part(ExpandedParams p, ExpandedTile* lds) {
-    expanded_part<NW, NB, true>(p, lds);
+    expanded_part<true>(p, lds);
 }
 
-template <int NW, int NB>
-__global__ __launch_bounds__(64 * NW, 2) void expanded_kernel(ExpandedParams p) {
+__global__ __launch_bounds__(64 * kWaves, 2) void expanded_kernel(ExpandedParams p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
     ExpandedTile* const lds = reinterpret_cast<ExpandedTile*>(lds_raw);
-    if (__builtin_expect(expanded_part<NW, NB, false>(p, lds), 0)) careful_part<NW, NB>(p, lds);
+    if (__builtin_expect(expanded_part<false>(p, lds), 0)) careful_part(p, lds);
 }
 
-// Waves of a work-group and parts of the keys: 256 queries where that gives
-// every CU a work-group, else 128; parts where 128 do not either.
+// Blocks of queries, and the parts that the keys are cut into where the blocks
+// leave CUs without one (of four tiles or more each).
 struct ExpandedShape {
-    int32_t waves, blocks, parts;
+    int32_t blocks, parts;
 };
 
 inline ExpandedShape expanded_shape(int32_t tokens, int32_t keys, int32_t batch, int32_t heads, int32_t max_q) {
-    const int64_t cus = device_cus();
     ExpandedShape s;
-    s.waves = (int64_t)heads * (tokens / (8 * kRows)) >= cus ? 8 : 4;
-    s.blocks = (int32_t)cdiv(max_q, s.waves * kRows);
-    const int64_t groups = std::min((int64_t)batch * s.blocks, batch + cdiv(tokens, s.waves * kRows)) * heads;
+    s.blocks = (int32_t)cdiv(max_q, kBlock);
+    const int64_t groups = std::min((int64_t)batch * s.blocks, batch + cdiv(tokens, kBlock)) * heads;
     const int64_t tiles = cdiv(keys, kTileKeys);
-    s.parts = (int32_t)std::max<int64_t>(1, std::min(2 * cus / std::max<int64_t>(1, groups), tiles / (4 * batch)));
+    s.parts = (int32_t)std::max<int64_t>(1, std::min(device_cus() / std::max<int64_t>(1, groups), tiles / (4 * batch)));
     return s;
-}
-
-template <int NW, int NB>
-int launch_expanded(const ExpandedParams& p, int64_t blocks, hipStream_t st) {
-    static OncePerDevice once;
-    constexpr size_t bytes = NB * sizeof(ExpandedTile);
-    const int rc = allow_lds(once, reinterpret_cast<const void*>(expanded_kernel<NW, NB>), bytes, "latent_expanded: LDS");
-    if (rc != V1_OK) return rc;
-    hipLaunchKernelGGL((expanded_kernel<NW, NB>), dim3((uint32_t)blocks), dim3(64 * NW), bytes, st, p);
-    return V1_LAUNCHED("latent_expanded");
 }
 
 }  // namespace
@@ -374,15 +399,24 @@ extern "C" int v1_latent_expanded(const v1_latent_expanded_args* a, void* stream
     const int64_t need = v1_latent_expanded_workspace(tokens, keys, batch, heads, max_q);
     V1_REQUIRE(workspace_bytes >= need && (need == 0 || workspace != nullptr),
                "latent_expanded: workspace of %lld bytes needed", (long long)need);
-    const int64_t pairs = (int64_t)batch * heads, by_pair = pairs % 8 == 0 || pairs >= 64;
-    const int64_t items = (by_pair ? 8 * cdiv(pairs, 8) : pairs) * s.blocks * s.parts;
-    V1_REQUIRE(items < 1ll << 30, "latent_expanded: too many work items");
+    // XCD by XCD where that leaves few of them short of work; groups of two
+    // work-groups for each of an XCD's CUs
+    const int64_t pairs = (int64_t)batch * heads;
+    const int32_t xcds = pairs % 8 == 0 || pairs >= 64 ? 8 : 1;
+    const int64_t items = cdiv(pairs, xcds) * xcds * s.blocks * s.parts;
+    V1_REQUIRE(pairs < 1ll << 30 && items < 1ll << 30, "latent_expanded: too many work items");
+    const int64_t group = std::min(cdiv(pairs, xcds), cdiv(2 * device_cus() / xcds, (int64_t)s.blocks * s.parts));
     ExpandedParams p{static_cast<const uint16_t*>(q), q_row, q_head, static_cast<const uint16_t*>(kv), kv_row, kv_head,
                      static_cast<const uint16_t*>(rope), rope_row, cu_q, cu_k, tokens, keys, batch, heads, s.blocks,
-                     causal, s.parts, (int32_t)by_pair, scale * kLog2e, static_cast<uint16_t*>(out), o_row, o_head, lse,
+                     causal, s.parts, xcds, (int32_t)group, scale * kLog2e, static_cast<uint16_t*>(out), o_row, o_head, lse,
                      parts_at(workspace, (int64_t)tokens * s.parts, heads, kValue)};
     const hipStream_t st = as_stream(stream);
-    const int rc = s.waves == 8 ? launch_expanded<8, 3>(p, items, st) : launch_expanded<4, 2>(p, items, st);
+    static OncePerDevice once;
+    constexpr size_t bytes = kBuffers * sizeof(ExpandedTile);
+    int rc = allow_lds(once, reinterpret_cast<const void*>(expanded_kernel), bytes, "latent_expanded: LDS");
+    if (rc != V1_OK) return rc;
+    hipLaunchKernelGGL(expanded_kernel, dim3((uint32_t)items), dim3(64 * kWaves), bytes, st, p);
+    rc = V1_LAUNCHED("latent_expanded");
     if (rc != V1_OK || s.parts == 1) return rc;
     // (as rows of s.parts one-tile parts)
     JoinParams j{Plan{nullptr, tokens, s.parts * kTileKeys, 1, 0}, p.partial, p.out, o_row, o_head, lse, heads, cu_q, batch};
