@@ -15,12 +15,13 @@
 // -> LDS two ahead; rows are laid with their 16-byte chunks XORed by the row so
 // that the fragments' reads meet different banks.
 //
-// Bound by the matrix units: 16 heads of 4096 queries over 32768 keys take 1232 us,
-// 1046 TFLOP/s (an 8192^3 library product: 1210).  With both waves of a SIMD in
-// the same step, matrix products and exponentials took turns: 1336 us.  Work-groups
-// of 128 queries, two to a CU: 1800 us there, 326 against 312 us for 32 sequences
-// of 100 queries and 4096 keys, and ahead only below some 300 keys a sequence
-// (64 sequences of 300, 8 heads: 70 against 78 us).
+// Bound by the matrix units: 16 heads of 4096 queries over 32768 keys take 1187 us,
+// 1087 TFLOP/s (an 8192^3 library product: 1210).  With both waves of a SIMD in
+// the same step, matrix products and exponentials took turns: 1336 us; with the
+// fragments' reads where the compiler puts them, 1232.  Work-groups of 128 queries,
+// two to a CU: 1800 us, 326 against 312 us for 32 sequences of 100 queries and 4096
+// keys, and ahead only below some 300 keys a sequence (64 sequences of 300, 8 heads:
+// 70 against 78 us).
 #include "attn.h"
 
 namespace v1 {
@@ -62,6 +63,18 @@ struct ExpandedTile {
 
 __device__ __forceinline__ f32x16 mfma32(const Frag& a, const Frag& b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, c, 0, 0, 0);
+}
+
+// Reads of LDS, EACH for one matrix product, kAhead products before it.
+constexpr int kAhead = 4;
+template <int N, int EACH>
+__device__ __forceinline__ void reads_ahead() {
+    __builtin_amdgcn_sched_group_barrier(0x100, EACH * kAhead, 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (i + kAhead < N) __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);
+    }
 }
 
 // A fragment of V^T, rows 32 d .., of 16 keys 16 kk ..: lanes 4r .. 4r + 3 of a
@@ -182,9 +195,6 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedT
             }
         }
     };
-    for (int t = 0; t < 2; ++t)
-        if (t < tiles) copy_tile(t);
-
     // B fragments of Q^T: column c = query i0 + c
     Frag q[12];
     {
@@ -192,6 +202,11 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedT
 #pragma unroll
         for (int s = 0; s < 12; ++s) q[s].u = *reinterpret_cast<const u32x4*>(src + 16 * s);
     }
+    for (int t = 0; t < 2; ++t)
+        if (t < tiles) copy_tile(t);
+    // (or the loop waits for them, and with them for its copies)
+#pragma unroll
+    for (int s = 0; s < 12; ++s) asm volatile("" : "+v"(q[s].u));
     f32x16 acc[4], s[2];
     Frag pf[4];
     float mx = -__builtin_inff(), total = 0.f;
@@ -206,23 +221,20 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedT
     auto scores = [&](int32_t t) __attribute__((always_inline)) {
         const ExpandedTile& tile = lds[t % kBuffers];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
-            const int32_t r = 32 * u + c;
 #pragma unroll
-            for (int st = 0; st < 8; ++st) {
+        for (int st = 0; st < 12; ++st)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int32_t r = 32 * u + c;
                 Frag k;
-                k.u = *reinterpret_cast<const u32x4*>(&tile.key[r][16 * ((2 * st + h) ^ (r & 15))]);
+                k.u = *reinterpret_cast<const u32x4*>(st < 8 ? &tile.key[r][16 * ((2 * st + h) ^ (r & 15))]
+                                                             : &tile.rope[r][16 * ((2 * st - 16 + h) ^ (r & 7))]);
                 s[u] = mfma32(k, q[st], s[u]);
             }
-#pragma unroll
-            for (int st = 0; st < 4; ++st) {
-                Frag k;
-                k.u = *reinterpret_cast<const u32x4*>(&tile.rope[r][16 * ((2 * st + h) ^ (r & 7))]);
-                s[u] = mfma32(k, q[8 + st], s[u]);
-            }
-        }
+        reads_ahead<24, 1>();
     };
     auto softmax = [&](int32_t t) __attribute__((always_inline)) {
         if (is_masked(t)) {
@@ -270,6 +282,7 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedT
             for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
                 for (int d = 0; d < 4; ++d) acc[d] = mfma32(values(tile, kk, d), pf[kk], acc[d]);
+            reads_ahead<16, 2>();
         }
     };
     const int32_t mine = min(tiles, max(tiles_of(wave_most) - first, 0));  // tiles that the wave sees something of
