@@ -95,7 +95,7 @@ __device__ __forceinline__ uint32_t lds_offset(const void* p) {
 
 // 16 bytes per lane, memory -> LDS at `lds` + 16 * lane (`lds` the same for the
 // wave).  Written as asm so that the compiler puts no waits of its own before
-// LDS reads; they are counted by the caller (vm_wait).  There is no output
+// LDS reads; the caller waits for them (wait_copies, wait_barrier).  There is no output
 // register that could be reused while the copy is in flight.
 __device__ __forceinline__ void copy_to_lds(const void* src, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
@@ -137,6 +137,7 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 //              from the lengths.
 constexpr int kTileKeys = 64;
 constexpr int kPlanRows = 256;
+constexpr int32_t kMostKeys = INT32_MAX - kTileKeys;  // (the last tile's positions stay below 2^31)
 
 struct Plan {
     const int32_t* lens;  // NULL: `keys` keys in every row
@@ -243,6 +244,9 @@ __device__ __forceinline__ void items_of(const Plan& p, int32_t row, int32_t& fi
     parts = __shfl(mine, row >> 2, kWave);
 }
 
+// Whether the device's lengths may decide: few rows, and their tiles can be added in 32 bits.
+inline bool planned(int64_t rows, int64_t tiles) { return rows <= kPlanRows && rows * tiles < 1ll << 30; }
+
 // Most work items that a call can have.
 inline int64_t items_at_most(const Plan& p) {
     if (p.chunk > 0) return (int64_t)p.rows * std::max<int64_t>(1, cdiv(cdiv(p.keys, kTileKeys), p.chunk));
@@ -284,8 +288,10 @@ struct JoinParams {
     int64_t o_row, o_head;
     float* lse;
     int32_t heads;
-    const int32_t* cu;  // not NULL: rows outside [cu[0], cu[batch]) are left as they are
-    int32_t batch;
+    // not NULL: only rows cu[b] .. min(cu[b + 1], cu[b] + most) - 1 have parts (the ends
+    // taken within [0, rows]); the others are left as they are
+    const int32_t* cu;
+    int32_t batch, most;
 };
 
 // One work-group per (row, head): D / 4 threads add four dims of every (1024 / D)-th
@@ -299,7 +305,14 @@ __global__ __launch_bounds__(256) void join_kernel(JoinParams p) {
     __shared__ float totals[G];
     const int32_t row = (int32_t)blockIdx.x, h = (int32_t)blockIdx.y, lane = (int32_t)threadIdx.x % kWave;
     const int32_t group = (int32_t)threadIdx.x / T, at4 = (int32_t)threadIdx.x % T;
-    if (p.cu && (row < p.cu[0] || row >= p.cu[p.batch])) return;
+    if (p.cu) {
+        int mine = 0;
+        for (int32_t b = (int32_t)threadIdx.x; b < p.batch; b += 256) {
+            const int32_t lo = min(max(p.cu[b], 0), p.plan.rows), hi = min(max(p.cu[b + 1], lo), p.plan.rows);
+            mine |= row >= lo && row < hi && row - lo < p.most;
+        }
+        if (!__syncthreads_or(mine)) return;
+    }
     int32_t first, parts;
     items_of(p.plan, row, first, parts);
     if (parts <= 1) return;

@@ -402,6 +402,7 @@ extern "C" int v1_latent_expanded(const v1_latent_expanded_args* a, void* stream
           workspace_bytes, tokens, keys, batch, heads, max_q, causal, scale] = *a;
     V1_REQUIRE(tokens >= 0 && keys >= 0 && batch >= 0 && heads > 0 && max_q >= 0, "latent_expanded: bad shape");
     V1_REQUIRE(heads < 1 << 16, "latent_expanded: too many heads");
+    V1_REQUIRE(keys <= kMostKeys && tokens <= kMostKeys, "latent_expanded: too many tokens or keys");
     V1_REQUIRE(scale > 0.f && scale < __builtin_inff(), "latent_expanded: scale must be positive and finite");
     const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kv) | reinterpret_cast<uintptr_t>(rope);
     V1_REQUIRE(all % 16 == 0 && (q_row | q_head | kv_row | kv_head | rope_row) % 8 == 0 &&
@@ -432,7 +433,8 @@ extern "C" int v1_latent_expanded(const v1_latent_expanded_args* a, void* stream
     rc = V1_LAUNCHED("latent_expanded");
     if (rc != V1_OK || s.parts == 1) return rc;
     // (as rows of s.parts one-tile parts)
-    JoinParams j{Plan{nullptr, tokens, s.parts * kTileKeys, 1, 0}, p.partial, p.out, o_row, o_head, lse, heads, cu_q, batch};
+    JoinParams j{Plan{nullptr, tokens, s.parts * kTileKeys, 1, 0}, p.partial, p.out, o_row, o_head, lse, heads, cu_q, batch,
+                 s.blocks * kBlock};
     hipLaunchKernelGGL(join_kernel<kValue>, dim3((uint32_t)tokens, (uint32_t)heads), dim3(256), 0, st, j);
     return V1_LAUNCHED("latent_expanded: join");
 }

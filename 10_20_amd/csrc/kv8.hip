@@ -381,7 +381,7 @@ inline Plan kv8_plan(const int32_t* lens, int32_t rows, int32_t kv_heads, int32_
     const int64_t together = kv8_together(kv_heads), streams = kWaves / together, steps = cdiv(cdiv(keys, kTileKeys), streams);
     const int64_t slots = std::max<int64_t>(1, 2 * device_cus() * together / kv_heads);
     Plan p{lens, rows, keys, 0, 0};
-    if (ragged && rows <= kPlanRows && rows < slots) p.target = (int32_t)std::max(slots - rows, (slots + 1) / 2);
+    if (ragged && planned(rows, cdiv(keys, kTileKeys)) && rows < slots) p.target = (int32_t)std::max(slots - rows, (slots + 1) / 2);
     else p.chunk = (int32_t)streams * chunk_for(rows, steps, slots, 2, 1);
     return p;
 }
@@ -433,6 +433,7 @@ extern "C" int v1_kv8_attend(const v1_kv8_attend_args* a, void* stream) {
     V1_REQUIRE(rows >= 0 && kv_heads > 0 && group > 0 && keys >= 0 && pages >= 0 && table_len >= 0 &&
                    (int64_t)kv_heads * group < 1ll << 16,
                "kv8_attend: bad shape");
+    V1_REQUIRE(keys <= kMostKeys, "kv8_attend: too many keys");
     V1_REQUIRE(group <= kMaxGroup, "kv8_attend: at most %d query heads per KV head", kMaxGroup);
     V1_REQUIRE(scale > 0.f && scale < __builtin_inff(), "kv8_attend: scale must be positive and finite");
     V1_REQUIRE(aligned16(q) && (q_row | q_head) % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0 &&
@@ -464,7 +465,7 @@ extern "C" int v1_kv8_attend(const v1_kv8_attend_args* a, void* stream) {
     hipLaunchKernelGGL(kv8_attend_kernel, dim3((uint32_t)(8 * spread)), dim3(64 * kWaves), sizeof(Kv8Lds), st, p);
     rc = V1_LAUNCHED("kv8_attend");
     if (rc != V1_OK || need == 0) return rc;
-    JoinParams j{plan, p.parts, p.out, o_row, o_head, lse, heads, nullptr, 0};
+    JoinParams j{plan, p.parts, p.out, o_row, o_head, lse, heads, nullptr, 0, 0};
     hipLaunchKernelGGL(join_kernel<kDim>, dim3((uint32_t)rows, (uint32_t)heads), dim3(256), 0, st, j);
     return V1_LAUNCHED("kv8_attend: join");
 }

@@ -519,16 +519,29 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
     }
 }
 
-// Heads of a work-group: 16, 32 or 64 (more: several work-groups a row).
-inline int32_t absorbed_heads(int32_t heads) { return heads <= 16 ? 16 : heads <= 32 ? 32 : 64; }
+// Heads of a work-group: 16, 32 or 64 (more: several work-groups a row).  More heads
+// share each key's conversion (1024 rows of 64 heads and 2048 keys: 16 / 32 / 64 of
+// them take 710 / 460 / 365 us); fewer start and end sooner.  So the fewest
+// whose work-groups all run at once and have little to do:
+//   8 rows, 64 heads, 2048 keys      16.7 / 20.0 / 25.6 us   (4 tiles a CU at 16)
+//   20 rows, 64 heads, to 6000 keys  35.4 / 31.9 / 35.4      (29 at 16, 15 at 32)
+//   128 rows, 64 heads, 2048 keys    87.2 / 60.0 / 66.5      (32 at 32)
+//   7 rows, 64 heads, to 60000 keys  76.5 / 61.0 / 57.1      (51 at 32)
+//   160 rows, 64 heads, 2048 keys     128 /  109 / 81.0      (320 work-groups at 32)
+inline int32_t absorbed_heads(int32_t rows, int32_t heads, int32_t keys) {
+    const int64_t cus = device_cus(), tiles = cdiv(keys, kTileKeys);
+    const int64_t of16 = (int64_t)rows * cdiv(heads, 16), of32 = (int64_t)rows * cdiv(heads, 32);
+    if (heads <= 16 || (of16 <= cus && of16 * tiles <= 8 * cus)) return 16;
+    return heads <= 32 || (of32 <= cus && of32 * tiles <= 32 * cus) ? 32 : 64;
+}
 
 // (One work-group a CU.  A part's start is two to four dependent loads, its sums
 // are three tiles' bytes at 64 heads and less than one at 16.)
 inline Plan absorbed_plan(const int32_t* lens, int32_t rows, int32_t heads, int32_t keys, bool ragged) {
-    const int32_t hb = absorbed_heads(heads);
+    const int32_t hb = absorbed_heads(rows, heads, keys);
     const int64_t splits = cdiv(heads, hb), tiles = cdiv(keys, kTileKeys), slots = std::max<int64_t>(1, device_cus() / splits);
     Plan p{lens, rows, keys, 0, 0};
-    if (ragged && rows <= kPlanRows && rows < slots) p.target = (int32_t)std::max(slots - rows, (slots + 1) / 2);
+    if (ragged && planned(rows, tiles) && rows < slots) p.target = (int32_t)std::max(slots - rows, (slots + 1) / 2);
     else p.chunk = chunk_for(rows, tiles, slots, 3, hb / 16);
     return p;
 }
@@ -579,6 +592,7 @@ extern "C" int v1_latent_attend(const v1_latent_attend_args* a, void* stream) {
           out, o_row, o_head, lse, workspace, workspace_bytes, map_shift, rows, heads, keys, scale] = *a;
     V1_REQUIRE(rows >= 0 && heads > 0 && keys >= 0 && pool_rows >= 0 && pool_rows < 1ll << 31, "latent_attend: bad shape");
     V1_REQUIRE(heads < 1 << 16, "latent_attend: too many heads");
+    V1_REQUIRE(keys <= kMostKeys, "latent_attend: too many keys");
     V1_REQUIRE(scale > 0.f && scale < __builtin_inff(), "latent_attend: scale must be positive and finite");
     V1_REQUIRE(map_shift >= 0 && map_shift < 31 && map_len >= 0, "latent_attend: bad page map");
     V1_REQUIRE(aligned16(q) && aligned16(pool) && reinterpret_cast<uintptr_t>(out) % 8 == 0 && q_row % 8 == 0 &&
@@ -591,7 +605,7 @@ extern "C" int v1_latent_attend(const v1_latent_attend_args* a, void* stream) {
     const int64_t items = items_at_most(plan), need = v1_latent_attend_workspace(rows, heads, keys, lens != nullptr);
     V1_REQUIRE(workspace_bytes >= need && (need == 0 || workspace != nullptr),
                "latent_attend: workspace of %lld bytes needed", (long long)need);
-    const int32_t hb = absorbed_heads(heads);
+    const int32_t hb = absorbed_heads(rows, heads, keys);
     const int64_t splits = cdiv(heads, hb), spread = cdiv(items, 8), blocks = 8 * spread * splits;
     V1_REQUIRE(blocks < 1ll << 31, "latent_attend: too many rows");
     AbsorbedParams p{static_cast<const uint16_t*>(q), q_row, q_head, static_cast<const uint8_t*>(pool), pool_rows,
@@ -603,7 +617,7 @@ extern "C" int v1_latent_attend(const v1_latent_attend_args* a, void* stream) {
                    : hb == 32 ? launch_absorbed<2, 1>(p, blocks, st)
                               : launch_absorbed<2, 2>(p, blocks, st);
     if (rc != V1_OK || need == 0) return rc;
-    JoinParams j{plan, p.parts, p.out, o_row, o_head, lse, heads, nullptr, 0};
+    JoinParams j{plan, p.parts, p.out, o_row, o_head, lse, heads, nullptr, 0, 0};
     hipLaunchKernelGGL(join_kernel<kLatent>, dim3((uint32_t)rows, (uint32_t)heads), dim3(256), 0, st, j);
     return V1_LAUNCHED("latent_attend: join");
 }

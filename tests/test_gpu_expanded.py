@@ -62,7 +62,8 @@ def check(out, lse, q, kv, rope, nq, nk, causal=True, scale=192 ** -0.5):
 @pytest.mark.parametrize("nq,nk,heads", [
     ([1], [1], 1), ([1], [700], 2), ([64], [64], 1), ([65], [65], 3), ([33, 1, 0, 127, 200], None, 2),
     ([5, 300], [70, 1000], 2), ([128], [128], 16), ([257], [1500], 1), ([100, 7], [50, 7], 2), ([40], [0], 1),
-    ([2, 3, 4], [9000, 30, 4], 1), ([1300, 900], None, 16), ([8, 8, 8, 8], [512, 512, 512, 512], 16)])
+    ([2, 3, 4], [9000, 30, 4], 1), ([1300, 900], None, 16), ([8, 8, 8, 8], [512, 512, 512, 512], 16),
+    ([3, 2100, 5, 1, 0, 2, 64, 300, 1, 1, 9, 4, 700], None, 5)])
 @pytest.mark.parametrize("causal", [True, False])
 def test_sequences(nq, nk, heads, causal):
     print("expanded", nq, nk, heads, causal, flush=True)
@@ -110,7 +111,7 @@ def test_strides_and_rows_behind_the_last_sequence():
 
 
 @gpu
-@pytest.mark.parametrize("heads,n", [(1, 300), (16, 2100)])
+@pytest.mark.parametrize("heads,n", [(1, 300), (16, 2100), (1, 2100)])
 def test_values_that_are_not_finite(heads, n):
     """An infinite or NaN value, or key, of a token that a query does not see changes
     nothing for that query; those that see it get what the formula gives."""

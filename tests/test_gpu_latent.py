@@ -82,15 +82,15 @@ def test_pool_rows(rows, heads, keys):
 
 
 @gpu
-@pytest.mark.parametrize("heads", [8, 32, 64])
+@pytest.mark.parametrize("heads,keys", [(8, 700), (32, 700), (64, 700), (32, 6000), (64, 45000)])  # (the last: 32, 64 heads a work-group)
 @pytest.mark.parametrize("shared", [True, False])
-def test_pages_masks_and_lengths(heads, shared):
+def test_pages_masks_and_lengths(heads, keys, shared):
     """Page tables with bad entries, ids that are not attended (also whole tiles
     and rows of them), ragged lengths of 0, 1, past the row; nothing outside the
     attended rows is read: the others hold NaN."""
-    print("latent pages", heads, shared, flush=True)
+    print("latent pages", heads, keys, shared, flush=True)
     g = torch.Generator(device=DEV).manual_seed(heads)
-    rows, pages, entries, keys = 13, 60, 11, 700
+    rows, pages, entries = 13, 60, 11
     pool, q = rand_pool(g, pages * 16), rand_q(g, rows, heads)
     table = torch.stack([torch.randperm(pages, device=DEV, generator=g)[:entries] for _ in range(rows)]).to(torch.int32)
     table[:, 3], table[:, 5] = -1, pages  # no page, and a page past the pool
@@ -116,7 +116,8 @@ def test_pages_masks_and_lengths(heads, shared):
 
 
 @gpu
-@pytest.mark.parametrize("rows,heads,entries", [(5, 16, 40), (3, 128, 33), (257, 16, 3), (40, 33, 7)])
+@pytest.mark.parametrize("rows,heads,entries", [(5, 16, 40), (3, 128, 33), (257, 16, 3), (40, 33, 7), (70, 128, 40),
+                                                (20, 64, 300), (3, 17, 2000)])
 def test_whole_contexts(rows, heads, entries):
     """No ids: the first lens positions of each row's pages, lengths far apart."""
     print("latent whole", rows, heads, entries, flush=True)
