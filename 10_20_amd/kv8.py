@@ -26,20 +26,31 @@ _DEFAULT_SCALE = 1.0 / math.sqrt(DIM)
 _BF16, _I32, _F32, _E4M3 = torch.bfloat16, torch.int32, torch.float32, torch.float8_e4m3fn
 
 
+def _bad_pool(name):
+    raise ValueError(f"{name} must be float8_e4m3fn [pages, {PAGE}, kv_heads, {DIM}] with a contiguous last dimension")
+
+
+# (each property of a tensor is asked for once: 0.1-0.3 us of a call whose kernels
+# may take 10)
 def _pools(k_pool, v_pool, k_scale, v_scale):
-    shape = k_pool.shape
-    if len(shape) != 4 or shape[1] != PAGE or shape[3] != DIM or not shape[2]:
-        raise ValueError(f"k_pool must be float8_e4m3fn [pages, {PAGE}, kv_heads, {DIM}] with a contiguous last dimension")
+    """Pages, KV heads, and the pointers and strides of the pools and scales."""
+    shape, kp, vp, ks, vs = k_pool.shape, k_pool.stride(), v_pool.stride(), k_scale.stride(), v_scale.stride()
+    if len(shape) != 4 or k_pool.dtype != _E4M3 or kp[3] != 1:
+        _bad_pool("k_pool")
+    pages, page, heads, dim = shape
+    if page != PAGE or dim != DIM or not heads:
+        _bad_pool("k_pool")
     if v_pool.shape != shape:
         raise ValueError("k_pool and v_pool must agree")
-    for name, t in (("k_pool", k_pool), ("v_pool", v_pool)):
-        if t.dtype != _E4M3 or t.stride(3) != 1:
-            raise ValueError(f"{name} must be float8_e4m3fn [pages, {PAGE}, kv_heads, {DIM}] with a contiguous last dimension")
-    pages, _, heads, _ = shape
-    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if t.dtype != _F32 or t.shape != (pages, heads) or (heads > 1 and t.stride(1) != 1):
-            raise ValueError(f"{name} must be float32 [pages, kv_heads] with unit inner stride")
-    return pages, heads
+    if v_pool.dtype != _E4M3 or vp[3] != 1:
+        _bad_pool("v_pool")
+    each = (pages, heads)
+    if k_scale.dtype != _F32 or k_scale.shape != each or (ks[1] != 1 and heads > 1):
+        raise ValueError("k_scale must be float32 [pages, kv_heads] with unit inner stride")
+    if v_scale.dtype != _F32 or v_scale.shape != each or (vs[1] != 1 and heads > 1):
+        raise ValueError("v_scale must be float32 [pages, kv_heads] with unit inner stride")
+    return pages, heads, (k_pool.data_ptr(), kp[0], kp[1], kp[2], v_pool.data_ptr(), vp[0], vp[1], vp[2],
+                          k_scale.data_ptr(), ks[0], v_scale.data_ptr(), vs[0], pages)
 
 
 def _vector(name, t, n):
@@ -68,22 +79,23 @@ def store(k, v, k_pool, v_pool, k_scale, v_scale, table, starts, cu_tokens):
     table, pages outside the pool and requests with a negative start are skipped; a
     page is appended to by one request of a call (pages shared by several are full)."""
     _lib.require_gpu(k, v, k_pool, v_pool, k_scale, v_scale, table, starts, cu_tokens)
-    pages, heads = _pools(k_pool, v_pool, k_scale, v_scale)
-    for name, t in (("k", k), ("v", v)):
-        if t.dtype != _BF16 or t.dim() != 3 or t.shape[1:] != (heads, DIM) or t.stride(2) != 1:
-            raise ValueError(f"{name} must be bfloat16 [tokens, {heads}, {DIM}] with a contiguous last dimension")
-    tokens = k.shape[0]
-    if v.shape[0] != tokens:
+    pages, heads, pools = _pools(k_pool, v_pool, k_scale, v_scale)
+    shape, ks, vs = k.shape, k.stride(), v.stride()
+    tokens = shape[0] if len(shape) == 3 else -1
+    if shape != (tokens, heads, DIM) or k.dtype != _BF16 or ks[2] != 1:
+        raise ValueError(f"k must be bfloat16 [tokens, {heads}, {DIM}] with a contiguous last dimension")
+    if v.shape != shape:
         raise ValueError("k and v must be of one shape")
-    if table.dtype != _I32 or table.dim() != 2 or (table.shape[1] and table.stride(1) != 1):
+    if v.dtype != _BF16 or vs[2] != 1:
+        raise ValueError(f"v must be bfloat16 [tokens, {heads}, {DIM}] with a contiguous last dimension")
+    ts = table.stride()
+    if table.dtype != _I32 or len(ts) != 2 or (ts[1] != 1 and table.shape[1]):
         raise ValueError("table must be int32 [requests, entries] with unit inner stride")
     requests, entries = table.shape
     _vector("starts", starts, requests)
     _vector("cu_tokens", cu_tokens, requests + 1)
-    _lib.call_packed("v1_kv8_store", k, k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2],
-                     k_pool.data_ptr(), *k_pool.stride()[:3], v_pool.data_ptr(), *v_pool.stride()[:3], k_scale.data_ptr(),
-                     k_scale.stride(0), v_scale.data_ptr(), v_scale.stride(0), pages, table.data_ptr(), table.stride(0),
-                     starts.data_ptr(), cu_tokens.data_ptr(), entries, tokens, requests, heads)
+    _lib.call_packed("v1_kv8_store", k, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], *pools,
+                     table.data_ptr(), ts[0], starts.data_ptr(), cu_tokens.data_ptr(), entries, tokens, requests, heads)
 
 
 def attend(q, k_pool, v_pool, k_scale, v_scale, table, lens=None, ids=None, softmax_scale=None, out=None, return_lse=False):
@@ -101,23 +113,27 @@ def attend(q, k_pool, v_pool, k_scale, v_scale, table, lens=None, ids=None, soft
     Returns out [rows, heads, 128] bf16, and with return_lse the natural log of the
     sum of exponentials, [rows, heads] fp32."""
     _lib.require_gpu(q, k_pool, v_pool, k_scale, v_scale, table, lens, ids, out)
-    pages, kv_heads = _pools(k_pool, v_pool, k_scale, v_scale)
-    if q.dim() != 3 or q.shape[2] != DIM or q.dtype != _BF16 or q.stride(2) != 1:
+    pages, kv_heads, pools = _pools(k_pool, v_pool, k_scale, v_scale)
+    shape, qs = q.shape, q.stride()
+    if len(shape) != 3 or shape[2] != DIM or q.dtype != _BF16 or qs[2] != 1:
         raise ValueError(f"q must be bfloat16 [rows, heads, {DIM}] with a contiguous last dimension")
-    rows, heads, _ = q.shape
+    rows, heads, _ = shape
     group = heads // kv_heads
     if not heads or heads % kv_heads or group > 16:
         raise ValueError("query heads must be a multiple of KV heads, at most 16 per KV head")
-    dims, entries = table.dim(), table.shape[-1]
-    if table.dtype != _I32 or not (dims == 1 or (dims == 2 and table.shape[0] == rows)):
+    of, ts = table.shape, table.stride()
+    dims = len(of)
+    if table.dtype != _I32 or not (dims == 1 or (dims == 2 and of[0] == rows)):
         raise ValueError("table must be int32 [entries] or [rows, entries]")
-    if entries and table.stride(-1) != 1:
+    entries = of[-1]
+    if entries and ts[-1] != 1:
         raise ValueError("table must have unit inner stride")
     ids_ptr = ids_stride = lens_ptr = 0
     if ids is not None:
-        if ids.dtype != _I32 or ids.dim() != 2 or ids.shape[0] != rows or (ids.shape[1] and ids.stride(1) != 1):
+        of, at = ids.shape, ids.stride()
+        if ids.dtype != _I32 or len(of) != 2 or of[0] != rows or (at[1] != 1 and of[1]):
             raise ValueError("ids must be int32 [rows, keys] with unit inner stride")
-        keys, ids_ptr, ids_stride = ids.shape[1], ids.data_ptr(), ids.stride(0)
+        keys, ids_ptr, ids_stride = of[1], ids.data_ptr(), at[0]
     else:
         keys = entries * PAGE
         if keys >= 1 << 31:
@@ -132,15 +148,14 @@ def attend(q, k_pool, v_pool, k_scale, v_scale, table, lens=None, ids=None, soft
         keys = 0
     if out is None:
         out = q.new_empty((rows, heads, DIM))
-    elif out.dtype != _BF16 or out.shape != (rows, heads, DIM) or out.stride(2) != 1:
+    o_row, o_head, o_dim = out.stride() if out.dim() == 3 else (0, 0, 0)
+    if o_dim != 1 or out.dtype != _BF16 or out.shape != shape:
         raise ValueError(f"out must be bfloat16 [{rows}, {heads}, {DIM}] with a contiguous last dimension")
     lse = q.new_empty((rows, heads), dtype=_F32) if return_lse else None
     # (the sums of a row's parts are the call's own, as in attention.attend_slots)
     ws_bytes = _workspace_bytes(q.get_device(), rows, kv_heads, group, keys, lens is not None)
     ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
-    _lib.call_packed("v1_kv8_attend", q, q.data_ptr(), *q.stride()[:2], k_pool.data_ptr(),
-                     *k_pool.stride()[:3], v_pool.data_ptr(), *v_pool.stride()[:3], k_scale.data_ptr(), k_scale.stride(0),
-                     v_scale.data_ptr(), v_scale.stride(0), pages, table.data_ptr(), table.stride(0) if dims == 2 else 0,
-                     ids_ptr, ids_stride, lens_ptr, out.data_ptr(), *out.stride()[:2], _lib.ptr(lse), _lib.ptr(ws),
-                     ws_bytes, entries, rows, kv_heads, group, keys, scale)
+    _lib.call_packed("v1_kv8_attend", q, q.data_ptr(), qs[0], qs[1], *pools, table.data_ptr(), ts[0] if dims == 2 else 0,
+                     ids_ptr, ids_stride, lens_ptr, out.data_ptr(), o_row, o_head, _lib.ptr(lse), _lib.ptr(ws), ws_bytes,
+                     entries, rows, kv_heads, group, keys, scale)
     return (out, lse) if return_lse else out

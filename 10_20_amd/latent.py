@@ -31,17 +31,24 @@ def _int32(name, t, n):
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape [{n}]")
 
 
+# (each property of a tensor is asked for once: 0.1-0.3 us of a call whose kernels
+# may take 10)
 def _pool(pool):
-    if pool.dtype != torch.uint8 or pool.dim() != 2 or pool.shape[1] != ROW_BYTES or pool.stride(1) != 1:
+    """Rows and their stride."""
+    shape, stride = pool.shape, pool.stride()
+    if pool.dtype != torch.uint8 or len(shape) != 2 or shape[1] != ROW_BYTES or stride[1] != 1:
         raise ValueError(f"pool must be a uint8 [rows, {ROW_BYTES}] tensor with unit inner stride")
+    return shape[0], stride[0]
 
 
 def _output(out, q, shape):
+    """The output and its strides."""
     if out is None:
-        return q.new_empty(shape)
-    if out.dtype != _BF16 or out.shape != shape or out.stride(2) != 1:
+        out = q.new_empty(shape)
+    stride = out.stride()
+    if out.dtype != _BF16 or out.shape != shape or stride[2] != 1:
         raise ValueError(f"out must be bfloat16 {list(shape)} with a contiguous last dimension")
-    return out
+    return out, stride[0], stride[1]
 
 
 _DEFAULT_SCALE = 1.0 / math.sqrt(HEAD + ROPE)
@@ -72,14 +79,15 @@ def store_rows(latent, rope, pool, slots):
     code the nearest e4m3 value of x / s (ties to even); infinities are stored as
     +-448 s, NaN as NaN."""
     _lib.require_gpu(latent, rope, pool, slots)
-    tokens = latent.shape[0]
-    for name, t, n in (("latent", latent, LATENT), ("rope", rope, ROPE)):
-        if t.dtype != _BF16 or t.shape != (tokens, n) or t.stride(1) != 1:
-            raise ValueError(f"{name} must be bfloat16 [tokens, {n}] with a contiguous last dimension")
-    _pool(pool)
+    tokens, ls, rs = latent.shape[0], latent.stride(), rope.stride()
+    if latent.shape != (tokens, LATENT) or latent.dtype != _BF16 or ls[1] != 1:
+        raise ValueError(f"latent must be bfloat16 [tokens, {LATENT}] with a contiguous last dimension")
+    if rope.shape != (tokens, ROPE) or rope.dtype != _BF16 or rs[1] != 1:
+        raise ValueError(f"rope must be bfloat16 [tokens, {ROPE}] with a contiguous last dimension")
+    rows, stride = _pool(pool)
     _int32("slots", slots, tokens)
-    _lib.call_packed("v1_latent_store", pool, latent.data_ptr(), latent.stride(0), rope.data_ptr(),
-                     rope.stride(0), slots.data_ptr(), pool.data_ptr(), pool.shape[0], pool.stride(0), tokens)
+    _lib.call_packed("v1_latent_store", pool, latent.data_ptr(), ls[0], rope.data_ptr(), rs[0], slots.data_ptr(),
+                     pool.data_ptr(), rows, stride, tokens)
     return pool
 
 
@@ -101,27 +109,30 @@ def attend(q, pool, ids=None, table=None, page_bits=0, lens=None, softmax_scale=
     1 / sqrt(192), that of the expanded form.  Returns out [rows, heads, 512] bf16,
     and with return_lse the natural log of the sum of exponentials, [rows, heads] fp32."""
     _lib.require_gpu(q, pool, ids, table, lens, out)
-    if q.dim() != 3 or q.shape[2] != LATENT + ROPE or q.dtype != _BF16 or q.stride(2) != 1 or not q.shape[1]:
+    shape, qs = q.shape, q.stride()
+    if len(shape) != 3 or shape[2] != LATENT + ROPE or q.dtype != _BF16 or qs[2] != 1 or not shape[1]:
         raise ValueError(f"q must be bfloat16 [rows, heads, {LATENT + ROPE}] with a contiguous last dimension")
-    _pool(pool)
-    rows, heads, _ = q.shape
+    slots, slot_stride = _pool(pool)
+    rows, heads, _ = shape
     page_bits = int(page_bits)
     if not 0 <= page_bits < 31:
         raise ValueError("page_bits must be in [0, 31)")
     map_ptr = map_len = map_stride = ids_ptr = ids_stride = lens_ptr = 0
     if table is not None:
-        dims = table.dim()
-        if table.dtype != _I32 or not (dims == 1 or (dims == 2 and table.shape[0] == rows)):
+        of, at = table.shape, table.stride()
+        dims = len(of)
+        if table.dtype != _I32 or not (dims == 1 or (dims == 2 and of[0] == rows)):
             raise ValueError("table must be int32 [entries] or [rows, entries]")
-        map_ptr, map_len, map_stride = table.data_ptr(), table.shape[-1], table.stride(0) if dims == 2 else 0
-        if map_len and table.stride(-1) != 1:
+        map_ptr, map_len, map_stride = table.data_ptr(), of[-1], at[0] if dims == 2 else 0
+        if map_len and at[-1] != 1:
             raise ValueError("table must have unit inner stride")
     if ids is not None:
-        if ids.dtype != _I32 or ids.dim() != 2 or ids.shape[0] != rows or (ids.shape[1] and ids.stride(1) != 1):
+        of, at = ids.shape, ids.stride()
+        if ids.dtype != _I32 or len(of) != 2 or of[0] != rows or (at[1] != 1 and of[1]):
             raise ValueError("ids must be int32 [rows, keys] with unit inner stride")
-        keys, ids_ptr, ids_stride = ids.shape[1], ids.data_ptr(), ids.stride(0)
+        keys, ids_ptr, ids_stride = of[1], ids.data_ptr(), at[0]
     else:
-        keys = map_len << page_bits if table is not None else pool.shape[0]
+        keys = map_len << page_bits if table is not None else slots
         if keys >= 1 << 31:
             raise ValueError("positions must stay below 2**31")
     if table is not None and map_len == 0:
@@ -130,16 +141,14 @@ def attend(q, pool, ids=None, table=None, page_bits=0, lens=None, softmax_scale=
         _int32("lens", lens, rows)
         lens_ptr = lens.data_ptr()
     scale = _scale(softmax_scale)
-    out = _output(out, q, (rows, heads, LATENT))
+    out, o_row, o_head = _output(out, q, (rows, heads, LATENT))
     lse = q.new_empty((rows, heads), dtype=torch.float32) if return_lse else None
     # (the sums of a row's parts are the call's own, as in attention.attend_slots)
     ws_bytes = _workspace_bytes("v1_latent_attend_workspace", q.get_device(), rows, heads, keys, lens is not None)
     ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
-    o_row, o_head, _ = out.stride()
-    q_row, q_head, _ = q.stride()
-    _lib.call_packed("v1_latent_attend", q, q.data_ptr(), q_row, q_head, pool.data_ptr(), pool.shape[0],
-                     pool.stride(0), map_ptr, map_len, map_stride, ids_ptr, ids_stride, lens_ptr, out.data_ptr(), o_row,
-                     o_head, _lib.ptr(lse), _lib.ptr(ws), ws_bytes, page_bits, rows, heads, keys, scale)
+    _lib.call_packed("v1_latent_attend", q, q.data_ptr(), qs[0], qs[1], pool.data_ptr(), slots, slot_stride, map_ptr, map_len,
+                     map_stride, ids_ptr, ids_stride, lens_ptr, out.data_ptr(), o_row, o_head, _lib.ptr(lse), _lib.ptr(ws),
+                     ws_bytes, page_bits, rows, heads, keys, scale)
     return (out, lse) if return_lse else out
 
 
@@ -183,11 +192,10 @@ def attend_expanded(q, kv, k_rope, cu_q, cu_k=None, max_q=None, softmax_scale=No
     if max_q < 0:
         raise ValueError("max_q must not be negative")
     scale = _scale(softmax_scale)
-    out = _output(out, q, (tokens, heads, HEAD))
+    out, o_row, o_head = _output(out, q, (tokens, heads, HEAD))
     lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
     ws_bytes = _workspace_bytes("v1_latent_expanded_workspace", q.get_device(), tokens, keys, batch, heads, max_q)
     ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
-    o_row, o_head, _ = out.stride()
     q_row, q_head, _ = q.stride()
     _lib.call_packed("v1_latent_expanded", q, q.data_ptr(), q_row, q_head, kv.data_ptr(), kv.stride(0),
                      kv.stride(1), k_rope.data_ptr(), k_rope.stride(0), cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(),
