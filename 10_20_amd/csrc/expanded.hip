@@ -146,6 +146,7 @@ __device__ __forceinline__ void careful_product(f32x16 (&sums)[4], const Frag (&
 template <bool CAREFUL>
 __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedTile* lds) {
     constexpr int COPIES = (int)(sizeof(ExpandedTile) / 1024) / kWaves;
+    static_assert(COPIES == 5 && kWaves * 4 * 2 == kTileKeys, "copies of a tile");
     const int32_t wave = __builtin_amdgcn_readfirstlane((int32_t)threadIdx.x / kWave);
     const int32_t lane = (int32_t)threadIdx.x % kWave, c = lane & 31, h = lane >> 5;
 
@@ -176,25 +177,28 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedT
     const int32_t each = (all_tiles + p.parts - 1) / p.parts;
     const int32_t first = min(part * each, all_tiles), tiles = min(each, all_tiles - first);
 
-    auto copy_tile = [&](int32_t t) __attribute__((always_inline)) {
+    // Copy j of the wave's five of a tile: four keys twice, four values twice, eight
+    // rows of rope numbers.  (Rows and tiles past the last are copies of the last key.)
+    auto copy = [&](int32_t t, auto which) __attribute__((always_inline)) {
+        constexpr int j = which.value;
         ExpandedTile& to = lds[t % kBuffers];
         const int32_t k0 = (first + t) * kTileKeys;
-#pragma unroll
-        for (int j = 0; j < COPIES; ++j) {
-            const int32_t i = j * kWaves + wave;
-            if (i < 32) {  // keys (16 copies of 4 rows), then values
-                const int32_t r = 4 * (i & 15) + (lane >> 4), at = lane & 15;
-                const int32_t chunk = i < 16 ? at ^ (r & 15) : 16 + (at ^ (4 * (r & 3)));
-                const int64_t key = k_lo + min(k0 + r, nk - 1);
-                copy_to_lds(p.kv + key * p.kv_row + head * p.kv_head + 8 * chunk,
-                            lds_offset(i < 16 ? &to.key[4 * i][0] : &to.value[4 * (i - 16)][0]));
-            } else {
-                const int32_t r = 8 * (i - 32) + (lane >> 3);
-                const int64_t key = k_lo + min(k0 + r, nk - 1);
-                copy_to_lds(p.rope + key * p.rope_row + 8 * ((lane & 7) ^ (r & 7)), lds_offset(&to.rope[8 * (i - 32)][0]));
-            }
+        if constexpr (j < 4) {
+            const int32_t i = (j & 1) * kWaves + wave, r = 4 * i + (lane >> 4), at = lane & 15;
+            const int32_t chunk = j < 2 ? at ^ (r & 15) : 16 + (at ^ (4 * (r & 3)));
+            const int64_t key = k_lo + min(k0 + r, nk - 1);
+            copy_to_lds(p.kv + key * p.kv_row + head * p.kv_head + 8 * chunk,
+                        lds_offset(j < 2 ? &to.key[4 * i][0] : &to.value[4 * i][0]));
+        } else {
+            const int32_t r = 8 * wave + (lane >> 3);
+            const int64_t key = k_lo + min(k0 + r, nk - 1);
+            copy_to_lds(p.rope + key * p.rope_row + 8 * ((lane & 7) ^ (r & 7)), lds_offset(&to.rope[8 * wave][0]));
         }
     };
+    auto copy_tile = [&](int32_t t) __attribute__((always_inline)) {
+        each_of<COPIES>([&](auto j) __attribute__((always_inline)) { copy(t, j); });
+    };
+
     // B fragments of Q^T: column c = query i0 + c
     Frag q[12];
     {
@@ -202,8 +206,7 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedT
 #pragma unroll
         for (int s = 0; s < 12; ++s) q[s].u = *reinterpret_cast<const u32x4*>(src + 16 * s);
     }
-    for (int t = 0; t < 2; ++t)
-        if (t < tiles) copy_tile(t);
+    if (tiles > 0) copy_tile(0), copy_tile(1);
     // (or the loop waits for them, and with them for its copies)
 #pragma unroll
     for (int s = 0; s < 12; ++s) asm volatile("" : "+v"(q[s].u));
@@ -224,17 +227,22 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedT
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
+        // key rows 32u .., numbers 16 (n / 2) ..
+        Frag k[kAhead];
+        auto fetch = [&](int n) __attribute__((always_inline)) {
+            const int32_t st = n / 2, r = 32 * (n & 1) + c;
+            k[n % kAhead].u = *reinterpret_cast<const u32x4*>(st < 8 ? &tile.key[r][16 * ((2 * st + h) ^ (r & 15))]
+                                                                     : &tile.rope[r][16 * ((2 * st - 16 + h) ^ (r & 7))]);
+        };
 #pragma unroll
-        for (int st = 0; st < 12; ++st)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int32_t r = 32 * u + c;
-                Frag k;
-                k.u = *reinterpret_cast<const u32x4*>(st < 8 ? &tile.key[r][16 * ((2 * st + h) ^ (r & 15))]
-                                                             : &tile.rope[r][16 * ((2 * st - 16 + h) ^ (r & 7))]);
-                s[u] = mfma32(k, q[st], s[u]);
-            }
-        reads_ahead<24, 1>();
+        for (int n = 0; n < kAhead; ++n) fetch(n);
+        each_of<24>([&](auto number) __attribute__((always_inline)) {
+            constexpr int n = number.value;
+            s[n & 1] = mfma32(k[n % kAhead], q[n / 2], s[n & 1]);
+            if constexpr (n + kAhead < 24) fetch(n + kAhead);
+            if constexpr (n % 4 == 1 && n / 4 < COPIES) copy(t + 2, Number<n / 4>{});
+            __builtin_amdgcn_sched_barrier(0);
+        });
     };
     auto softmax = [&](int32_t t) __attribute__((always_inline)) {
         if (is_masked(t)) {
@@ -287,29 +295,28 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedT
     };
     const int32_t mine = min(tiles, max(tiles_of(wave_most) - first, 0));  // tiles that the wave sees something of
     // The two waves of a SIMD half a tile apart: one multiplies (the last tile's
-    // values, this one's keys) while the other makes probabilities.  Half-steps
-    // are divided by barriers; the even ones begin with tile `to_come` in LDS and
-    // the one after the next asked for, whose buffer was read until the last.
+    // values, this one's keys) and asks for its copies of the tile after the next,
+    // whose buffer was read until two steps ago, while the other makes
+    // probabilities.  Steps are divided by barriers, every other one of them behind a
+    // wait for the copies of the tile whose keys come next.  (The copies in one piece
+    // behind the barrier hold both waves up: 800 of a tile's 6300 cycles.)
     const bool second = wave >= kWaves / 2;
-    auto sync = [&](bool even, int32_t to_come) __attribute__((always_inline)) {
-        if (even) {
-            if (to_come + 1 < tiles) wait_barrier<COPIES>();
-            else wait_barrier<0>();
-            if (to_come + 2 < tiles) copy_tile(to_come + 2);
-        } else {
-            lds_barrier();
-        }
+    auto sync = [&](bool landed) __attribute__((always_inline)) {
+        if (landed) wait_barrier<COPIES>();
+        else lds_barrier();
     };
-    if (second) sync(true, 0);
+    if (second) sync(true);
 #pragma unroll 1
     for (int32_t t = 0; t <= tiles; ++t) {
-        sync(!second, t);
+        sync(!second);
         if (t > 0 && t <= mine) products(t - 1);
         if (t < mine) scores(t);
-        sync(second, t + 1);
+        else if (t < tiles) copy_tile(t + 2);
+        sync(second);
         if (t < mine) softmax(t);
     }
     if (!second) lds_barrier();
+    wait_copies<0>();
     if constexpr (!CAREFUL) {
         float odd = 0.f;  // NaN if a sum is not finite
 #pragma unroll
