@@ -297,6 +297,28 @@ struct JoinParams {
     int32_t batch, most;
 };
 
+// Whether the row has parts (asked by a whole work-group).
+__device__ __forceinline__ bool joined_row(const JoinParams& p, int32_t row) {
+    if (!p.cu) return true;
+    int mine = 0;
+    for (int32_t b = (int32_t)threadIdx.x; b < p.batch; b += 256) {
+        const int32_t lo = min(max(p.cu[b], 0), p.plan.rows), hi = min(max(p.cu[b + 1], lo), p.plan.rows);
+        mine |= row >= lo && row < hi && row - lo < p.most;
+    }
+    return __syncthreads_or(mine);
+}
+
+__device__ __forceinline__ void write_joined(const JoinParams& p, int32_t row, int32_t h, int32_t at4, f32x4 o, float top, float total) {
+    const bool none = total == 0.f;  // no key attended
+    const float inv = none ? 0.f : 1.0f / total;
+    *reinterpret_cast<u32x2*>(p.out + row * p.o_row + h * p.o_head + 4 * at4) =
+        none ? u32x2{0, 0} : u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
+    if (p.lse && at4 == 0)
+        p.lse[(int64_t)row * p.heads + h] = none ? -__builtin_inff() : (top + __builtin_amdgcn_logf(total)) * kLn2;
+}
+
+constexpr int kFewParts = 8;
+
 // One work-group per (row, head): D / 4 threads add four dims of every (1024 / D)-th
 // part, scaled to the largest of the parts' maxima, and the groups meet in LDS (one
 // thread per two dims over all parts took 30 us for 37 parts of 7 rows x 64 heads x
@@ -309,14 +331,7 @@ __global__ __launch_bounds__(256) void join_kernel(JoinParams p) {
     __shared__ float totals[G];
     const int32_t row = (int32_t)blockIdx.x, h = (int32_t)blockIdx.y, lane = (int32_t)threadIdx.x % kWave;
     const int32_t group = (int32_t)threadIdx.x / T, at4 = (int32_t)threadIdx.x % T;
-    if (p.cu) {
-        int mine = 0;
-        for (int32_t b = (int32_t)threadIdx.x; b < p.batch; b += 256) {
-            const int32_t lo = min(max(p.cu[b], 0), p.plan.rows), hi = min(max(p.cu[b + 1], lo), p.plan.rows);
-            mine |= row >= lo && row < hi && row - lo < p.most;
-        }
-        if (!__syncthreads_or(mine)) return;
-    }
+    if (!joined_row(p, row)) return;
     int32_t first, parts;
     items_of(p.plan, row, first, parts);
     if (parts <= 1) return;
@@ -345,12 +360,50 @@ __global__ __launch_bounds__(256) void join_kernel(JoinParams p) {
         o += sums[k][at4];
         total += totals[k];
     }
-    const bool none = total == 0.f;  // no key attended
-    const float inv = none ? 0.f : 1.0f / total;
-    *reinterpret_cast<u32x2*>(p.out + row * p.o_row + h * p.o_head + 4 * at4) =
-        none ? u32x2{0, 0} : u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
-    if (p.lse && at4 == 0)
-        p.lse[(int64_t)row * p.heads + h] = none ? -__builtin_inff() : (top + __builtin_amdgcn_logf(total)) * kLn2;
+    write_joined(p, row, h, at4, o, top, total);
+}
+
+// The same for rows of a few parts, known on the host: D / 4 threads for each (row,
+// head), several of them a work-group.
+template <int D>
+__global__ __launch_bounds__(256) void join_few_kernel(JoinParams p) {
+    constexpr int T = D / 4, G = 256 / T;
+    const int32_t row = (int32_t)blockIdx.x, h = (int32_t)blockIdx.y * G + (int32_t)threadIdx.x / T, at4 = (int32_t)threadIdx.x % T;
+    if (!joined_row(p, row) || h >= p.heads) return;
+    const int32_t parts = (tiles_of(p.plan.keys) + p.plan.chunk - 1) / p.plan.chunk;
+    const int64_t first = (int64_t)row * parts * p.heads + h;
+    f32x2 st[kFewParts];
+    f32x4 x[kFewParts];
+    float top = -__builtin_inff(), total = 0.f;
+#pragma unroll
+    for (int i = 0; i < kFewParts; ++i) {
+        const int64_t at = first + (int64_t)min(i, parts - 1) * p.heads;
+        st[i] = p.parts.stats[at];
+        x[i] = *reinterpret_cast<const f32x4*>(p.parts.sums + at * D + 4 * at4);
+        top = fmaxf(top, st[i][0]);
+    }
+    const float sub = top == -__builtin_inff() ? 0.f : top;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kFewParts; ++i) {
+        if (i >= parts) break;
+        const float f = __builtin_amdgcn_exp2f(st[i][0] - sub);
+        total = fmaf(f, st[i][1], total);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = fmaf(f, x[i][k], o[k]);
+    }
+    write_joined(p, row, h, at4, o, top, total);
+}
+
+template <int D>
+int launch_join(const JoinParams& p, hipStream_t st, const char* what) {
+    const int64_t parts = p.plan.chunk > 0 ? cdiv(cdiv(p.plan.keys, kTileKeys), p.plan.chunk) : kPlanRows;
+    constexpr int G = 256 / (D / 4);
+    if (parts <= kFewParts)
+        hipLaunchKernelGGL(join_few_kernel<D>, dim3((uint32_t)p.plan.rows, (uint32_t)cdiv(p.heads, G)), dim3(256), 0, st, p);
+    else
+        hipLaunchKernelGGL(join_kernel<D>, dim3((uint32_t)p.plan.rows, (uint32_t)p.heads), dim3(256), 0, st, p);
+    return V1_LAUNCHED(what);
 }
 
 }  // namespace attn

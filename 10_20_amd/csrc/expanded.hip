@@ -162,8 +162,13 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedT
     const int32_t part = at % p.parts, block = p.blocks - 1 - at / p.parts;
     const int32_t head = index % p.heads, b = index / p.heads;
     if (b >= p.batch) return false;
-    const int32_t q_lo = min(max(p.cu_q[b], 0), p.tokens), q_hi = min(max(p.cu_q[b + 1], q_lo), p.tokens);
-    const int32_t k_lo = min(max(p.cu_k[b], 0), p.keys), k_hi = min(max(p.cu_k[b + 1], k_lo), p.keys);
+    int32_t ends[4] = {p.cu_q[b], p.cu_q[b + 1], p.cu_k[b], p.cu_k[b + 1]};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(ends[i]));  // (one wait for the four)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ends[i] = __builtin_amdgcn_readfirstlane(ends[i]);
+    const int32_t q_lo = min(max(ends[0], 0), p.tokens), q_hi = min(max(ends[1], q_lo), p.tokens);
+    const int32_t k_lo = min(max(ends[2], 0), p.keys), k_hi = min(max(ends[3], k_lo), p.keys);
     const int32_t nq = q_hi - q_lo, nk = k_hi - k_lo;
     const int32_t q0 = block * kBlock;
     if (q0 >= nq) return false;
@@ -199,17 +204,30 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedT
         each_of<COPIES>([&](auto j) __attribute__((always_inline)) { copy(t, j); });
     };
 
-    // B fragments of Q^T: column c = query i0 + c
+    // B fragments of Q^T: column c = query i0 + c.  The rows come through LDS (rows of
+    // 24 chunks of 16 bytes end to end, eight of them XORed by the row, in the last
+    // three buffers): fragments read from memory are 32 rows' lines for every one.
     Frag q[12];
     {
-        const uint16_t* src = p.q + (q_lo + (int64_t)min(i0 + c, nq - 1)) * p.q_row + head * p.q_head + 8 * h;
+        uint8_t* const rows = reinterpret_cast<uint8_t*>(lds + kBuffers) - (kWaves - wave) * (kRows * 2 * (kKey + kRopeDims));
 #pragma unroll
-        for (int s = 0; s < 12; ++s) q[s].u = *reinterpret_cast<const u32x4*>(src + 16 * s);
+        for (int j = 0; j < 12; ++j) {
+            const int32_t r = (kWave * j + lane) / 24, chunk = (kWave * j + lane) % 24;
+            copy_to_lds(p.q + (q_lo + (int64_t)min(i0 + r, nq - 1)) * p.q_row + head * p.q_head + 8 * (chunk ^ (r & 7)),
+                        lds_offset(rows + 1024 * j));
+        }
+        if (tiles > 0) {
+            copy_tile(0);
+            wait_copies<COPIES>();
+        } else {
+            wait_copies<0>();
+        }
+#pragma unroll
+        for (int s = 0; s < 12; ++s)
+            q[s].u = *reinterpret_cast<const u32x4*>(rows + 384 * c + 16 * ((2 * s + h) ^ (c & 7)));
+        lds_barrier();
+        if (tiles > 0) copy_tile(1);
     }
-    if (tiles > 0) copy_tile(0), copy_tile(1);
-    // (or the loop waits for them, and with them for its copies)
-#pragma unroll
-    for (int s = 0; s < 12; ++s) asm volatile("" : "+v"(q[s].u));
     f32x16 acc[4], s[2];
     Frag pf[4];
     float mx = -__builtin_inff(), total = 0.f;
@@ -317,50 +335,66 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedT
     }
     if (!second) lds_barrier();
     wait_copies<0>();
+    __syncthreads();  // the tiles' memory is free
     if constexpr (!CAREFUL) {
-        float odd = 0.f;  // NaN if a sum is not finite
+        float odd = 0.f;
 #pragma unroll
         for (int d = 0; d < 4; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) odd = fmaf(acc[d][i], 0.f, odd);
-        int32_t* const flag = reinterpret_cast<int32_t*>(lds);
+        int32_t* const flags = reinterpret_cast<int32_t*>(lds);
+        const bool mine_odd = __ballot(odd != odd) != 0;
+        if (lane == 0) flags[wave] = mine_odd;
         __syncthreads();
-        if (threadIdx.x == 0) *flag = 0;
-        __syncthreads();
-        if (odd != odd) *flag = 1;
-        __syncthreads();
-        if (*flag != 0) {
+        int32_t any = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) any |= flags[w];
+        if (__builtin_amdgcn_readfirstlane(any)) {
             __syncthreads();
             return true;
         }
     }
     total += __shfl_xor(total, 32, kWave);
-    const int32_t i = i0 + c;
-    if (i >= nq) return false;
     const bool none = total == 0.f;  // no key seen
-    const int64_t row = q_lo + i;
+    // Rows leave through LDS as well, whole ones at a time: row c's numbers 32 d + 8 a
+    // + 4 h .. are its piece 8 d + 2 a + h of four, pieces XORed by the row.
+    static_assert(kBuffers * sizeof(ExpandedTile) >= kWaves * (kRows * 4 * kValue + 4), "rows and the flags before them");
+    uint8_t* const rows = reinterpret_cast<uint8_t*>(lds + kBuffers) - (kWaves - wave) * (kRows * 4 * kValue);
+    const int32_t left = nq - i0;
     if (p.parts == 1) {
         const float inv = none ? 0.f : 1.0f / total;
-        uint16_t* out = p.out + row * p.o_row + head * p.o_head + 4 * h;
 #pragma unroll
         for (int d = 0; d < 4; ++d)
 #pragma unroll
             for (int a = 0; a < 4; ++a)
-                *reinterpret_cast<u32x2*>(out + 32 * d + 8 * a) =
+                *reinterpret_cast<u32x2*>(rows + 256 * c + 8 * ((8 * d + 2 * a + h) ^ c)) =
                     none ? u32x2{0, 0} : u32x2{pack_bf16(acc[d][4 * a] * inv, acc[d][4 * a + 1] * inv),
                                                pack_bf16(acc[d][4 * a + 2] * inv, acc[d][4 * a + 3] * inv)};
-        if (p.lse && h == 0)
-            p.lse[row * p.heads + head] = none ? -__builtin_inff() : (mx + __builtin_amdgcn_logf(total)) * kLn2;
+        wait_lds();
+#pragma unroll
+        for (int j = 0; j < kRows / 2; ++j) {
+            const int32_t r = 2 * j + h;
+            const u32x2 x = *reinterpret_cast<const u32x2*>(rows + 256 * r + 8 * (c ^ r));
+            if (r < left) *reinterpret_cast<u32x2*>(p.out + (q_lo + i0 + r) * p.o_row + head * p.o_head + 4 * c) = x;
+        }
+        if (p.lse && h == 0 && c < left)
+            p.lse[(int64_t)(q_lo + i0 + c) * p.heads + head] = none ? -__builtin_inff() : (mx + __builtin_amdgcn_logf(total)) * kLn2;
     } else {
-        const int64_t at = (row * p.parts + part) * p.heads + head;
-        float* o = p.partial.sums + at * kValue + 4 * h;
+        const int64_t at = ((int64_t)(q_lo + i0) * p.parts + part) * p.heads + head, step = (int64_t)p.parts * p.heads;
 #pragma unroll
         for (int d = 0; d < 4; ++d)
 #pragma unroll
             for (int a = 0; a < 4; ++a)
-                *reinterpret_cast<f32x4*>(o + 32 * d + 8 * a) =
+                *reinterpret_cast<f32x4*>(rows + 512 * c + 16 * ((8 * d + 2 * a + h) ^ c)) =
                     f32x4{acc[d][4 * a], acc[d][4 * a + 1], acc[d][4 * a + 2], acc[d][4 * a + 3]};
-        if (h == 0) p.partial.stats[at] = f32x2{mx, total};
+        wait_lds();
+#pragma unroll
+        for (int j = 0; j < kRows / 2; ++j) {
+            const int32_t r = 2 * j + h;
+            const f32x4 x = *reinterpret_cast<const f32x4*>(rows + 512 * r + 16 * (c ^ r));
+            if (r < left) *reinterpret_cast<f32x4*>(p.partial.sums + (at + r * step) * kValue + 4 * c) = x;
+        }
+        if (h == 0 && c < left) p.partial.stats[at + c * step] = f32x2{mx, total};
     }
     return false;
 }
@@ -444,6 +478,5 @@ extern "C" int v1_latent_expanded(const v1_latent_expanded_args* a, void* stream
     // (as rows of s.parts one-tile parts)
     JoinParams j{Plan{nullptr, tokens, s.parts * kTileKeys, 1, 0}, p.partial, p.out, o_row, o_head, lse, heads, cu_q, batch,
                  s.blocks * kBlock};
-    hipLaunchKernelGGL(join_kernel<kValue>, dim3((uint32_t)tokens, (uint32_t)heads), dim3(256), 0, st, j);
-    return V1_LAUNCHED("latent_expanded: join");
+    return launch_join<kValue>(j, st, "latent_expanded: join");
 }

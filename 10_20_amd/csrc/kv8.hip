@@ -476,6 +476,5 @@ extern "C" int v1_kv8_attend(const v1_kv8_attend_args* a, void* stream) {
     rc = V1_LAUNCHED("kv8_attend");
     if (rc != V1_OK || need == 0) return rc;
     JoinParams j{plan, p.parts, p.out, o_row, o_head, lse, heads, nullptr, 0, 0};
-    hipLaunchKernelGGL(join_kernel<kDim>, dim3((uint32_t)rows, (uint32_t)heads), dim3(256), 0, st, j);
-    return V1_LAUNCHED("kv8_attend: join");
+    return launch_join<kDim>(j, st, "kv8_attend: join");
 }

@@ -630,6 +630,5 @@ extern "C" int v1_latent_attend(const v1_latent_attend_args* a, void* stream) {
                               : launch_absorbed<2, 2>(p, blocks, st);
     if (rc != V1_OK || need == 0) return rc;
     JoinParams j{plan, p.parts, p.out, o_row, o_head, lse, heads, nullptr, 0, 0};
-    hipLaunchKernelGGL(join_kernel<kLatent>, dim3((uint32_t)rows, (uint32_t)heads), dim3(256), 0, st, j);
-    return V1_LAUNCHED("latent_attend: join");
+    return launch_join<kLatent>(j, st, "latent_attend: join");
 }
