@@ -364,7 +364,8 @@ __global__ __launch_bounds__(256) void join_kernel(JoinParams p) {
 }
 
 // The same for rows of a few parts, known on the host: D / 4 threads for each (row,
-// head), several of them a work-group.
+// head), several of them a work-group.  (1024 rows of 16 heads x 128, four parts: 22 us
+// a work-group each, 8 so.)
 template <int D>
 __global__ __launch_bounds__(256) void join_few_kernel(JoinParams p) {
     constexpr int T = D / 4, G = 256 / T;

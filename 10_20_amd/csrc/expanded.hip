@@ -15,13 +15,19 @@
 // -> LDS two ahead; rows are laid with their 16-byte chunks XORed by the row so
 // that the fragments' reads meet different banks.
 //
-// Bound by the matrix units: 16 heads of 4096 queries over 32768 keys take 1187 us,
-// 1087 TFLOP/s (an 8192^3 library product: 1210).  With both waves of a SIMD in
-// the same step, matrix products and exponentials took turns: 1336 us; with the
-// fragments' reads where the compiler puts them, 1232.  Work-groups of 128 queries,
-// two to a CU: 1800 us, 326 against 312 us for 32 sequences of 100 queries and 4096
-// keys, and ahead only below some 300 keys a sequence (64 sequences of 300, 8 heads:
-// 70 against 78 us).
+// Bound by the matrix units at the clock under load: 16 heads of 4096 queries over
+// 32768 keys take 1136-1185 us by card, 1090-1134 TFLOP/s (an 8192^3 library product:
+// 1210).  On the way there: both waves of a SIMD in the same step, products and
+// exponentials by turns, 1336; fragments' reads where the compiler puts them 1233;
+// copies in one piece behind the barrier 1187.  Short sequences are bound by their
+// longest block, 8 us and 1.7 for each tile of its keys: 16 heads of 256 queries and
+// keys 15.6 us (18.7 with queries and outputs straight from and to the fragments, 32
+// rows' lines an instruction).
+// Work-groups of 128 queries, two to a CU, took 1800 us where this form took 1233, 326
+// against 312 for 32 sequences of 100 queries and 4096 keys, and were ahead only below
+// some 300 keys a sequence (64 sequences of 300, 8 heads: 70 against 78 us).  Parts by a
+// plan from the lengths, so that the longest blocks alone are cut, took 36 us for
+// nine prompts of 1 to 1000 tokens (39 without parts), but 95 for nine of 1500 (54).
 #include "attn.h"
 
 namespace v1 {

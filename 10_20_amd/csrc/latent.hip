@@ -142,12 +142,12 @@ __device__ __forceinline__ void copy_block(uint64_t src, uint32_t region) {
 //           once (2^-8 of each at most, as the output's rounding), and its codes
 //           transposed by the LDS read (ds_read_b64_tr_b8), exact in bf16.
 //
-// 1024 rows of 128 heads over 2048 chosen rows each: 680 us, 858 TFLOP/s (an 8192^3
+// 1024 rows of 128 heads over 2048 chosen rows each: 665 us, 834 TFLOP/s (an 8192^3
 // library product: 1210), bound by the issue of the two waves of a SIMD: a tile of
 // 64 heads is 72 products of 16 cycles a wave, and a conversion or fold for every
-// third of them cycles; 14 of a work-group's 80 us are its start and end.  128
-// rows of 16 heads: 49 us, 3.5 TB/s, in the loop the 6.1 TB/s at which memory gives
-// random rows of 656 bytes.  7 contexts of 5000 to 131072, 64 heads: 73 us, 9 of
+// third of their cycles; 12 of a work-group's 80 us are its start and end.  128
+// rows of 16 heads: 47 us, 3.6 TB/s, in the loop the 6.1 TB/s at which memory gives
+// random rows of 656 bytes.  7 contexts of 5000 to 131072, 64 heads: 71 us, 9 of
 // them the join.  On the way: all eight waves doing both halves, a tile at a time,
 // 2786 us for the first; scorers and multipliers apart 1280; products between the
 // conversions and the copies 768; tiles by blocks of 16 rows 680.
@@ -502,32 +502,62 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
     __syncthreads();
     const bool whole = it.parts == 1;
     const bool none = !(lds.seen[0] | lds.seen[1] | lds.seen[2] | lds.seen[3]);  // no key attended
+    // The sums leave through the tiles' memory, a head's columns end to end: as they
+    // lie in the registers a store would be 16 heads' pieces of 32 or 64 bytes.
+    uint8_t* const rows = lds.tile[0] + wave * (HB * 256);
+    static_assert(4 * HB * 256 <= 3 * kTileBytes, "a wave's rows of 256 bytes");
+    if (whole) {
+        float inv[PT];
 #pragma unroll
-    for (int ht = 0; ht < PT; ++ht) {
-        const int32_t h = 16 * ht + c, head = head0 + h;
-        if (head >= p.heads) continue;
-        float sum = lds.total[0][h];
+        for (int ht = 0; ht < PT; ++ht) {
+            const int32_t h = 16 * ht + c, head = head0 + h;
+            float sum = lds.total[0][h];
 #pragma unroll
-        for (int k = 1; k < KQ; ++k) sum += lds.total[k][h];
-        const float top = none ? -__builtin_inff() : lds.top[0][h];
-        if (whole) {
-            const float inv = 1.0f / sum;
-            uint16_t* out = p.out + it.row * p.o_row + head * p.o_head + wave * 128 + 4 * g;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-                *reinterpret_cast<u32x2*>(out + 16 * d) =
-                    none ? u32x2{0, 0} : u32x2{pack_bf16(acc[d][ht][0] * inv, acc[d][ht][1] * inv),
-                                               pack_bf16(acc[d][ht][2] * inv, acc[d][ht][3] * inv)};
-            if (p.lse && wave == 0 && g == 0)
-                p.lse[(int64_t)it.row * p.heads + head] = none ? top : (top + __builtin_amdgcn_logf(sum)) * kLn2;
-        } else {
-            const int64_t at = (int64_t)index * p.heads + head;
-            float* o = p.parts.sums + at * kLatent + wave * 128 + 4 * g;
+            for (int k = 1; k < KQ; ++k) sum += lds.total[k][h];
+            inv[ht] = 1.0f / sum;
+            if (p.lse && wave == 0 && g == 0 && head < p.heads)
+                p.lse[(int64_t)it.row * p.heads + head] =
+                    none ? -__builtin_inff() : (lds.top[0][h] + __builtin_amdgcn_logf(sum)) * kLn2;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
-                *reinterpret_cast<f32x4*>(o + 16 * d) = none ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[d][ht];
-            if (wave == 0 && g == 0) p.parts.stats[at] = f32x2{top, none ? 0.f : sum};
+                *reinterpret_cast<u32x2*>(rows + 256 * h + 8 * ((4 * d + g) ^ (2 * c))) =
+                    none ? u32x2{0, 0} : u32x2{pack_bf16(acc[d][ht][0] * inv[ht], acc[d][ht][1] * inv[ht]),
+                                               pack_bf16(acc[d][ht][2] * inv[ht], acc[d][ht][3] * inv[ht])};
         }
+        wait_lds();
+        uint16_t* out = p.out + it.row * p.o_row + wave * 128 + 4 * (lane & 31);
+#pragma unroll
+        for (int j = 0; j < HB / 2; ++j) {
+            const int32_t h = 2 * j + (lane >> 5);
+            const u32x2 x = *reinterpret_cast<const u32x2*>(rows + 256 * h + 8 * ((lane & 31) ^ (2 * (h & 15))));
+            if (head0 + h < p.heads) *reinterpret_cast<u32x2*>(out + (head0 + h) * p.o_head) = x;
+        }
+        return;
+    }
+    const int64_t at = (int64_t)index * p.heads + head0;
+    if (wave == 0 && lane < HB && head0 + lane < p.heads) {
+        float sum = lds.total[0][lane];
+#pragma unroll
+        for (int k = 1; k < KQ; ++k) sum += lds.total[k][lane];
+        p.parts.stats[at + lane] = f32x2{none ? -__builtin_inff() : lds.top[0][lane], none ? 0.f : sum};
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int ht = 0; ht < PT; ++ht)
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+                *reinterpret_cast<f32x4*>(rows + 256 * (16 * ht + c) + 16 * ((4 * d + g) ^ c)) =
+                    none ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[4 * half + d][ht];
+        wait_lds();
+#pragma unroll
+        for (int j = 0; j < HB / 4; ++j) {
+            const int32_t h = 4 * j + g;
+            const f32x4 x = *reinterpret_cast<const f32x4*>(rows + 256 * h + 16 * (c ^ (h & 15)));
+            if (head0 + h < p.heads)
+                *reinterpret_cast<f32x4*>(p.parts.sums + (at + h) * kLatent + wave * 128 + 64 * half + 4 * c) = x;
+        }
+        wait_lds();
     }
 }
 
