@@ -20,8 +20,8 @@ constexpr int kMaxGroup = 16;  // query heads of a KV head: the columns of a fra
 // rounded again at the new scale (off by half a step once more for each growth).
 // Bound by latency (a page and head is 16 KB at most): the request is found from the
 // lengths by every work-group, its page and the scale by two loads more.  128
-// requests of a token, 8 heads: 8.8 us; 4096 tokens of three requests: 12 us, 25 MB
-// at 2.1 TB/s.
+// requests of a token, 8 heads: 8.8 us; 4096 tokens of three requests: 9.1 us, 25 MB
+// at 2.8 TB/s (11 with the tokens asked for behind the page and divided one by one).
 struct Kv8StoreParams {
     const uint16_t* x[2];  // k, v
     int64_t x_token[2], x_head[2];
@@ -67,23 +67,26 @@ __global__ __launch_bounds__(256) void kv8_store_kernel(Kv8StoreParams p) {
     const int32_t entry = start / kTileKeys + left;
     if (entry >= p.table_len) return;
     const int32_t page = p.table[request * p.table_stride + entry];
-    if (page < 0 || page >= p.pages) return;
     const int64_t first = (int64_t)entry * kTileKeys;
-    const int32_t a = (int32_t)max((int64_t)start - first, (int64_t)0);                       // rows a .. b - 1 of the page are new
+    const int32_t a = (int32_t)max((int64_t)start - first, (int64_t)0);  // rows a .. b - 1 of the page are new
     const int32_t b = (int32_t)min((int64_t)start + n - first, (int64_t)kTileKeys);
-    const int64_t token0 = lo + (first - start);                                               // of the page's row 0
-
-    uint8_t* codes = p.pool[w] + page * p.page[w] + head * p.head[w];
-    float* scale_at = p.scale[w] + page * p.s_page[w] + head;
+    const int64_t token0 = lo + (first - start);  // of the page's row 0
     const int32_t row = (int32_t)threadIdx.x / 16, d = 8 * ((int32_t)threadIdx.x % 16);
-    u32x4 x[4];
-    float amax = 0.f;
+    u32x4 x[4];  // (asked for beside the page)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int32_t r = row + 16 * i;
         x[i] = u32x4{0, 0, 0, 0};
         if (r >= a && r < b)
             x[i] = *reinterpret_cast<const u32x4*>(p.x[w] + (token0 + r) * p.x_token[w] + head * p.x_head[w] + d);
+    }
+    if (page < 0 || page >= p.pages) return;
+    uint8_t* codes = p.pool[w] + page * p.page[w] + head * p.head[w];
+    float* scale_at = p.scale[w] + page * p.s_page[w] + head;
+    const float old = a > 0 ? *scale_at : 0.f;
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
             amax = fmaxf(amax, fmaxf(finite_abs(__uint_as_float(x[i][k] << 16)),
@@ -92,7 +95,6 @@ __global__ __launch_bounds__(256) void kv8_store_kernel(Kv8StoreParams p) {
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off, kWave));
     if (lane == 0) amax_of[wave] = amax;
-    const float old = a > 0 ? *scale_at : 0.f;
     __syncthreads();
     amax = fmaxf(fmaxf(amax_of[0], amax_of[1]), fmaxf(amax_of[2], amax_of[3]));
     const float need = exp2i(scale_exponent(amax));
@@ -100,6 +102,9 @@ __global__ __launch_bounds__(256) void kv8_store_kernel(Kv8StoreParams p) {
     if (threadIdx.x == 0) *scale_at = scale;
     const bool grew = a > 0 && scale > old;
     const float again = old / scale;  // (scale is a power of two where it grew)
+    // (a power of two, unless the caller's old one is not: x / scale is x * inv, exactly)
+    const bool power = __builtin_amdgcn_readfirstlane((__float_as_uint(scale) & 0x807fffffu) == 0 && scale >= 0x1p-126f && scale <= 0x1p120f);
+    const float inv = 1.0f / scale;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int32_t r = row + 16 * i;
@@ -108,8 +113,15 @@ __global__ __launch_bounds__(256) void kv8_store_kernel(Kv8StoreParams p) {
             float v[8];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                v[2 * k] = __uint_as_float(x[i][k] << 16) / scale;
-                v[2 * k + 1] = __uint_as_float(x[i][k] & 0xffff0000u) / scale;
+                v[2 * k] = __uint_as_float(x[i][k] << 16);
+                v[2 * k + 1] = __uint_as_float(x[i][k] & 0xffff0000u);
+            }
+            if (power) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] *= inv;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] /= scale;
             }
             *at = u32x2{codes4(v[0], v[1], v[2], v[3]), codes4(v[4], v[5], v[6], v[7])};
         } else if (grew && r < a) {
