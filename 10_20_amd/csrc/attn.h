@@ -139,7 +139,7 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 //              176 (103), 48 contexts of 4 KV heads in 8 bits 376 (305).
 constexpr int kTileKeys = 64;
 constexpr int kPlanRows = 256;
-constexpr int32_t kMostKeys = INT32_MAX - kTileKeys;  // (the last tile's positions stay below 2^31)
+constexpr int32_t kMostKeys = INT32_MAX - 32 * kTileKeys;  // (positions of the tiles asked for ahead stay below 2^31)
 
 struct Plan {
     const int32_t* lens;  // NULL: `keys` keys in every row

@@ -138,9 +138,12 @@ __device__ __forceinline__ void copy_block(uint64_t src, uint32_t region) {
 //   softmax the key groups exchange their maxima through LDS; probabilities and
 //           their sums stay fp32.
 //   output  O^T = C^T P^T: a wave takes a block of 128 columns of all heads: the
-//           probabilities times their keys' scale of that block, rounded to bf16
-//           once (2^-8 of each at most, as the output's rounding), and its codes
-//           transposed by the LDS read (ds_read_b64_tr_b8), exact in bf16.
+//           probabilities times their keys' scale of that block, and its codes
+//           transposed by the LDS read (ds_read_b64_tr_b8), exact in bf16.  Up to 32
+//           heads the former are two bf16 numbers, which leaves 2^-17 (1 us of 44 for
+//           128 rows of 16 heads, 20 of 265 for 1024 rows of 32); 64 heads round them
+//           once (2^-9 of each at most, as the output is), since the second products
+//           and their 32 registers would cost more than the waves have.
 //
 // 1024 rows of 128 heads over 2048 chosen rows each: 665 us, 834 TFLOP/s (an 8192^3
 // library product: 1210), bound by the issue of the two waves of a SIMD: a tile of
@@ -155,6 +158,7 @@ template <int HT, int HG>
 __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
     constexpr int HB = 16 * HT * HG, KT = HG, KQ = 4 / HG, RPW = kRegionRows, GT = kWave / RPW;
     constexpr int DT = 8, PT = HB / 16;
+    constexpr bool TWICE = HB < 64;  // probabilities in two bf16 numbers
     extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
     auto& lds = *reinterpret_cast<AbsorbedLds<HT, HG>*>(lds_raw);
     const int32_t wave = __builtin_amdgcn_readfirstlane((int32_t)threadIdx.x / kWave) & 3;
@@ -445,7 +449,7 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
         asm volatile("" : "+v"(g), "+v"(c));
         wait_barrier<kCopies>();
         begin_tile(t + 2);
-        Frag pf[2][PT];
+        Frag pf[2][PT], rest[2][TWICE ? PT : 1];
         float keep[PT];
         bool any = false;
 #pragma unroll
@@ -461,11 +465,16 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
             for (int h = 0; h < PT; ++h) {
                 const f32x4 x = *reinterpret_cast<const f32x4*>(&lds.prob[16 * h + c][4 * ((8 * ks + 2 * g) ^ c)]);
                 const f32x4 y = *reinterpret_cast<const f32x4*>(&lds.prob[16 * h + c][4 * ((8 * ks + 2 * g + 1) ^ c)]);
-                pf[ks][h].w[0] = pack_bf16(x[0] * a[0], x[1] * a[1]);
-                pf[ks][h].w[1] = pack_bf16(x[2] * a[2], x[3] * a[3]);
-                pf[ks][h].w[2] = pack_bf16(y[0] * b[0], y[1] * b[1]);
-                pf[ks][h].w[3] = pack_bf16(y[2] * b[2], y[3] * b[3]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float p0 = i < 2 ? x[2 * i] * a[2 * i] : y[2 * i - 4] * b[2 * i - 4];
+                    const float p1 = i < 2 ? x[2 * i + 1] * a[2 * i + 1] : y[2 * i - 3] * b[2 * i - 3];
+                    const uint32_t w = pack_bf16(p0, p1);
+                    pf[ks][h].w[i] = w;
+                    if constexpr (TWICE) rest[ks][h].w[i] = pack_bf16(p0 - __uint_as_float(w << 16), p1 - __uint_as_float(w & 0xffff0000u));
+                }
                 asm volatile("" : "+v"(pf[ks][h].u));  // (here, not where they are used)
+                if constexpr (TWICE) asm volatile("" : "+v"(rest[ks][h].u));
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -482,6 +491,7 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
 #pragma unroll
                 for (int h = 0; h < PT; ++h) {
                     acc[d.value][h] = mfma16(a[d.value & 1], pf[ks.value][h], acc[d.value][h]);
+                    if constexpr (TWICE) acc[d.value][h] = mfma16(a[d.value & 1], rest[ks.value][h], acc[d.value][h]);
                     if (h == 0 && d.value + 1 < DT)
                         a[(d.value + 1) & 1] = bf16_of_codes((uint32_t)v[ks.value][(d.value + 1) % DT][0],
                                                              (uint32_t)v[ks.value][(d.value + 1) % DT][1]);
@@ -562,19 +572,21 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
 }
 
 // Heads of a work-group: 16, 32 or 64 (more: several work-groups a row).  More heads
-// share each key's conversion (1024 rows of 64 heads and 2048 keys: 16 / 32 / 64 of
-// them take 710 / 460 / 365 us); fewer start and end sooner.  So the fewest
-// whose work-groups all run at once and have little to do:
-//   8 rows, 64 heads, 2048 keys      16.7 / 20.0 / 25.6 us   (4 tiles a CU at 16)
-//   20 rows, 64 heads, to 6000 keys  35.4 / 31.9 / 35.4      (29 at 16, 15 at 32)
-//   128 rows, 64 heads, 2048 keys    87.2 / 60.0 / 66.5      (32 at 32)
-//   7 rows, 64 heads, to 60000 keys  76.5 / 61.0 / 57.1      (51 at 32)
-//   160 rows, 64 heads, 2048 keys     128 /  109 / 81.0      (320 work-groups at 32)
+// share each key's conversion; fewer start and end sooner.  So the fewest whose
+// work-groups all run at once with at most eight tiles a CU.  64 heads, 2048 keys, in
+// work-groups of 16 / 32 / 64:
+//      8 rows  18.6 / 21.0 / 25.7 us  (4 tiles at 16)
+//     32 rows  34.9 / 34.2 / 36.0     (16 at 16, 8 at 32)
+//     64 rows  48.4 / 47.3 / 43.9
+//    128 rows  95.5 / 73.5 / 63.9
+//   1024 rows   754 /  534 /  360
 inline int32_t absorbed_heads(int32_t rows, int32_t heads, int32_t keys) {
     const int64_t cus = device_cus(), tiles = cdiv(keys, kTileKeys);
-    const int64_t of16 = (int64_t)rows * cdiv(heads, 16), of32 = (int64_t)rows * cdiv(heads, 32);
-    if (heads <= 16 || (of16 <= cus && of16 * tiles <= 8 * cus)) return 16;
-    return heads <= 32 || (of32 <= cus && of32 * tiles <= 32 * cus) ? 32 : 64;
+    auto few = [&](int32_t of) {
+        const int64_t groups = (int64_t)rows * cdiv(heads, of);
+        return heads <= of || (groups <= cus && groups * tiles <= 8 * cus);
+    };
+    return few(16) ? 16 : few(32) ? 32 : 64;
 }
 
 // (One work-group a CU.  A part's start is two to four dependent loads, its sums

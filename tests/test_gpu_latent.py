@@ -71,7 +71,7 @@ def rand_q(g, rows, heads, amp=1.5):
 @gpu
 @pytest.mark.parametrize("rows,heads,keys", [(1, 1, 1), (1, 16, 64), (3, 16, 65), (2, 5, 130), (5, 24, 200), (3, 32, 63),
                                              (2, 64, 129), (2, 40, 1000), (1, 128, 2048), (300, 16, 100), (270, 64, 70),
-                                             (9, 100, 33), (2, 200, 257), (7, 17, 2047)])
+                                             (9, 100, 33), (2, 200, 257), (7, 17, 2047), (24, 50, 1900)])
 def test_pool_rows(rows, heads, keys):
     print("latent", rows, heads, keys, flush=True)
     g = torch.Generator(device=DEV).manual_seed(rows * 1000 + heads + keys)
