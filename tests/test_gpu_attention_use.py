@@ -7,7 +7,10 @@ operators' own tests."""
 import contextlib
 import importlib
 import math
+import re
+import struct
 import threading
+from pathlib import Path
 
 import pytest
 import torch
@@ -309,3 +312,18 @@ def test_too_many_positions():
              b"keys")):
         assert getattr(h, name)(L.PACKED[name].pack(*fields), None) == L.V1_ERR_INVALID, name
         assert text in h.v1_last_error(), h.v1_last_error()
+
+
+def test_argument_structures_match_the_header():
+    """The packed formats hold the header's fields in its order, padded as C does."""
+    L = pkg("_lib")
+    text = re.sub(r"/\*.*?\*/", "", (Path(__file__).resolve().parents[1] / "include" / "v1idx.h").read_text(), flags=re.S)
+    for name, packed in L.PACKED.items():
+        body = re.search(r"typedef struct \{([^}]*)\} %s_args;" % name, text).group(1)
+        want = ""
+        for line in body.split(";"):
+            kind = "q" if "*" in line or "int64_t" in line else "i" if "int32_t" in line else "f" if "float" in line else ""
+            want += kind * (line.count(",") + 1) if kind else ""
+        got = "".join(c * int(n or 1) for n, c in re.findall(r"(\d*)([a-z])", packed.format) if c != "x")
+        assert got == want, name
+        assert packed.size == -(-struct.calcsize(want) // 8) * 8, name

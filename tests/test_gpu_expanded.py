@@ -135,6 +135,22 @@ def test_values_that_are_not_finite(heads, n):
 
 
 @gpu
+def test_rows_past_32_bits():
+    """Queries, keys, rope keys and outputs whose last rows lie 2^32 numbers behind the first."""
+    print("expanded far rows", flush=True)
+    n, heads, row = 300, 2, 1 << 24
+    q, kv, rope, cu, _ = inputs(11, [n], [n], heads)
+    base = torch.empty(n * row, device=DEV, dtype=torch.bfloat16)
+    far = lambda t, at: base.as_strided((n, *t.shape[1:]), (row, *t.stride()[1:]), at).copy_(t)
+    fq, fkv, frope = far(q, 0), far(kv, 8192), far(rope, 16384)
+    out = base.as_strided((n, heads, 128), (row, 128, 1), 32768).fill_(7)
+    _, lse = LT.attend_expanded(fq, fkv, frope, cu, out=out, return_lse=True)
+    check(out, lse, q, kv, rope, [n], [n])
+    whole, whole_lse = LT.attend_expanded(q, kv, rope, cu, return_lse=True)
+    assert torch.equal(out, whole) and torch.equal(lse, whole_lse)
+
+
+@gpu
 def test_lengths_outside_the_tensors():
     """cu_q and cu_k past the tensors or descending are clamped."""
     print("expanded clamped", flush=True)
