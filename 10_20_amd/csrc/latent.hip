@@ -426,7 +426,6 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
     // and the waits count the same for every tile)
     copy_tile(0);
     copy_tile(1);
-    copy_tile(2);
     i32x2 v[2][DT];  // this wave's codes of the last tile, transposed: its buffer is free for the next copies
     // lanes 2r, 2r + 1 of a group hand in 16 columns of key 8g + r; lane c gets column c of its eight keys
     auto fetch = [&](int32_t t, int ks) __attribute__((always_inline)) {
@@ -440,8 +439,9 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
                 v[ks][d] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
                     (__attribute__((address_space(3))) i32x2*)((at ^ (16 * q)) + 1024 * (d / 4)));
     };
-    wait_barrier<2 * kCopies>();
+    wait_barrier<kCopies>();
     fetch(0, 0);
+    copy_tile(2);  // (asked for before, it held the first scores up)
     lds_barrier();
     fetch(0, 1);
 #pragma unroll 1
