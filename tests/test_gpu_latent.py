@@ -116,6 +116,48 @@ def test_pages_masks_and_lengths(heads, keys, shared):
 
 
 @gpu
+@pytest.mark.parametrize("rows,heads,keys", [(700, 16, 1), (700, 16, 64), (600, 64, 100), (530, 100, 150), (300, 33, 200), (1100, 7, 257),
+                                             (520, 64, 300), (2100, 16, 130)])
+def test_many_rows_of_equal_capacity(rows, heads, keys):
+    """More rows than CUs, without lengths: rows without keys, with bad pages and with
+    all keys among them; what no row attends holds NaN."""
+    print("latent many", rows, heads, keys, flush=True)
+    g = torch.Generator(device=DEV).manual_seed(rows + keys)
+    pages, entries = 60, 11
+    pool, q = rand_pool(g, pages * 16), rand_q(g, rows, heads)
+    table = torch.stack([torch.randperm(pages, device=DEV, generator=g)[:entries] for _ in range(rows)]).to(torch.int32)
+    table[::3, 3], table[1::3, 5] = -1, pages
+    ids = torch.randint(0, entries * 16, (rows, keys), device=DEV, generator=g, dtype=torch.int32)
+    ids[torch.rand(ids.shape, device=DEV, generator=g) < 0.2] = -1
+    ids[5::7] = -1
+    ids[6::7, : keys // 2] = -1
+    ids[-1] = -1
+    slots, used = [], torch.zeros(pages * 16, device=DEV, dtype=torch.bool)
+    for r in range(rows):
+        i = ids[r].long()
+        i = i[i >= 0]
+        t = table[r].long()[i >> 4]
+        slots.append((t * 16 + (i & 15))[(t >= 0) & (t < pages)])
+        used[slots[-1]] = True
+    used[40] = False
+    slots = [s[s != 40] for s in slots]
+    for r in range(rows):
+        at = torch.where(ids[r] < 0, 0, ids[r]).long()
+        t = table[r].long()[at >> 4].clamp(0, pages - 1) * 16 + (at & 15)
+        ids[r, (t == 40) & (ids[r] >= 0)] = -1
+    pool[~used] = 0x7f
+    pool[~used, 640:] = 0xff
+    out, lse = LT.attend(q, pool, ids, table=table, page_bits=4, return_lse=True)
+    some = list(range(0, rows, max(1, rows // 97))) + [rows - 1]
+    check(out[some], lse[some], q[some], pool, [slots[r] for r in some], 192 ** -0.5)
+    # a row alone gives what it gives among the others
+    for r in (0, 6, rows // 2, rows - 2):
+        one, one_lse = LT.attend(q[r:r + 1].expand(rows, -1, -1), pool, ids[r:r + 1].expand(rows, -1), table=table[r:r + 1].expand(rows, -1),
+                                 page_bits=4, return_lse=True)
+        assert torch.equal(one, out[r:r + 1].expand_as(one)) and torch.equal(one_lse, lse[r:r + 1].expand_as(one_lse))
+
+
+@gpu
 @pytest.mark.parametrize("rows,heads,entries", [(5, 16, 40), (3, 128, 33), (257, 16, 3), (40, 33, 7), (70, 128, 40),
                                                 (20, 64, 300), (3, 17, 2000)])
 def test_whole_contexts(rows, heads, entries):
