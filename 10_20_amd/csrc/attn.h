@@ -132,9 +132,10 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 // them.  Two rules, both functions of the call's shapes and lengths alone:
 //   chunk > 0  every row in the same number of parts (rows of one capacity);
 //   chunk == 0 rows of different lengths (`lens` on the device, at most
-//              kPlanRows of them): parts of at most about sum(tiles) / target
-//              tiles, at most target + rows of them, found by every work-group
-//              from the lengths.  By the capacity instead, 7 rows of 64 heads and
+//              kPlanRows of them): the smallest of nine sizes of a part, from
+//              sum(tiles) / slots to sum(tiles) / target, with no more than
+//              `slots` parts, else the last (at most target + rows parts), found
+//              by every work-group from the lengths.  By the capacity instead, 7 rows of 64 heads and
 //              up to 60000 latent rows take 72 us (57 so), 40 rows of up to 30000
 //              176 (103), 48 contexts of 4 KV heads in 8 bits 376 (305).
 constexpr int kTileKeys = 64;
@@ -143,7 +144,7 @@ constexpr int32_t kMostKeys = INT32_MAX - 32 * kTileKeys;  // (positions of the 
 
 struct Plan {
     const int32_t* lens;  // NULL: `keys` keys in every row
-    int32_t rows, keys, chunk, target;
+    int32_t rows, keys, chunk, target, slots;
 };
 
 struct Item {
@@ -176,14 +177,30 @@ __device__ __forceinline__ int32_t plan_parts(const Plan& p, int32_t (&keys)[4],
         tiles += tiles_of(keys[i]);
     }
     const int32_t all = __shfl((int32_t)wave_inclusive_sum((uint32_t)tiles), kWave - 1, kWave);
-    const int32_t chunk = max(1, (all + p.target - 1) / p.target);
-    int32_t mine = 0;
+    const int32_t most = max(1, (all + p.target - 1) / p.target), least = max(1, (all + p.slots - 1) / p.slots);
+    const int32_t step = max(1, (most - least + 7) / 8);
+    int32_t mine, upto, lo = 0, hi = 8;
+    for (;;) {
+        const int32_t at = (lo + hi) / 2, chunk = at == 8 ? most : min(least + at * step, most);
+        const float inv = 1.0f / (float)chunk;
+        mine = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        parts[i] = 4 * lane + i < p.rows ? max(1, (tiles_of(keys[i]) + chunk - 1) / chunk) : 0;
-        mine += parts[i];
+        for (int i = 0; i < 4; ++i) {
+            // ceil(tiles / chunk): the product is off by less than one (tiles stay below 2^26, parts below 2^22)
+            const int32_t n = tiles_of(keys[i]);
+            int32_t q = (int32_t)((float)n * inv);
+            q -= q * chunk > n;
+            q += q * chunk < n;
+            q += q * chunk < n;
+            parts[i] = 4 * lane + i < p.rows ? max(1, q) : 0;
+            mine += parts[i];
+        }
+        upto = (int32_t)wave_inclusive_sum((uint32_t)mine);
+        if (lo == hi) break;
+        if (__shfl(upto, kWave - 1, kWave) <= p.slots) hi = at;
+        else lo = at + 1;
     }
-    return (int32_t)wave_inclusive_sum((uint32_t)mine) - mine;
+    return upto - mine;
 }
 
 // Work item `index`; false: there is none.  (Every wave finds it by itself.)
@@ -225,34 +242,13 @@ __device__ __forceinline__ bool find_item(const Plan& p, int32_t index, Item& it
     return true;
 }
 
-// First work item and number of parts of a row.
-__device__ __forceinline__ void items_of(const Plan& p, int32_t row, int32_t& first, int32_t& parts) {
-    if (p.chunk > 0) {
-        parts = max(1, (tiles_of(p.keys) + p.chunk - 1) / p.chunk);
-        first = row * parts;
-        return;
-    }
-    int32_t keys[4], of[4];
-    int32_t at = plan_parts(p, keys, of), mine_at = 0, mine = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if ((row & 3) == i) {
-            mine_at = at;
-            mine = of[i];
-        }
-        at += of[i];
-    }
-    first = __shfl(mine_at, row >> 2, kWave);
-    parts = __shfl(mine, row >> 2, kWave);
-}
-
 // Whether the device's lengths may decide: few rows, and their tiles can be added in 32 bits.
 inline bool planned(int64_t rows, int64_t tiles) { return rows <= kPlanRows && rows * tiles < 1ll << 30; }
 
 // Most work items that a call can have.
 inline int64_t items_at_most(const Plan& p) {
     if (p.chunk > 0) return (int64_t)p.rows * std::max<int64_t>(1, cdiv(cdiv(p.keys, kTileKeys), p.chunk));
-    return (int64_t)p.rows + p.target;
+    return std::max<int64_t>(p.slots, (int64_t)p.rows + p.target);
 }
 
 // Tiles of a part of rows of `tiles` tiles: the number of parts whose work-groups
@@ -269,19 +265,23 @@ inline int32_t chunk_for(int64_t rows, int64_t tiles, int64_t slots, int64_t sta
     return (int32_t)std::max<int64_t>(1, best);
 }
 
-// Workspace: sums [items][heads][dims], then maxima and totals [items][heads].
+// Workspace: sums [items][heads][dims], maxima and totals [items][heads], and of a
+// planned call each row's first item and number of parts, written with its first part.
 struct Parts {
     float* sums;
     f32x2* stats;
+    i32x2* of_row;
 };
 
-inline int64_t parts_bytes(int64_t items, int32_t heads, int32_t dims) {
-    return items * heads * (dims + 2) * (int64_t)sizeof(float);
+inline int64_t parts_bytes(const Plan& plan, int32_t heads, int32_t dims) {
+    return items_at_most(plan) * heads * (dims + 2) * (int64_t)sizeof(float) + (plan.chunk > 0 ? 0 : plan.rows * (int64_t)sizeof(i32x2));
 }
 
-inline Parts parts_at(void* ws, int64_t items, int32_t heads, int32_t dims) {
+inline Parts parts_at(void* ws, const Plan& plan, int32_t heads, int32_t dims) {
+    const int64_t items = items_at_most(plan);
     float* sums = static_cast<float*>(ws);
-    return {sums, reinterpret_cast<f32x2*>(sums + items * heads * dims)};
+    f32x2* stats = reinterpret_cast<f32x2*>(sums + items * heads * dims);
+    return {sums, stats, reinterpret_cast<i32x2*>(stats + items * heads)};
 }
 
 struct JoinParams {
@@ -332,8 +332,14 @@ __global__ __launch_bounds__(256) void join_kernel(JoinParams p) {
     const int32_t row = (int32_t)blockIdx.x, h = (int32_t)blockIdx.y, lane = (int32_t)threadIdx.x % kWave;
     const int32_t group = (int32_t)threadIdx.x / T, at4 = (int32_t)threadIdx.x % T;
     if (!joined_row(p, row)) return;
-    int32_t first, parts;
-    items_of(p.plan, row, first, parts);
+    int32_t parts, first;
+    if (p.plan.chunk > 0) {
+        parts = (tiles_of(p.plan.keys) + p.plan.chunk - 1) / p.plan.chunk;
+        first = row * parts;
+    } else {
+        const i32x2 of = p.parts.of_row[row];
+        first = of[0], parts = of[1];
+    }
     if (parts <= 1) return;
     float top = -__builtin_inff(), total = 0.f;
     for (int32_t i = lane; i < parts; i += kWave) top = fmaxf(top, p.parts.stats[(int64_t)(first + i) * p.heads + h][0]);

@@ -432,6 +432,9 @@ inline ExpandedShape expanded_shape(int32_t tokens, int32_t keys, int32_t batch,
     return s;
 }
 
+// For the join: as many rows of s.parts parts of a tile each.
+inline Plan rows_of_parts(int32_t tokens, const ExpandedShape& s) { return Plan{nullptr, tokens, s.parts * kTileKeys, 1, 0, 0}; }
+
 }  // namespace
 }  // namespace v1
 
@@ -441,7 +444,7 @@ extern "C" int64_t v1_latent_expanded_workspace(int32_t tokens, int32_t keys, in
                                                 int32_t max_q) {
     if (tokens <= 0 || keys <= 0 || batch <= 0 || heads <= 0 || max_q <= 0) return 0;
     const ExpandedShape s = expanded_shape(tokens, keys, batch, heads, max_q);
-    return s.parts == 1 ? 0 : attn::parts_bytes((int64_t)tokens * s.parts, heads, kValue);
+    return s.parts == 1 ? 0 : attn::parts_bytes(rows_of_parts(tokens, s), heads, kValue);
 }
 
 extern "C" int v1_latent_expanded(const v1_latent_expanded_args* a, void* stream) {
@@ -472,7 +475,7 @@ extern "C" int v1_latent_expanded(const v1_latent_expanded_args* a, void* stream
     ExpandedParams p{static_cast<const uint16_t*>(q), q_row, q_head, static_cast<const uint16_t*>(kv), kv_row, kv_head,
                      static_cast<const uint16_t*>(rope), rope_row, cu_q, cu_k, tokens, keys, batch, heads, s.blocks,
                      causal, s.parts, xcds, (int32_t)group, scale * kLog2e, static_cast<uint16_t*>(out), o_row, o_head, lse,
-                     parts_at(workspace, (int64_t)tokens * s.parts, heads, kValue)};
+                     parts_at(workspace, rows_of_parts(tokens, s), heads, kValue)};
     const hipStream_t st = as_stream(stream);
     static OncePerDevice once;
     constexpr size_t bytes = kBuffers * sizeof(ExpandedTile);
@@ -481,8 +484,7 @@ extern "C" int v1_latent_expanded(const v1_latent_expanded_args* a, void* stream
     hipLaunchKernelGGL(expanded_kernel, dim3((uint32_t)items), dim3(64 * kWaves), bytes, st, p);
     rc = V1_LAUNCHED("latent_expanded");
     if (rc != V1_OK || s.parts == 1) return rc;
-    // (as rows of s.parts one-tile parts)
-    JoinParams j{Plan{nullptr, tokens, s.parts * kTileKeys, 1, 0}, p.partial, p.out, o_row, o_head, lse, heads, cu_q, batch,
+    JoinParams j{rows_of_parts(tokens, s), p.partial, p.out, o_row, o_head, lse, heads, cu_q, batch,
                  s.blocks * kBlock};
     return launch_join<kValue>(j, st, "latent_expanded: join");
 }

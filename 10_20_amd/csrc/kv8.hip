@@ -195,11 +195,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_attend_kernel(Kv8Params p)
     auto& lds = *reinterpret_cast<Kv8Lds*>(lds_raw);
     const int32_t wave = __builtin_amdgcn_readfirstlane((int32_t)threadIdx.x / kWave);
     const int32_t lane = (int32_t)threadIdx.x % kWave, g = lane >> 4, c = lane & 15;
-    int32_t index = ((int32_t)blockIdx.x % 8) * p.spread + (int32_t)blockIdx.x / 8;
-    const int32_t sets = p.kv_heads / p.together, set = index % sets;
-    index /= sets;
+    const int32_t xcd = (int32_t)blockIdx.x % 8, turn = (int32_t)blockIdx.x / 8, sets = p.kv_heads / p.together;
+    const int32_t set = p.plan.chunk > 0 ? (xcd * p.spread + turn) % sets : turn % sets;
+    const int32_t index = p.plan.chunk > 0 ? (xcd * p.spread + turn) / sets : turn / sets * 8 + xcd;
     Item it;
     if (!find_item(p.plan, index, it)) return;
+    if (p.plan.chunk == 0 && it.part == 0 && set == 0 && threadIdx.x == 0) p.parts.of_row[it.row] = i32x2{index, it.parts};
     const int32_t streams = kWaves / p.together, stream = wave / p.together, kvh = set * p.together + wave % p.together;
     const int32_t mine = (it.tiles - stream + streams - 1) / streams;  // this wave's tiles: stream, stream + streams, ...
     const int32_t* ids = p.ids ? p.ids + it.row * p.ids_stride : nullptr;
@@ -402,8 +403,9 @@ inline int32_t kv8_together(int32_t kv_heads) { return kv_heads % 4 == 0 ? 4 : k
 inline Plan kv8_plan(const int32_t* lens, int32_t rows, int32_t kv_heads, int32_t keys, bool ragged) {
     const int64_t together = kv8_together(kv_heads), streams = kWaves / together, steps = cdiv(cdiv(keys, kTileKeys), streams);
     const int64_t slots = std::max<int64_t>(1, 2 * device_cus() * together / kv_heads);
-    Plan p{lens, rows, keys, 0, 0};
-    if (ragged && planned(rows, cdiv(keys, kTileKeys)) && rows < slots) p.target = (int32_t)std::max(slots - rows, (slots + 1) / 2);
+    Plan p{lens, rows, keys, 0, 0, (int32_t)slots};
+    if (ragged && keys > 0 && planned(rows, cdiv(keys, kTileKeys)) && rows < slots)
+        p.target = (int32_t)std::max(slots - rows, (slots + 1) / 2);
     else p.chunk = (int32_t)streams * chunk_for(rows, steps, slots, 2, 1);
     return p;
 }
@@ -444,7 +446,7 @@ extern "C" int64_t v1_kv8_attend_workspace(int32_t rows, int32_t kv_heads, int32
     if (rows <= 0 || kv_heads <= 0 || group <= 0 || keys <= 0) return 0;
     const attn::Plan plan = kv8_plan(nullptr, rows, kv_heads, keys, ragged != 0);
     const int64_t items = attn::items_at_most(plan);
-    return plan.chunk > 0 && items == rows ? 0 : attn::parts_bytes(items, kv_heads * group, kDim);
+    return plan.chunk > 0 && items == rows ? 0 : attn::parts_bytes(plan, kv_heads * group, kDim);
 }
 
 extern "C" int v1_kv8_attend(const v1_kv8_attend_args* a, void* stream) {
@@ -468,7 +470,8 @@ extern "C" int v1_kv8_attend(const v1_kv8_attend_args* a, void* stream) {
     if (pages == 0 || table_len == 0) keys = 0;
     const Plan plan = kv8_plan(lens, rows, kv_heads, keys, lens != nullptr);
     const int32_t together = kv8_together(kv_heads);
-    const int64_t items = items_at_most(plan), spread = cdiv(items * (kv_heads / together), 8);
+    const int64_t items = items_at_most(plan), sets = kv_heads / together;
+    const int64_t spread = plan.chunk > 0 ? cdiv(items * sets, 8) : cdiv(items, 8) * sets;
     const int64_t need = v1_kv8_attend_workspace(rows, kv_heads, group, keys, lens != nullptr);
     V1_REQUIRE(workspace_bytes >= need && (need == 0 || workspace != nullptr),
                "kv8_attend: workspace of %lld bytes needed", (long long)need);
@@ -479,7 +482,7 @@ extern "C" int v1_kv8_attend(const v1_kv8_attend_args* a, void* stream) {
                 {kp_page, vp_page}, {kp_token, vp_token}, {kp_head, vp_head},
                 {k_scale, v_scale}, {ks_page, vs_page}, pages, table, table_stride, table_len, ids, ids_stride, plan,
                 kv_heads, group, (int32_t)spread, together, scale * kLog2e, static_cast<uint16_t*>(out), o_row, o_head, lse,
-                parts_at(workspace, items, heads, kDim)};
+                parts_at(workspace, plan, heads, kDim)};
     static OncePerDevice once;
     int rc = allow_lds(once, reinterpret_cast<const void*>(kv8_attend_kernel), sizeof(Kv8Lds), "kv8_attend: LDS");
     if (rc != V1_OK) return rc;

@@ -167,11 +167,12 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
     int32_t g = lane >> 4, c = lane & 15;  // (opaque in the loops, as buffer_of)
 
     // work-groups reach the XCDs in turn: the splits of an item follow each other on one of them
-    const int32_t xcd = (int32_t)blockIdx.x % 8, turn = (int32_t)blockIdx.x / 8;
-    const int32_t index = xcd * p.spread + turn / p.splits, split = turn % p.splits;
+    const int32_t xcd = (int32_t)blockIdx.x % 8, turn = (int32_t)blockIdx.x / 8, split = turn % p.splits;
+    const int32_t index = p.plan.chunk > 0 ? xcd * p.spread + turn / p.splits : turn / p.splits * 8 + xcd;
     Item it;
     if (!find_item(p.plan, index, it)) return;
     const int32_t head0 = split * HB, tiles = it.tiles;
+    if (p.plan.chunk == 0 && it.part == 0 && split == 0 && threadIdx.x == 0) p.parts.of_row[it.row] = i32x2{index, it.parts};
 
     if (scorer) {
         const int32_t hg = wave / KQ, kq = wave % KQ;
@@ -594,8 +595,8 @@ inline int32_t absorbed_heads(int32_t rows, int32_t heads, int32_t keys) {
 inline Plan absorbed_plan(const int32_t* lens, int32_t rows, int32_t heads, int32_t keys, bool ragged) {
     const int32_t hb = absorbed_heads(rows, heads, keys);
     const int64_t splits = cdiv(heads, hb), tiles = cdiv(keys, kTileKeys), slots = std::max<int64_t>(1, device_cus() / splits);
-    Plan p{lens, rows, keys, 0, 0};
-    if (ragged && planned(rows, tiles) && rows < slots) p.target = (int32_t)std::max(slots - rows, (slots + 1) / 2);
+    Plan p{lens, rows, keys, 0, 0, (int32_t)slots};
+    if (ragged && keys > 0 && planned(rows, tiles) && rows < slots) p.target = (int32_t)std::max(slots - rows, (slots + 1) / 2);
     else p.chunk = chunk_for(rows, tiles, slots, 3, hb / 16);
     return p;
 }
@@ -637,7 +638,7 @@ extern "C" int64_t v1_latent_attend_workspace(int32_t rows, int32_t heads, int32
     if (rows <= 0 || heads <= 0 || keys <= 0) return 0;
     const attn::Plan plan = absorbed_plan(nullptr, rows, heads, keys, ragged != 0);
     const int64_t items = attn::items_at_most(plan);
-    return plan.chunk > 0 && items == rows ? 0 : attn::parts_bytes(items, heads, kLatent);
+    return plan.chunk > 0 && items == rows ? 0 : attn::parts_bytes(plan, heads, kLatent);
 }
 
 extern "C" int v1_latent_attend(const v1_latent_attend_args* a, void* stream) {
@@ -665,7 +666,7 @@ extern "C" int v1_latent_attend(const v1_latent_attend_args* a, void* stream) {
     AbsorbedParams p{static_cast<const uint16_t*>(q), q_row, q_head, static_cast<const uint8_t*>(pool), pool_rows,
                      pool_stride_bytes, map, map_len, map_stride, map_shift, ids, ids_stride, plan, heads,
                      (int32_t)splits, (int32_t)spread, scale * kLog2e, static_cast<uint16_t*>(out), o_row, o_head, lse,
-                     parts_at(workspace, items, heads, kLatent)};
+                     parts_at(workspace, plan, heads, kLatent)};
     const hipStream_t st = as_stream(stream);
     const int rc = hb == 16   ? launch_absorbed<1, 1>(p, blocks, st)
                    : hb == 32 ? launch_absorbed<2, 1>(p, blocks, st)

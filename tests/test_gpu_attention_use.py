@@ -327,3 +327,25 @@ def test_argument_structures_match_the_header():
         got = "".join(c * int(n or 1) for n, c in re.findall(r"(\d*)([a-z])", packed.format) if c != "x")
         assert got == want, name
         assert packed.size == -(-struct.calcsize(want) // 8) * 8, name
+
+
+@gpu
+@pytest.mark.parametrize("ragged", [False, True])
+def test_nothing_to_attend(ragged):
+    """Tables, pools and ids without an entry: rows of zeros and -inf."""
+    print("nothing", ragged, flush=True)
+    rows = 3
+    q = torch.randn((rows, 4, 576), device=DEV).to(BF16)
+    lens = torch.full((rows,), 5, device=DEV, dtype=I32) if ragged else None
+    pool, none = torch.zeros((8, 656), device=DEV, dtype=torch.uint8), torch.zeros((rows, 0), device=DEV, dtype=I32)
+    pools = lambda pages: (*(torch.zeros((pages, 64, 2, 128), device=DEV, dtype=torch.uint8).view(kv8.F8) for _ in range(2)),
+                           *(torch.ones((pages, 2), device=DEV) for _ in range(2)))
+    table = torch.zeros((rows, 2), device=DEV, dtype=I32)
+    ids = torch.zeros((rows, 3), device=DEV, dtype=I32)
+    narrow = q[..., :128].contiguous()
+    for out, lse in (LT.attend(q, pool, none, lens=lens, return_lse=True), LT.attend(q, pool, table=none, page_bits=6, lens=lens, return_lse=True),
+                     LT.attend(q, pool[:0], lens=lens, return_lse=True), LT.attend(q, pool[:0], ids, lens=lens, return_lse=True),
+                     K8.attend(narrow, *pools(4), none, lens, return_lse=True), K8.attend(narrow, *pools(0), table, lens, return_lse=True),
+                     K8.attend(narrow, *pools(4), table, lens, none, return_lse=True),
+                     K8.attend(narrow, *pools(0), table, lens, ids, return_lse=True)):
+        assert bool((out == 0).all()) and bool((lse == -math.inf).all())
