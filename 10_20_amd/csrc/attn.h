@@ -135,9 +135,13 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 //              kPlanRows of them): the smallest of nine sizes of a part, from
 //              sum(tiles) / slots to sum(tiles) / target, with no more than
 //              `slots` parts, else the last (at most target + rows parts), found
-//              by every work-group from the lengths.  By the capacity instead, 7 rows of 64 heads and
-//              up to 60000 latent rows take 72 us (57 so), 40 rows of up to 30000
-//              176 (103), 48 contexts of 4 KV heads in 8 bits 376 (305).
+//              by every work-group from the lengths.  By the capacity instead, 7 rows
+//              of 64 heads and up to 60000 latent rows take 69 us (58 so), 40 rows of
+//              up to 30000 171 (89), 48 contexts of 4 KV heads in 8 bits 337 (202).
+//              Parts go to the XCDs in turn, since their number is known there alone:
+//              a range of the most there could be for each XCD left the last ones
+//              without work (200 rows of 16 heads, up to 8000 latent rows: 157 us, 102
+//              so, and 98 with as many parts as run at once).
 constexpr int kTileKeys = 64;
 constexpr int kPlanRows = 256;
 constexpr int32_t kMostKeys = INT32_MAX - 32 * kTileKeys;  // (positions of the tiles asked for ahead stay below 2^31)

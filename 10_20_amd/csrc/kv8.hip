@@ -188,7 +188,7 @@ struct Kv8Lds {
 //           probabilities, times the page's V scale, rounded to bf16 once.
 //
 // Bound by memory: 48 contexts of 4096 to 65536 tokens, 4 KV heads of 8 query heads,
-// 203 us for 1.09 GB, 5.4 TB/s (a 1 GiB copy moves 5.2).  8 rows of 2048 chosen tokens, one KV head: 7 us
+// 202 us for 1.09 GB, 5.4 TB/s (a 1 GiB copy moves 5.2).  8 rows of 2048 chosen tokens, one KV head: 7 us
 // and 3 for the join, a chain of four loads (lengths, id, page, key).
 __global__ __launch_bounds__(64 * kWaves, 2) void kv8_attend_kernel(Kv8Params p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
@@ -394,9 +394,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_attend_kernel(Kv8Params p)
 
 // KV heads of a work-group: as many as divide them.  The rows of a token's heads lie
 // side by side, and four heads in step read them in one go: 48 contexts as above, one
-// head to a work-group 247 us, two 211, four 203; 8 rows of 8 heads and up to 32768
-// tokens 72, 63, 60.  Contexts of 2000 tokens have little for a wave that has a head
-// to itself: 256 of them 137, 133, 149.
+// head to a work-group 230 us, two 207, four 202; 8 rows of 8 heads and up to 32768
+// tokens 68, 61, 58; 256 contexts of 2000 tokens, 4 heads, 136, 131, 123.
 inline int32_t kv8_together(int32_t kv_heads) { return kv_heads % 4 == 0 ? 4 : kv_heads % 2 == 0 ? 2 : 1; }
 
 // (Two work-groups a CU, a tile of each wave at a time.)

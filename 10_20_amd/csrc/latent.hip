@@ -166,7 +166,8 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
     const int32_t lane = (int32_t)threadIdx.x % kWave;
     int32_t g = lane >> 4, c = lane & 15;  // (opaque in the loops, as buffer_of)
 
-    // work-groups reach the XCDs in turn: the splits of an item follow each other on one of them
+    // Work-groups reach the XCDs in turn: the splits of an item follow each other on one
+    // of them, and so do rows of equal capacity, which may choose from one context.
     const int32_t xcd = (int32_t)blockIdx.x % 8, turn = (int32_t)blockIdx.x / 8, split = turn % p.splits;
     const int32_t index = p.plan.chunk > 0 ? xcd * p.spread + turn / p.splits : turn / p.splits * 8 + xcd;
     Item it;
