@@ -52,7 +52,9 @@ struct ExpandedParams {
     int64_t rope_row;
     const int32_t* cu_q;
     const int32_t* cu_k;
-    int32_t tokens, keys, batch, heads, blocks;  // blocks: of queries, of the longest sequence
+    int32_t tokens, keys, batch, heads;
+    int32_t blocks;           // of every sequence; 0: windows of slots
+    int32_t window, windows;  // blocks or slots of one, and their number
     int32_t causal, parts, xcds, group;
     float scale2;
     uint16_t* out;
@@ -69,6 +71,98 @@ struct ExpandedTile {
 
 __device__ __forceinline__ f32x16 mfma32(const Frag& a, const Frag& b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ int32_t keys_seen(const ExpandedParams& p, int32_t nq, int32_t nk, int32_t i) {
+    return p.causal ? min(max(nk - nq + i + 1, 0), nk) : nk;
+}
+
+struct Work {
+    int32_t q_lo, nq, k_lo, nk;  // the sequence of its block
+    int32_t q0;                  // the block's first query there
+    int32_t head, part;
+};
+
+// Slots: sequence b's blocks of queries lie in slots cu_q[b] / kBlock + b and on, as many as
+// its queries can need wherever they begin; tokens / kBlock + batch in all, taken in
+// windows of a wave's lanes.
+constexpr int kWindow = kWave;
+
+// The block of the window with the rank-th most tiles of keys (equal ones in the
+// slots' order); false: there are no more.  Every wave finds it by itself, in two
+// rounds of loads for up to 64 sequences and one more for every factor of 64.
+__device__ __forceinline__ bool find_block(const ExpandedParams& p, int32_t window, int32_t rank, Work& w) {
+    const int32_t lane = (int32_t)threadIdx.x % kWave, first = window * kWindow, slot = first + lane;
+    int32_t from = 0;  // a sequence whose slots begin at the first one or before: the lanes take 64 from there on
+    if (p.batch > kWave) {
+        auto start = [&](int32_t b) __attribute__((always_inline)) { return min(max(p.cu_q[b], 0), p.tokens) / kBlock + b; };
+        for (int32_t n = p.batch; n > 1;) {
+            const int32_t step = (n + kWave - 1) / kWave;
+            const bool past = lane * step >= n || start(from + min(lane * step, n - 1)) > first;
+            const int32_t skip = (max(__popcll(__ballot(!past)), 1) - 1) * step;
+            from += skip;
+            n = min(step, n - skip);
+        }
+        from = __builtin_amdgcn_readfirstlane(from);
+    }
+    const int32_t b = from + lane, at = min(b, p.batch - 1);
+    int32_t ends[4] = {p.cu_q[at], p.cu_q[at + 1], p.cu_k[at], p.cu_k[at + 1]};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(ends[i]));  // (one wait for the four)
+    int32_t q_lo = min(max(ends[0], 0), p.tokens), nq = min(max(ends[1], q_lo), p.tokens) - q_lo;
+    int32_t k_lo = min(max(ends[2], 0), p.keys), nk = min(max(ends[3], k_lo), p.keys) - k_lo;
+    int32_t begin = b >= p.batch ? INT32_MAX : q_lo / kBlock + b;
+    int32_t j = 0;  // from the sequences' lanes to the slots'
+#pragma unroll
+    for (int step = kWave / 2; step > 0; step /= 2)
+        if (__shfl(begin, j + step, kWave) <= slot) j += step;
+    q_lo = __shfl(q_lo, j, kWave), nq = __shfl(nq, j, kWave);
+    k_lo = __shfl(k_lo, j, kWave), nk = __shfl(nk, j, kWave);
+    begin = __shfl(begin, j, kWave);
+    const int32_t q0 = slot < begin ? nq : (slot - begin) * kBlock;
+    // bit by bit of the number of tiles, from the largest: those with the bit come first
+    const int32_t tiles = tiles_of(keys_seen(p, nq, nk, min(q0 + kBlock, nq) - 1));
+    uint64_t left = __ballot(lane < p.window && q0 < nq);
+    if (rank >= __popcll(left)) return false;
+    for (int32_t bit = 31 - __clz(tiles_of(p.keys) | 1); bit >= 0; --bit) {
+        const uint64_t more = __ballot((tiles >> bit) & 1) & left;
+        const int32_t n = __popcll(more);
+        left = rank < n ? more : left & ~more;
+        rank -= rank < n ? 0 : n;
+    }
+    const uint64_t who = __ballot(((left >> lane) & 1) && (int32_t)lanes_below(left) == rank);
+    const int32_t src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)who) - 1);
+    w.q_lo = __builtin_amdgcn_readlane(q_lo, src), w.nq = __builtin_amdgcn_readlane(nq, src);
+    w.k_lo = __builtin_amdgcn_readlane(k_lo, src), w.nk = __builtin_amdgcn_readlane(nk, src);
+    w.q0 = __builtin_amdgcn_readlane(q0, src);
+    return true;
+}
+
+// The work-group's part of the attention; false: there is none.  (Found by the
+// kernel before the rest: inside expanded_part its loops cost the tiles' loop its registers.)
+__device__ __forceinline__ bool find_work(const ExpandedParams& p, Work& w) {
+    // Work-groups reach the XCDs in turn.  An XCD takes whole units, a head of a sequence
+    // or of a window, `group` of them at a time: the group's blocks longest first, so that
+    // the last ones to end are short and blocks of the same keys meet in one L2.
+    // Of 4 sequences of 4096, 32 heads: a pair at a time 803 us, so 740; of 2 times
+    // 4096 queries, 16384 keys, 128 heads: all pairs at a time 10290 us, so 9200.
+    const int32_t per = p.window * p.parts, units = (p.windows * p.heads + p.xcds - 1) / p.xcds;
+    const int32_t turn = (int32_t)blockIdx.x / p.xcds, before = turn / (p.group * per) * p.group;
+    const int32_t size = min(p.group, units - before), within = turn - before * per, at = within / size;
+    const int32_t index = (before + within % size) * p.xcds + (int32_t)blockIdx.x % p.xcds;
+    const int32_t rank = at / p.parts, b = index / p.heads;
+    w.part = at % p.parts, w.head = index % p.heads;
+    if (b >= p.windows) return false;
+    if (p.blocks == 0) return find_block(p, p.windows - 1 - b, rank, w);
+    int32_t ends[4] = {p.cu_q[b], p.cu_q[b + 1], p.cu_k[b], p.cu_k[b + 1]};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(ends[i]));  // (one wait for the four)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ends[i] = __builtin_amdgcn_readfirstlane(ends[i]);
+    w.q_lo = min(max(ends[0], 0), p.tokens), w.nq = min(max(ends[1], w.q_lo), p.tokens) - w.q_lo;
+    w.k_lo = min(max(ends[2], 0), p.keys), w.nk = min(max(ends[3], w.k_lo), p.keys) - w.k_lo;
+    w.q0 = (p.blocks - 1 - rank) * kBlock;
+    return w.q0 < w.nq;
 }
 
 // Reads of LDS, EACH for one matrix product, kAhead products before it.
@@ -150,37 +244,15 @@ __device__ __forceinline__ void careful_product(f32x16 (&sums)[4], const Frag (&
 // end up not finite (true is returned, nothing written) are found again by the
 // CAREFUL form.
 template <bool CAREFUL>
-__device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedTile* lds) {
+__device__ __forceinline__ bool expanded_part(const ExpandedParams& p, const Work& w, ExpandedTile* lds) {
     constexpr int COPIES = (int)(sizeof(ExpandedTile) / 1024) / kWaves;
     static_assert(COPIES == 5 && kWaves * 4 * 2 == kTileKeys, "copies of a tile");
     const int32_t wave = __builtin_amdgcn_readfirstlane((int32_t)threadIdx.x / kWave);
     const int32_t lane = (int32_t)threadIdx.x % kWave, c = lane & 31, h = lane >> 5;
 
-    // Work-groups reach the XCDs in turn.  An XCD takes whole (sequence, head)
-    // pairs, `group` of them at a time: the group's blocks longest first, so that
-    // the last ones to end are short and blocks of the same keys meet in one L2.
-    // Of 4 sequences of 4096, 32 heads: a pair at a time 803 us, so 740; of 2 times
-    // 4096 queries, 16384 keys, 128 heads: all pairs at a time 10290 us, so 9200.
-    const int32_t per = p.blocks * p.parts, pairs = ((int32_t)p.batch * p.heads + p.xcds - 1) / p.xcds;
-    const int32_t turn = (int32_t)blockIdx.x / p.xcds, before = turn / (p.group * per) * p.group;
-    const int32_t size = min(p.group, pairs - before), within = turn - before * per, at = within / size;
-    const int32_t index = (before + within % size) * p.xcds + (int32_t)blockIdx.x % p.xcds;
-    const int32_t part = at % p.parts, block = p.blocks - 1 - at / p.parts;
-    const int32_t head = index % p.heads, b = index / p.heads;
-    if (b >= p.batch) return false;
-    int32_t ends[4] = {p.cu_q[b], p.cu_q[b + 1], p.cu_k[b], p.cu_k[b + 1]};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(ends[i]));  // (one wait for the four)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) ends[i] = __builtin_amdgcn_readfirstlane(ends[i]);
-    const int32_t q_lo = min(max(ends[0], 0), p.tokens), q_hi = min(max(ends[1], q_lo), p.tokens);
-    const int32_t k_lo = min(max(ends[2], 0), p.keys), k_hi = min(max(ends[3], k_lo), p.keys);
-    const int32_t nq = q_hi - q_lo, nk = k_hi - k_lo;
-    const int32_t q0 = block * kBlock;
-    if (q0 >= nq) return false;
-
+    const int32_t q_lo = w.q_lo, nq = w.nq, k_lo = w.k_lo, nk = w.nk, q0 = w.q0, head = w.head, part = w.part;
     // keys that query i sees: the first seen(i)
-    auto seen = [&](int32_t i) __attribute__((always_inline)) { return p.causal ? min(max(nk - nq + i + 1, 0), nk) : nk; };
+    auto seen = [&](int32_t i) __attribute__((always_inline)) { return keys_seen(p, nq, nk, i); };
     const int32_t i0 = q0 + wave * kRows;                                // this wave's first query
     const int32_t my_seen = seen(min(i0 + c, nq - 1));
     const int32_t wave_least = i0 < nq ? seen(i0) : 0, wave_most = i0 < nq ? seen(min(i0 + kRows, nq) - 1) : 0;
@@ -407,28 +479,51 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, ExpandedT
 
 // (A call, so that its registers are not the common form's.)
 __device__ __attribute__((noinline)) void careful_part(ExpandedParams p, ExpandedTile* lds) {
-    expanded_part<true>(p, lds);
+    Work w;
+    if (find_work(p, w)) expanded_part<true>(p, w, lds);
 }
 
 __global__ __launch_bounds__(64 * kWaves, 2) void expanded_kernel(ExpandedParams p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
     ExpandedTile* const lds = reinterpret_cast<ExpandedTile*>(lds_raw);
-    if (__builtin_expect(expanded_part<false>(p, lds), 0)) careful_part(p, lds);
+    Work w;
+    if (!find_work(p, w)) return;
+    // (as they are from here on: without this line 27 more scalar registers spill, 0.7 us of a work-group)
+    asm volatile("" : "+s"(w.q_lo), "+s"(w.nq), "+s"(w.k_lo), "+s"(w.nk), "+s"(w.q0), "+s"(w.head), "+s"(w.part));
+    if (__builtin_expect(expanded_part<false>(p, w, lds), 0)) careful_part(p, lds);
 }
 
 // Blocks of queries, and the parts that the keys are cut into where the blocks
 // leave CUs without one (of four tiles or more each): 512 queries of 16 heads over
 // 32768 keys 187 us in eight parts, one for each CU; in sixteen 202.
+//
+// Every sequence gets as many blocks as the longest can have, unless the slots are less
+// than a third of those: an empty work-group takes all of a CU's LDS for the time of its
+// loads, finding a slot's block takes 2-3 us of a work-group.  Blocks and slots, us:
+//   9 prompts of 1 to 1000 tokens, 16 heads      36, 16          35.7, 36.7
+//   200 of 10 to 3000, 8 heads                   2400, 609        610, 592
+//   64 of 512, 16 heads, max_q not given         8192, 192        737, 221
+//   1000 of 100, 16 heads, max_q not given       391000, 1390   21100, 774
+//   63 of 100 and one of 16000, 16 heads         4032, 150       1426, 1301
+constexpr int64_t kMostGroups = (1ll << 32) / (64 * kWaves);  // (a launch has fewer than 2^32 work-items a dimension)
+
 struct ExpandedShape {
-    int32_t blocks, parts;
+    int32_t blocks, window, windows, parts;
 };
 
 inline ExpandedShape expanded_shape(int32_t tokens, int32_t keys, int32_t batch, int32_t heads, int32_t max_q) {
+    const int64_t blocks = cdiv(max_q, kBlock), slots = (int64_t)tokens / kBlock + batch, tiles = cdiv(keys, kTileKeys);
+    const int64_t groups = std::min(batch * blocks, slots) * heads;
     ExpandedShape s;
-    s.blocks = (int32_t)cdiv(max_q, kBlock);
-    const int64_t groups = std::min((int64_t)batch * s.blocks, batch + cdiv(tokens, kBlock)) * heads;
-    const int64_t tiles = cdiv(keys, kTileKeys);
-    s.parts = (int32_t)std::max<int64_t>(1, std::min(device_cus() / std::max<int64_t>(1, groups), tiles / (4 * batch)));
+    s.parts = (int32_t)std::max<int64_t>(1, std::min(device_cus() / std::max<int64_t>(1, groups), tiles / (4 * (int64_t)batch)));
+    if (batch * blocks <= 3 * slots && ((int64_t)batch * heads + 7) * blocks * s.parts < kMostGroups) {
+        s.blocks = s.window = (int32_t)blocks;
+        s.windows = batch;
+    } else {
+        s.blocks = 0;
+        s.window = (int32_t)std::min<int64_t>(slots, kWindow);
+        s.windows = (int32_t)cdiv(slots, s.window);
+    }
     return s;
 }
 
@@ -467,14 +562,14 @@ extern "C" int v1_latent_expanded(const v1_latent_expanded_args* a, void* stream
     // XCD by XCD where that leaves few of them short of work (12 heads of 8192 queries
     // 338 us so, 295 in turn; 9 sequences of 1500, 4 heads, 59 either way); groups of
     // two work-groups for each of an XCD's CUs
-    const int64_t pairs = (int64_t)batch * heads;
-    const int32_t xcds = pairs % 8 == 0 || pairs >= 64 ? 8 : 1;
-    const int64_t items = cdiv(pairs, xcds) * xcds * s.blocks * s.parts;
-    V1_REQUIRE(pairs < 1ll << 30 && items < 1ll << 30, "latent_expanded: too many work items");
-    const int64_t group = std::min(cdiv(pairs, xcds), cdiv(2 * device_cus() / xcds, (int64_t)s.blocks * s.parts));
+    const int64_t units = (int64_t)s.windows * heads;
+    const int32_t xcds = units % 8 == 0 || units >= 64 ? 8 : 1;
+    const int64_t items = cdiv(units, xcds) * xcds * s.window * s.parts;
+    V1_REQUIRE(items < kMostGroups, "latent_expanded: too many sequences, queries and heads for a launch");
+    const int64_t group = std::min(cdiv(units, xcds), cdiv(2 * device_cus() / xcds, (int64_t)s.window * s.parts));
     ExpandedParams p{static_cast<const uint16_t*>(q), q_row, q_head, static_cast<const uint16_t*>(kv), kv_row, kv_head,
-                     static_cast<const uint16_t*>(rope), rope_row, cu_q, cu_k, tokens, keys, batch, heads, s.blocks,
-                     causal, s.parts, xcds, (int32_t)group, scale * kLog2e, static_cast<uint16_t*>(out), o_row, o_head, lse,
+                     static_cast<const uint16_t*>(rope), rope_row, cu_q, cu_k, tokens, keys, batch, heads, s.blocks, s.window,
+                     s.windows, causal, s.parts, xcds, (int32_t)group, scale * kLog2e, static_cast<uint16_t*>(out), o_row, o_head, lse,
                      parts_at(workspace, rows_of_parts(tokens, s), heads, kValue)};
     const hipStream_t st = as_stream(stream);
     static OncePerDevice once;
@@ -485,6 +580,6 @@ extern "C" int v1_latent_expanded(const v1_latent_expanded_args* a, void* stream
     rc = V1_LAUNCHED("latent_expanded");
     if (rc != V1_OK || s.parts == 1) return rc;
     JoinParams j{rows_of_parts(tokens, s), p.partial, p.out, o_row, o_head, lse, heads, cu_q, batch,
-                 s.blocks * kBlock};
+                 (int32_t)std::min<int64_t>(cdiv(max_q, kBlock) * kBlock, INT32_MAX)};
     return launch_join<kValue>(j, st, "latent_expanded: join");
 }

@@ -1,0 +1,101 @@
+"""Attention over expanded keys and values where the batch's sequences are far from
+alike: lengths not given on the host, many short sequences, long ones among short
+ones, padded buffers.  Against float64 with the bounds of the operator's own tests,
+and against the same sequences in calls that know their lengths (a block of queries
+does the same sums wherever it lies in the launch, so those are equal)."""
+import random
+
+import pytest
+import torch
+
+import test_gpu_expanded as expanded
+from conftest import pkg
+
+LT = pkg("latent")
+DEV = "cuda:0"
+gpu = pytest.mark.gpu
+
+
+def lengths(kind, n):
+    rng = random.Random(n)
+    if kind == "short":
+        return [rng.choice([0, 1, 2, 7, 64, 100]) for _ in range(n)]
+    if kind == "one long":
+        return [rng.choice([0, 1, 90]) for _ in range(n // 2)] + [5000] + [rng.choice([0, 1, 256, 257]) for _ in range(n // 2)]
+    return [rng.choice([0, 1, 255, 256, 257, 511, 513, 900]) for _ in range(n)]
+
+
+@gpu
+@pytest.mark.parametrize("n", [2, 9, 63, 64, 65, 130, 700])
+@pytest.mark.parametrize("kind", ["short", "one long", "mixed"])
+@pytest.mark.parametrize("causal", [True, False])
+def test_batches_without_max_q(n, kind, causal):
+    print("expanded batch", n, kind, causal, flush=True)
+    nq = lengths(kind, n)
+    nk = [max(0, m + (17, 0, -3, 400)[i % 4]) for i, m in enumerate(nq)]
+    q, kv, rope, cu_q, cu_k = expanded.inputs(n, nq, nk, 2, behind=300)
+    out = torch.full((q.shape[0], 2, 128), 7.0, device=DEV, dtype=torch.bfloat16)
+    _, lse = LT.attend_expanded(q, kv, rope, cu_q, cu_k, causal=causal, out=out, return_lse=True)
+    assert bool((out[sum(nq):] == 7).all())
+    known, known_lse = LT.attend_expanded(q, kv, rope, cu_q, cu_k, max(nq), causal=causal, return_lse=True)
+    if n >= 63:  # (too few keys a sequence for parts, either way)
+        assert torch.equal(out[:sum(nq)], known[:sum(nq)]) and torch.equal(lse[:sum(nq)], known_lse[:sum(nq)])
+    few = sorted(random.Random(1).sample(range(len(nq)), min(len(nq), 12)) + [nq.index(max(nq))])
+    for b in few:
+        i, j = int(cu_q[b]), int(cu_k[b])
+        for o, l in ((out, lse), (known, known_lse)):
+            expanded.check(o[i:i + nq[b]], l[i:i + nq[b]], q[i:i + nq[b]], kv[j:j + nk[b]], rope[j:j + nk[b]], [nq[b]], [nk[b]], causal)
+
+
+@gpu
+def test_sequences_that_begin_behind_the_first_row():
+    """Rows before the first sequence, and a batch that ends before the buffer does."""
+    print("expanded begin", flush=True)
+    for n, first in ((70, 1000), (3, 300), (1, 256)):
+        nq = [1, 300, 40] * 30
+        nq = nq[:n]
+        q, kv, rope, cu, _ = expanded.inputs(n, nq, nq, 2, behind=4000)
+        out = torch.full((q.shape[0], 2, 128), 7.0, device=DEV, dtype=torch.bfloat16)
+        want, want_lse = LT.attend_expanded(q[first:], kv[first:], rope[first:], cu, return_lse=True)
+        _, lse = LT.attend_expanded(q, kv, rope, cu + first, out=out, return_lse=True)
+        end = first + sum(nq)
+        assert bool((out[:first] == 7).all()) and bool((out[end:] == 7).all())
+        expanded.check(out[first:end], lse[first:end], q[first:], kv[first:], rope[first:], nq, nq)
+        expanded.check(want[:sum(nq)], want_lse[:sum(nq)], q[first:], kv[first:], rope[first:], nq, nq)
+
+
+@gpu
+def test_more_blocks_than_a_launch_holds():
+    """2048 sequences whose lengths only the device knows, 512 heads: a block of the
+    longest possible for each would be more work-groups than a launch can have."""
+    print("expanded launch", flush=True)
+    heads, nq = 512, [(1, 0, 2, 1)[i % 4] for i in range(2047)] + [60]
+    g = torch.Generator(device=DEV).manual_seed(0)
+    r = lambda *s: torch.randn(s, device=DEV, generator=g, dtype=torch.bfloat16)
+    q, kv, rope = r(sum(nq) + 600, heads, 192), r(sum(nq), heads, 256), r(sum(nq), 64)
+    cu = torch.tensor([0] + nq, device=DEV).cumsum(0).to(torch.int32)
+    assert len(nq) * -(-q.shape[0] // 256) * heads >= (1 << 32) // 512
+    out, lse = LT.attend_expanded(q, kv, rope, cu, return_lse=True)
+    n = sum(nq)
+    known, known_lse = LT.attend_expanded(q, kv, rope, cu, max_q=60, return_lse=True)
+    assert torch.equal(out[:n], known[:n]) and torch.equal(lse[:n], known_lse[:n])
+    for b in (0, 1, 2, 1000, 2046, 2047):
+        i = int(cu[b])
+        pick = lambda t: t[i:i + nq[b], 5::100]
+        expanded.check(pick(out), pick(lse), pick(q), pick(kv), rope[i:i + nq[b]], [nq[b]], [nq[b]])
+
+
+def library_call(**change):
+    L = pkg("_lib")
+    if not L.LIB_PATH.exists():
+        pkg("build").build()
+    base = dict(q=256, qr=384, qh=192, kv=256, kr=512, kh=256, rope=256, rr=64, cu_q=256, cu_k=256, out=256, o_row=256, o_head=128,
+                lse=0, ws=0, wsb=0, tokens=4096, keys=4096, batch=1, heads=16, max_q=4096, causal=1, scale=0.1)
+    return L.lib().v1_latent_expanded(L.PACKED["v1_latent_expanded"].pack(*{**base, **change}.values()), None), L
+
+
+def test_too_many_sequences_for_a_launch():
+    for change in (dict(batch=1 << 16, heads=128, max_q=1), dict(batch=1 << 17, heads=64), dict(batch=(1 << 31) - 1, heads=1),
+                   dict(batch=(1 << 31) - 1, heads=65535, tokens=1 << 30, max_q=1 << 30)):
+        rc, L = library_call(**change)
+        assert rc == L.V1_ERR_INVALID and b"launch" in L.lib().v1_last_error(), change
