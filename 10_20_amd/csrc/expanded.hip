@@ -52,7 +52,7 @@ struct ExpandedParams {
     int64_t rope_row;
     const int32_t* cu_q;
     const int32_t* cu_k;
-    int32_t tokens, keys, batch, heads;
+    int32_t tokens, keys, batch, heads, max_q;
     int32_t blocks;           // of every sequence; 0: windows of slots
     int32_t window, windows;  // blocks or slots of one, and their number
     int32_t causal, parts, xcds, group;
@@ -73,13 +73,16 @@ __device__ __forceinline__ f32x16 mfma32(const Frag& a, const Frag& b, f32x16 c)
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, c, 0, 0, 0);
 }
 
-__device__ __forceinline__ int32_t keys_seen(const ExpandedParams& p, int32_t nq, int32_t nk, int32_t i) {
-    return p.causal ? min(max(nk - nq + i + 1, 0), nk) : nk;
+// Keys that query i of a sequence sees: the first of them.
+__device__ __forceinline__ int32_t keys_seen(const ExpandedParams& p, int32_t before, int32_t nk, int32_t i) {
+    return p.causal ? min(max(before + i + 1, 0), nk) : nk;
 }
 
 struct Work {
-    int32_t q_lo, nq, k_lo, nk;  // the sequence of its block
-    int32_t q0;                  // the block's first query there
+    // the sequence of its block: where its queries begin, how many there are (max_q at
+    // most), its keys, and those before its first query (nk less all of its queries)
+    int32_t q_lo, nq, k_lo, nk, before;
+    int32_t q0;  // the block's first query there
     int32_t head, part;
 };
 
@@ -110,7 +113,8 @@ __device__ __forceinline__ bool find_block(const ExpandedParams& p, int32_t wind
 #pragma unroll
     for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(ends[i]));  // (one wait for the four)
     int32_t q_lo = min(max(ends[0], 0), p.tokens), nq = min(max(ends[1], q_lo), p.tokens) - q_lo;
-    int32_t k_lo = min(max(ends[2], 0), p.keys), nk = min(max(ends[3], k_lo), p.keys) - k_lo;
+    int32_t k_lo = min(max(ends[2], 0), p.keys), nk = min(max(ends[3], k_lo), p.keys) - k_lo, before = nk - nq;
+    nq = min(nq, p.max_q);
     int32_t begin = b >= p.batch ? INT32_MAX : q_lo / kBlock + b;
     int32_t j = 0;  // from the sequences' lanes to the slots'
 #pragma unroll
@@ -118,10 +122,10 @@ __device__ __forceinline__ bool find_block(const ExpandedParams& p, int32_t wind
         if (__shfl(begin, j + step, kWave) <= slot) j += step;
     q_lo = __shfl(q_lo, j, kWave), nq = __shfl(nq, j, kWave);
     k_lo = __shfl(k_lo, j, kWave), nk = __shfl(nk, j, kWave);
-    begin = __shfl(begin, j, kWave);
+    begin = __shfl(begin, j, kWave), before = __shfl(before, j, kWave);
     const int32_t q0 = slot < begin ? nq : (slot - begin) * kBlock;
     // bit by bit of the number of tiles, from the largest: those with the bit come first
-    const int32_t tiles = tiles_of(keys_seen(p, nq, nk, min(q0 + kBlock, nq) - 1));
+    const int32_t tiles = tiles_of(keys_seen(p, before, nk, min(q0 + kBlock, nq) - 1));
     uint64_t left = __ballot(lane < p.window && q0 < nq);
     if (rank >= __popcll(left)) return false;
     for (int32_t bit = 31 - __clz(tiles_of(p.keys) | 1); bit >= 0; --bit) {
@@ -134,7 +138,7 @@ __device__ __forceinline__ bool find_block(const ExpandedParams& p, int32_t wind
     const int32_t src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)who) - 1);
     w.q_lo = __builtin_amdgcn_readlane(q_lo, src), w.nq = __builtin_amdgcn_readlane(nq, src);
     w.k_lo = __builtin_amdgcn_readlane(k_lo, src), w.nk = __builtin_amdgcn_readlane(nk, src);
-    w.q0 = __builtin_amdgcn_readlane(q0, src);
+    w.before = __builtin_amdgcn_readlane(before, src), w.q0 = __builtin_amdgcn_readlane(q0, src);
     return true;
 }
 
@@ -161,6 +165,7 @@ __device__ __forceinline__ bool find_work(const ExpandedParams& p, Work& w) {
     for (int i = 0; i < 4; ++i) ends[i] = __builtin_amdgcn_readfirstlane(ends[i]);
     w.q_lo = min(max(ends[0], 0), p.tokens), w.nq = min(max(ends[1], w.q_lo), p.tokens) - w.q_lo;
     w.k_lo = min(max(ends[2], 0), p.keys), w.nk = min(max(ends[3], w.k_lo), p.keys) - w.k_lo;
+    w.before = w.nk - w.nq, w.nq = min(w.nq, p.max_q);
     w.q0 = (p.blocks - 1 - rank) * kBlock;
     return w.q0 < w.nq;
 }
@@ -250,9 +255,8 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, const Wor
     const int32_t wave = __builtin_amdgcn_readfirstlane((int32_t)threadIdx.x / kWave);
     const int32_t lane = (int32_t)threadIdx.x % kWave, c = lane & 31, h = lane >> 5;
 
-    const int32_t q_lo = w.q_lo, nq = w.nq, k_lo = w.k_lo, nk = w.nk, q0 = w.q0, head = w.head, part = w.part;
-    // keys that query i sees: the first seen(i)
-    auto seen = [&](int32_t i) __attribute__((always_inline)) { return keys_seen(p, nq, nk, i); };
+    const int32_t q_lo = w.q_lo, nq = w.nq, k_lo = w.k_lo, nk = w.nk, before = w.before, q0 = w.q0, head = w.head, part = w.part;
+    auto seen = [&](int32_t i) __attribute__((always_inline)) { return keys_seen(p, before, nk, i); };
     const int32_t i0 = q0 + wave * kRows;                                // this wave's first query
     const int32_t my_seen = seen(min(i0 + c, nq - 1));
     const int32_t wave_least = i0 < nq ? seen(i0) : 0, wave_most = i0 < nq ? seen(min(i0 + kRows, nq) - 1) : 0;
@@ -489,7 +493,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void expanded_kernel(ExpandedParams
     Work w;
     if (!find_work(p, w)) return;
     // (as they are from here on: without this line 27 more scalar registers spill, 0.7 us of a work-group)
-    asm volatile("" : "+s"(w.q_lo), "+s"(w.nq), "+s"(w.k_lo), "+s"(w.nk), "+s"(w.q0), "+s"(w.head), "+s"(w.part));
+    asm volatile("" : "+s"(w.q_lo), "+s"(w.nq), "+s"(w.k_lo), "+s"(w.nk), "+s"(w.before), "+s"(w.q0), "+s"(w.head), "+s"(w.part));
     if (__builtin_expect(expanded_part<false>(p, w, lds), 0)) careful_part(p, lds);
 }
 
@@ -568,7 +572,7 @@ extern "C" int v1_latent_expanded(const v1_latent_expanded_args* a, void* stream
     V1_REQUIRE(items < kMostGroups, "latent_expanded: too many sequences, queries and heads for a launch");
     const int64_t group = std::min(cdiv(units, xcds), cdiv(2 * device_cus() / xcds, (int64_t)s.window * s.parts));
     ExpandedParams p{static_cast<const uint16_t*>(q), q_row, q_head, static_cast<const uint16_t*>(kv), kv_row, kv_head,
-                     static_cast<const uint16_t*>(rope), rope_row, cu_q, cu_k, tokens, keys, batch, heads, s.blocks, s.window,
+                     static_cast<const uint16_t*>(rope), rope_row, cu_q, cu_k, tokens, keys, batch, heads, max_q, s.blocks, s.window,
                      s.windows, causal, s.parts, xcds, (int32_t)group, scale * kLog2e, static_cast<uint16_t*>(out), o_row, o_head, lse,
                      parts_at(workspace, rows_of_parts(tokens, s), heads, kValue)};
     const hipStream_t st = as_stream(stream);
@@ -580,6 +584,6 @@ extern "C" int v1_latent_expanded(const v1_latent_expanded_args* a, void* stream
     rc = V1_LAUNCHED("latent_expanded");
     if (rc != V1_OK || s.parts == 1) return rc;
     JoinParams j{rows_of_parts(tokens, s), p.partial, p.out, o_row, o_head, lse, heads, cu_q, batch,
-                 (int32_t)std::min<int64_t>(cdiv(max_q, kBlock) * kBlock, INT32_MAX)};
+                 max_q};
     return launch_join<kValue>(j, st, "latent_expanded: join");
 }

@@ -166,11 +166,11 @@ def attend_expanded(q, kv, k_rope, cu_q, cu_k=None, max_q=None, softmax_scale=No
     cu_q, cu_k: [batch + 1] int32, where each sequence's queries and keys begin and
             end (cu_k None: cu_q).  With `causal`, query i of nq sees keys
             j <= nk - nq + i of its nk (a chunk at the end of its context), else all.
-    max_q:  at least the longest sequence's queries (queries past it are not
-            computed); None: tokens.
+    max_q:  at least the longest sequence's queries; None: tokens.  The first max_q
+            queries of a longer one are computed, their keys counted from its end as ever.
 
-    A query without keys gives zeros and -inf; rows outside [cu_q[0], cu_q[-1]) of
-    `out` are left as they are.  softmax_scale > 0, default 1 / sqrt(192).  Returns
+    A query without keys gives zeros and -inf; rows of `out` outside [cu_q[0],
+    cu_q[-1]) or past a sequence's first max_q are left as they are.  softmax_scale > 0, default 1 / sqrt(192).  Returns
     out [tokens, heads, 128] bf16, and with return_lse the natural log of the sum
     of exponentials, [tokens, heads] fp32."""
     cu_k = cu_q if cu_k is None else cu_k

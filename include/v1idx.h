@@ -637,8 +637,9 @@ int64_t v1_latent_attend_workspace(int32_t rows, int32_t heads, int32_t keys, in
  * keys cu_k[b] .. cu_k[b + 1] (clamped to the tensors).  out[i, h] (bf16, 128) =
  * softmax over the keys that query i sees of scale * q . (k_j, rope_j), times
  * v_j; causal: query i of nq sees keys j <= nk - nq + i, else all.  No key: zeros
- * and an lse of -inf.  max_q: at least the longest sequence's queries.  lse (may
- * be NULL): [tokens, heads].  Rows outside the sequences are not written.
+ * and an lse of -inf.  max_q: at least the longest sequence's queries; of a longer
+ * one the first max_q are computed.  lse (may be NULL): [tokens, heads].  Rows
+ * outside the sequences or past max_q are not written.
  * workspace: v1_latent_expanded_workspace bytes, as above.  scale > 0. */
 typedef struct {
     const void* q;

@@ -85,6 +85,27 @@ def test_more_blocks_than_a_launch_holds():
         expanded.check(pick(out), pick(lse), pick(q), pick(kv), rope[i:i + nq[b]], [nq[b]], [nq[b]])
 
 
+@gpu
+@pytest.mark.parametrize("max_q", [1, 100, 256, 257, 1500])
+@pytest.mark.parametrize("heads,nq", [(1, [900]), (1, [90, 0, 3000, 300]), (40, [700, 20, 1600]), (2, [3, 40, 1] * 30 + [4000] + [5, 257] * 20)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_only_the_first_max_q_queries(heads, nq, max_q, causal):
+    """Each sequence's first max_q queries, at their places before the end of its
+    keys; every other row of the output is left alone."""
+    print("expanded max_q", heads, len(nq), max_q, causal, flush=True)
+    nk = [n + (0, 30, -1)[i % 3] for i, n in enumerate(nq)]
+    nk = [max(0, m) for m in nk]
+    q, kv, rope, cu_q, cu_k = expanded.inputs(max_q, nq, nk, heads)
+    out = torch.full((sum(nq), heads, 128), 7.0, device=DEV, dtype=torch.bfloat16)
+    _, lse = LT.attend_expanded(q, kv, rope, cu_q, cu_k, max_q, causal=causal, out=out, return_lse=True)
+    whole, whole_lse = LT.attend_expanded(q, kv, rope, cu_q, cu_k, causal=causal, return_lse=True)
+    some = torch.cat([torch.arange(n, device=DEV) < max_q for n in nq])
+    assert bool((out[~some] == 7).all())
+    whole[some], whole_lse[some] = out[some], lse[some]
+    for h in range(0, heads, 9):
+        expanded.check(whole[:, h:h + 1], whole_lse[:, h:h + 1], q[:, h:h + 1], kv[:, h:h + 1], rope, nq, nk, causal)
+
+
 def library_call(**change):
     L = pkg("_lib")
     if not L.LIB_PATH.exists():
