@@ -295,21 +295,28 @@ struct JoinParams {
     int64_t o_row, o_head;
     float* lse;
     int32_t heads;
-    // not NULL: only rows cu[b] .. min(cu[b + 1], cu[b] + most) - 1 have parts (the ends
-    // taken within [0, rows]); the others are left as they are
+    // not NULL: only rows cu[b] .. min(cu[b + 1], cu[b] + most) - 1 of the output have parts (the
+    // ends taken within [0, tokens]), the others are left as they are.  The plan's rows are those
+    // of the output, or (by_sequence) `most` for each of the sequences.
     const int32_t* cu;
-    int32_t batch, most;
+    int32_t tokens, batch, most;
+    bool by_sequence;
 };
 
-// Whether the row has parts (asked by a whole work-group).
-__device__ __forceinline__ bool joined_row(const JoinParams& p, int32_t row) {
-    if (!p.cu) return true;
+// The output's row of a row of the plan; -1: it has no parts (asked by a whole work-group).
+__device__ __forceinline__ int32_t joined_row(const JoinParams& p, int32_t row) {
+    if (!p.cu) return row;
+    auto begin = [&](int32_t b) __attribute__((always_inline)) { return min(max(p.cu[b], 0), p.tokens); };
+    if (p.by_sequence) {
+        const int32_t b = row / p.most, i = row - b * p.most, lo = begin(b);
+        return i < begin(b + 1) - lo ? lo + i : -1;
+    }
     int mine = 0;
     for (int32_t b = (int32_t)threadIdx.x; b < p.batch; b += 256) {
-        const int32_t lo = min(max(p.cu[b], 0), p.plan.rows), hi = min(max(p.cu[b + 1], lo), p.plan.rows);
+        const int32_t lo = begin(b), hi = begin(b + 1);
         mine |= row >= lo && row < hi && row - lo < p.most;
     }
-    return __syncthreads_or(mine);
+    return __syncthreads_or(mine) ? row : -1;
 }
 
 __device__ __forceinline__ void write_joined(const JoinParams& p, int32_t row, int32_t h, int32_t at4, f32x4 o, float top, float total) {
@@ -335,7 +342,8 @@ __global__ __launch_bounds__(256) void join_kernel(JoinParams p) {
     __shared__ float totals[G];
     const int32_t row = (int32_t)blockIdx.x, h = (int32_t)blockIdx.y, lane = (int32_t)threadIdx.x % kWave;
     const int32_t group = (int32_t)threadIdx.x / T, at4 = (int32_t)threadIdx.x % T;
-    if (!joined_row(p, row)) return;
+    const int32_t to = joined_row(p, row);
+    if (to < 0) return;
     int32_t parts, first;
     if (p.plan.chunk > 0) {
         parts = (tiles_of(p.plan.keys) + p.plan.chunk - 1) / p.plan.chunk;
@@ -370,7 +378,7 @@ __global__ __launch_bounds__(256) void join_kernel(JoinParams p) {
         o += sums[k][at4];
         total += totals[k];
     }
-    write_joined(p, row, h, at4, o, top, total);
+    write_joined(p, to, h, at4, o, top, total);
 }
 
 // The same for rows of a few parts, known on the host: D / 4 threads for each (row,
@@ -380,7 +388,8 @@ template <int D>
 __global__ __launch_bounds__(256) void join_few_kernel(JoinParams p) {
     constexpr int T = D / 4, G = 256 / T;
     const int32_t row = (int32_t)blockIdx.x, h = (int32_t)blockIdx.y * G + (int32_t)threadIdx.x / T, at4 = (int32_t)threadIdx.x % T;
-    if (!joined_row(p, row) || h >= p.heads) return;
+    const int32_t to = joined_row(p, row);
+    if (to < 0 || h >= p.heads) return;
     const int32_t parts = (tiles_of(p.plan.keys) + p.plan.chunk - 1) / p.plan.chunk;
     const int64_t first = (int64_t)row * parts * p.heads + h;
     f32x2 st[kFewParts];
@@ -403,7 +412,7 @@ __global__ __launch_bounds__(256) void join_few_kernel(JoinParams p) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[k] = fmaf(f, x[i][k], o[k]);
     }
-    write_joined(p, row, h, at4, o, top, total);
+    write_joined(p, to, h, at4, o, top, total);
 }
 
 template <int D>

@@ -60,6 +60,7 @@ struct ExpandedParams {
     uint16_t* out;
     int64_t o_row, o_head;
     float* lse;
+    bool by_sequence;  // workspace rows: max_q for each sequence, else one for each token
     Parts partial;
 };
 
@@ -82,7 +83,8 @@ struct Work {
     // the sequence of its block: where its queries begin, how many there are (max_q at
     // most), its keys, and those before its first query (nk less all of its queries)
     int32_t q_lo, nq, k_lo, nk, before;
-    int32_t q0;  // the block's first query there
+    int32_t q0;   // the block's first query there
+    int32_t row;  // its row in the workspace
     int32_t head, part;
 };
 
@@ -139,6 +141,7 @@ __device__ __forceinline__ bool find_block(const ExpandedParams& p, int32_t wind
     w.q_lo = __builtin_amdgcn_readlane(q_lo, src), w.nq = __builtin_amdgcn_readlane(nq, src);
     w.k_lo = __builtin_amdgcn_readlane(k_lo, src), w.nk = __builtin_amdgcn_readlane(nk, src);
     w.before = __builtin_amdgcn_readlane(before, src), w.q0 = __builtin_amdgcn_readlane(q0, src);
+    w.row = w.q_lo + w.q0;  // (by_sequence has fewer rows than tokens, batch x max_q, and then blocks are fewer than slots)
     return true;
 }
 
@@ -167,6 +170,7 @@ __device__ __forceinline__ bool find_work(const ExpandedParams& p, Work& w) {
     w.k_lo = min(max(ends[2], 0), p.keys), w.nk = min(max(ends[3], w.k_lo), p.keys) - w.k_lo;
     w.before = w.nk - w.nq, w.nq = min(w.nq, p.max_q);
     w.q0 = (p.blocks - 1 - rank) * kBlock;
+    w.row = (p.by_sequence ? b * p.max_q : w.q_lo) + w.q0;
     return w.q0 < w.nq;
 }
 
@@ -462,7 +466,7 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, const Wor
         if (p.lse && h == 0 && c < left)
             p.lse[(int64_t)(q_lo + i0 + c) * p.heads + head] = none ? -__builtin_inff() : (mx + __builtin_amdgcn_logf(total)) * kLn2;
     } else {
-        const int64_t at = ((int64_t)(q_lo + i0) * p.parts + part) * p.heads + head, step = (int64_t)p.parts * p.heads;
+        const int64_t at = ((int64_t)(w.row + wave * kRows) * p.parts + part) * p.heads + head, step = (int64_t)p.parts * p.heads;
 #pragma unroll
         for (int d = 0; d < 4; ++d)
 #pragma unroll
@@ -493,7 +497,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void expanded_kernel(ExpandedParams
     Work w;
     if (!find_work(p, w)) return;
     // (as they are from here on: without this line 27 more scalar registers spill, 0.7 us of a work-group)
-    asm volatile("" : "+s"(w.q_lo), "+s"(w.nq), "+s"(w.k_lo), "+s"(w.nk), "+s"(w.before), "+s"(w.q0), "+s"(w.head), "+s"(w.part));
+    asm volatile("" : "+s"(w.q_lo), "+s"(w.nq), "+s"(w.k_lo), "+s"(w.nk), "+s"(w.before), "+s"(w.q0), "+s"(w.row), "+s"(w.head), "+s"(w.part));
     if (__builtin_expect(expanded_part<false>(p, w, lds), 0)) careful_part(p, lds);
 }
 
@@ -531,8 +535,11 @@ inline ExpandedShape expanded_shape(int32_t tokens, int32_t keys, int32_t batch,
     return s;
 }
 
-// For the join: as many rows of s.parts parts of a tile each.
-inline Plan rows_of_parts(int32_t tokens, const ExpandedShape& s) { return Plan{nullptr, tokens, s.parts * kTileKeys, 1, 0, 0}; }
+// For the join: as many rows of s.parts parts of a tile each as there are tokens, or, if that is less
+// (a padded buffer), max_q for each sequence: 256 rows for every work-group at most, 34 MB.
+inline Plan rows_of_parts(int32_t tokens, int32_t batch, int32_t max_q, const ExpandedShape& s) {
+    return Plan{nullptr, (int32_t)std::min<int64_t>(tokens, (int64_t)batch * max_q), s.parts * kTileKeys, 1, 0, 0};
+}
 
 }  // namespace
 }  // namespace v1
@@ -543,7 +550,7 @@ extern "C" int64_t v1_latent_expanded_workspace(int32_t tokens, int32_t keys, in
                                                 int32_t max_q) {
     if (tokens <= 0 || keys <= 0 || batch <= 0 || heads <= 0 || max_q <= 0) return 0;
     const ExpandedShape s = expanded_shape(tokens, keys, batch, heads, max_q);
-    return s.parts == 1 ? 0 : attn::parts_bytes(rows_of_parts(tokens, s), heads, kValue);
+    return s.parts == 1 ? 0 : attn::parts_bytes(rows_of_parts(tokens, batch, max_q, s), heads, kValue);
 }
 
 extern "C" int v1_latent_expanded(const v1_latent_expanded_args* a, void* stream) {
@@ -571,10 +578,12 @@ extern "C" int v1_latent_expanded(const v1_latent_expanded_args* a, void* stream
     const int64_t items = cdiv(units, xcds) * xcds * s.window * s.parts;
     V1_REQUIRE(items < kMostGroups, "latent_expanded: too many sequences, queries and heads for a launch");
     const int64_t group = std::min(cdiv(units, xcds), cdiv(2 * device_cus() / xcds, (int64_t)s.window * s.parts));
+    const Plan plan = rows_of_parts(tokens, batch, max_q, s);
+    const bool by_sequence = plan.rows < tokens;
     ExpandedParams p{static_cast<const uint16_t*>(q), q_row, q_head, static_cast<const uint16_t*>(kv), kv_row, kv_head,
                      static_cast<const uint16_t*>(rope), rope_row, cu_q, cu_k, tokens, keys, batch, heads, max_q, s.blocks, s.window,
                      s.windows, causal, s.parts, xcds, (int32_t)group, scale * kLog2e, static_cast<uint16_t*>(out), o_row, o_head, lse,
-                     parts_at(workspace, rows_of_parts(tokens, s), heads, kValue)};
+                     by_sequence, parts_at(workspace, plan, heads, kValue)};
     const hipStream_t st = as_stream(stream);
     static OncePerDevice once;
     constexpr size_t bytes = kBuffers * sizeof(ExpandedTile);
@@ -583,7 +592,6 @@ extern "C" int v1_latent_expanded(const v1_latent_expanded_args* a, void* stream
     hipLaunchKernelGGL(expanded_kernel, dim3((uint32_t)items), dim3(64 * kWaves), bytes, st, p);
     rc = V1_LAUNCHED("latent_expanded");
     if (rc != V1_OK || s.parts == 1) return rc;
-    JoinParams j{rows_of_parts(tokens, s), p.partial, p.out, o_row, o_head, lse, heads, cu_q, batch,
-                 max_q};
+    JoinParams j{plan, p.partial, p.out, o_row, o_head, lse, heads, cu_q, tokens, batch, max_q, by_sequence};
     return launch_join<kValue>(j, st, "latent_expanded: join");
 }

@@ -489,6 +489,6 @@ extern "C" int v1_kv8_attend(const v1_kv8_attend_args* a, void* stream) {
     hipLaunchKernelGGL(kv8_attend_kernel, dim3((uint32_t)(8 * spread)), dim3(64 * kWaves), sizeof(Kv8Lds), st, p);
     rc = V1_LAUNCHED("kv8_attend");
     if (rc != V1_OK || need == 0) return rc;
-    JoinParams j{plan, p.parts, p.out, o_row, o_head, lse, heads, nullptr, 0, 0};
+    JoinParams j{plan, p.parts, p.out, o_row, o_head, lse, heads, nullptr, 0, 0, 0, false};
     return launch_join<kDim>(j, st, "kv8_attend: join");
 }

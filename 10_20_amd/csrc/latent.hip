@@ -673,6 +673,6 @@ extern "C" int v1_latent_attend(const v1_latent_attend_args* a, void* stream) {
                    : hb == 32 ? launch_absorbed<2, 1>(p, blocks, st)
                               : launch_absorbed<2, 2>(p, blocks, st);
     if (rc != V1_OK || need == 0) return rc;
-    JoinParams j{plan, p.parts, p.out, o_row, o_head, lse, heads, nullptr, 0, 0};
+    JoinParams j{plan, p.parts, p.out, o_row, o_head, lse, heads, nullptr, 0, 0, 0, false};
     return launch_join<kLatent>(j, st, "latent_attend: join");
 }

@@ -106,6 +106,50 @@ def test_only_the_first_max_q_queries(heads, nq, max_q, causal):
         expanded.check(whole[:, h:h + 1], whole_lse[:, h:h + 1], q[:, h:h + 1], kv[:, h:h + 1], rope, nq, nk, causal)
 
 
+@gpu
+@pytest.mark.parametrize("nq,nk,max_q,heads,behind", [
+    ([200], [20000], 200, 2, 100000), ([1], [3000], 1, 16, 100000), ([3, 0, 70, 1], [5000, 40, 900, 0], 70, 2, 100000),
+    ([3, 0, 90, 1], [5000, 40, 900, 1], 70, 2, 100000), ([400, 300], [9000, 8000], 400, 1, 100000),
+    ([1] * 40 + [900] + [2] * 20, [3000] * 61, 900, 1, 100000), ([1] * 40 + [900] + [2] * 20, [3000] * 61, 900, 1, 0)])
+def test_parts_of_a_padded_buffer(nq, nk, max_q, heads, behind):
+    """Few queries in a buffer for many, their keys in several parts (but for the last
+    batch with its padding, whose blocks could be as many as the CUs): the sums take
+    the room of the sequences or of the tokens, and rows outside the sequences stay."""
+    print("expanded padded", nq[:4], max_q, behind, flush=True)
+    L = pkg("_lib")
+    first = 9
+    need = L.lib().v1_latent_expanded_workspace(sum(nq) + behind + first, sum(nk), len(nq), heads, max_q)
+    assert need <= (1 << 16) * 130 * 4 and (need > 0) == (max_q < 900 or behind == 0), need
+    q, kv, rope, cu_q, cu_k = expanded.inputs(7, nq, nk, heads)
+    wide = torch.full((sum(nq) + behind + first, heads, 192), float("nan"), device=DEV, dtype=torch.bfloat16)
+    wide[first:first + sum(nq)] = q
+    out = torch.full((wide.shape[0], heads, 128), 7.0, device=DEV, dtype=torch.bfloat16)
+    _, lse = LT.attend_expanded(wide, kv, rope, cu_q + first, cu_k, max_q, out=out, return_lse=True)
+    some = torch.zeros(wide.shape[0], device=DEV, dtype=torch.bool)
+    some[first:first + sum(nq)] = torch.cat([torch.arange(n, device=DEV) < max_q for n in nq])
+    assert bool((out[~some] == 7).all())
+    whole, whole_lse = LT.attend_expanded(q, kv, rope, cu_q, cu_k, return_lse=True)
+    mine = some[first:first + sum(nq)]
+    whole[mine], whole_lse[mine] = out[some], lse[some]
+    expanded.check(whole, whole_lse, q, kv, rope, nq, nk)
+
+
+def test_room_for_parts():
+    """Never more than 256 rows of sums for each work-group of one round."""
+    L = pkg("_lib")
+    if not L.LIB_PATH.exists():
+        pkg("build").build()
+    room = L.lib().v1_latent_expanded_workspace
+    for tokens in (1, 200, 8192, 100000, 1 << 20):
+        for batch in (1, 3, 60):
+            for max_q in (1, 200, 300, 5000, tokens):
+                for heads in (1, 16, 100):
+                    for keys in (100, 65536, 1 << 24):
+                        assert room(tokens, keys, batch, heads, min(max_q, tokens)) <= (1 << 16) * 130 * 4, (tokens, keys, batch, heads, max_q)
+    assert room(8192, 65536, 1, 16, 200) == room(200, 65536, 1, 16, 200) > 0
+    assert room(16384, 1 << 20, 1, 1, 1) == room(1, 1 << 20, 1, 1, 1) > 0
+
+
 def library_call(**change):
     L = pkg("_lib")
     if not L.LIB_PATH.exists():
