@@ -125,6 +125,9 @@ __device__ __forceinline__ void wait_barrier() {
 // The work-group's barrier for LDS data alone: copies stay in flight.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// Whether one launch holds so many work-groups (fewer than 2^32 work-items a dimension).
+inline bool launchable(int64_t groups, int threads) { return groups < (1ll << 32) / threads; }
+
 // ------------------------------------------------ parts of a row's keys
 // A row's keys, in tiles of 64, are split over several work-groups where the
 // rows alone would not fill the GPU.  Each part leaves its unnormalised sums

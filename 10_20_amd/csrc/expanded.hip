@@ -513,8 +513,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void expanded_kernel(ExpandedParams
 //   64 of 512, 16 heads, max_q not given         8192, 192        737, 221
 //   1000 of 100, 16 heads, max_q not given       391000, 1390   21100, 774
 //   63 of 100 and one of 16000, 16 heads         4032, 150       1426, 1301
-constexpr int64_t kMostGroups = (1ll << 32) / (64 * kWaves);  // (a launch has fewer than 2^32 work-items a dimension)
-
 struct ExpandedShape {
     int32_t blocks, window, windows, parts;
 };
@@ -524,7 +522,7 @@ inline ExpandedShape expanded_shape(int32_t tokens, int32_t keys, int32_t batch,
     const int64_t groups = std::min(batch * blocks, slots) * heads;
     ExpandedShape s;
     s.parts = (int32_t)std::max<int64_t>(1, std::min(device_cus() / std::max<int64_t>(1, groups), tiles / (4 * (int64_t)batch)));
-    if (batch * blocks <= 3 * slots && ((int64_t)batch * heads + 7) * blocks * s.parts < kMostGroups) {
+    if (batch * blocks <= 3 * slots && launchable(((int64_t)batch * heads + 7) * blocks * s.parts, 64 * kWaves)) {
         s.blocks = s.window = (int32_t)blocks;
         s.windows = batch;
     } else {
@@ -576,7 +574,7 @@ extern "C" int v1_latent_expanded(const v1_latent_expanded_args* a, void* stream
     const int64_t units = (int64_t)s.windows * heads;
     const int32_t xcds = units % 8 == 0 || units >= 64 ? 8 : 1;
     const int64_t items = cdiv(units, xcds) * xcds * s.window * s.parts;
-    V1_REQUIRE(items < kMostGroups, "latent_expanded: too many sequences, queries and heads for a launch");
+    V1_REQUIRE(launchable(items, 64 * kWaves), "latent_expanded: too many sequences, queries and heads for a launch");
     const int64_t group = std::min(cdiv(units, xcds), cdiv(2 * device_cus() / xcds, (int64_t)s.window * s.parts));
     const Plan plan = rows_of_parts(tokens, batch, max_q, s);
     const bool by_sequence = plan.rows < tokens;

@@ -437,6 +437,7 @@ extern "C" int v1_kv8_store(const v1_kv8_store_args* a, void* stream) {
                      requests, kv_heads, pages};
     // n tokens of a request touch at most min(n, n / 64 + 2) pages
     const int64_t most = std::min<int64_t>(tokens, (int64_t)tokens / kTileKeys + 2ll * requests);
+    V1_REQUIRE(launchable(most, 256), "kv8_store: too many tokens for a launch");
     hipLaunchKernelGGL(kv8_store_kernel, dim3((uint32_t)most, (uint32_t)(2 * kv_heads)), dim3(256), 0, as_stream(stream), p);
     return V1_LAUNCHED("kv8_store");
 }
@@ -474,7 +475,7 @@ extern "C" int v1_kv8_attend(const v1_kv8_attend_args* a, void* stream) {
     const int64_t need = v1_kv8_attend_workspace(rows, kv_heads, group, keys, lens != nullptr);
     V1_REQUIRE(workspace_bytes >= need && (need == 0 || workspace != nullptr),
                "kv8_attend: workspace of %lld bytes needed", (long long)need);
-    V1_REQUIRE(8 * spread < 1ll << 31, "kv8_attend: too many rows");
+    V1_REQUIRE(launchable(8 * spread, 64 * kWaves), "kv8_attend: too many rows and heads for a launch");
     const int32_t heads = kv_heads * group;
     Kv8Params p{static_cast<const uint16_t*>(q), q_row, q_head,
                 {static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool)},

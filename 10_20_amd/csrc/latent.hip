@@ -628,6 +628,7 @@ extern "C" int v1_latent_store(const v1_latent_store_args* a, void* stream) {
                "latent_store: inputs and pool must be 16-byte aligned, strides multiples of 8");
     V1_REQUIRE(pool_stride_bytes % 16 == 0 && pool_stride_bytes >= kRowBytes,
                "latent_store: pool stride must be a multiple of 16 and >= %d", kRowBytes);
+    V1_REQUIRE(launchable(cdiv(tokens, 4), 256), "latent_store: too many tokens for a launch");
     if (tokens == 0) return V1_OK;
     StoreParams p{static_cast<const uint16_t*>(latent), latent_stride, static_cast<const uint16_t*>(rope), rope_stride,
                   slots, tokens, static_cast<uint8_t*>(pool), pool_rows, pool_stride_bytes};
@@ -663,7 +664,7 @@ extern "C" int v1_latent_attend(const v1_latent_attend_args* a, void* stream) {
                "latent_attend: workspace of %lld bytes needed", (long long)need);
     const int32_t hb = absorbed_heads(rows, heads, keys);
     const int64_t splits = cdiv(heads, hb), spread = cdiv(items, 8), blocks = 8 * spread * splits;
-    V1_REQUIRE(blocks < 1ll << 31, "latent_attend: too many rows");
+    V1_REQUIRE(launchable(blocks, 512), "latent_attend: too many rows and heads for a launch");
     AbsorbedParams p{static_cast<const uint16_t*>(q), q_row, q_head, static_cast<const uint8_t*>(pool), pool_rows,
                      pool_stride_bytes, map, map_len, map_stride, map_shift, ids, ids_stride, plan, heads,
                      (int32_t)splits, (int32_t)spread, scale * kLog2e, static_cast<uint16_t*>(out), o_row, o_head, lse,
