@@ -223,7 +223,11 @@ def call_packed(name, t, *fields):
     """An entry point of PACKED, with its structure's fields in order, on the
     current stream of t's device (which need not be the current one)."""
     index = t.get_device()
-    entry, args = getattr(_lib or lib(), name), PACKED[name].pack(*fields)
+    entry = getattr(_lib or lib(), name)
+    try:
+        args = PACKED[name].pack(*fields)
+    except struct.error:
+        raise ValueError(f"{name}: a size past 2**31") from None
     if index == torch._C._cuda_getDevice():
         rc = entry(args, torch._C._cuda_getCurrentRawStream(index))
     else:
@@ -231,6 +235,14 @@ def call_packed(name, t, *fields):
             rc = entry(args, torch._C._cuda_getCurrentRawStream(index))
     if rc != V1_OK:
         check(rc, name)
+
+
+def workspace_bytes(name, index, *sizes):
+    """What the entry point asks for on a device."""
+    if any(n >> 31 for n in sizes):  # (ctypes would take the low 32 bits)
+        raise ValueError(f"{name}: a size past 2**31")
+    with torch.cuda.device(index):
+        return getattr(lib(), name)(*sizes)
 
 
 def ptr(t):

@@ -61,8 +61,7 @@ def _vector(name, t, n):
 # (sizes alone decide: asked of the library once for each)
 @functools.lru_cache(maxsize=4096)
 def _workspace_bytes(index, *sizes):
-    with torch.cuda.device(index):
-        return _lib.lib().v1_kv8_attend_workspace(*sizes)
+    return _lib.workspace_bytes("v1_kv8_attend_workspace", index, *sizes)
 
 
 def store(k, v, k_pool, v_pool, k_scale, v_scale, table, starts, cu_tokens):

@@ -64,8 +64,7 @@ def _scale(softmax_scale):
 # (sizes alone decide: asked of the library once for each)
 @functools.lru_cache(maxsize=4096)
 def _workspace_bytes(entry, index, *sizes):
-    with torch.cuda.device(index):
-        return getattr(_lib.lib(), entry)(*sizes)
+    return _lib.workspace_bytes(entry, index, *sizes)
 
 
 def store_rows(latent, rope, pool, slots):
@@ -79,8 +78,9 @@ def store_rows(latent, rope, pool, slots):
     code the nearest e4m3 value of x / s (ties to even); infinities are stored as
     +-448 s, NaN as NaN."""
     _lib.require_gpu(latent, rope, pool, slots)
-    tokens, ls, rs = latent.shape[0], latent.stride(), rope.stride()
-    if latent.shape != (tokens, LATENT) or latent.dtype != _BF16 or ls[1] != 1:
+    shape, ls, rs = latent.shape, latent.stride(), rope.stride()
+    tokens = shape[0] if len(shape) == 2 else -1
+    if shape != (tokens, LATENT) or latent.dtype != _BF16 or ls[1] != 1:
         raise ValueError(f"latent must be bfloat16 [tokens, {LATENT}] with a contiguous last dimension")
     if rope.shape != (tokens, ROPE) or rope.dtype != _BF16 or rs[1] != 1:
         raise ValueError(f"rope must be bfloat16 [tokens, {ROPE}] with a contiguous last dimension")
@@ -178,7 +178,7 @@ def attend_expanded(q, kv, k_rope, cu_q, cu_k=None, max_q=None, softmax_scale=No
     if q.dim() != 3 or q.shape[2] != HEAD + ROPE or q.dtype != _BF16 or q.stride(2) != 1 or not q.shape[1]:
         raise ValueError(f"q must be bfloat16 [tokens, heads, {HEAD + ROPE}] with a contiguous last dimension")
     tokens, heads, _ = q.shape
-    keys = kv.shape[0]
+    keys = kv.shape[0] if kv.dim() == 3 else -1
     if kv.dtype != _BF16 or kv.shape != (keys, heads, 2 * HEAD) or kv.stride(2) != 1:
         raise ValueError(f"kv must be bfloat16 [keys, heads, {2 * HEAD}] with a contiguous last dimension")
     if k_rope.dtype != _BF16 or k_rope.shape != (keys, ROPE) or k_rope.stride(1) != 1:

@@ -1,8 +1,14 @@
 """Calls of the attention over latent rows and 8-bit pages, and of their writers, that
 the library refuses before it launches anything."""
+import importlib
+
 import pytest
+import torch
 
 from conftest import pkg
+
+LT, K8 = pkg("latent"), pkg("kv8")
+BF16, F32, I32, F8 = torch.bfloat16, torch.float32, torch.int32, torch.float8_e4m3fn
 
 
 def refused(name, **fields):
@@ -32,3 +38,66 @@ KV8_STORE = dict(k=256, kt=128, kh=128, v=256, vt=128, vh=128, kp=256, kpp=8192,
 def test_more_work_groups_than_a_launch_holds(name, fields, change):
     """(A launch has fewer than 2^32 work-items a dimension.)"""
     assert "for a launch" in (refused(name, **{**fields, **change}) or ""), (name, change)
+
+
+# ------------------------------------------------- arguments that do not fit are ValueErrors
+@pytest.fixture
+def on_meta(monkeypatch):
+    """The modules' own checks, with tensors that have shapes and no memory; a call that
+    reaches the library fails the test."""
+    L = importlib.import_module("10_20_amd._lib")
+
+    class Lib:
+        def __getattr__(self, name):
+            def entry(*args):
+                raise AssertionError(f"{name} was called")
+            return entry
+
+    monkeypatch.setattr(L, "require_gpu", lambda *t: None)
+    monkeypatch.setattr(L, "_lib", Lib())
+    return lambda *shape, dtype=BF16: torch.empty(shape, device="meta", dtype=dtype)
+
+
+def test_sizes_past_32_bits(on_meta):
+    z, n = on_meta, 1 << 31
+    pool = z(8, 656, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="2\\*\\*31"):
+        LT.store_rows(z(n, 512), z(n, 64), pool, z(n, dtype=I32))
+    for many in (n, 2 * n, 2 * n + 1):  # (the last: one key or row, if its low 32 bits were taken)
+        for call in (lambda: LT.attend(z(many, 1, 576), pool, z(many, 3, dtype=I32), return_lse=True),
+                     lambda: LT.attend(z(2, 1, 576), pool, z(2, many, dtype=I32)), lambda: LT.attend(z(2, many, 576), pool, z(2, 3, dtype=I32)),
+                     lambda: LT.attend_expanded(z(many, 1, 192), z(5, 1, 256), z(5, 64), z(2, dtype=I32)),
+                     lambda: LT.attend_expanded(z(5, 1, 192), z(many, 1, 256), z(many, 64), z(2, dtype=I32)),
+                     lambda: LT.attend_expanded(z(5, 1, 192), z(5, 1, 256), z(5, 64), z(many + 1, dtype=I32))):
+            with pytest.raises(ValueError, match="2\\*\\*31"):
+                call()
+        pools = z(3, 64, 1, 128, dtype=F8), z(3, 64, 1, 128, dtype=F8), z(3, 1, dtype=F32), z(3, 1, dtype=F32)
+        for call in (lambda: K8.attend(z(2, 1, 128), *pools, z(2, 9, dtype=I32), ids=z(2, many, dtype=I32)),
+                     lambda: K8.attend(z(many, 1, 128), *pools, z(9, dtype=I32)), lambda: K8.attend(z(2, 1, 128), *pools, z(many, dtype=I32)),
+                     lambda: K8.store(z(many, 1, 128), z(many, 1, 128), *pools, z(2, 9, dtype=I32), z(2, dtype=I32), z(3, dtype=I32)),
+                     lambda: K8.store(z(5, 1, 128), z(5, 1, 128), *pools, z(many, 9, dtype=I32), z(many, dtype=I32), z(many + 1, dtype=I32))):
+            with pytest.raises(ValueError, match="2\\*\\*31"):
+                call()
+
+
+def test_dimensions_that_are_not_there(on_meta):
+    z = on_meta
+    pool = z(8, 656, dtype=torch.uint8)
+    for latent, rope in ((z(), z(5, 64)), (z(512), z(5, 64)), (z(5, 512), z()), (z(5, 512), z(64)), (z(1, 5, 512), z(5, 64))):
+        with pytest.raises(ValueError, match="must be"):
+            LT.store_rows(latent, rope, pool, z(5, dtype=I32))
+    for bad in (dict(kv=z()), dict(kv=z(5, 256)), dict(k_rope=z()), dict(k_rope=z(64)), dict(q=z()), dict(cu_q=z(dtype=I32)), dict(out=z())):
+        with pytest.raises(ValueError, match="must be"):
+            LT.attend_expanded(**{**dict(q=z(5, 1, 192), kv=z(5, 1, 256), k_rope=z(5, 64), cu_q=z(2, dtype=I32)), **bad})
+    for bad in (dict(q=z()), dict(pool=z(dtype=torch.uint8)), dict(ids=z(dtype=I32)), dict(table=z(dtype=I32)), dict(lens=z(dtype=I32)), dict(out=z())):
+        with pytest.raises(ValueError, match="must be"):
+            LT.attend(**{**dict(q=z(5, 1, 576), pool=pool, ids=z(5, 3, dtype=I32)), **bad})
+    codes, scales, table = z(3, 64, 1, 128, dtype=F8), z(3, 1, dtype=F32), z(2, 9, dtype=I32)
+    base = dict(k_pool=codes, v_pool=codes, k_scale=scales, v_scale=scales, table=table)
+    for bad in (dict(q=z()), dict(k_pool=z(dtype=F8)), dict(k_scale=z(dtype=F32)), dict(table=z(dtype=I32)), dict(lens=z(dtype=I32)),
+                dict(ids=z(dtype=I32)), dict(out=z())):
+        with pytest.raises(ValueError, match="must be"):
+            K8.attend(**{**base, "q": z(2, 1, 128), **bad})
+    for bad in (dict(k=z()), dict(table=z(dtype=I32)), dict(starts=z(dtype=I32)), dict(cu_tokens=z(dtype=I32)), dict(v_scale=z(dtype=F32))):
+        with pytest.raises(ValueError, match="must be"):
+            K8.store(**{**base, "k": z(5, 1, 128), "v": z(5, 1, 128), "starts": z(2, dtype=I32), "cu_tokens": z(3, dtype=I32), **bad})
