@@ -558,7 +558,7 @@ extern "C" int v1_latent_expanded(const v1_latent_expanded_args* a, void* stream
     V1_REQUIRE(tokens >= 0 && keys >= 0 && batch >= 0 && heads > 0 && max_q >= 0, "latent_expanded: bad shape");
     V1_REQUIRE(heads < 1 << 16, "latent_expanded: too many heads");
     V1_REQUIRE(keys <= kMostKeys && tokens <= kMostKeys, "latent_expanded: too many tokens or keys");
-    V1_REQUIRE(scale > 0.f && scale < __builtin_inff(), "latent_expanded: scale must be positive and finite");
+    V1_REQUIRE(scale > 0.f && scale * kLog2e < __builtin_inff(), "latent_expanded: scale must be positive and finite");
     const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kv) | reinterpret_cast<uintptr_t>(rope);
     V1_REQUIRE(all % 16 == 0 && (q_row | q_head | kv_row | kv_head | rope_row) % 8 == 0 &&
                    reinterpret_cast<uintptr_t>(out) % 8 == 0 && (o_row | o_head) % 4 == 0,

@@ -459,7 +459,7 @@ extern "C" int v1_kv8_attend(const v1_kv8_attend_args* a, void* stream) {
                "kv8_attend: bad shape");
     V1_REQUIRE(keys <= kMostKeys, "kv8_attend: too many keys");
     V1_REQUIRE(group <= kMaxGroup, "kv8_attend: at most %d query heads per KV head", kMaxGroup);
-    V1_REQUIRE(scale > 0.f && scale < __builtin_inff(), "kv8_attend: scale must be positive and finite");
+    V1_REQUIRE(scale > 0.f && scale * kLog2e < __builtin_inff(), "kv8_attend: scale must be positive and finite");
     V1_REQUIRE(aligned16(q) && (q_row | q_head) % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0 &&
                    (o_row | o_head) % 4 == 0,
                "kv8_attend: q must be 16-byte aligned with strides in multiples of 8, out 8-byte and 4");

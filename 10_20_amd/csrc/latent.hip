@@ -650,7 +650,7 @@ extern "C" int v1_latent_attend(const v1_latent_attend_args* a, void* stream) {
     V1_REQUIRE(rows >= 0 && heads > 0 && keys >= 0 && pool_rows >= 0 && pool_rows < 1ll << 31, "latent_attend: bad shape");
     V1_REQUIRE(heads < 1 << 16, "latent_attend: too many heads");
     V1_REQUIRE(keys <= kMostKeys, "latent_attend: too many keys");
-    V1_REQUIRE(scale > 0.f && scale < __builtin_inff(), "latent_attend: scale must be positive and finite");
+    V1_REQUIRE(scale > 0.f && scale * kLog2e < __builtin_inff(), "latent_attend: scale must be positive and finite");
     V1_REQUIRE(map_shift >= 0 && map_shift < 31 && map_len >= 0, "latent_attend: bad page map");
     V1_REQUIRE(aligned16(q) && aligned16(pool) && reinterpret_cast<uintptr_t>(out) % 8 == 0 && q_row % 8 == 0 &&
                    q_head % 8 == 0 && o_row % 4 == 0 && o_head % 4 == 0,

@@ -101,3 +101,11 @@ def test_dimensions_that_are_not_there(on_meta):
     for bad in (dict(k=z()), dict(table=z(dtype=I32)), dict(starts=z(dtype=I32)), dict(cu_tokens=z(dtype=I32)), dict(v_scale=z(dtype=F32))):
         with pytest.raises(ValueError, match="must be"):
             K8.store(**{**base, "k": z(5, 1, 128), "v": z(5, 1, 128), "starts": z(2, dtype=I32), "cu_tokens": z(3, dtype=I32), **bad})
+
+
+def test_scales_that_the_library_refuses():
+    expanded = dict(q=256, qr=384, qh=192, kv=256, kr=512, kh=256, rope=256, rr=64, cu_q=256, cu_k=256, out=256, o_row=256, o_head=128,
+                    lse=0, ws=0, wsb=0, tokens=8, keys=8, batch=1, heads=1, max_q=8, causal=1, scale=0.1)
+    for name, fields in (("v1_latent_attend", ATTEND), ("v1_kv8_attend", KV8), ("v1_latent_expanded", expanded)):
+        for s in (3e38, 1e39, float("inf"), float("nan"), 0.0, 1e-60):  # (3e38 times log2(e) is no float32, 1e39 neither)
+            assert "scale" in (refused(name, **{**fields, "scale": s}) or ""), (name, s)
