@@ -19,6 +19,9 @@ using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 // rescaled only past that (probabilities keep their relative precision; at 2^6
 // every third tile of 64 heads had a head to rescale, 4% of the time).
 constexpr float kLag = 16.f;
+// The maximum of keys whose scores are all -inf, which give 0 / 0 as the formula
+// does, told from that of no keys, -inf, which give zeros.
+constexpr float kLowest = -3.4028234663852886e38f;
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 
 union Frag {
@@ -323,7 +326,7 @@ __device__ __forceinline__ int32_t joined_row(const JoinParams& p, int32_t row) 
 }
 
 __device__ __forceinline__ void write_joined(const JoinParams& p, int32_t row, int32_t h, int32_t at4, f32x4 o, float top, float total) {
-    const bool none = total == 0.f;  // no key attended
+    const bool none = top == -__builtin_inff() && total == 0.f;  // no key attended
     const float inv = none ? 0.f : 1.0f / total;
     *reinterpret_cast<u32x2*>(p.out + row * p.o_row + h * p.o_head + 4 * at4) =
         none ? u32x2{0, 0} : u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};

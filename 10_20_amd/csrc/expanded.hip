@@ -441,7 +441,7 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, const Wor
         }
     }
     total += __shfl_xor(total, 32, kWave);
-    const bool none = total == 0.f;  // no key seen
+    const bool none = my_seen <= first * kTileKeys;  // no key seen
     // Rows leave through LDS as well, whole ones at a time: row c's numbers 32 d + 8 a
     // + 4 h .. are its piece 8 d + 2 a + h of four, pieces XORed by the row.
     static_assert(kBuffers * sizeof(ExpandedTile) >= kWaves * (kRows * 4 * kValue + 4), "rows and the flags before them");
@@ -480,7 +480,7 @@ __device__ __forceinline__ bool expanded_part(const ExpandedParams& p, const Wor
             const f32x4 x = *reinterpret_cast<const f32x4*>(rows + 512 * r + 16 * (c ^ r));
             if (r < left) *reinterpret_cast<f32x4*>(p.partial.sums + (at + r * step) * kValue + 4 * c) = x;
         }
-        if (h == 0 && c < left) p.partial.stats[at + c * step] = f32x2{mx, total};
+        if (h == 0 && c < left) p.partial.stats[at + c * step] = f32x2{none ? mx : fmaxf(mx, kLowest), total};
     }
     return false;
 }

@@ -260,6 +260,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_attend_kernel(Kv8Params p)
 #pragma unroll
     for (int d = 0; d < 8; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     float mx = -__builtin_inff(), total = 0.f;
+    bool some = false;  // a key that is attended
 
     int32_t id = fetch_id(0), id1 = fetch_id(1), id2 = fetch_id(2);
     int32_t page = fetch_page(id), page1 = fetch_page(id1);
@@ -279,7 +280,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_attend_kernel(Kv8Params p)
         // scales of this tile, by key
         lds.ks[wave][lane] = ks * p.scale2;
         lds.vs[wave][lane] = page < 0 ? 0.f : vs;
-        const uint64_t seen = __ballot(page >= 0) >> (4 * g);  // bit 16u + i: key 16u + 4g + i is attended
+        const uint64_t attended = __ballot(page >= 0), seen = attended >> (4 * g);  // bit 16u + i: key 16u + 4g + i is attended
+        some |= attended != 0;
         f32x4 d[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -359,7 +361,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_attend_kernel(Kv8Params p)
 #pragma unroll
     for (int i = 0; i < 8; ++i) *reinterpret_cast<f32x4*>(&lds.u[wave].out[c][16 * i + 4 * g]) = acc[i];
     if (g == 0) {
-        lds.top[wave][c] = mx;
+        lds.top[wave][c] = some ? fmaxf(mx, kLowest) : mx;
         lds.total[wave][c] = total;
     }
     __syncthreads();
@@ -377,7 +379,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_attend_kernel(Kv8Params p)
             o1 = fmaf(f, lds.u[w].out[h][dim + 1], o1);
         }
         if (it.parts == 1) {
-            const bool none = sum == 0.f;  // no key attended
+            const bool none = top == -__builtin_inff() && sum == 0.f;  // no key attended
             const float inv = none ? 0.f : 1.0f / sum;
             *reinterpret_cast<uint32_t*>(p.out + it.row * p.o_row + head * p.o_head + dim) =
                 none ? 0u : pack_bf16(o0 * inv, o1 * inv);

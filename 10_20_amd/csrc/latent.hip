@@ -551,7 +551,7 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
         float sum = lds.total[0][lane];
 #pragma unroll
         for (int k = 1; k < KQ; ++k) sum += lds.total[k][lane];
-        p.parts.stats[at + lane] = f32x2{none ? -__builtin_inff() : lds.top[0][lane], none ? 0.f : sum};
+        p.parts.stats[at + lane] = f32x2{none ? -__builtin_inff() : fmaxf(lds.top[0][lane], kLowest), none ? 0.f : sum};
     }
 #pragma unroll
     for (int half = 0; half < 2; ++half) {

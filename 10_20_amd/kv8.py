@@ -108,7 +108,8 @@ def attend(q, k_pool, v_pool, k_scale, v_scale, table, lens=None, ids=None, soft
            None: all
 
     Ids below zero, past the table or in pages outside the pool are not attended.  A
-    row without keys gives zeros and -inf.  softmax_scale > 0, default 1 / sqrt(128).
+    row without keys gives zeros and -inf, one whose keys all score -inf NaN and
+    -inf.  softmax_scale > 0, default 1 / sqrt(128).
     Returns out [rows, heads, 128] bf16, and with return_lse the natural log of the
     sum of exponentials, [rows, heads] fp32."""
     _lib.require_gpu(q, k_pool, v_pool, k_scale, v_scale, table, lens, ids, out)

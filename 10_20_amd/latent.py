@@ -105,7 +105,8 @@ def attend(q, pool, ids=None, table=None, page_bits=0, lens=None, softmax_scale=
            Without ids and lens every position of the table (or pool) is attended.
 
     Ids below zero, past the table or outside the pool are not attended.  A row
-    without keys gives zeros and a log-sum-exp of -inf.  softmax_scale > 0: default
+    without keys gives zeros and a log-sum-exp of -inf, one whose keys all score
+    -inf NaN and -inf.  softmax_scale > 0: default
     1 / sqrt(192), that of the expanded form.  Returns out [rows, heads, 512] bf16,
     and with return_lse the natural log of the sum of exponentials, [rows, heads] fp32."""
     _lib.require_gpu(q, pool, ids, table, lens, out)
@@ -169,7 +170,8 @@ def attend_expanded(q, kv, k_rope, cu_q, cu_k=None, max_q=None, softmax_scale=No
     max_q:  at least the longest sequence's queries; None: tokens.  The first max_q
             queries of a longer one are computed, their keys counted from its end as ever.
 
-    A query without keys gives zeros and -inf; rows of `out` outside [cu_q[0],
+    A query without keys gives zeros and -inf, one whose keys all score -inf NaN
+    and -inf; rows of `out` outside [cu_q[0],
     cu_q[-1]) or past a sequence's first max_q are left as they are.  softmax_scale > 0, default 1 / sqrt(192).  Returns
     out [tokens, heads, 128] bf16, and with return_lse the natural log of the sum
     of exponentials, [tokens, heads] fp32."""
