@@ -427,9 +427,10 @@ extern "C" int v1_kv8_store(const v1_kv8_store_args* a, void* stream) {
     V1_REQUIRE(kv_heads <= 32767, "kv8_store: too many heads");
     V1_REQUIRE(aligned16(k) && aligned16(v) && (k_token | k_head | v_token | v_head) % 8 == 0,
                "kv8_store: k and v must be 16-byte aligned with strides in multiples of 8");
-    V1_REQUIRE((reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool)) % 8 == 0 &&
-                   (kp_page | kp_token | kp_head | vp_page | vp_token | vp_head) % 8 == 0,
-               "kv8_store: pools must be 8-byte aligned with strides in multiples of 8");
+    // (the store's own pieces are of 8 bytes; the attention that reads the pools takes 16)
+    V1_REQUIRE(aligned16(k_pool) && aligned16(v_pool) &&
+                   (kp_page | kp_token | kp_head | vp_page | vp_token | vp_head) % 16 == 0,
+               "kv8_store: pools must be 16-byte aligned with strides in multiples of 16");
     if (tokens == 0 || requests == 0 || table_len == 0 || pages == 0) return V1_OK;
     Kv8StoreParams p{{static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v)},
                      {k_token, v_token}, {k_head, v_head},

@@ -2,8 +2,9 @@
 e4m3fn codes with one fp32 scale for each page and KV head, half the bytes of the
 bf16 pools that attention.attend_slots reads.
 
-Pools: k_pool, v_pool [pages, 64, kv_heads, 128] float8_e4m3fn (any strides, the
-last dimension contiguous: token-major and head-major pages alike), k_scale,
+Pools: k_pool, v_pool [pages, 64, kv_heads, 128] float8_e4m3fn (16-byte aligned, any
+strides in multiples of 16, the last dimension contiguous: token-major and
+head-major pages alike), k_scale,
 v_scale [pages, kv_heads] fp32.  Position i of a request lies in page
 table[i // 64], the layout of the page manager.  `store` appends tokens, `attend`
 reads them for one query position per row: the first positions of a context or

@@ -662,7 +662,7 @@ int v1_latent_expanded(const v1_latent_expanded_args* a, void* stream);
 int64_t v1_latent_expanded_workspace(int32_t tokens, int32_t keys, int32_t batch, int32_t heads, int32_t max_q);
 /* ------------------------------------------------------------------------
  * K / V pages of 64 tokens in OCP e4m3fn codes, [pages, 64, kv_heads, 128] with
- * any strides (bytes: page, token, head), and one fp32 scale for each page and
+ * any strides (bytes, multiples of 16: page, token, head; 16-byte aligned), and one fp32 scale for each page and
  * head, [pages, kv_heads] (K and V their own; *_page: row strides).  No
  * counterpart in the reference, whose K / V pools are bf16.
  *

@@ -109,3 +109,9 @@ def test_scales_that_the_library_refuses():
     for name, fields in (("v1_latent_attend", ATTEND), ("v1_kv8_attend", KV8), ("v1_latent_expanded", expanded)):
         for s in (3e38, 1e39, float("inf"), float("nan"), 0.0, 1e-60):  # (3e38 times log2(e) is no float32, 1e39 neither)
             assert "scale" in (refused(name, **{**fields, "scale": s}) or ""), (name, s)
+
+
+@pytest.mark.parametrize("change", [dict(kp=264), dict(vp=8), dict(kpp=8200), dict(vpt=136), dict(kph=8)])
+def test_pools_that_only_one_of_writer_and_reader_would_take(change):
+    for name, fields in (("v1_kv8_store", KV8_STORE), ("v1_kv8_attend", KV8)):
+        assert "pools must be 16-byte aligned" in (refused(name, **{**fields, **change}) or ""), name
