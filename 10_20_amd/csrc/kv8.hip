@@ -185,7 +185,10 @@ struct Kv8Lds {
 //           c is query head c of the group.
 //   output  O^T = V^T P^T: V codes go memory -> LDS and come back transposed
 //           (ds_read_b64_tr_b8); the lane's own scores are its B fragment's
-//           probabilities, times the page's V scale, rounded to bf16 once.
+//           probabilities, times the page's V scale, in two bf16 numbers, which leaves
+//           2^-17 of each (one number, 2^-8: 1.33 times the error of a rounded exact
+//           result; 200.5 us where two take 201, 60.5 where 62.8 for 600 rows of one KV head and
+//           1000-3000 tokens).
 //
 // Bound by memory: 48 contexts of 4096 to 65536 tokens, 4 KV heads of 8 query heads,
 // 202 us for 1.09 GB, 5.4 TB/s (a 1 GiB copy moves 5.2).  8 rows of 2048 chosen tokens, one KV head: 7 us
@@ -322,7 +325,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_attend_kernel(Kv8Params p)
             for (int i = 0; i < 8; ++i) acc[i] *= keep;
         }
         const float sub = mx == -__builtin_inff() ? 0.f : mx;
-        Frag pf[2];
+        Frag pf[2], rest[2];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const f32x4 f = *reinterpret_cast<const f32x4*>(&lds.vs[wave][16 * u + 4 * g]);
@@ -332,8 +335,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_attend_kernel(Kv8Params p)
                 x[i] = __builtin_amdgcn_exp2f(s[u][i] - sub);
                 total += x[i];
             }
-            pf[u / 2].w[2 * (u & 1)] = pack_bf16(x[0] * f[0], x[1] * f[1]);
-            pf[u / 2].w[2 * (u & 1) + 1] = pack_bf16(x[2] * f[2], x[3] * f[3]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float p0 = x[2 * i] * f[2 * i], p1 = x[2 * i + 1] * f[2 * i + 1];
+                const uint32_t w = pack_bf16(p0, p1);
+                pf[u / 2].w[2 * (u & 1) + i] = w;
+                rest[u / 2].w[2 * (u & 1) + i] = pack_bf16(p0 - __uint_as_float(w << 16), p1 - __uint_as_float(w & 0xffff0000u));
+            }
         }
         // this tile's values have landed: behind them at least the next tile's 8 loads of keys were issued, if there is one
         if (t + 1 < mine) {
@@ -351,7 +359,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_attend_kernel(Kv8Params p)
             for (int i = 0; i < 8; ++i) {
                 const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
                     (__attribute__((address_space(3))) i32x2*)(v + 16 * (i ^ (r & 7)) + 8 * (c & 1)));
-                acc[i] = mfma16(bf16_of_codes((uint32_t)w[0], (uint32_t)w[1]), pf[step], acc[i]);
+                const Frag a = bf16_of_codes((uint32_t)w[0], (uint32_t)w[1]);
+                acc[i] = mfma16(a, pf[step], acc[i]);
+                acc[i] = mfma16(a, rest[step], acc[i]);
             }
         }
     }
