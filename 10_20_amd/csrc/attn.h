@@ -17,7 +17,9 @@ using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 
 // The maximum that is subtracted may lag the true one by 2^kLag: sums are
 // rescaled only past that (probabilities keep their relative precision; at 2^6
-// every third tile of 64 heads had a head to rescale, 4% of the time).
+// every third tile of 64 heads had a head to rescale, 4% of the time).  So sums
+// hold up to 2^16 times the number of keys times a value before they are divided
+// by their total: values past some 2^100 may overflow where their mean does not.
 constexpr float kLag = 16.f;
 // The maximum of keys whose scores are all -inf, which give 0 / 0 as the formula
 // does, told from that of no keys, -inf, which give zeros.
@@ -141,7 +143,12 @@ inline bool launchable(int64_t groups, int threads) { return groups < (1ll << 32
 //              kPlanRows of them): the smallest of nine sizes of a part, from
 //              sum(tiles) / slots to sum(tiles) / target, with no more than
 //              `slots` parts, else the last (at most target + rows parts), found
-//              by every work-group from the lengths.  By the capacity instead, 7 rows
+//              by every work-group from the lengths.  Where the rows alone are
+//              `slots` or more, or past kPlanRows, the first rule holds, one part a
+//              row, and the longest row is a work-group's: contexts of 4096 to
+//              131072, us on both sides of that: 127 and 128 rows of 128 heads 2330,
+//              4240; 255 and 256 of 16 1600, 2760; 8-bit, 255 and 256 of 8 KV heads
+//              4090, 6130, 256 and 257 of 4 1540, 4400.  By the capacity instead below it, 7 rows
 //              of 64 heads and up to 60000 latent rows take 69 us (58 so), 40 rows of
 //              up to 30000 171 (89), 48 contexts of 4 KV heads in 8 bits 337 (202).
 //              Parts go to the XCDs in turn, since their number is known there alone:
@@ -264,8 +271,8 @@ inline int64_t items_at_most(const Plan& p) {
 // Tiles of a part of rows of `tiles` tiles: the number of parts whose work-groups
 // end first, `slots` of them running at a time, where a part costs `start` tiles'
 // time beside its own and each part of several another `leave` (its sums, written
-// and joined).  128 rows of 16 heads over 2048 latent rows take 44 us in the two
-// parts a row that this finds, 51 in four, 70 in eight.
+// and joined).  128 rows of 16 heads over 2048 of two million latent rows take 43 us in
+// the two parts a row that this finds, 51 in one, 52 in four, 69 in eight.
 inline int32_t chunk_for(int64_t rows, int64_t tiles, int64_t slots, int64_t start, int64_t leave) {
     int64_t best = tiles, least = cdiv(rows, slots) * (tiles + start);
     for (int64_t parts = 2; parts <= tiles && rows * (parts - 1) < slots; ++parts) {

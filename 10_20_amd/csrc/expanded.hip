@@ -10,7 +10,10 @@
 //   scores  S^T = K Q^T, a tile of 64 keys at a time from LDS;
 //   output  O^T = V^T P^T: a lane's scores are already the probabilities of its
 //           B fragment (the key order inside 16 keys is chosen so), rounded to
-//           bf16 once; V comes transposed from LDS (ds_read_b64_tr_b16).
+//           bf16 once, 2^-8 of each at most, as the output is (1.38 times the error of
+//           a rounded exact result; a second number for the rest would be 16 products
+//           more beside a tile's 40, of the units that bound the kernel); V comes
+//           transposed from LDS (ds_read_b64_tr_b16).
 // Scores, maxima and sums stay fp32, exponentials are base 2.  Tiles come memory
 // -> LDS two ahead; rows are laid with their 16-byte chunks XORed by the row so
 // that the fragments' reads meet different banks.

@@ -142,16 +142,17 @@ __device__ __forceinline__ void copy_block(uint64_t src, uint32_t region) {
 //           transposed by the LDS read (ds_read_b64_tr_b8), exact in bf16.  Up to 32
 //           heads the former are two bf16 numbers, which leaves 2^-17 (1 us of 44 for
 //           128 rows of 16 heads, 20 of 265 for 1024 rows of 32); 64 heads round them
-//           once (2^-9 of each at most, as the output is), since the second products
+//           once (2^-8 of each at most, as the output is), since the second products
 //           and their 32 registers would cost more than the waves have.
 //
-// 1024 rows of 128 heads over 2048 chosen rows each: 665 us, 834 TFLOP/s (an 8192^3
+// 1024 rows of 128 heads over 2048 chosen rows each: 650-665 us, 834-853 TFLOP/s (an 8192^3
 // library product: 1210), bound by the issue of the two waves of a SIMD: a tile of
 // 64 heads is 72 products of 16 cycles a wave, and a conversion or fold for every
 // third of their cycles; 12 of a work-group's 80 us are its start and end.  128
-// rows of 16 heads: 47 us, 3.6 TB/s, in the loop the 6.1 TB/s at which memory gives
-// random rows of 656 bytes.  7 contexts of 5000 to 131072, 64 heads: 71 us, 9 of
-// them the join.  On the way: all eight waves doing both halves, a tile at a time,
+// rows of 16 heads: 42-50 us with the join, 3.4-4.1 TB/s; in the loop 1.80 us a tile, 6.0
+// TB/s (256 rows of 2048 and of 4096 of two million latent rows, 67 and 125 us), where
+// copies of random rows to LDS alone reach 6.2.  7 contexts of 5000 to 131072, 64
+// heads: 62-70 us, 9 of them the join.  On the way: all eight waves doing both halves, a tile at a time,
 // 2786 us for the first; scorers and multipliers apart 1280; products between the
 // conversions and the copies 768; tiles by blocks of 16 rows 680.
 template <int HT, int HG>
@@ -582,6 +583,10 @@ __global__ __launch_bounds__(512, 2) void absorbed_kernel(AbsorbedParams p) {
 //     64 rows  48.4 / 47.3 / 43.9
 //    128 rows  95.5 / 73.5 / 63.9
 //   1024 rows   754 /  534 /  360
+// (Keys are the row's capacity: a call does not wait for the device to know its
+// lengths.  8 rows of 64 heads and some 2000 tokens take 21 us in tables of 2048, 29
+// in tables of 16384 and more.  So a row's heads, and with them its probabilities' bits,
+// depend on the batch.)
 inline int32_t absorbed_heads(int32_t rows, int32_t heads, int32_t keys) {
     const int64_t cus = device_cus(), tiles = cdiv(keys, kTileKeys);
     auto few = [&](int32_t of) {

@@ -2,9 +2,10 @@
 where one latent vector per token serves every head.
 
 A cache row is 656 bytes: 512 OCP e4m3fn codes, 64 bf16 rope-key numbers, 4 fp32
-scales (code j stands for code * scale[j // 128]); the row that
-native_kernels.gather_rows, the page manager and the tail staging move as opaque
-bytes.  `store_rows` writes rows, `attend` reads them with queries that already
+scales, in this order (code j stands for code * scale[j // 128]; a cache with its
+scales before the rope numbers is another format of the same size, and is not told
+apart); the row that native_kernels.gather_rows, the page manager and the tail
+staging move as opaque bytes.  `store_rows` writes rows, `attend` reads them with queries that already
 carry the key projection ("absorbed": one key of 512 + 64 numbers for all heads,
 its first 512 the value), `attend_expanded` is the prompt's form over keys and
 values expanded per head from the latent.
