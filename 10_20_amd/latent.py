@@ -5,10 +5,10 @@ A cache row is 656 bytes: 512 OCP e4m3fn codes, 64 bf16 rope-key numbers, 4 fp32
 scales, in this order (code j stands for code * scale[j // 128]; a cache with its
 scales before the rope numbers is another format of the same size, and is not told
 apart); the row that native_kernels.gather_rows, the page manager and the tail
-staging move as opaque bytes.  `store_rows` writes rows, `attend` reads them with queries that already
-carry the key projection ("absorbed": one key of 512 + 64 numbers for all heads,
-its first 512 the value), `attend_expanded` is the prompt's form over keys and
-values expanded per head from the latent.
+staging move as opaque bytes.  `store_rows` writes rows, `attend` reads them with
+queries that already carry the key projection ("absorbed": one key of 512 + 64
+numbers for all heads, its first 512 the value), `attend_expanded` is the prompt's
+form over keys and values expanded per head from the latent.
 
 Every call launches on the current stream of its tensors' device, never
 synchronises, and raises ValueError for arguments that do not fit.
@@ -172,8 +172,8 @@ def attend_expanded(q, kv, k_rope, cu_q, cu_k=None, max_q=None, softmax_scale=No
             queries of a longer one are computed, their keys counted from its end as ever.
 
     A query without keys gives zeros and -inf, one whose keys all score -inf NaN
-    and -inf; rows of `out` outside [cu_q[0],
-    cu_q[-1]) or past a sequence's first max_q are left as they are.  softmax_scale > 0, default 1 / sqrt(192).  Returns
+    and -inf; rows of `out` outside [cu_q[0], cu_q[-1]) or past a sequence's first
+    max_q are left as they are (their log-sum-exps are not set).  softmax_scale > 0, default 1 / sqrt(192).  Returns
     out [tokens, heads, 128] bf16, and with return_lse the natural log of the sum
     of exponentials, [tokens, heads] fp32."""
     cu_k = cu_q if cu_k is None else cu_k

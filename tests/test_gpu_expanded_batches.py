@@ -134,6 +134,48 @@ def test_parts_of_a_padded_buffer(nq, nk, max_q, heads, behind):
     expanded.check(whole, whole_lse, q, kv, rope, nq, nk)
 
 
+@gpu
+@pytest.mark.parametrize("batch,tokens,keys,max_q,heads", [(70, 3000, 3000, None, 2), (3, 20000, 9000, 40, 2), (61, 1000, 60000, 900, 1)])
+def test_graphs_whose_lengths_change(batch, tokens, keys, max_q, heads):
+    """Captured once (slots; a padded buffer in parts; slots in parts) and replayed with
+    other sequences, lengths of 0 and rows behind the last one among them."""
+    print("expanded graph", batch, max_q, flush=True)
+    rng = random.Random(batch)
+    q, kv, rope, _, _ = expanded.inputs(batch, [tokens], [keys], heads)
+    cu_q, cu_k = (torch.zeros(batch + 1, device=DEV, dtype=torch.int32) for _ in range(2))
+    out = torch.zeros((tokens, heads, 128), device=DEV, dtype=torch.bfloat16)
+
+    def refill():
+        most = min(max_q or tokens, tokens // batch)
+        nq = [rng.choice([0, 1, rng.randint(0, most), most]) for _ in range(batch)]
+        if batch > 3:
+            nq[rng.randrange(batch)] = (max_q or 1500) // 2
+        nk = [rng.randint(0, keys // batch) for _ in nq]
+        for cu, n in ((cu_q, nq), (cu_k, nk)):
+            cu.copy_(torch.tensor([0] + n).cumsum(0))
+        out.fill_(7.0)
+        return nq, nk
+
+    refill()
+    LT.attend_expanded(q, kv, rope, cu_q, cu_k, max_q, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _, lse = LT.attend_expanded(q, kv, rope, cu_q, cu_k, max_q, out=out, return_lse=True)
+    for _ in range(4):
+        nq, nk = refill()
+        n = sum(nq)
+        assert n <= tokens
+        want, want_lse = LT.attend_expanded(q, kv, rope, cu_q, cu_k, max_q, return_lse=True)
+        torch.randn(1 << 20, device=DEV).sort()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[:n], want[:n]) and torch.equal(lse[:n], want_lse[:n]) and bool((out[n:] == 7).all())
+        b = nq.index(max(nq))
+        i, j = int(cu_q[b]), int(cu_k[b])
+        expanded.check(out[i:i + nq[b]], lse[i:i + nq[b]], q[i:i + nq[b]], kv[j:j + nk[b]], rope[j:j + nk[b]], [nq[b]], [nk[b]])
+
+
 def test_room_for_parts():
     """Never more than 256 rows of sums for each work-group of one round."""
     L = pkg("_lib")
