@@ -10,6 +10,9 @@ table[i // 64], the layout of the page manager.  `store` appends tokens, `attend
 reads them for one query position per row: the first positions of a context or
 the Top-K's ids.
 
+Sums are fp32, undivided until the end, and may carry 2^16 times the keys' number
+times a value: they are kept for magnitudes between 2^-100 and 2^100.
+
 Every call launches on the current stream of its tensors' device, never
 synchronises, and raises ValueError for arguments that do not fit.
 """

@@ -10,6 +10,9 @@ queries that already carry the key projection ("absorbed": one key of 512 + 64
 numbers for all heads, its first 512 the value), `attend_expanded` is the prompt's
 form over keys and values expanded per head from the latent.
 
+Sums are fp32, undivided until the end, and may carry 2^16 times the keys' number
+times a value: they are kept for magnitudes between 2^-100 and 2^100.
+
 Every call launches on the current stream of its tensors' device, never
 synchronises, and raises ValueError for arguments that do not fit.
 """
