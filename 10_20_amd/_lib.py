@@ -166,6 +166,10 @@ _SIGNATURES = {
     "v1_kv8_attend": (_c_i32, [ctypes.c_char_p, _vp]),
     "v1_kv8_attend_workspace": (_c_i64, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32]),
     "v1_latent_expanded_workspace": (_c_i64, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32]),
+    "v1_paged_append": (_c_i32, [ctypes.c_char_p, _vp]),
+    "v1_paged_keep": (_c_i32, [ctypes.c_char_p, _vp]),
+    "v1_paged_attend": (_c_i32, [ctypes.c_char_p, _vp]),
+    "v1_paged_attend_workspace": (_c_i64, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32]),
 }
 
 # Arguments of the entry points that take them in a structure, packed by
@@ -177,6 +181,9 @@ PACKED = {
     "v1_latent_expanded": struct.Struct("16q6if4x"),
     "v1_kv8_store": struct.Struct("23q4i"),
     "v1_kv8_attend": struct.Struct("27q5if"),
+    "v1_paged_append": struct.Struct("29q8i"),
+    "v1_paged_keep": struct.Struct("14q4i"),
+    "v1_paged_attend": struct.Struct("26q8i2f"),
 }
 
 _lock = threading.Lock()

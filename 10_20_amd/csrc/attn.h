@@ -181,15 +181,16 @@ __device__ __forceinline__ void cut(Item& it) {
     it.tiles = min(each, tiles - it.first);
 }
 
-// The planned parts of up to kPlanRows rows, four rows a lane (row 4 lane + i);
-// returns the number of parts before the lane's first row.
-__device__ __forceinline__ int32_t plan_parts(const Plan& p, int32_t (&keys)[4], int32_t (&parts)[4]) {
+// The planned parts of up to kPlanRows rows, four rows a lane (row 4 lane + i), of
+// keys_of_row(row) keys each; returns the number of parts before the lane's first row.
+template <class Keys>
+__device__ __forceinline__ int32_t plan_parts(const Plan& p, int32_t (&keys)[4], int32_t (&parts)[4], Keys keys_of_row) {
     const int32_t lane = (int32_t)threadIdx.x % kWave;
     int32_t tiles = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int32_t r = 4 * lane + i;
-        keys[i] = min(max(p.lens[min(r, p.rows - 1)], 0), p.keys);
+        keys[i] = keys_of_row(min(r, p.rows - 1));
         if (r >= p.rows) keys[i] = 0;
         tiles += tiles_of(keys[i]);
     }
@@ -221,17 +222,18 @@ __device__ __forceinline__ int32_t plan_parts(const Plan& p, int32_t (&keys)[4],
 }
 
 // Work item `index`; false: there is none.  (Every wave finds it by itself.)
-__device__ __forceinline__ bool find_item(const Plan& p, int32_t index, Item& it) {
+template <class Keys>
+__device__ __forceinline__ bool find_item(const Plan& p, int32_t index, Item& it, Keys keys_of_row) {
     if (p.chunk > 0) {
         it.parts = max(1, (tiles_of(p.keys) + p.chunk - 1) / p.chunk);
         it.row = index / it.parts;
         it.part = index - it.row * it.parts;
         if (it.row >= p.rows) return false;
-        it.keys = keys_of(p, it.row);
+        it.keys = keys_of_row(it.row);
     } else {
         int32_t keys[4], parts[4];
         const int32_t lane = (int32_t)threadIdx.x % kWave;
-        int32_t at = plan_parts(p, keys, parts);
+        int32_t at = plan_parts(p, keys, parts, keys_of_row);
         int32_t row = -1, part = 0, n = 0, of = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -257,6 +259,10 @@ __device__ __forceinline__ bool find_item(const Plan& p, int32_t index, Item& it
     it.parts = __builtin_amdgcn_readfirstlane(it.parts);
     cut(it);
     return true;
+}
+
+__device__ __forceinline__ bool find_item(const Plan& p, int32_t index, Item& it) {
+    return find_item(p, index, it, [&](int32_t row) __attribute__((always_inline)) { return keys_of(p, row); });
 }
 
 // Whether the device's lengths may decide: few rows, and their tiles can be added in 32 bits.

@@ -731,6 +731,113 @@ typedef struct {
 } v1_kv8_attend_args;
 int v1_kv8_attend(const v1_kv8_attend_args* a, void* stream);
 int64_t v1_kv8_attend_workspace(int32_t rows, int32_t kv_heads, int32_t group, int32_t keys, int32_t ragged);
+/* ------------------------------------------------------------------------
+ * K / V pages of 64 tokens of bf16 (fp16 != 0: fp16) numbers, [pages, 64,
+ * kv_heads, 128] with any strides (numbers, multiples of 8: page, token, head;
+ * 16-byte aligned), position i of request r in page table[r * table_stride + i / 64].
+ * No counterpart in the reference, whose pools are read by an external library or
+ * slot by slot.
+ *
+ * v1_paged_append writes tokens cu_tokens[r] .. cu_tokens[r + 1] - 1 of k, v
+ * [tokens, kv_heads, 128] at positions starts[r], starts[r] + 1, ... of request r,
+ * keys rotated, and q [tokens, heads, 128] rotated to out (which may be q; heads
+ * may be 0).  rotations [rotation_rows, rotated] fp32: cosines, then sines, of an
+ * angle's rotated / 2 pairs; pair i is numbers i and i + rotated / 2, or
+ * (interleaved) 2i and 2i + 1; numbers from `rotated` (16, 32, .. 128) on are
+ * copied.  A token's angle is its position, or positions[t] (NULL: none).  Tokens of
+ * no request or with an angle outside the table are skipped; positions below zero or
+ * past the table and pages outside the pool are not written to.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+    const void* q;
+    int64_t q_token, q_head;
+    const void* k;
+    int64_t k_token, k_head;
+    const void* v;
+    int64_t v_token, v_head;
+    void* out;
+    int64_t o_token, o_head;
+    void* k_pool;
+    int64_t kp_page, kp_token, kp_head;
+    void* v_pool;
+    int64_t vp_page, vp_token, vp_head;
+    int64_t pages;
+    const int32_t* table;
+    int64_t table_stride;
+    const int32_t* starts;
+    const int32_t* cu_tokens;
+    const float* rotations;
+    int64_t rotation_row, rotation_rows;
+    const int32_t* positions;
+    int32_t table_len, tokens, requests, heads, kv_heads, rotated, interleaved, fp16;
+} v1_paged_append_args;
+int v1_paged_append(const v1_paged_append_args* a, void* stream);
+/* Row starts[r] + i of request r := row starts[r] + ids[cu_ids[r] + i], K and V, for
+ * all i at once; ids of a request ascend from zero or above (an id below its own
+ * index is not moved).  Positions past the table and pages outside the pool are
+ * skipped. */
+typedef struct {
+    void* k_pool;
+    int64_t kp_page, kp_token, kp_head;
+    void* v_pool;
+    int64_t vp_page, vp_token, vp_head;
+    int64_t pages;
+    const int32_t* table;
+    int64_t table_stride;
+    const int32_t* starts;
+    const int32_t* ids;
+    const int32_t* cu_ids;
+    int32_t table_len, count, requests, kv_heads;
+} v1_paged_keep_args;
+int v1_paged_keep(const v1_paged_keep_args* a, void* stream);
+/* Attention of ragged queries over the pages: q [tokens, kv_heads * group, 128],
+ * request r's queries cu_q[r] .. cu_q[r + 1] - 1 (cu_q NULL: query r) at the end of
+ * its lens[r] keys (within [0, 64 * table_len]): query i of nq at position
+ * lens[r] - nq + i.  With d = scale q . k_j, softcap tanh(d / softcap) where softcap
+ * > 0, less slopes[head] |position - j| (slopes NULL: 0), out (same type, 128) =
+ * softmax over the keys seen, times v_j.  Seen: j < prefix[r] (NULL: 0), and
+ * max(document[token] (NULL: 0), position - window + 1 (window 0: 0)) <= j <= position.
+ *
+ * parents (not NULL; prefix and document NULL, max_q <= 256): the queries are
+ * drafted tokens, each a child of the request's draft parents[token] (0 .. its own
+ * index - 1; others: of the context).  Draft i sees the lens[r] - nq keys before the
+ * drafts (those of its window), itself and its ancestors; its position is lens[r] - nq
+ * + its depth.
+ *
+ * Keys in pages outside the pool are not attended; no key: zeros and an lse of -inf;
+ * keys that all score -inf: NaN and -inf.  max_q: at least the longest request's
+ * queries; of a longer one the first max_q are computed.  lse (may be NULL): [tokens,
+ * kv_heads * group].  Rows outside the requests or past max_q are not written.
+ * workspace: v1_paged_attend_workspace(tokens, requests, kv_heads, group, max_q (1
+ * without cu_q), 64 * table_len, window) bytes, the call's own until the stream has
+ * passed it.  scale > 0. */
+typedef struct {
+    const void* q;
+    int64_t q_token, q_head;
+    const void* k_pool;
+    int64_t kp_page, kp_token, kp_head;
+    const void* v_pool;
+    int64_t vp_page, vp_token, vp_head;
+    int64_t pages;
+    const int32_t* table;
+    int64_t table_stride;
+    const int32_t* lens;
+    const int32_t* cu_q;
+    const int32_t* prefix;
+    const int32_t* document;
+    const int32_t* parents;
+    const float* slopes;
+    void* out;
+    int64_t o_token, o_head;
+    float* lse;
+    void* workspace;
+    int64_t workspace_bytes;
+    int32_t table_len, tokens, requests, max_q, kv_heads, group, window, fp16;
+    float scale, softcap;
+} v1_paged_attend_args;
+int v1_paged_attend(const v1_paged_attend_args* a, void* stream);
+int64_t v1_paged_attend_workspace(int32_t tokens, int32_t requests, int32_t kv_heads, int32_t group, int32_t max_q,
+                                  int32_t keys, int32_t window);
 #ifdef __cplusplus
 }
 #endif
