@@ -1,0 +1,457 @@
+// Attention of many queries of each request over K / V pages of 16-bit numbers (the
+// same sums as those of few queries, with the keys' tiles shared by 256 columns).
+#include "paged_attend.h"
+
+namespace v1 {
+namespace {
+
+using namespace paged;
+
+constexpr int kRows = 32;                           // columns of a wave
+constexpr int kWaves = 8, kBlock = kWaves * kRows;  // of a work-group
+constexpr int kBuffers = 4;                         // tiles in LDS
+static_assert(kBlock == kBlockColumns);
+
+using f32x16 = __attribute__((ext_vector_type(16))) float;
+using i16x4 = __attribute__((ext_vector_type(4))) short;
+
+struct PageTile {
+    uint8_t key[kTileKeys][2 * kDim];
+    uint8_t value[kTileKeys][2 * kDim];
+};
+
+struct BlocksLds {
+    PageTile tile[kBuffers];
+    Tree tree;
+    int32_t lo[kWaves], hi[kWaves];
+};
+
+template <class T>
+__device__ __forceinline__ f32x16 mfma32(const Frag& a, const Frag& b, f32x16 c) {
+    if constexpr (__is_same(T, __bf16)) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, c, 0, 0, 0);
+    } else {
+        using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a.v), __builtin_bit_cast(f16x8, b.v), c, 0, 0, 0);
+    }
+}
+
+// A fragment of V^T, rows 32 d .., of 16 keys 16 kk ..: lanes 4r .. 4r + 3 of a
+// group of 16 hand in 16 columns of a key, lane n gets column n of four keys.
+__device__ __forceinline__ Frag values(const PageTile& tile, int kk, int d) {
+    const int32_t lane = (int32_t)threadIdx.x % kWave;
+    const int32_t r = 16 * kk + 4 * (lane >> 5) + ((lane & 15) >> 2);
+    const int32_t chunk = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    Frag v;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const uint8_t* at = &tile.value[r + 8 * e][16 * (chunk ^ (4 * (r & 3))) + 8 * (lane & 1)];
+        const u32x2 w = __builtin_bit_cast(
+            u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)at));
+        v.w[2 * e] = w[0];
+        v.w[2 * e + 1] = w[1];
+    }
+    return v;
+}
+
+// Reads of LDS, EACH for one matrix product, kAhead products before it.
+constexpr int kAhead = 4;
+template <int N, int EACH>
+__device__ __forceinline__ void reads_ahead() {
+    __builtin_amdgcn_sched_group_barrier(0x100, EACH * kAhead, 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (i + kAhead < N) __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);
+    }
+}
+
+struct BlocksWork {
+    Request w;
+    int32_t request, kv, block;  // block: of columns
+    int32_t part, parts;
+    int64_t unit;  // its sums' place in the workspace
+};
+
+// The work-group's part of the attention; false: there is none.
+__device__ __forceinline__ bool find_work(const AttendParams& p, BlocksWork& work) {
+    // Work-groups reach the XCDs in turn.  An XCD takes whole units, a KV head of an item
+    // (a request, or a part of its keys), `together` of them at a time, the longest
+    // blocks of all of them first: blocks of the same keys meet in one L2, and the last
+    // ones to end are short.
+    const int32_t units = (p.units + p.xcds - 1) / p.xcds, turn = (int32_t)blockIdx.x / p.xcds;
+    const int32_t before = turn / (p.together * p.blocks) * p.together, size = min(p.together, units - before);
+    const int32_t within = turn - before * p.blocks, rank = within / size;
+    const int32_t unit = (before + within % size) * p.xcds + (int32_t)blockIdx.x % p.xcds;
+    if (unit >= p.units) return false;
+    work.kv = unit % p.kv_heads;
+    if (p.slots > 0) {
+        // slots: request r's blocks lie in slots cu[r] group / 256 + r and on, as many as it can need wherever it begins
+        const int32_t slot = p.slots - 1 - unit / p.kv_heads;
+        auto start = [&](int32_t r) __attribute__((always_inline)) {
+            return (int32_t)((int64_t)min(max(p.cu[r], 0), p.tokens) * p.group / kBlock) + r;
+        };
+        const int32_t r = last_at_most(p.requests, slot, start);
+        work.request = r;
+        work.block = slot - __builtin_amdgcn_readfirstlane(start(r));
+        work.part = 0, work.parts = 1, work.unit = 0;
+        if (work.block < 0) return false;
+    } else {
+        Item it;
+        const int32_t index = unit / p.kv_heads;
+        if (!find_item(p.plan, index, it, [&](int32_t r) __attribute__((always_inline)) { return planned_keys(p, r); })) return false;
+        work.block = p.blocks - 1 - rank;
+        work.request = it.row, work.part = it.part, work.parts = it.parts;
+        work.unit = ((int64_t)index * p.kv_heads + work.kv) * p.blocks + work.block;
+        if (p.plan.chunk == 0 && it.part == 0 && work.kv == 0 && rank == 0 && threadIdx.x == 0)
+            p.parts.of_row[it.row] = i32x2{index, it.parts};
+    }
+    work.w = request_at(p, work.request);
+    return (int64_t)work.block * kBlock < (int64_t)work.w.nq * p.group;
+}
+
+// Masked keys of infinite or NaN values: sums that end up not finite (true is returned,
+// nothing written) are found again by the CAREFUL form.
+template <class T, int MODE, bool CAREFUL>
+__device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksWork& work, BlocksLds& lds) {
+    constexpr int COPIES = (int)(sizeof(PageTile) / 1024) / kWaves;
+    static_assert(COPIES == 4, "copies of a tile");
+    const Request& w = work.w;
+    const int32_t wave = __builtin_amdgcn_readfirstlane((int32_t)threadIdx.x / kWave);
+    const int32_t lane = (int32_t)threadIdx.x % kWave, c = lane & 31, h = lane >> 5;
+    const int32_t m0 = work.block * kBlock, columns = min(w.nq * p.group - m0, kBlock) - wave * kRows;  // (of this wave, or less)
+    const int32_t* table = p.table + work.request * p.table_stride;
+
+    const Column col = column_at(p, w, lds.tree, m0, wave * kRows + c);
+    int32_t least_lo = INT32_MAX, most_lo = 0, least_hi = INT32_MAX, most_hi = 0;
+    if (c < columns) least_lo = most_lo = col.lo, least_hi = most_hi = col.hi;
+    least_lo = wave_min(least_lo), most_lo = wave_max(most_lo), least_hi = wave_min(least_hi), most_hi = wave_max(most_hi);
+    float slope = 0.f;
+    if (MODE == kBiased && p.slopes) slope = p.slopes[work.kv * p.group + col.head] * kLog2e;
+    if (lane == 0) lds.lo[wave] = least_lo, lds.hi[wave] = most_hi;
+    lds_barrier();
+    int32_t all_lo = INT32_MAX, all_hi = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) all_lo = min(all_lo, lds.lo[i]), all_hi = max(all_hi, lds.hi[i]);
+    all_lo = __builtin_amdgcn_readfirstlane(all_lo), all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+    const Tiles list = tiles_seen(p, w, all_lo, all_hi);
+    const int32_t each = (list.count + work.parts - 1) / work.parts;
+    const int32_t first = min(work.part * each, list.count), tiles = min(each, list.count - first);
+    const int32_t end = p.parents ? w.len : max(all_hi, w.pre);  // no column sees a key from here on
+
+    // pages of the next 64 tiles, one a lane; -1: no page
+    int32_t page_of = -1;
+    auto fetch_pages = [&](int32_t t) __attribute__((always_inline)) {
+        page_of = table[list.at(first + min(t + lane, tiles - 1))];
+        if (page_of >= p.pages) page_of = -1;
+    };
+    auto page_at = [&](int32_t t) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(page_of, t & 63); };
+    auto first_key = [&](int32_t t) __attribute__((always_inline)) { return list.at(first + t) * kTileKeys; };
+
+    // Copy j of the wave's four of a tile: four keys twice, four values twice.  (Rows that no column
+    // sees are copies of the last that one may; tiles without a page, which nobody reads, are page 0's.)
+    auto copy = [&](int32_t t, int32_t k0, int32_t page, auto which) __attribute__((always_inline)) {
+        constexpr int j = which.value, v = j / 2;
+        PageTile& to = lds.tile[t % kBuffers];
+        const int32_t i = (j & 1) * kWaves + wave, r = 4 * i + (lane >> 4), at = lane & 15;
+        const int32_t chunk = v == 0 ? at ^ (r & 15) : at ^ (4 * (r & 3));
+        const uint16_t* from = p.pool[v] + work.kv * p.head[v] + max(page, 0) * p.page[v];
+        copy_to_lds(from + min(r, end - k0 - 1) * p.token[v] + 8 * chunk, lds_offset(v == 0 ? &to.key[4 * i][0] : &to.value[4 * i][0]));
+    };
+    auto copy_tile = [&](int32_t t, int32_t k0, int32_t page) __attribute__((always_inline)) {
+        each_of<COPIES>([&](auto j) __attribute__((always_inline)) { copy(t, k0, page, j); });
+    };
+
+    // B fragments of Q^T: column c.  The rows come through LDS (rows of 16 chunks of 16
+    // bytes end to end, XORed by the row, in the last two buffers): fragments read from
+    // memory are 32 rows' lines for every one.
+    Frag q[8];
+    int32_t page0 = -1, page1 = -1, key0 = 0, key1 = 0;  // of this tile and the next
+    {
+        uint8_t* const rows = &lds.tile[2].key[0][0] + wave * (kRows * 2 * kDim);
+        static_assert(kWaves * kRows * 2 * kDim == 2 * sizeof(PageTile), "queries in two buffers");
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int32_t r = 4 * j + (lane >> 4), chunk = (lane & 15) ^ (r & 15);
+            const int32_t query = __shfl(col.query, r, kWave), head = __shfl(col.head, r, kWave);
+            copy_to_lds(p.q + (w.q_lo + (int64_t)query) * p.q_token + (int64_t)(work.kv * p.group + head) * p.q_head + 8 * chunk,
+                        lds_offset(rows + 1024 * j));
+        }
+        if (tiles > 0) {
+            fetch_pages(0);
+            page0 = page_at(0), key0 = first_key(0);
+            page1 = page_at(min(1, tiles - 1)), key1 = first_key(min(1, tiles - 1));
+            copy_tile(0, key0, page0);
+            wait_copies<COPIES>();
+        } else {
+            wait_copies<0>();
+        }
+#pragma unroll
+        for (int s = 0; s < 8; ++s) q[s].u = *reinterpret_cast<const u32x4*>(rows + 256 * c + 16 * ((2 * s + h) ^ (c & 15)));
+        lds_barrier();
+        if (tiles > 0) copy_tile(1, key1, page1);
+    }
+    f32x16 acc[4], s[2];
+    Frag pf[4];
+    float mx = -__builtin_inff(), total = 0.f;
+    bool some = false;  // a key of the column is attended
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+    // whether the wave sees a key of a tile, and whether all of its columns see all of them
+    auto sees = [&](int32_t k0, int32_t page) __attribute__((always_inline)) {
+        return page >= 0 && columns > 0 &&
+               ((k0 + kTileKeys > least_lo && k0 < most_hi) || k0 < w.pre || (p.parents && k0 + kTileKeys > w.before));
+    };
+    auto sees_all = [&](int32_t k0) __attribute__((always_inline)) {
+        return (k0 >= most_lo && k0 + kTileKeys <= least_hi) || k0 + kTileKeys <= w.pre;
+    };
+    // scores: register i of half u is key 32u + 8 (i / 4) + 4h + i % 4
+    auto scores = [&](int32_t t, int32_t key2, int32_t page2) __attribute__((always_inline)) {
+        const PageTile& tile = lds.tile[t % kBuffers];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
+        // key rows 32u .., numbers 16 (n / 2) ..
+        Frag k[kAhead];
+        auto fetch = [&](int n) __attribute__((always_inline)) {
+            const int32_t st = n / 2, r = 32 * (n & 1) + c;
+            k[n % kAhead].u = *reinterpret_cast<const u32x4*>(&tile.key[r][16 * ((2 * st + h) ^ (r & 15))]);
+        };
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) fetch(n);
+        each_of<16>([&](auto number) __attribute__((always_inline)) {
+            constexpr int n = number.value;
+            s[n & 1] = mfma32<T>(k[n % kAhead], q[n / 2], s[n & 1]);
+            if constexpr (n + kAhead < 16) fetch(n + kAhead);
+            if constexpr (n % 4 == 1) copy(t + 2, key2, page2, Number<n / 4>{});
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    auto each_score = [&](auto&& f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[u][i] = f(s[u][i], 32 * u + 8 * (i / 4) + i % 4);  // (the key, but for 4h)
+    };
+    uint64_t seen = ~0ull;  // bit 32u + 8 a + i: key 32u + 8a + 4h + i of the tile in `pf`
+    auto softmax = [&](int32_t k0) __attribute__((always_inline)) {
+        float factor = p.scale2;
+        if constexpr (MODE != kPlain) {
+            factor = 1.f;
+            if (MODE == kCapped || p.cap2 > 0.f) {
+                float big = 0.f;
+                each_score([&](float x, int) { x *= p.cap_in, big = fmaxf(big, fabsf(x)); return x; });
+                if (__ballot(big > kSmall)) each_score([&](float x, int) { return capped_any(x, p.cap2); });
+                else each_score([&](float x, int) { return capped_small(x, p.cap2); });
+            } else {
+                each_score([&](float x, int) { return x * p.scale2; });
+            }
+            if constexpr (MODE == kBiased) {
+                if (p.slopes) {
+                    if (p.parents && k0 + kTileKeys > w.before) {
+                        each_score([&](float x, int key) {
+                            int32_t at = k0 + key + 4 * h;
+                            if (at >= w.before) at = w.before + lds.tree.depth[min(at - w.before, kMostDrafts - 1)];
+                            return fmaf(-slope, fabsf((float)(col.position - at)), x);
+                        });
+                    } else {
+                        const float away = (float)(col.position - k0 - 4 * h);
+                        each_score([&](float x, int key) { return fmaf(-slope, fabsf(away - (float)key), x); });
+                    }
+                }
+            }
+        }
+        seen = ~0ull;
+        if (!sees_all(k0)) {
+            seen = column_sees(p, w, lds.tree, col, k0);
+            some |= seen != 0;
+            seen >>= 4 * h;
+            each_score([&](float x, int key) { return (seen >> key) & 1 ? x : -__builtin_inff(); });
+        } else {
+            some = true;
+        }
+        float top = s[0][0];
+        each_score([&](float x, int) { top = fmaxf(top, x); return x; });
+        top = fmaxf(top, __shfl_xor(top, 32, kWave)) * factor;
+        if (__ballot(top > mx + Range<T>::most)) {
+            const float next = top > mx + Range<T>::most ? top - Range<T>::head : mx;
+            const float keep = mx == -__builtin_inff() ? (next == mx ? 1.f : 0.f) : __builtin_amdgcn_exp2f(mx - next);
+            mx = next;
+            total *= keep;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) acc[d] *= keep;
+        }
+        const float sub = mx == -__builtin_inff() ? 0.f : mx;
+        each_score([&](float x, int) {
+            x = __builtin_amdgcn_exp2f(MODE == kPlain ? fmaf(x, factor, -sub) : x - sub);
+            total += x;
+            return x;
+        });
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                pf[kk].w[i] = pack<T>(s[kk / 2][8 * (kk & 1) + 2 * i], s[kk / 2][8 * (kk & 1) + 2 * i + 1]);
+    };
+    auto products = [&](int32_t t) __attribute__((always_inline)) {
+        const PageTile& tile = lds.tile[t % kBuffers];
+        if constexpr (CAREFUL) {
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                f32x16 up, down;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) up[i] = down[i] = 0.f;
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {
+                    const Frag v = values(tile, kk, d);
+                    Frag plain, pos, neg, see;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        split_odd<T>(v.w[i], plain.w[i], pos.w[i], neg.w[i]);
+                        const int32_t bit = 16 * kk + 8 * (i / 2) + 2 * (i & 1);  // (of the lane's numbers 2i, 2i + 1)
+                        see.w[i] = ((seen >> bit) & 1 ? kOne<T> : 0u) | ((seen >> (bit + 1)) & 1 ? kOne<T> << 16 : 0u);
+                    }
+                    acc[d] = mfma32<T>(plain, pf[kk], acc[d]);
+                    up = mfma32<T>(pos, see, up);
+                    down = mfma32<T>(neg, see, down);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    acc[d][i] += (up[i] > 0.f ? __builtin_inff() : 0.f) - (down[i] > 0.f ? __builtin_inff() : 0.f);
+            }
+        } else {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) acc[d] = mfma32<T>(values(tile, kk, d), pf[kk], acc[d]);
+            reads_ahead<16, 2>();
+        }
+    };
+    // The two waves of a SIMD half a tile apart: one multiplies (the last tile's
+    // values, this one's keys) and asks for its copies of the tile after the next,
+    // whose buffer was read until two steps ago, while the other makes
+    // probabilities.  Steps are divided by barriers, every other one of them behind a
+    // wait for the copies of the tile whose keys come next.
+    const bool second = wave >= kWaves / 2;
+    auto sync = [&](bool landed) __attribute__((always_inline)) {
+        if (landed) wait_barrier<COPIES>();
+        else lds_barrier();
+    };
+    if (second) sync(true);
+    bool saw = false;
+#pragma unroll 1
+    for (int32_t t = 0; t <= tiles; ++t) {
+        const bool now = t < tiles && sees(key0, page0);
+        sync(!second);
+        if (saw) products(t - 1);
+        const int32_t later = min(t + 2, tiles - 1);
+        if (((t + 2) & 63) == 0 && t + 2 < tiles) fetch_pages(t + 2);
+        const int32_t page2 = page_at(later), key2 = first_key(later);
+        if (now) scores(t, key2, page2);
+        else if (t < tiles) copy_tile(t + 2, key2, page2);
+        sync(second);
+        if (now) softmax(key0);
+        saw = now;
+        key0 = key1, page0 = page1, key1 = key2, page1 = page2;
+    }
+    if (!second) lds_barrier();
+    wait_copies<0>();
+    __syncthreads();  // the tiles' memory is free
+    if constexpr (!CAREFUL) {
+        float odd = 0.f;
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) odd = fmaf(acc[d][i], 0.f, odd);
+        if (__syncthreads_or(odd != odd)) return true;
+    }
+    total += __shfl_xor(total, 32, kWave);
+    const bool none = !some;  // no key seen
+    // Rows leave through LDS as well, whole ones at a time: row c's numbers 32 d + 8 a
+    // + 4 h .. are its piece 8 d + 2 a + h of four, pieces XORed by the row.
+    static_assert(sizeof(PageTile) * kBuffers >= kWaves * kRows * 4 * kDim, "rows");
+    uint8_t* const rows = &lds.tile[0].key[0][0] + wave * (kRows * 4 * kDim);
+    if (work.parts == 1) {
+        const float inv = none ? 0.f : 1.0f / total;
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int a = 0; a < 4; ++a)
+                *reinterpret_cast<u32x2*>(rows + 256 * c + 8 * ((8 * d + 2 * a + h) ^ c)) =
+                    none ? u32x2{0, 0} : u32x2{pack<T>(acc[d][4 * a] * inv, acc[d][4 * a + 1] * inv),
+                                               pack<T>(acc[d][4 * a + 2] * inv, acc[d][4 * a + 3] * inv)};
+        wait_lds();
+#pragma unroll
+        for (int j = 0; j < kRows / 2; ++j) {
+            const int32_t r = 2 * j + h;
+            const u32x2 x = *reinterpret_cast<const u32x2*>(rows + 256 * r + 8 * (c ^ r));
+            const int32_t query = __shfl(col.query, r, kWave), head = work.kv * p.group + __shfl(col.head, r, kWave);
+            if (r < columns) *reinterpret_cast<u32x2*>(p.out + (w.q_lo + (int64_t)query) * p.o_token + head * p.o_head + 4 * c) = x;
+        }
+        if (p.lse && h == 0 && c < columns)
+            p.lse[(w.q_lo + (int64_t)col.query) * p.kv_heads * p.group + work.kv * p.group + col.head] =
+                none ? -__builtin_inff() : (mx + __builtin_amdgcn_logf(total)) * kLn2;
+    } else {
+        const int64_t at = work.unit * kBlock + wave * kRows;
+        if (tiles > 0) {
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int a = 0; a < 4; ++a)
+                    *reinterpret_cast<f32x4*>(rows + 512 * c + 16 * ((8 * d + 2 * a + h) ^ c)) =
+                        f32x4{acc[d][4 * a], acc[d][4 * a + 1], acc[d][4 * a + 2], acc[d][4 * a + 3]};
+            wait_lds();
+#pragma unroll
+            for (int j = 0; j < kRows / 2; ++j) {
+                const int32_t r = 2 * j + h;
+                const f32x4 x = *reinterpret_cast<const f32x4*>(rows + 512 * r + 16 * (c ^ r));
+                if (r < columns) *reinterpret_cast<f32x4*>(p.parts.sums + (at + r) * kDim + 4 * c) = x;
+            }
+        }
+        if (h == 0 && c < columns) p.parts.stats[at + c] = f32x2{none ? -__builtin_inff() : fmaxf(mx, kLowest), none ? 0.f : total};
+    }
+    return false;
+}
+
+// (A call, so that its registers are not the common form's.)
+template <class T, int MODE>
+__device__ __attribute__((noinline)) void careful_block(AttendParams p, BlocksLds* lds) {
+    BlocksWork work;
+    if (find_work(p, work)) blocks_part<T, MODE, true>(p, work, *lds);
+}
+
+template <class T, int MODE>
+__global__ __launch_bounds__(64 * kWaves, 2) void blocks_kernel(AttendParams p) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
+    auto& lds = *reinterpret_cast<BlocksLds*>(lds_raw);
+    BlocksWork work;
+    if (!find_work(p, work)) return;
+    if (p.parents) find_tree(p, work.w, lds.tree);
+    if (__builtin_expect(blocks_part<T, MODE, false>(p, work, lds), 0)) careful_block<T, MODE>(p, &lds);
+}
+
+template <class T, int MODE>
+int launch(const AttendParams& p, int64_t groups, hipStream_t st) {
+    static OncePerDevice once;
+    const auto kernel = blocks_kernel<T, MODE>;
+    const int rc = allow_lds(once, reinterpret_cast<const void*>(kernel), sizeof(BlocksLds), "paged_attend: LDS");
+    if (rc != V1_OK) return rc;
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)groups), dim3(64 * kWaves), sizeof(BlocksLds), st, p);
+    return V1_LAUNCHED("paged_attend: blocks");
+}
+
+template <class T>
+int launch(int mode, const AttendParams& p, int64_t groups, hipStream_t st) {
+    return mode == kPlain ? launch<T, kPlain>(p, groups, st) : mode == kCapped ? launch<T, kCapped>(p, groups, st) : launch<T, kBiased>(p, groups, st);
+}
+
+}  // namespace
+
+int paged::launch_blocks(bool fp16, int mode, const AttendParams& p, int64_t groups, hipStream_t st) {
+    return fp16 ? launch<_Float16>(mode, p, groups, st) : launch<__bf16>(mode, p, groups, st);
+}
+
+}  // namespace v1

@@ -2,7 +2,7 @@
 //   S[m, j] = scale q_m . k_j, capped and biased, O[m] = sum_j softmax_j(S[m, :]) v_j
 // for the columns m of a request (its queries times the heads of a KV head) and the
 // keys j that column m sees.
-#include "paged.h"
+#include "paged_attend.h"
 
 namespace v1 {
 namespace {
@@ -10,7 +10,6 @@ namespace {
 using namespace paged;
 
 constexpr int kWaves = 4;
-constexpr int kPlain = 0, kCapped = 1, kBiased = 2;  // what a score takes (kBiased: distance, and a cap if there is one)
 
 template <int NC>
 struct RowsLds {
@@ -400,8 +399,8 @@ struct RowsJoin {
 template <class T>
 __global__ __launch_bounds__(256) void rows_join(RowsJoin j) {
     const AttendParams& p = j.a;
-    const int32_t r = (int32_t)blockIdx.x, each = p.blocks * j.cols / 8, kv = (int32_t)blockIdx.y / each;
-    const int32_t m = (int32_t)blockIdx.y % each * 8 + (int32_t)threadIdx.x / 32, at4 = (int32_t)threadIdx.x % 32;
+    const int32_t r = (int32_t)blockIdx.y, each = p.blocks * j.cols / 8, kv = (int32_t)blockIdx.x / each;
+    const int32_t m = (int32_t)blockIdx.x % each * 8 + (int32_t)threadIdx.x / 32, at4 = (int32_t)threadIdx.x % 32;
     const Request w = request_at(p, r);
     if (m >= w.nq * p.group) return;
     int32_t parts, first;
@@ -424,6 +423,7 @@ __global__ __launch_bounds__(256) void rows_join(RowsJoin j) {
     for (int32_t i = 0; i < parts; ++i) {
         const int64_t at = base + i * step;
         const f32x2 st = p.parts.stats[at];
+        if (st[0] == -__builtin_inff() && st[1] == 0.f) continue;  // (no key of it is seen: its sums are not written)
         const f32x4 x = *reinterpret_cast<const f32x4*>(p.parts.sums + at * kDim + 4 * at4);
         const float f = __builtin_amdgcn_exp2f(st[0] - sub);
         total = fmaf(f, st[1], total);
@@ -446,32 +446,60 @@ inline int32_t reach_of(int32_t window, int32_t max_q) {
     return window > 0 ? (int32_t)std::min<int64_t>((int64_t)window + max_q + kTileKeys, INT32_MAX) : 0;
 }
 
-struct RowsShape {
-    int32_t cols, blocks, together, reach;
+struct Shape {
+    int32_t cols, blocks, together, reach;  // cols: of a block; 256: the kernel of many queries
+    int32_t slots, units, xcds;
     int64_t items;
     Plan plan;
 };
 
-inline RowsShape rows_shape(const int32_t* lens, int32_t requests, int32_t kv_heads, int32_t group, int32_t max_q, int32_t keys, int32_t window) {
-    RowsShape s;
+constexpr int kFewColumns = 64;  // the most that the kernel of few queries takes
+
+inline Shape shape_of(const int32_t* lens, int32_t tokens, int32_t requests, int32_t kv_heads, int32_t group, int32_t max_q, int32_t keys,
+                      int32_t window) {
+    Shape s;
     s.reach = reach_of(window, max_q);
     const int64_t columns = (int64_t)max_q * group;
-    s.cols = columns <= 16 ? 16 : columns <= 32 ? 32 : 64;
+    const bool few = columns <= kFewColumns;
+    s.cols = !few ? kBlockColumns : columns <= 16 ? 16 : columns <= 32 ? 32 : 64;
     s.blocks = (int32_t)cdiv(columns, s.cols);
-    s.together = kv_heads % 4 == 0 ? 4 : kv_heads % 2 == 0 ? 2 : 1;
+    s.together = !few ? 1 : kv_heads % 4 == 0 ? 4 : kv_heads % 2 == 0 ? 2 : 1;
+    s.slots = s.units = 0, s.xcds = 1;
     if (s.reach > 0) keys = std::min(keys, s.reach);
-    const int64_t sets = (int64_t)kv_heads / s.together * s.blocks, streams = kWaves / s.together;
-    const int64_t slots = std::max<int64_t>(1, device_cus() / sets), steps = cdiv(cdiv(keys, kTileKeys), streams);
-    s.plan = Plan{lens, requests, keys, 0, 0, (int32_t)slots};
-    if (keys > 0 && planned(requests, cdiv(keys, kTileKeys)) && requests < slots)
-        s.plan.target = (int32_t)std::max(slots - requests, (slots + 1) / 2);
-    else s.plan.chunk = (int32_t)streams * chunk_for(requests, steps, slots, 2, 1);
+    const int64_t sets = (int64_t)kv_heads / s.together * s.blocks, streams = few ? kWaves / s.together : 1;
+    const int64_t running = std::max<int64_t>(1, device_cus() / sets), tiles = cdiv(keys, kTileKeys);
+    const int64_t most = few ? running : std::max<int64_t>(1, 2 * device_cus() / sets);
+    s.plan = Plan{lens, requests, keys, 0, 0, (int32_t)most};
+    if (keys > 0 && planned(requests, tiles) && requests < most)
+        s.plan.target = (int32_t)std::max(most - requests, (most + 1) / 2);
+    else s.plan.chunk = (int32_t)streams * chunk_for(requests, cdiv(tiles, streams), running, few ? 2 : 6, few ? 1 : 2);
     s.items = items_at_most(s.plan);
+    if (!few) {
+        // Every request gets as many blocks as the longest can have, unless the blocks that the queries can need are
+        // less than a third of those.
+        const int64_t slots = (int64_t)tokens * group / s.cols + requests;
+        if (max_q > 1 && ((int64_t)requests * s.blocks > 3 * slots || !launchable(((int64_t)s.items * kv_heads + 7) * s.blocks, 512))) {
+            s.slots = (int32_t)slots, s.blocks = 1, s.items = slots;
+            s.plan.chunk = (int32_t)std::max<int64_t>(1, tiles);
+        }
+        const int64_t units = s.items * kv_heads;
+        s.xcds = units % 8 == 0 || units >= 64 ? 8 : 1;
+        s.units = (int32_t)std::min<int64_t>(units, INT32_MAX);
+        s.together = (int32_t)std::max<int64_t>(1, std::min(cdiv(units, s.xcds), cdiv(2 * device_cus() / s.xcds, s.blocks)));
+    }
     return s;
 }
 
-inline int64_t rows_workspace(const RowsShape& s, int32_t kv_heads) {
-    return s.plan.chunk > 0 && s.items == s.plan.rows ? 0 : parts_bytes(s.plan, kv_heads * s.blocks * s.cols, kDim);
+inline int64_t workspace_of(const Shape& s, int32_t kv_heads) {
+    if (s.slots > 0 || (s.plan.chunk > 0 && s.items == s.plan.rows)) return 0;
+    return s.items * kv_heads * s.blocks * s.cols * (kDim + 2) * (int64_t)sizeof(float) + (s.plan.chunk > 0 ? 0 : s.plan.rows * (int64_t)sizeof(i32x2));
+}
+
+inline Parts parts_of(void* ws, const Shape& s, int32_t kv_heads) {
+    const int64_t columns = s.items * kv_heads * s.blocks * s.cols;
+    float* sums = static_cast<float*>(ws);
+    f32x2* stats = reinterpret_cast<f32x2*>(sums + columns * kDim);
+    return {sums, stats, reinterpret_cast<i32x2*>(stats + columns)};
 }
 
 template <class T, int NC, int MODE>
@@ -491,17 +519,23 @@ int launch_rows(int mode, const AttendParams& p, int64_t groups, hipStream_t st)
 }
 
 template <class T>
-int attend_rows(AttendParams& p, const RowsShape& s, int mode, hipStream_t st) {
-    const int64_t sets = (int64_t)p.kv_heads / s.together * s.blocks;
-    const int64_t spread = s.plan.chunk > 0 ? cdiv(s.items * sets, 8) : cdiv(s.items, 8) * sets;
-    V1_REQUIRE(launchable(8 * spread, 64 * kWaves) && (int64_t)p.kv_heads * s.blocks * s.cols < 1 << 18,
-               "paged_attend: too many requests, queries and heads for a launch");
-    p.spread = (int32_t)spread;
-    const int rc = s.cols == 16 ? launch_rows<T, 1>(mode, p, 8 * spread, st)
-                 : s.cols == 32 ? launch_rows<T, 2>(mode, p, 8 * spread, st) : launch_rows<T, 4>(mode, p, 8 * spread, st);
-    if (rc != V1_OK || rows_workspace(s, p.kv_heads) == 0) return rc;
-    hipLaunchKernelGGL(rows_join<T>, dim3((uint32_t)p.requests, (uint32_t)(p.kv_heads * s.blocks * s.cols / 8)), dim3(256), 0, st,
-                       RowsJoin{p, s.cols});
+int attend(AttendParams& p, const Shape& s, int mode, hipStream_t st) {
+    int rc;
+    if (s.cols == kBlockColumns) {
+        const int64_t groups = cdiv(s.items * p.kv_heads, s.xcds) * s.xcds * s.blocks;
+        V1_REQUIRE(launchable(groups, 512) && s.items * p.kv_heads <= INT32_MAX, "paged_attend: too many requests, queries and heads for a launch");
+        rc = launch_blocks(__is_same(T, _Float16), mode, p, groups, st);
+    } else {
+        const int64_t sets = (int64_t)p.kv_heads / s.together * s.blocks;
+        const int64_t spread = s.plan.chunk > 0 ? cdiv(s.items * sets, 8) : cdiv(s.items, 8) * sets;
+        V1_REQUIRE(launchable(8 * spread, 64 * kWaves), "paged_attend: too many requests and heads for a launch");
+        p.spread = (int32_t)spread;
+        rc = s.cols == 16 ? launch_rows<T, 1>(mode, p, 8 * spread, st)
+           : s.cols == 32 ? launch_rows<T, 2>(mode, p, 8 * spread, st) : launch_rows<T, 4>(mode, p, 8 * spread, st);
+    }
+    if (rc != V1_OK || workspace_of(s, p.kv_heads) == 0) return rc;
+    const int64_t eights = cdiv((int64_t)s.blocks * s.cols, 8);
+    hipLaunchKernelGGL(rows_join<T>, dim3((uint32_t)(p.kv_heads * eights), (uint32_t)p.requests), dim3(256), 0, st, RowsJoin{p, s.cols});
     return V1_LAUNCHED("paged_attend: join");
 }
 
@@ -513,7 +547,7 @@ using namespace v1;
 extern "C" int64_t v1_paged_attend_workspace(int32_t tokens, int32_t requests, int32_t kv_heads, int32_t group, int32_t max_q,
                                              int32_t keys, int32_t window) {
     if (tokens <= 0 || requests <= 0 || kv_heads <= 0 || group <= 0 || max_q <= 0 || keys <= 0) return 0;
-    return rows_workspace(rows_shape(nullptr, requests, kv_heads, group, max_q, keys, window), kv_heads);
+    return workspace_of(shape_of(nullptr, tokens, requests, kv_heads, group, max_q, keys, window), kv_heads);
 }
 
 extern "C" int v1_paged_attend(const v1_paged_attend_args* a, void* stream) {
@@ -541,8 +575,8 @@ extern "C" int v1_paged_attend(const v1_paged_attend_args* a, void* stream) {
     if (pages == 0) table_len = 0;
     const int32_t keys = table_len * kTileKeys;
     if (!cu_q) max_q = 1;
-    const RowsShape s = rows_shape(lens, requests, kv_heads, group, max_q, keys, window);
-    const int64_t need = rows_workspace(s, kv_heads);
+    const Shape s = shape_of(lens, tokens, requests, kv_heads, group, max_q, keys, window);
+    const int64_t need = workspace_of(s, kv_heads);
     V1_REQUIRE(workspace_bytes >= need && (need == 0 || workspace != nullptr), "paged_attend: workspace of %lld bytes needed", (long long)need);
     const int mode = slopes ? kBiased : softcap > 0.f ? kCapped : kPlain;
     AttendParams p{static_cast<const uint16_t*>(q), q_token, q_head,
@@ -551,6 +585,6 @@ extern "C" int v1_paged_attend(const v1_paged_attend_args* a, void* stream) {
                    parents, slopes, table_len, tokens, requests, max_q, kv_heads, group, small_div_magic((uint32_t)group),
                    window, scale * kLog2e, softcap > 0.f ? scale / softcap : 0.f, softcap * kLog2e,
                    static_cast<uint16_t*>(out), o_token, o_head, lse, s.plan, s.reach, s.blocks, 0, s.together,
-                   parts_at(workspace, s.plan, kv_heads * s.blocks * s.cols, kDim)};
-    return fp16 ? attend_rows<_Float16>(p, s, mode, as_stream(stream)) : attend_rows<__bf16>(p, s, mode, as_stream(stream));
+                   s.units, s.xcds, s.slots, parts_of(workspace, s, kv_heads)};
+    return fp16 ? attend<_Float16>(p, s, mode, as_stream(stream)) : attend<__bf16>(p, s, mode, as_stream(stream));
 }
