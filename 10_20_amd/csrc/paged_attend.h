@@ -31,7 +31,32 @@ __device__ __forceinline__ f32x4 mfma16(const Frag& a, const Frag& b, f32x4 c) {
     }
 }
 
-constexpr int kPlain = 0, kCapped = 1, kBiased = 2;  // what a score takes (kBiased: distance, and a cap if there is one)
+// tanh(t) / t in t^2 for |t| up to 0.33 and up to 0.75, and the same polynomials of
+// cap log2(e) tanh(d scale / cap) / d in d^2 for |d| up to so much.
+constexpr float kCapNear[4] = {0.9999999780542091f, -0.3333268647142513f, 0.1330338186573907f, -0.04948183016008989f}, kCapNearMost = 0.33f;
+constexpr float kCapFar[6] = {0.9999999710131235f, -0.33332958872695295f, 0.13325405922016131f, -0.053344425407917576f,
+                              0.019582898606222813f, -0.0047162504597644895f}, kCapFarMost = 0.75f;
+struct Cap {
+    float near[4], far[6];
+    float near_most, far_most;
+};
+
+inline Cap cap_of(float scale, float softcap) {
+    Cap c{};
+    if (softcap <= 0.f) return c;
+    const double in = (double)scale / softcap;
+    double by = (double)scale * kLog2e;
+    for (int i = 0; i < 6; ++i, by *= in * in) {
+        if (i < 4) c.near[i] = (float)(kCapNear[i] * by);
+        c.far[i] = (float)(kCapFar[i] * by);
+    }
+    c.near_most = (float)(kCapNearMost / in), c.far_most = (float)(kCapFarMost / in);
+    return c;
+}
+
+// What a score takes: nothing, a cap (of 2^-12 .. 2^12 times the scale, so that the
+// polynomials' coefficients are normal numbers), a distance, or any cap and a distance.
+constexpr int kPlain = 0, kCapped = 1, kBiased = 2, kBoth = 3;
 
 struct AttendParams {
     const uint16_t* q;
@@ -52,6 +77,7 @@ struct AttendParams {
     int32_t window;           // 0: none
     float scale2;             // scores times log2(e)
     float cap_in, cap2;       // scale / cap, cap log2(e); 0: no cap
+    Cap cap;
     uint16_t* out;
     int64_t o_token, o_head;
     float* lse;
@@ -207,29 +233,43 @@ __device__ __forceinline__ int32_t wave_min(int32_t x) {
 __device__ __forceinline__ int32_t wave_max(int32_t x) { return -wave_min(-x); }
 
 // ------------------------------------------------------------------ capped scores
-// cap tanh(x / cap), base 2, of a product d = q . k: with t = d scale / cap it is
-// t G(t^2), a polynomial fitted to tanh(t) / t on |t| <= 0.75 (off by 3e-8 of the value
-// at most, half a step of fp32), and past that cap (1 - 2 / (e^2t + 1)).  Scores that
-// are all small, as of every model that was trained with a cap far above them, take
-// the polynomial alone: eight operations where the exponential and the reciprocal
-// occupy their unit for eight as well, beside three more.
-constexpr float kSmall = 0.75f;
-
-__device__ __forceinline__ float capped_small(float t, float cap2) {
+// cap tanh(x / cap), base 2, of a product d = q . k, t = d scale / cap: past |t| = 0.75
+// cap (1 - 2 / (e^2t + 1)), below it t G(t^2) with a polynomial G fitted to tanh(t) / t
+// (off by 3e-8 of the value at most, half a step of fp32; the other form there is off by
+// as much of the cap).
+__device__ __forceinline__ float capped(float t, float cap2) {
     const float z = t * t;
-    float g = -0.0047162504597644895f;
-    g = fmaf(g, z, 0.019582898606222813f);
-    g = fmaf(g, z, -0.053344425407917576f);
-    g = fmaf(g, z, 0.13325405922016131f);
-    g = fmaf(g, z, -0.33332958872695295f);
-    g = fmaf(g, z, 0.9999999710131235f);
-    return t * cap2 * g;
+    float g = kCapFar[5];
+#pragma unroll
+    for (int i = 4; i >= 0; --i) g = fmaf(g, z, kCapFar[i]);
+    const float e = __builtin_amdgcn_exp2f(2.f * kLog2e * t);
+    const float past = fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(e + 1.f), cap2);
+    return fabsf(t) <= kCapFarMost ? t * cap2 * g : past;
 }
 
-__device__ __forceinline__ float capped_any(float t, float cap2) {
-    const float e = __builtin_amdgcn_exp2f(2.f * kLog2e * t);
-    const float far = fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(e + 1.f), cap2);
-    return fabsf(t) <= kSmall ? capped_small(t, cap2) : far;
+// capped(d scale / cap) - sub of a tile's scores: where all of them are small, as those of
+// a model trained with a cap far above them are, by the shorter of two polynomials in
+// d^2, whose coefficients have the scale and the cap in them.  (4096 queries over 32K
+// keys, a cap of 50: 1.7 us a tile of 256 columns of `capped` alone, 1.2 so.)
+// `far`: the largest |d| of the lane's; each(f): d := f(d) for all of them.
+template <class Each>
+__device__ __forceinline__ void cap_scores(const Cap& cap, float cap_in, float cap2, float far, Each each) {
+    if (__ballot(far > cap.near_most) == 0) {
+        each([&](float d, float sub) __attribute__((always_inline)) {
+            const float z = d * d;
+            return fmaf(d, fmaf(fmaf(fmaf(cap.near[3], z, cap.near[2]), z, cap.near[1]), z, cap.near[0]), -sub);
+        });
+    } else if (__ballot(far > cap.far_most) == 0) {
+        each([&](float d, float sub) __attribute__((always_inline)) {
+            const float z = d * d;
+            float g = fmaf(cap.far[5], z, cap.far[4]);
+#pragma unroll
+            for (int i = 3; i >= 0; --i) g = fmaf(g, z, cap.far[i]);
+            return fmaf(d, g, -sub);
+        });
+    } else {
+        each([&](float d, float sub) __attribute__((always_inline)) { return capped(d * cap_in, cap2) - sub; });
+    }
 }
 
 // ----------------------------------------------- infinite and NaN values that are masked

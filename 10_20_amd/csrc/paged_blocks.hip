@@ -54,17 +54,17 @@ __device__ __forceinline__ Frag values(const PageTile& tile, int kk, int d) {
     return v;
 }
 
-// Reads of LDS, EACH for one matrix product, kAhead products before it.
-constexpr int kAhead = 4;
-template <int N, int EACH>
-__device__ __forceinline__ void reads_ahead() {
-    __builtin_amdgcn_sched_group_barrier(0x100, EACH * kAhead, 0);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        if (i + kAhead < N) __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);
-    }
+// 16 bytes per lane, memory -> LDS as copy_to_lds does, from a base of the whole wave's.
+__device__ __forceinline__ void copy_from(const void* base, uint32_t offset, uint32_t lds) {
+    const uint64_t at = reinterpret_cast<uint64_t>(base);
+    const uint64_t same = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32 |
+                          (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at);
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :: "v"(offset), "s"(same), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory", "m0");
 }
+
+// Products between the read of a fragment from LDS and its own.
+constexpr int kAhead = 5;
 
 struct BlocksWork {
     Request w;
@@ -127,7 +127,7 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
     if (c < columns) least_lo = most_lo = col.lo, least_hi = most_hi = col.hi;
     least_lo = wave_min(least_lo), most_lo = wave_max(most_lo), least_hi = wave_min(least_hi), most_hi = wave_max(most_hi);
     float slope = 0.f;
-    if (MODE == kBiased && p.slopes) slope = p.slopes[work.kv * p.group + col.head] * kLog2e;
+    if ((MODE == kBiased || MODE == kBoth) && p.slopes) slope = p.slopes[work.kv * p.group + col.head] * kLog2e;
     if (lane == 0) lds.lo[wave] = least_lo, lds.hi[wave] = most_hi;
     lds_barrier();
     int32_t all_lo = INT32_MAX, all_hi = 0;
@@ -150,16 +150,30 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
 
     // Copy j of the wave's four of a tile: four keys twice, four values twice.  (Rows that no column
     // sees are copies of the last that one may; tiles without a page, which nobody reads, are page 0's.)
-    auto copy = [&](int32_t t, int32_t k0, int32_t page, auto which) __attribute__((always_inline)) {
+    struct From {
+        const uint16_t* page[2];  // of keys, of values
+        int32_t rows;             // of it that may be seen
+    };
+    auto from_page = [&](int32_t k0, int32_t page) __attribute__((always_inline)) {
+        From f;
+#pragma unroll
+        for (int v = 0; v < 2; ++v) f.page[v] = p.pool[v] + work.kv * p.head[v] + max(page, 0) * p.page[v];
+        f.rows = end - k0;
+        return f;
+    };
+    const int32_t row0 = 4 * wave + (lane >> 4);
+    const uint32_t stride[2] = {(uint32_t)p.token[0] * 2, (uint32_t)p.token[1] * 2};  // (below 2^26: a page's rows lie within 2^32 bytes)
+    // (rows 32 apart have the same chunks)
+    const uint32_t chunk[2] = {16u * ((lane & 15) ^ (row0 & 15)), 16u * ((lane & 15) ^ (4 * (row0 & 3)))};
+    auto copy = [&](int32_t t, const From& f, auto which) __attribute__((always_inline)) {
         constexpr int j = which.value, v = j / 2;
         PageTile& to = lds.tile[t % kBuffers];
-        const int32_t i = (j & 1) * kWaves + wave, r = 4 * i + (lane >> 4), at = lane & 15;
-        const int32_t chunk = v == 0 ? at ^ (r & 15) : at ^ (4 * (r & 3));
-        const uint16_t* from = p.pool[v] + work.kv * p.head[v] + max(page, 0) * p.page[v];
-        copy_to_lds(from + min(r, end - k0 - 1) * p.token[v] + 8 * chunk, lds_offset(v == 0 ? &to.key[4 * i][0] : &to.value[4 * i][0]));
+        const int32_t i = (j & 1) * kWaves + wave;
+        copy_from(f.page[v], (uint32_t)min(row0 + 32 * (j & 1), f.rows - 1) * stride[v] + chunk[v],
+                  lds_offset(v == 0 ? &to.key[4 * i][0] : &to.value[4 * i][0]));
     };
-    auto copy_tile = [&](int32_t t, int32_t k0, int32_t page) __attribute__((always_inline)) {
-        each_of<COPIES>([&](auto j) __attribute__((always_inline)) { copy(t, k0, page, j); });
+    auto copy_tile = [&](int32_t t, const From& f) __attribute__((always_inline)) {
+        each_of<COPIES>([&](auto j) __attribute__((always_inline)) { copy(t, f, j); });
     };
 
     // B fragments of Q^T: column c.  The rows come through LDS (rows of 16 chunks of 16
@@ -181,7 +195,7 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
             fetch_pages(0);
             page0 = page_at(0), key0 = first_key(0);
             page1 = page_at(min(1, tiles - 1)), key1 = first_key(min(1, tiles - 1));
-            copy_tile(0, key0, page0);
+            copy_tile(0, from_page(key0, page0));
             wait_copies<COPIES>();
         } else {
             wait_copies<0>();
@@ -189,7 +203,7 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
 #pragma unroll
         for (int s = 0; s < 8; ++s) q[s].u = *reinterpret_cast<const u32x4*>(rows + 256 * c + 16 * ((2 * s + h) ^ (c & 15)));
         lds_barrier();
-        if (tiles > 0) copy_tile(1, key1, page1);
+        if (tiles > 0) copy_tile(1, from_page(key1, page1));
     }
     f32x16 acc[4], s[2];
     Frag pf[4];
@@ -207,26 +221,36 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
     auto sees_all = [&](int32_t k0) __attribute__((always_inline)) {
         return (k0 >= most_lo && k0 + kTileKeys <= least_hi) || k0 + kTileKeys <= w.pre;
     };
-    // scores: register i of half u is key 32u + 8 (i / 4) + 4h + i % 4
-    auto scores = [&](int32_t t, int32_t key2, int32_t page2) __attribute__((always_inline)) {
-        const PageTile& tile = lds.tile[t % kBuffers];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
-        // key rows 32u .., numbers 16 (n / 2) ..
-        Frag k[kAhead];
-        auto fetch = [&](int n) __attribute__((always_inline)) {
-            const int32_t st = n / 2, r = 32 * (n & 1) + c;
-            k[n % kAhead].u = *reinterpret_cast<const u32x4*>(&tile.key[r][16 * ((2 * st + h) ^ (r & 15))]);
+    // Sixteen products, of the last tile's values (which 0) or of this one's keys (1), each
+    // fragment read kAhead products before its own.  Scores: register i of half u is key
+    // 32u + 8 (i / 4) + 4h + i % 4.
+    auto multiply = [&](int32_t t, const From& f, auto which) __attribute__((always_inline)) {
+        constexpr bool SCORES = which.value != 0;
+        const PageTile& tile = lds.tile[(SCORES ? t : t - 1) % kBuffers];
+        Frag x[kAhead];
+        auto fetch = [&](auto number) __attribute__((always_inline)) {
+            constexpr int n = number.value;
+            if constexpr (!SCORES) {
+                x[n % kAhead] = values(tile, n / 4, n % 4);
+            } else {  // key rows 32 (n & 1) .., numbers 16 (n / 2) ..
+                const int32_t r = 32 * (n & 1) + c;
+                x[n % kAhead].u = *reinterpret_cast<const u32x4*>(&tile.key[r][16 * ((n - (n & 1) + h) ^ (r & 15))]);
+            }
         };
+        if constexpr (SCORES) {
 #pragma unroll
-        for (int n = 0; n < kAhead; ++n) fetch(n);
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
+        }
+        each_of<kAhead>(fetch);
+        __builtin_amdgcn_sched_barrier(0);
         each_of<16>([&](auto number) __attribute__((always_inline)) {
             constexpr int n = number.value;
-            s[n & 1] = mfma32<T>(k[n % kAhead], q[n / 2], s[n & 1]);
-            if constexpr (n + kAhead < 16) fetch(n + kAhead);
-            if constexpr (n % 4 == 1) copy(t + 2, key2, page2, Number<n / 4>{});
+            if constexpr (!SCORES) acc[n % 4] = mfma32<T>(x[n % kAhead], pf[n / 4], acc[n % 4]);
+            else s[n & 1] = mfma32<T>(x[n % kAhead], q[n / 2], s[n & 1]);
+            if constexpr (n + kAhead < 16) fetch(Number<n + kAhead>{});
+            if constexpr (SCORES && n % 4 == 1) copy(t + 2, f, Number<n / 4>{});
             __builtin_amdgcn_sched_barrier(0);
         });
     };
@@ -236,98 +260,96 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[u][i] = f(s[u][i], 32 * u + 8 * (i / 4) + i % 4);  // (the key, but for 4h)
     };
+    Cap cap = p.cap;
+    if constexpr (MODE == kCapped) {  // (in registers of the loop's own: there are too few scalar ones)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(cap.near[i]));
+    }
     uint64_t seen = ~0ull;  // bit 32u + 8 a + i: key 32u + 8a + 4h + i of the tile in `pf`
     auto softmax = [&](int32_t k0) __attribute__((always_inline)) {
-        float factor = p.scale2;
-        if constexpr (MODE != kPlain) {
-            factor = 1.f;
-            if (MODE == kCapped || p.cap2 > 0.f) {
-                float big = 0.f;
-                each_score([&](float x, int) { x *= p.cap_in, big = fmaxf(big, fabsf(x)); return x; });
-                if (__ballot(big > kSmall)) each_score([&](float x, int) { return capped_any(x, p.cap2); });
-                else each_score([&](float x, int) { return capped_small(x, p.cap2); });
+        if constexpr (MODE == kBoth) each_score([&](float x, int) { return capped(x * p.cap_in, p.cap2); });
+        if constexpr (MODE == kBiased || MODE == kBoth) {
+            const float factor = MODE == kBoth ? 1.f : p.scale2;
+            if (k0 + kTileKeys <= least_hi) {  // (no key behind a query: the distances fall by one a key)
+                const float base = -slope * (float)(col.position - k0 - 4 * h);
+                each_score([&](float x, int key) { return fmaf(x, factor, fmaf(slope, (float)key, base)); });
             } else {
-                each_score([&](float x, int) { return x * p.scale2; });
-            }
-            if constexpr (MODE == kBiased) {
-                if (p.slopes) {
-                    if (p.parents && k0 + kTileKeys > w.before) {
-                        each_score([&](float x, int key) {
-                            int32_t at = k0 + key + 4 * h;
-                            if (at >= w.before) at = w.before + lds.tree.depth[min(at - w.before, kMostDrafts - 1)];
-                            return fmaf(-slope, fabsf((float)(col.position - at)), x);
-                        });
-                    } else {
-                        const float away = (float)(col.position - k0 - 4 * h);
-                        each_score([&](float x, int key) { return fmaf(-slope, fabsf(away - (float)key), x); });
-                    }
-                }
+                // (a draft's depth in place of its number; read for every key, without branches)
+                const int32_t draft0 = k0 + 4 * h - w.before, from = p.parents ? 0 : INT32_MAX;
+                each_score([&](float x, int key) {
+                    const int32_t draft = draft0 + key, depth = lds.tree.depth[min(max(draft, 0), kMostDrafts - 1)];
+                    return fmaf(-slope, fabsf((float)(col.position - w.before - (draft >= from ? depth : draft))), x * factor);
+                });
             }
         }
+        const bool whole = sees_all(k0);
+        bool sees_some = true;
         seen = ~0ull;
-        if (!sees_all(k0)) {
+        if (!whole) {
             seen = column_sees(p, w, lds.tree, col, k0);
-            some |= seen != 0;
+            sees_some = seen != 0;
             seen >>= 4 * h;
-            each_score([&](float x, int key) { return (seen >> key) & 1 ? x : -__builtin_inff(); });
-        } else {
-            some = true;
         }
-        float top = s[0][0];
-        each_score([&](float x, int) { top = fmaxf(top, x); return x; });
-        top = fmaxf(top, __shfl_xor(top, 32, kWave)) * factor;
-        if (__ballot(top > mx + Range<T>::most)) {
-            const float next = top > mx + Range<T>::most ? top - Range<T>::head : mx;
-            const float keep = mx == -__builtin_inff() ? (next == mx ? 1.f : 0.f) : __builtin_amdgcn_exp2f(mx - next);
-            mx = next;
-            total *= keep;
+        some |= sees_some;
+        // The largest magnitude bounds the scores; their maximum is looked for where the bound may pass the subtracted one.
+        float far = 0.f;
+        each_score([&](float x, int) { far = fmaxf(far, fabsf(x)); return x; });
+        const float bound = MODE == kPlain ? far * p.scale2 : MODE == kCapped ? far * p.cap.far[0] : far;
+        if (__ballot(bound > mx + Range<T>::most || mx == -__builtin_inff())) {
+            float top = -__builtin_inff();
+            if (whole) each_score([&](float x, int) { top = fmaxf(top, x); return x; });
+            else each_score([&](float x, int key) { top = fmaxf(top, (seen >> key) & 1 ? x : -__builtin_inff()); return x; });
+            top = fmaxf(top, __shfl_xor(top, 32, kWave));
+            if (MODE == kPlain) top *= p.scale2;
+            if (MODE == kCapped) top = sees_some ? capped(top * p.cap_in, p.cap2) : -__builtin_inff();
+            if (__ballot(top > mx + Range<T>::most)) {
+                const float next = top > mx + Range<T>::most ? top - Range<T>::head : mx;
+                const float keep = mx == -__builtin_inff() ? (next == mx ? 1.f : 0.f) : __builtin_amdgcn_exp2f(mx - next);
+                mx = next;
+                total *= keep;
 #pragma unroll
-            for (int d = 0; d < 4; ++d) acc[d] *= keep;
+                for (int d = 0; d < 4; ++d) acc[d] *= keep;
+            }
         }
         const float sub = mx == -__builtin_inff() ? 0.f : mx;
+        if constexpr (MODE == kCapped) {
+            cap_scores(cap, p.cap_in, p.cap2, far, [&](auto f) __attribute__((always_inline)) { each_score([&](float x, int) { return f(x, sub); }); });
+        }
         each_score([&](float x, int) {
-            x = __builtin_amdgcn_exp2f(MODE == kPlain ? fmaf(x, factor, -sub) : x - sub);
-            total += x;
-            return x;
+            return __builtin_amdgcn_exp2f(MODE == kPlain ? fmaf(x, p.scale2, -sub) : MODE == kCapped ? x : x - sub);
         });
+        if (!whole) each_score([&](float x, int key) { return (seen >> key) & 1 ? x : 0.f; });
+        each_score([&](float x, int) { total += x; return x; });
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 pf[kk].w[i] = pack<T>(s[kk / 2][8 * (kk & 1) + 2 * i], s[kk / 2][8 * (kk & 1) + 2 * i + 1]);
     };
-    auto products = [&](int32_t t) __attribute__((always_inline)) {
+    auto careful_products = [&](int32_t t) __attribute__((always_inline)) {
         const PageTile& tile = lds.tile[t % kBuffers];
-        if constexpr (CAREFUL) {
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                f32x16 up, down;
+        for (int d = 0; d < 4; ++d) {
+            f32x16 up, down;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) up[i] = down[i] = 0.f;
+            for (int i = 0; i < 16; ++i) up[i] = down[i] = 0.f;
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk) {
-                    const Frag v = values(tile, kk, d);
-                    Frag plain, pos, neg, see;
+            for (int kk = 0; kk < 4; ++kk) {
+                const Frag v = values(tile, kk, d);
+                Frag plain, pos, neg, see;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        split_odd<T>(v.w[i], plain.w[i], pos.w[i], neg.w[i]);
-                        const int32_t bit = 16 * kk + 8 * (i / 2) + 2 * (i & 1);  // (of the lane's numbers 2i, 2i + 1)
-                        see.w[i] = ((seen >> bit) & 1 ? kOne<T> : 0u) | ((seen >> (bit + 1)) & 1 ? kOne<T> << 16 : 0u);
-                    }
-                    acc[d] = mfma32<T>(plain, pf[kk], acc[d]);
-                    up = mfma32<T>(pos, see, up);
-                    down = mfma32<T>(neg, see, down);
+                for (int i = 0; i < 4; ++i) {
+                    split_odd<T>(v.w[i], plain.w[i], pos.w[i], neg.w[i]);
+                    const int32_t bit = 16 * kk + 8 * (i / 2) + 2 * (i & 1);  // (of the lane's numbers 2i, 2i + 1)
+                    see.w[i] = ((seen >> bit) & 1 ? kOne<T> : 0u) | ((seen >> (bit + 1)) & 1 ? kOne<T> << 16 : 0u);
                 }
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    acc[d][i] += (up[i] > 0.f ? __builtin_inff() : 0.f) - (down[i] > 0.f ? __builtin_inff() : 0.f);
+                acc[d] = mfma32<T>(plain, pf[kk], acc[d]);
+                up = mfma32<T>(pos, see, up);
+                down = mfma32<T>(neg, see, down);
             }
-        } else {
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-#pragma unroll
-                for (int d = 0; d < 4; ++d) acc[d] = mfma32<T>(values(tile, kk, d), pf[kk], acc[d]);
-            reads_ahead<16, 2>();
+            for (int i = 0; i < 16; ++i)
+                acc[d][i] += (up[i] > 0.f ? __builtin_inff() : 0.f) - (down[i] > 0.f ? __builtin_inff() : 0.f);
         }
     };
     // The two waves of a SIMD half a tile apart: one multiplies (the last tile's
@@ -345,13 +367,18 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
 #pragma unroll 1
     for (int32_t t = 0; t <= tiles; ++t) {
         const bool now = t < tiles && sees(key0, page0);
-        sync(!second);
-        if (saw) products(t - 1);
         const int32_t later = min(t + 2, tiles - 1);
         if (((t + 2) & 63) == 0 && t + 2 < tiles) fetch_pages(t + 2);
         const int32_t page2 = page_at(later), key2 = first_key(later);
-        if (now) scores(t, key2, page2);
-        else if (t < tiles) copy_tile(t + 2, key2, page2);
+        const From f = from_page(key2, page2);
+        sync(!second);
+        // (one place for each: variants of both together cost copies of the sums between them)
+        if (saw) {
+            if constexpr (CAREFUL) careful_products(t - 1);
+            else multiply(t, f, Number<0>{});
+        }
+        if (now) multiply(t, f, Number<1>{});
+        else if (t < tiles) copy_tile(t + 2, f);
         sync(second);
         if (now) softmax(key0);
         saw = now;
@@ -429,6 +456,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void blocks_kernel(AttendParams p) 
     auto& lds = *reinterpret_cast<BlocksLds*>(lds_raw);
     BlocksWork work;
     if (!find_work(p, work)) return;
+    // (the same for the work-group, and in scalar registers from here on)
+    for (int32_t* x : {&work.request, &work.kv, &work.block, &work.part, &work.parts}) *x = __builtin_amdgcn_readfirstlane(*x);
     if (p.parents) find_tree(p, work.w, lds.tree);
     if (__builtin_expect(blocks_part<T, MODE, false>(p, work, lds), 0)) careful_block<T, MODE>(p, &lds);
 }
@@ -445,7 +474,8 @@ int launch(const AttendParams& p, int64_t groups, hipStream_t st) {
 
 template <class T>
 int launch(int mode, const AttendParams& p, int64_t groups, hipStream_t st) {
-    return mode == kPlain ? launch<T, kPlain>(p, groups, st) : mode == kCapped ? launch<T, kCapped>(p, groups, st) : launch<T, kBiased>(p, groups, st);
+    return mode == kPlain ? launch<T, kPlain>(p, groups, st) : mode == kCapped ? launch<T, kCapped>(p, groups, st)
+         : mode == kBiased ? launch<T, kBiased>(p, groups, st) : launch<T, kBoth>(p, groups, st);
 }
 
 }  // namespace

@@ -52,7 +52,7 @@ __device__ __forceinline__ bool rows_part(const AttendParams& p, const RowsWork&
             least_hi = min(least_hi, col[n].hi), most_hi = max(most_hi, col[n].hi);
         }
         slope[n] = 0.f;
-        if (MODE == kBiased && p.slopes) slope[n] = p.slopes[kvh * p.group + col[n].head] * kLog2e;
+        if ((MODE == kBiased || MODE == kBoth) && p.slopes) slope[n] = p.slopes[kvh * p.group + col[n].head] * kLog2e;
     }
     least_lo = wave_min(least_lo), most_lo = wave_max(most_lo), least_hi = wave_min(least_hi), most_hi = wave_max(most_hi);
     const Tiles tiles = tiles_seen(p, w, least_lo, most_hi);
@@ -153,32 +153,26 @@ __device__ __forceinline__ bool rows_part(const AttendParams& p, const RowsWork&
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s[n][u][i] *= p.scale2;
         } else {
-            if (MODE == kCapped || p.cap2 > 0.f) {
-                float big = 0.f;
+            if constexpr (MODE == kCapped || MODE == kBoth) {
+                float far = 0.f;
 #pragma unroll
                 for (int n = 0; n < NC; ++n)
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            s[n][u][i] *= p.cap_in;
-                            big = fmaxf(big, fabsf(s[n][u][i]));
+                            if constexpr (MODE == kBoth) s[n][u][i] = capped(s[n][u][i] * p.cap_in, p.cap2);
+                            else far = fmaxf(far, fabsf(s[n][u][i]));
                         }
-                if (__ballot(big > kSmall)) {
+                if constexpr (MODE == kCapped)
+                    cap_scores(p.cap, p.cap_in, p.cap2, far, [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int n = 0; n < NC; ++n)
+                        for (int n = 0; n < NC; ++n)
 #pragma unroll
-                        for (int u = 0; u < 4; ++u)
+                            for (int u = 0; u < 4; ++u)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) s[n][u][i] = capped_any(s[n][u][i], p.cap2);
-                } else {
-#pragma unroll
-                    for (int n = 0; n < NC; ++n)
-#pragma unroll
-                        for (int u = 0; u < 4; ++u)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) s[n][u][i] = capped_small(s[n][u][i], p.cap2);
-                }
+                                for (int i = 0; i < 4; ++i) s[n][u][i] = f(s[n][u][i], 0.f);
+                    });
             } else {
 #pragma unroll
                 for (int n = 0; n < NC; ++n)
@@ -187,8 +181,8 @@ __device__ __forceinline__ bool rows_part(const AttendParams& p, const RowsWork&
 #pragma unroll
                         for (int i = 0; i < 4; ++i) s[n][u][i] *= p.scale2;
             }
-            if constexpr (MODE == kBiased) {
-                if (p.slopes) {
+            if constexpr (MODE == kBiased || MODE == kBoth) {
+                {
                     const bool drafts = p.parents && k0 + kTileKeys > w.before;
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
@@ -390,19 +384,22 @@ __global__ __launch_bounds__(64 * kWaves, 1) void rows_kernel(AttendParams p) {
     if (__builtin_expect(rows_part<T, NC, MODE, false>(p, work, lds), 0)) careful_rows<T, NC, MODE>(p, work, &lds);
 }
 
-// A work-group of the join: a request's columns of a KV head, 32 threads for each one.
+// A work-group of the join: 8 / G columns of a request and KV head, G groups of 32
+// threads for each, every group every G-th part.
 struct RowsJoin {
     AttendParams a;
     int32_t cols;  // of a block
 };
 
-template <class T>
+template <class T, int G>
 __global__ __launch_bounds__(256) void rows_join(RowsJoin j) {
+    __shared__ f32x4 sums[8][32];
+    __shared__ float totals[8];
     const AttendParams& p = j.a;
-    const int32_t r = (int32_t)blockIdx.y, each = p.blocks * j.cols / 8, kv = (int32_t)blockIdx.x / each;
-    const int32_t m = (int32_t)blockIdx.x % each * 8 + (int32_t)threadIdx.x / 32, at4 = (int32_t)threadIdx.x % 32;
-    const Request w = request_at(p, r);
-    if (m >= w.nq * p.group) return;
+    constexpr int C = 8 / G;
+    const int32_t r = (int32_t)blockIdx.y, each = p.blocks * j.cols / C, kv = (int32_t)blockIdx.x / each;
+    const int32_t who = (int32_t)threadIdx.x / 32, at4 = (int32_t)threadIdx.x % 32, group = who % G;
+    const int32_t m = (int32_t)blockIdx.x % each * C + who / G;
     int32_t parts, first;
     if (p.plan.chunk > 0) {
         parts = (tiles_of(p.plan.keys) + p.plan.chunk - 1) / p.plan.chunk;
@@ -411,25 +408,40 @@ __global__ __launch_bounds__(256) void rows_join(RowsJoin j) {
         const i32x2 of = p.parts.of_row[r];
         first = of[0], parts = of[1];
     }
-    if (parts <= 1) return;
+    const Request w = request_at(p, r);
+    if (parts <= 1 || (m - who / G) >= w.nq * p.group) return;
     const int64_t step = (int64_t)p.kv_heads * p.blocks * j.cols, base = first * step + (int64_t)kv * p.blocks * j.cols + m;
     float top = -__builtin_inff(), total = 0.f;
+    const bool there = m < w.nq * p.group;
+    if (!there) parts = 0;
     for (int32_t i = at4; i < parts; i += 32) top = fmaxf(top, p.parts.stats[base + i * step][0]);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
     const float sub = top == -__builtin_inff() ? 0.f : top;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int32_t i = 0; i < parts; ++i) {
+    for (int32_t i = group; i < parts; i += G) {
         const int64_t at = base + i * step;
         const f32x2 st = p.parts.stats[at];
-        if (st[0] == -__builtin_inff() && st[1] == 0.f) continue;  // (no key of it is seen: its sums are not written)
-        const f32x4 x = *reinterpret_cast<const f32x4*>(p.parts.sums + at * kDim + 4 * at4);
+        f32x4 x = *reinterpret_cast<const f32x4*>(p.parts.sums + at * kDim + 4 * at4);
+        const bool none = st[0] == -__builtin_inff() && st[1] == 0.f;  // (no key of it is seen: its sums may not be written)
         const float f = __builtin_amdgcn_exp2f(st[0] - sub);
         total = fmaf(f, st[1], total);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[k] = fmaf(f, x[k], o[k]);
+        for (int k = 0; k < 4; ++k) o[k] = fmaf(f, none ? 0.f : x[k], o[k]);
     }
+    if constexpr (G > 1) {
+        sums[who][at4] = o;
+        if (at4 == 0) totals[who] = total;
+        __syncthreads();
+        if (group != 0) return;
+#pragma unroll
+        for (int k = 1; k < G; ++k) {
+            o += sums[who + k][at4];
+            total += totals[who + k];
+        }
+    }
+    if (!there) return;
     const int32_t i = m / p.group, head = kv * p.group + m % p.group;
     const int64_t token = w.q_lo + i;
     const bool none = top == -__builtin_inff() && total == 0.f;  // no key attended
@@ -438,6 +450,13 @@ __global__ __launch_bounds__(256) void rows_join(RowsJoin j) {
         none ? u32x2{0, 0} : u32x2{pack<T>(o[0] * inv, o[1] * inv), pack<T>(o[2] * inv, o[3] * inv)};
     if (p.lse && at4 == 0)
         p.lse[token * p.kv_heads * p.group + head] = none ? -__builtin_inff() : (top + __builtin_amdgcn_logf(total)) * kLn2;
+}
+
+template <class T, int G>
+int launch_join(const AttendParams& p, int32_t cols, hipStream_t st) {
+    const int64_t groups = (int64_t)p.kv_heads * p.blocks * cols / (8 / G);
+    hipLaunchKernelGGL((rows_join<T, G>), dim3((uint32_t)groups, (uint32_t)p.requests), dim3(256), 0, st, RowsJoin{p, cols});
+    return V1_LAUNCHED("paged_attend: join");
 }
 
 // -------------------------------------------------------------- the host's side
@@ -514,8 +533,8 @@ int launch_rows(const AttendParams& p, int64_t groups, hipStream_t st) {
 
 template <class T, int NC>
 int launch_rows(int mode, const AttendParams& p, int64_t groups, hipStream_t st) {
-    return mode == kPlain ? launch_rows<T, NC, kPlain>(p, groups, st)
-         : mode == kCapped ? launch_rows<T, NC, kCapped>(p, groups, st) : launch_rows<T, NC, kBiased>(p, groups, st);
+    return mode == kPlain ? launch_rows<T, NC, kPlain>(p, groups, st) : mode == kCapped ? launch_rows<T, NC, kCapped>(p, groups, st)
+         : mode == kBiased ? launch_rows<T, NC, kBiased>(p, groups, st) : launch_rows<T, NC, kBoth>(p, groups, st);
 }
 
 template <class T>
@@ -534,9 +553,9 @@ int attend(AttendParams& p, const Shape& s, int mode, hipStream_t st) {
            : s.cols == 32 ? launch_rows<T, 2>(mode, p, 8 * spread, st) : launch_rows<T, 4>(mode, p, 8 * spread, st);
     }
     if (rc != V1_OK || workspace_of(s, p.kv_heads) == 0) return rc;
-    const int64_t eights = cdiv((int64_t)s.blocks * s.cols, 8);
-    hipLaunchKernelGGL(rows_join<T>, dim3((uint32_t)(p.kv_heads * eights), (uint32_t)p.requests), dim3(256), 0, st, RowsJoin{p, s.cols});
-    return V1_LAUNCHED("paged_attend: join");
+    // (about as many groups as a request has parts)
+    const int64_t parts = cdiv(s.items, p.requests);
+    return parts > 8 ? launch_join<T, 8>(p, s.cols, st) : parts > 2 ? launch_join<T, 2>(p, s.cols, st) : launch_join<T, 1>(p, s.cols, st);
 }
 
 }  // namespace
@@ -571,6 +590,8 @@ extern "C" int v1_paged_attend(const v1_paged_attend_args* a, void* stream) {
     V1_REQUIRE(paged::aligned16(k_pool) && paged::aligned16(v_pool) &&
                    (kp_page | kp_token | kp_head | vp_page | vp_token | vp_head) % 8 == 0,
                "paged_attend: pools must be 16-byte aligned with strides in multiples of 8");
+    V1_REQUIRE(kp_token >= 0 && kp_token < 1 << 25 && vp_token >= 0 && vp_token < 1 << 25,
+               "paged_attend: a page's tokens must lie less than 2^25 numbers apart");
     if (tokens == 0 || requests == 0 || max_q == 0) return V1_OK;
     if (pages == 0) table_len = 0;
     const int32_t keys = table_len * kTileKeys;
@@ -578,12 +599,13 @@ extern "C" int v1_paged_attend(const v1_paged_attend_args* a, void* stream) {
     const Shape s = shape_of(lens, tokens, requests, kv_heads, group, max_q, keys, window);
     const int64_t need = workspace_of(s, kv_heads);
     V1_REQUIRE(workspace_bytes >= need && (need == 0 || workspace != nullptr), "paged_attend: workspace of %lld bytes needed", (long long)need);
-    const int mode = slopes ? kBiased : softcap > 0.f ? kCapped : kPlain;
+    const float in = softcap > 0.f ? scale / softcap : 0.f;
+    const int mode = softcap == 0.f ? (slopes ? kBiased : kPlain) : !slopes && in >= 0x1p-12f && in <= 0x1p12f ? kCapped : kBoth;
     AttendParams p{static_cast<const uint16_t*>(q), q_token, q_head,
                    {static_cast<const uint16_t*>(k_pool), static_cast<const uint16_t*>(v_pool)}, {kp_page, vp_page},
                    {kp_token, vp_token}, {kp_head, vp_head}, pages, table, table_stride, lens, cu_q, prefix, document,
                    parents, slopes, table_len, tokens, requests, max_q, kv_heads, group, small_div_magic((uint32_t)group),
-                   window, scale * kLog2e, softcap > 0.f ? scale / softcap : 0.f, softcap * kLog2e,
+                   window, scale * kLog2e, in, softcap * kLog2e, cap_of(scale, softcap),
                    static_cast<uint16_t*>(out), o_token, o_head, lse, s.plan, s.reach, s.blocks, 0, s.together,
                    s.units, s.xcds, s.slots, parts_of(workspace, s, kv_heads)};
     return fp16 ? attend<_Float16>(p, s, mode, as_stream(stream)) : attend<__bf16>(p, s, mode, as_stream(stream));
