@@ -230,7 +230,35 @@ __device__ __forceinline__ int32_t wave_min(int32_t x) {
     for (int off = 32; off > 0; off >>= 1) x = min(x, __shfl_xor(x, off, kWave));
     return __builtin_amdgcn_readfirstlane(x);
 }
-__device__ __forceinline__ int32_t wave_max(int32_t x) { return -wave_min(-x); }
+
+// Bounds of what the columns of lanes 0 .. n - 1 see.  They ascend with the columns,
+// unless documents or depths decide.
+struct Bounds {
+    int32_t least_lo, most_lo, least_hi, most_hi;
+};
+
+__device__ __forceinline__ Bounds bounds_of(const AttendParams& p, const Column& c, int32_t lane, int32_t n) {
+    if (n <= 0) return {INT32_MAX, 0, INT32_MAX, 0};
+    const int32_t last = min(n, kWave) - 1;
+    Bounds b;
+    b.least_hi = __builtin_amdgcn_readlane(c.hi, 0), b.most_hi = __builtin_amdgcn_readlane(c.hi, last);
+    if (p.document || (p.parents && p.window > 0)) {
+        b.least_lo = wave_min(lane <= last ? c.lo : INT32_MAX);
+        b.most_lo = -wave_min(lane <= last ? -c.lo : 0);
+    } else {
+        b.least_lo = __builtin_amdgcn_readlane(c.lo, 0), b.most_lo = __builtin_amdgcn_readlane(c.lo, last);
+    }
+    return b;
+}
+
+// All bits of a register where the bit of a key among 64 is set.
+__device__ __forceinline__ uint32_t mask_of(uint64_t seen, int key) {
+    return (uint32_t)__builtin_amdgcn_sbfe((int)(uint32_t)(key < 32 ? seen : seen >> 32), key & 31, 1);
+}
+__device__ __forceinline__ float if_seen(uint32_t mask, float x) { return __uint_as_float(mask & __float_as_uint(x)); }
+__device__ __forceinline__ float if_seen_or_least(uint32_t mask, float x) {
+    return __uint_as_float((mask & __float_as_uint(x)) | (~mask & 0xff800000u));
+}
 
 // ------------------------------------------------------------------ capped scores
 // cap tanh(x / cap), base 2, of a product d = q . k, t = d scale / cap: past |t| = 0.75

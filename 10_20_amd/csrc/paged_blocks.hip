@@ -123,9 +123,8 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
     const int32_t* table = p.table + work.request * p.table_stride;
 
     const Column col = column_at(p, w, lds.tree, m0, wave * kRows + c);
-    int32_t least_lo = INT32_MAX, most_lo = 0, least_hi = INT32_MAX, most_hi = 0;
-    if (c < columns) least_lo = most_lo = col.lo, least_hi = most_hi = col.hi;
-    least_lo = wave_min(least_lo), most_lo = wave_max(most_lo), least_hi = wave_min(least_hi), most_hi = wave_max(most_hi);
+    const Bounds mine = bounds_of(p, col, c, min(columns, kRows));
+    const int32_t least_lo = mine.least_lo, most_lo = mine.most_lo, least_hi = mine.least_hi, most_hi = mine.most_hi;
     float slope = 0.f;
     if ((MODE == kBiased || MODE == kBoth) && p.slopes) slope = p.slopes[work.kv * p.group + col.head] * kLog2e;
     if (lane == 0) lds.lo[wave] = least_lo, lds.hi[wave] = most_hi;
@@ -298,7 +297,7 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
         if (__ballot(bound > mx + Range<T>::most || mx == -__builtin_inff())) {
             float top = -__builtin_inff();
             if (whole) each_score([&](float x, int) { top = fmaxf(top, x); return x; });
-            else each_score([&](float x, int key) { top = fmaxf(top, (seen >> key) & 1 ? x : -__builtin_inff()); return x; });
+            else each_score([&](float x, int key) { top = fmaxf(top, if_seen_or_least(mask_of(seen, key), x)); return x; });
             top = fmaxf(top, __shfl_xor(top, 32, kWave));
             if (MODE == kPlain) top *= p.scale2;
             if (MODE == kCapped) top = sees_some ? capped(top * p.cap_in, p.cap2) : -__builtin_inff();
@@ -318,7 +317,7 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
         each_score([&](float x, int) {
             return __builtin_amdgcn_exp2f(MODE == kPlain ? fmaf(x, p.scale2, -sub) : MODE == kCapped ? x : x - sub);
         });
-        if (!whole) each_score([&](float x, int key) { return (seen >> key) & 1 ? x : 0.f; });
+        if (!whole) each_score([&](float x, int key) { return if_seen(mask_of(seen, key), x); });
         each_score([&](float x, int) { total += x; return x; });
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)

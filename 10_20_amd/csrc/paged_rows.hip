@@ -47,14 +47,12 @@ __device__ __forceinline__ bool rows_part(const AttendParams& p, const RowsWork&
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
         col[n] = column_at(p, w, lds.tree, m0, 16 * n + c);
-        if (16 * n + c < columns) {
-            least_lo = min(least_lo, col[n].lo), most_lo = max(most_lo, col[n].lo);
-            least_hi = min(least_hi, col[n].hi), most_hi = max(most_hi, col[n].hi);
-        }
+        const Bounds b = bounds_of(p, col[n], c, min(columns - 16 * n, 16));
+        least_lo = min(least_lo, b.least_lo), most_lo = max(most_lo, b.most_lo);
+        least_hi = min(least_hi, b.least_hi), most_hi = max(most_hi, b.most_hi);
         slope[n] = 0.f;
         if ((MODE == kBiased || MODE == kBoth) && p.slopes) slope[n] = p.slopes[kvh * p.group + col[n].head] * kLog2e;
     }
-    least_lo = wave_min(least_lo), most_lo = wave_max(most_lo), least_hi = wave_min(least_hi), most_hi = wave_max(most_hi);
     const Tiles tiles = tiles_seen(p, w, least_lo, most_hi);
     const int32_t each = (tiles.count + it.parts - 1) / it.parts;
     const int32_t first = min(it.part * each, tiles.count), count = min(each, tiles.count - first);
@@ -209,7 +207,7 @@ __device__ __forceinline__ bool rows_part(const AttendParams& p, const RowsWork&
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[n][u][i] = (seen[n] >> (16 * u + i)) & 1 ? s[n][u][i] : -__builtin_inff();
+                    for (int i = 0; i < 4; ++i) s[n][u][i] = if_seen_or_least(mask_of(seen[n], 16 * u + i), s[n][u][i]);
             }
         } else {
             some = -1;
@@ -480,15 +478,16 @@ inline Shape shape_of(const int32_t* lens, int32_t tokens, int32_t requests, int
     s.reach = reach_of(window, max_q);
     const int64_t columns = (int64_t)max_q * group;
     const bool few = columns <= kFewColumns;
-    s.cols = !few ? kBlockColumns : columns <= 16 ? 16 : columns <= 32 ? 32 : 64;
+    s.cols = !few ? kBlockColumns : columns <= 16 ? 16 : 32;
     s.blocks = (int32_t)cdiv(columns, s.cols);
     s.together = !few ? 1 : kv_heads % 4 == 0 ? 4 : kv_heads % 2 == 0 ? 2 : 1;
     s.slots = s.units = 0, s.xcds = 1;
     if (s.reach > 0) keys = std::min(keys, s.reach);
     const int64_t sets = (int64_t)kv_heads / s.together * s.blocks, streams = few ? kWaves / s.together : 1;
     const int64_t running = std::max<int64_t>(1, device_cus() / sets), tiles = cdiv(keys, kTileKeys);
-    const int64_t most = few ? running : std::max<int64_t>(1, 2 * device_cus() / sets);
-    s.plan = Plan{lens, requests, keys, 0, 0, (int32_t)most};
+    // (many queries: parts enough for two work-groups a CU, or twice the requests where that is four at most)
+    const int64_t most = few ? running : std::max<int64_t>({1, 2 * device_cus() / sets, std::min<int64_t>(4 * device_cus() / sets, 2ll * requests)});
+    s.plan = Plan{lens, requests, keys, 0, 0, (int32_t)most, few ? 1 : 4};
     if (keys > 0 && planned(requests, tiles) && requests < most)
         s.plan.target = (int32_t)std::max(most - requests, (most + 1) / 2);
     else s.plan.chunk = (int32_t)streams * chunk_for(requests, cdiv(tiles, streams), running, few ? 2 : 6, few ? 1 : 2);
@@ -549,8 +548,7 @@ int attend(AttendParams& p, const Shape& s, int mode, hipStream_t st) {
         const int64_t spread = s.plan.chunk > 0 ? cdiv(s.items * sets, 8) : cdiv(s.items, 8) * sets;
         V1_REQUIRE(launchable(8 * spread, 64 * kWaves), "paged_attend: too many requests and heads for a launch");
         p.spread = (int32_t)spread;
-        rc = s.cols == 16 ? launch_rows<T, 1>(mode, p, 8 * spread, st)
-           : s.cols == 32 ? launch_rows<T, 2>(mode, p, 8 * spread, st) : launch_rows<T, 4>(mode, p, 8 * spread, st);
+        rc = s.cols == 16 ? launch_rows<T, 1>(mode, p, 8 * spread, st) : launch_rows<T, 2>(mode, p, 8 * spread, st);
     }
     if (rc != V1_OK || workspace_of(s, p.kv_heads) == 0) return rc;
     // (about as many groups as a request has parts)
