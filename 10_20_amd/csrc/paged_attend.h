@@ -50,12 +50,13 @@ inline Cap cap_of(float scale, float softcap) {
         if (i < 4) c.near[i] = (float)(kCapNear[i] * by);
         c.far[i] = (float)(kCapFar[i] * by);
     }
-    c.near_most = (float)(kCapNearMost / in), c.far_most = (float)(kCapFarMost / in);
+    // (a cap so far from the scale that the coefficients would not be normal numbers: neither polynomial)
+    const bool normal = in >= 0x1p-12 && in <= 0x1p12;
+    c.near_most = normal ? (float)(kCapNearMost / in) : -1.f, c.far_most = normal ? (float)(kCapFarMost / in) : -1.f;
     return c;
 }
 
-// What a score takes: nothing, a cap (of 2^-12 .. 2^12 times the scale, so that the
-// polynomials' coefficients are normal numbers), a distance, or any cap and a distance.
+// What a score takes: nothing, a cap, a distance, or both.
 constexpr int kPlain = 0, kCapped = 1, kBiased = 2, kBoth = 3;
 
 struct AttendParams {

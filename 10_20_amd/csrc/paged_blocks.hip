@@ -140,12 +140,14 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
 
     // pages of the next 64 tiles, one a lane; -1: no page
     int32_t page_of = -1;
+    constexpr bool BACK = MODE == kBiased || MODE == kBoth;
+    auto tile_at = [&](int32_t t) __attribute__((always_inline)) { return list.at(first + (BACK ? tiles - 1 - t : t)); };
     auto fetch_pages = [&](int32_t t) __attribute__((always_inline)) {
-        page_of = table[list.at(first + min(t + lane, tiles - 1))];
+        page_of = table[tile_at(min(t + lane, tiles - 1))];
         if (page_of >= p.pages) page_of = -1;
     };
     auto page_at = [&](int32_t t) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(page_of, t & 63); };
-    auto first_key = [&](int32_t t) __attribute__((always_inline)) { return list.at(first + t) * kTileKeys; };
+    auto first_key = [&](int32_t t) __attribute__((always_inline)) { return tile_at(t) * kTileKeys; };
 
     // Copy j of the wave's four of a tile: four keys twice, four values twice.  (Rows that no column
     // sees are copies of the last that one may; tiles without a page, which nobody reads, are page 0's.)
@@ -266,7 +268,11 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
     }
     uint64_t seen = ~0ull;  // bit 32u + 8 a + i: key 32u + 8a + 4h + i of the tile in `pf`
     auto softmax = [&](int32_t k0) __attribute__((always_inline)) {
-        if constexpr (MODE == kBoth) each_score([&](float x, int) { return capped(x * p.cap_in, p.cap2); });
+        if constexpr (MODE == kBoth) {
+            float far = 0.f;
+            each_score([&](float x, int) { far = fmaxf(far, fabsf(x)); return x; });
+            cap_scores(p.cap, p.cap_in, p.cap2, far, [&](auto f) __attribute__((always_inline)) { each_score([&](float x, int) { return f(x, 0.f); }); });
+        }
         if constexpr (MODE == kBiased || MODE == kBoth) {
             const float factor = MODE == kBoth ? 1.f : p.scale2;
             if (k0 + kTileKeys <= least_hi) {  // (no key behind a query: the distances fall by one a key)
@@ -291,8 +297,8 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
         }
         some |= sees_some;
         // The largest magnitude bounds the scores; their maximum is looked for where the bound may pass the subtracted one.
-        float far = 0.f;
-        each_score([&](float x, int) { far = fmaxf(far, fabsf(x)); return x; });
+        float far = BACK ? -__builtin_inff() : 0.f;
+        each_score([&](float x, int) { far = fmaxf(far, BACK ? x : fabsf(x)); return x; });
         const float bound = MODE == kPlain ? far * p.scale2 : MODE == kCapped ? far * p.cap.far[0] : far;
         if (__ballot(bound > mx + Range<T>::most || mx == -__builtin_inff())) {
             float top = -__builtin_inff();
@@ -387,12 +393,13 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
     wait_copies<0>();
     __syncthreads();  // the tiles' memory is free
     if constexpr (!CAREFUL) {
-        float odd = 0.f;
+        float odd[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int d = 0; d < 4; ++d)
+        for (int i = 0; i < 16; ++i)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) odd = fmaf(acc[d][i], 0.f, odd);
-        if (__syncthreads_or(odd != odd)) return true;
+            for (int d = 0; d < 4; ++d) odd[d] = fmaf(acc[d][i], 0.f, odd[d]);
+        const float sum = (odd[0] + odd[1]) + (odd[2] + odd[3]);
+        if (__syncthreads_or(sum != sum)) return true;
     }
     total += __shfl_xor(total, 32, kWave);
     const bool none = !some;  // no key seen

@@ -158,19 +158,15 @@ __device__ __forceinline__ bool rows_part(const AttendParams& p, const RowsWork&
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            if constexpr (MODE == kBoth) s[n][u][i] = capped(s[n][u][i] * p.cap_in, p.cap2);
-                            else far = fmaxf(far, fabsf(s[n][u][i]));
-                        }
-                if constexpr (MODE == kCapped)
-                    cap_scores(p.cap, p.cap_in, p.cap2, far, [&](auto f) __attribute__((always_inline)) {
+                        for (int i = 0; i < 4; ++i) far = fmaxf(far, fabsf(s[n][u][i]));
+                cap_scores(p.cap, p.cap_in, p.cap2, far, [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
-                        for (int n = 0; n < NC; ++n)
+                    for (int n = 0; n < NC; ++n)
 #pragma unroll
-                            for (int u = 0; u < 4; ++u)
+                        for (int u = 0; u < 4; ++u)
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) s[n][u][i] = f(s[n][u][i], 0.f);
-                    });
+                            for (int i = 0; i < 4; ++i) s[n][u][i] = f(s[n][u][i], 0.f);
+                });
             } else {
 #pragma unroll
                 for (int n = 0; n < NC; ++n)
@@ -180,19 +176,18 @@ __device__ __forceinline__ bool rows_part(const AttendParams& p, const RowsWork&
                         for (int i = 0; i < 4; ++i) s[n][u][i] *= p.scale2;
             }
             if constexpr (MODE == kBiased || MODE == kBoth) {
-                {
-                    const bool drafts = p.parents && k0 + kTileKeys > w.before;
+                // (a draft's depth in place of its number; read for every key, without branches)
+                const int32_t draft0 = k0 + 4 * g - w.before, from = p.parents ? 0 : INT32_MAX;
 #pragma unroll
-                    for (int u = 0; u < 4; ++u)
+                for (int u = 0; u < 4; ++u)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            int32_t key = k0 + 16 * u + 4 * g + i;
-                            if (drafts && key >= w.before) key = w.before + lds.tree.depth[min(key - w.before, kMostDrafts - 1)];
+                    for (int i = 0; i < 4; ++i) {
+                        const int32_t draft = draft0 + 16 * u + i, depth = lds.tree.depth[min(max(draft, 0), kMostDrafts - 1)];
+                        const int32_t at = w.before + (draft >= from ? depth : draft);
 #pragma unroll
-                            for (int n = 0; n < NC; ++n)
-                                s[n][u][i] = fmaf(-slope[n], fabsf((float)(col[n].position - key)), s[n][u][i]);
-                        }
-                }
+                        for (int n = 0; n < NC; ++n)
+                            s[n][u][i] = fmaf(-slope[n], fabsf((float)(col[n].position - at)), s[n][u][i]);
+                    }
             }
         }
         uint64_t seen[NC];
@@ -470,7 +465,7 @@ struct Shape {
     Plan plan;
 };
 
-constexpr int kFewColumns = 64;  // the most that the kernel of few queries takes
+constexpr int kFewColumns = 32;  // the most that the kernel of few queries takes
 
 inline Shape shape_of(const int32_t* lens, int32_t tokens, int32_t requests, int32_t kv_heads, int32_t group, int32_t max_q, int32_t keys,
                       int32_t window) {
@@ -485,10 +480,19 @@ inline Shape shape_of(const int32_t* lens, int32_t tokens, int32_t requests, int
     if (s.reach > 0) keys = std::min(keys, s.reach);
     const int64_t sets = (int64_t)kv_heads / s.together * s.blocks, streams = few ? kWaves / s.together : 1;
     const int64_t running = std::max<int64_t>(1, device_cus() / sets), tiles = cdiv(keys, kTileKeys);
-    // (many queries: parts enough for two work-groups a CU, or twice the requests where that is four at most)
-    const int64_t most = few ? running : std::max<int64_t>({1, 2 * device_cus() / sets, std::min<int64_t>(4 * device_cus() / sets, 2ll * requests)});
-    s.plan = Plan{lens, requests, keys, 0, 0, (int32_t)most, few ? 1 : 4};
-    if (keys > 0 && planned(requests, tiles) && requests < most)
+    // Parts at most, and tiles of a part at least.  Few queries: as many as run at once; where the requests alone are that
+    // many, two for each of the longer ones, unless a window makes them alike: 130 requests of 1000 to 20000 tokens, 32 heads
+    // of 8 KV heads, 1013 us in one part each and 625 so; 250 of 8000, 4 KV heads, 685 and 694; 128 of 500, which parts of
+    // less than 32 tiles would cut, 46 and 59.  Many queries: enough for two work-groups a CU (32 trees of 64 drafts over
+    // 4K-64K tokens 1110 us, three a CU 1056, four 1085; 8 such trees 282, 303, 313), or for twice the requests where that is
+    // four a CU or less (8 chunks of 512 behind 1000 to 32000 tokens, 32 heads: 1250 us in one part each, 706 so).
+    const bool crowded = few && requests >= running;
+    const int64_t most = !few ? std::max<int64_t>({1, 2 * device_cus() / sets, std::min<int64_t>(4 * device_cus() / sets, 2ll * requests)})
+                       : crowded && s.reach == 0 ? std::min<int64_t>(4 * running, 2ll * requests) : running;
+    s.plan = Plan{lens, requests, keys, 0, 0, (int32_t)most, !few ? 4 : crowded ? (int32_t)(32 * streams) : 1};
+    // (a request of few tiles is one work-group's: the join would take longer than its tiles)
+    if (few && tiles <= 4 * streams) s.plan.chunk = (int32_t)std::max<int64_t>(1, tiles);
+    else if (keys > 0 && planned(requests, tiles) && requests < most)
         s.plan.target = (int32_t)std::max(most - requests, (most + 1) / 2);
     else s.plan.chunk = (int32_t)streams * chunk_for(requests, cdiv(tiles, streams), running, few ? 2 : 6, few ? 1 : 2);
     s.items = items_at_most(s.plan);
@@ -598,7 +602,7 @@ extern "C" int v1_paged_attend(const v1_paged_attend_args* a, void* stream) {
     const int64_t need = workspace_of(s, kv_heads);
     V1_REQUIRE(workspace_bytes >= need && (need == 0 || workspace != nullptr), "paged_attend: workspace of %lld bytes needed", (long long)need);
     const float in = softcap > 0.f ? scale / softcap : 0.f;
-    const int mode = softcap == 0.f ? (slopes ? kBiased : kPlain) : !slopes && in >= 0x1p-12f && in <= 0x1p12f ? kCapped : kBoth;
+    const int mode = softcap == 0.f ? (slopes ? kBiased : kPlain) : slopes ? kBoth : kCapped;
     AttendParams p{static_cast<const uint16_t*>(q), q_token, q_head,
                    {static_cast<const uint16_t*>(k_pool), static_cast<const uint16_t*>(v_pool)}, {kp_page, vp_page},
                    {kp_token, vp_token}, {kp_head, vp_head}, pages, table, table_stride, lens, cu_q, prefix, document,
