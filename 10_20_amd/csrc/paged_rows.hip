@@ -576,6 +576,7 @@ extern "C" int v1_paged_attend(const v1_paged_attend_args* a, void* stream) {
     auto [q, q_token, q_head, k_pool, kp_page, kp_token, kp_head, v_pool, vp_page, vp_token, vp_head, pages, table,
           table_stride, lens, cu_q, prefix, document, parents, slopes, out, o_token, o_head, lse, workspace,
           workspace_bytes, table_len, tokens, requests, max_q, kv_heads, group, window, fp16, scale, softcap] = *a;
+    if (!cu_q) max_q = 1;
     V1_REQUIRE(tokens >= 0 && requests >= 0 && max_q >= 0 && kv_heads > 0 && group > 0 && pages >= 0 && table_len >= 0 &&
                    window >= 0 && (int64_t)kv_heads * group < 1 << 15,
                "paged_attend: bad shape");
@@ -584,7 +585,7 @@ extern "C" int v1_paged_attend(const v1_paged_attend_args* a, void* stream) {
     V1_REQUIRE(parents == nullptr || (max_q <= kMostDrafts && document == nullptr && prefix == nullptr),
                "paged_attend: at most %d drafted tokens of a request", kMostDrafts);
     V1_REQUIRE(scale > 0.f && scale * kLog2e < __builtin_inff(), "paged_attend: scale must be positive and finite");
-    V1_REQUIRE(softcap >= 0.f && (softcap == 0.f || (softcap * 4.f < __builtin_inff() && scale / softcap >= 0x1p-126f &&
+    V1_REQUIRE(softcap >= 0.f && (softcap == 0.f || (softcap >= 0x1p-126f && softcap * 4.f < __builtin_inff() && scale / softcap >= 0x1p-126f &&
                                                       scale / softcap < __builtin_inff())),
                "paged_attend: softcap must be zero or positive, and softcap and scale / softcap normal numbers");
     V1_REQUIRE(paged::aligned16(q) && (q_token | q_head) % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0 && (o_token | o_head) % 4 == 0,
@@ -597,7 +598,6 @@ extern "C" int v1_paged_attend(const v1_paged_attend_args* a, void* stream) {
     if (tokens == 0 || requests == 0 || max_q == 0) return V1_OK;
     if (pages == 0) table_len = 0;
     const int32_t keys = table_len * kTileKeys;
-    if (!cu_q) max_q = 1;
     const Shape s = shape_of(lens, tokens, requests, kv_heads, group, max_q, keys, window);
     const int64_t need = workspace_of(s, kv_heads);
     V1_REQUIRE(workspace_bytes >= need && (need == 0 || workspace != nullptr), "paged_attend: workspace of %lld bytes needed", (long long)need);

@@ -6,7 +6,7 @@ Top-K's ids of single tokens; kv8 holds pages in 8 bits.)
 
 Pools: k_pool, v_pool [pages, 64, kv_heads, 128] bfloat16 or float16 (16-byte
 aligned, any strides in multiples of 8, the last dimension contiguous: token-major
-and head-major pages alike).  Position i of a request lies in page table[r, i // 64],
+and head-major pages alike; `attend` takes tokens of a page less than 2**25 numbers apart).  Position i of a request lies in page table[r, i // 64],
 the layout of the page manager.
 
 A step of drafted trees: `append` writes the drafts behind the context, each at the
@@ -193,6 +193,8 @@ def _attend(q, k_pool, v_pool, table, lens, cu_q, max_q, scale, softcap, slopes,
         _vector("document", document, tokens)
         of_document = document.data_ptr()
     if parents is not None:
+        if max_q > MOST_DRAFTS:
+            raise ValueError(f"max_q must be given, at most {MOST_DRAFTS}, for more drafted tokens than that")
         _vector("parents", parents, tokens)
         of_parents = parents.data_ptr()
     if slopes is not None:
@@ -269,7 +271,5 @@ def attend_tree(q, k_pool, v_pool, table, lens, parents, cu_q=None, max_q=None, 
     count from it, a window hides positions of the context alone."""
     if parents is None:
         raise ValueError("parents must be a contiguous int32 tensor")
-    if cu_q is not None and (q.shape[0] if max_q is None else min(int(max_q), q.shape[0])) > MOST_DRAFTS:
-        raise ValueError(f"max_q must be given, at most {MOST_DRAFTS}, for more drafted tokens than that")
     return _attend(q, k_pool, v_pool, table, lens, cu_q, max_q, softmax_scale, softcap, slopes, window, None, None, parents, out,
                    return_lse)
