@@ -321,10 +321,11 @@ __device__ __forceinline__ void split_odd(uint32_t w, uint32_t& plain, uint32_t&
 template <class T>
 constexpr uint32_t kOne = __is_same(T, __bf16) ? 0x3f80u : 0x3c00u;
 
-constexpr int kBlockColumns = 256;
+// Columns of a work-group for many queries: 256, or 128 for work that leaves CUs idle.
+constexpr int kBlockColumns = 256, kSmallBlockColumns = 128;
 
 // The launch of paged_blocks.hip.
-int launch_blocks(bool fp16, int mode, const AttendParams& p, int64_t groups, hipStream_t st);
+int launch_blocks(bool fp16, int columns, int mode, const AttendParams& p, int64_t groups, hipStream_t st);
 
 }  // namespace paged
 }  // namespace v1

@@ -7,10 +7,7 @@ namespace {
 
 using namespace paged;
 
-constexpr int kRows = 32;                           // columns of a wave
-constexpr int kWaves = 8, kBlock = kWaves * kRows;  // of a work-group
-constexpr int kBuffers = 4;                         // tiles in LDS
-static_assert(kBlock == kBlockColumns);
+constexpr int kRows = 32;  // columns of a wave
 
 using f32x16 = __attribute__((ext_vector_type(16))) float;
 using i16x4 = __attribute__((ext_vector_type(4))) short;
@@ -20,10 +17,13 @@ struct PageTile {
     uint8_t value[kTileKeys][2 * kDim];
 };
 
+// Work-groups of WAVES waves: eight, which take all of a CU's LDS for four tiles, or
+// four, two work-groups a CU with two tiles each.
+template <int WAVES>
 struct BlocksLds {
-    PageTile tile[kBuffers];
+    PageTile tile[WAVES / 2];
     Tree tree;
-    int32_t lo[kWaves], hi[kWaves];
+    int32_t lo[WAVES], hi[WAVES];
 };
 
 template <class T>
@@ -74,11 +74,13 @@ struct BlocksWork {
 };
 
 // The work-group's part of the attention; false: there is none.
+template <int WAVES>
 __device__ __forceinline__ bool find_work(const AttendParams& p, BlocksWork& work) {
     // Work-groups reach the XCDs in turn.  An XCD takes whole units, a KV head of an item
     // (a request, or a part of its keys), `together` of them at a time, the longest
     // blocks of all of them first: blocks of the same keys meet in one L2, and the last
     // ones to end are short.
+    constexpr int kBlock = WAVES * kRows;
     const int32_t units = (p.units + p.xcds - 1) / p.xcds, turn = (int32_t)blockIdx.x / p.xcds;
     const int32_t before = turn / (p.together * p.blocks) * p.together, size = min(p.together, units - before);
     const int32_t within = turn - before * p.blocks, rank = within / size;
@@ -112,10 +114,11 @@ __device__ __forceinline__ bool find_work(const AttendParams& p, BlocksWork& wor
 
 // Masked keys of infinite or NaN values: sums that end up not finite (true is returned,
 // nothing written) are found again by the CAREFUL form.
-template <class T, int MODE, bool CAREFUL>
-__device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksWork& work, BlocksLds& lds) {
+template <class T, int MODE, int WAVES, bool CAREFUL>
+__device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksWork& work, BlocksLds<WAVES>& lds) {
+    constexpr int kWaves = WAVES, kBlock = WAVES * kRows, kBuffers = WAVES / 2;
     constexpr int COPIES = (int)(sizeof(PageTile) / 1024) / kWaves;
-    static_assert(COPIES == 4, "copies of a tile");
+    static_assert(COPIES * kWaves == 32, "copies of a tile");
     const Request& w = work.w;
     const int32_t wave = __builtin_amdgcn_readfirstlane((int32_t)threadIdx.x / kWave);
     const int32_t lane = (int32_t)threadIdx.x % kWave, c = lane & 31, h = lane >> 5;
@@ -149,7 +152,7 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
     auto page_at = [&](int32_t t) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(page_of, t & 63); };
     auto first_key = [&](int32_t t) __attribute__((always_inline)) { return tile_at(t) * kTileKeys; };
 
-    // Copy j of the wave's four of a tile: four keys twice, four values twice.  (Rows that no column
+    // Copy j of the wave's of a tile: four keys each in the first half, four values in the second.  (Rows that no column
     // sees are copies of the last that one may; tiles without a page, which nobody reads, are page 0's.)
     struct From {
         const uint16_t* page[2];  // of keys, of values
@@ -164,13 +167,13 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
     };
     const int32_t row0 = 4 * wave + (lane >> 4);
     const uint32_t stride[2] = {(uint32_t)p.token[0] * 2, (uint32_t)p.token[1] * 2};  // (below 2^26: a page's rows lie within 2^32 bytes)
-    // (rows 32 apart have the same chunks)
+    // (rows 16 and 32 apart have the same chunks)
     const uint32_t chunk[2] = {16u * ((lane & 15) ^ (row0 & 15)), 16u * ((lane & 15) ^ (4 * (row0 & 3)))};
     auto copy = [&](int32_t t, const From& f, auto which) __attribute__((always_inline)) {
-        constexpr int j = which.value, v = j / 2;
+        constexpr int HALF = COPIES / 2, j = which.value % HALF, v = which.value / HALF;
         PageTile& to = lds.tile[t % kBuffers];
-        const int32_t i = (j & 1) * kWaves + wave;
-        copy_from(f.page[v], (uint32_t)min(row0 + 32 * (j & 1), f.rows - 1) * stride[v] + chunk[v],
+        const int32_t i = j * kWaves + wave;
+        copy_from(f.page[v], (uint32_t)min(row0 + 4 * kWaves * j, f.rows - 1) * stride[v] + chunk[v],
                   lds_offset(v == 0 ? &to.key[4 * i][0] : &to.value[4 * i][0]));
     };
     auto copy_tile = [&](int32_t t, const From& f) __attribute__((always_inline)) {
@@ -178,13 +181,13 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
     };
 
     // B fragments of Q^T: column c.  The rows come through LDS (rows of 16 chunks of 16
-    // bytes end to end, XORed by the row, in the last two buffers): fragments read from
+    // bytes end to end, XORed by the row, in the later buffers): fragments read from
     // memory are 32 rows' lines for every one.
     Frag q[8];
     int32_t page0 = -1, page1 = -1, key0 = 0, key1 = 0;  // of this tile and the next
     {
-        uint8_t* const rows = &lds.tile[2].key[0][0] + wave * (kRows * 2 * kDim);
-        static_assert(kWaves * kRows * 2 * kDim == 2 * sizeof(PageTile), "queries in two buffers");
+        uint8_t* const rows = &lds.tile[kBuffers / 2].key[0][0] + wave * (kRows * 2 * kDim);
+        static_assert(kWaves * kRows * 2 * kDim == kBuffers / 2 * sizeof(PageTile), "queries in the later half of the buffers");
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int32_t r = 4 * j + (lane >> 4), chunk = (lane & 15) ^ (r & 15);
@@ -204,7 +207,7 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
 #pragma unroll
         for (int s = 0; s < 8; ++s) q[s].u = *reinterpret_cast<const u32x4*>(rows + 256 * c + 16 * ((2 * s + h) ^ (c & 15)));
         lds_barrier();
-        if (tiles > 0) copy_tile(1, from_page(key1, page1));
+        if (WAVES == 8 && tiles > 0) copy_tile(1, from_page(key1, page1));
     }
     f32x16 acc[4], s[2];
     Frag pf[4];
@@ -222,12 +225,12 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
     auto sees_all = [&](int32_t k0) __attribute__((always_inline)) {
         return (k0 >= most_lo && k0 + kTileKeys <= least_hi) || k0 + kTileKeys <= w.pre;
     };
-    // Sixteen products, of the last tile's values (which 0) or of this one's keys (1), each
-    // fragment read kAhead products before its own.  Scores: register i of half u is key
-    // 32u + 8 (i / 4) + 4h + i % 4.
-    auto multiply = [&](int32_t t, const From& f, auto which) __attribute__((always_inline)) {
+    // Sixteen products, of tile t's values (which 0) or keys (1), each fragment read kAhead
+    // products before its own; beside those of the keys the copies of tile `next`.  Scores:
+    // register i of half u is key 32u + 8 (i / 4) + 4h + i % 4.
+    auto multiply = [&](int32_t t, int32_t next, const From& f, auto which) __attribute__((always_inline)) {
         constexpr bool SCORES = which.value != 0;
-        const PageTile& tile = lds.tile[(SCORES ? t : t - 1) % kBuffers];
+        const PageTile& tile = lds.tile[t % kBuffers];
         Frag x[kAhead];
         auto fetch = [&](auto number) __attribute__((always_inline)) {
             constexpr int n = number.value;
@@ -251,7 +254,7 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
             if constexpr (!SCORES) acc[n % 4] = mfma32<T>(x[n % kAhead], pf[n / 4], acc[n % 4]);
             else s[n & 1] = mfma32<T>(x[n % kAhead], q[n / 2], s[n & 1]);
             if constexpr (n + kAhead < 16) fetch(Number<n + kAhead>{});
-            if constexpr (SCORES && n % 4 == 1) copy(t + 2, f, Number<n / 4>{});
+            if constexpr (SCORES && n % (16 / COPIES) == 1) copy(next, f, Number<n / (16 / COPIES)>{});
             __builtin_amdgcn_sched_barrier(0);
         });
     };
@@ -357,39 +360,62 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
                 acc[d][i] += (up[i] > 0.f ? __builtin_inff() : 0.f) - (down[i] > 0.f ? __builtin_inff() : 0.f);
         }
     };
-    // The two waves of a SIMD half a tile apart: one multiplies (the last tile's
-    // values, this one's keys) and asks for its copies of the tile after the next,
-    // whose buffer was read until two steps ago, while the other makes
-    // probabilities.  Steps are divided by barriers, every other one of them behind a
-    // wait for the copies of the tile whose keys come next.
-    const bool second = wave >= kWaves / 2;
-    auto sync = [&](bool landed) __attribute__((always_inline)) {
-        if (landed) wait_barrier<COPIES>();
-        else lds_barrier();
+    constexpr Number<0> of_values;
+    constexpr Number<1> of_keys;
+    auto values_of = [&](int32_t t, const From& f) __attribute__((always_inline)) {
+        if constexpr (CAREFUL) careful_products(t);
+        else multiply(t, 0, f, of_values);
     };
-    if (second) sync(true);
-    bool saw = false;
+    if constexpr (WAVES == 8) {
+        // The two waves of a SIMD half a tile apart: one multiplies (the last tile's
+        // values, this one's keys) and asks for its copies of the tile after the next,
+        // whose buffer was read until two steps ago, while the other makes
+        // probabilities.  Steps are divided by barriers, every other one of them behind a
+        // wait for the copies of the tile whose keys come next.
+        const bool second = wave >= kWaves / 2;
+        auto sync = [&](bool landed) __attribute__((always_inline)) {
+            if (landed) wait_barrier<COPIES>();
+            else lds_barrier();
+        };
+        if (second) sync(true);
+        bool saw = false;
 #pragma unroll 1
-    for (int32_t t = 0; t <= tiles; ++t) {
-        const bool now = t < tiles && sees(key0, page0);
-        const int32_t later = min(t + 2, tiles - 1);
-        if (((t + 2) & 63) == 0 && t + 2 < tiles) fetch_pages(t + 2);
-        const int32_t page2 = page_at(later), key2 = first_key(later);
-        const From f = from_page(key2, page2);
-        sync(!second);
-        // (one place for each: variants of both together cost copies of the sums between them)
-        if (saw) {
-            if constexpr (CAREFUL) careful_products(t - 1);
-            else multiply(t, f, Number<0>{});
+        for (int32_t t = 0; t <= tiles; ++t) {
+            const bool now = t < tiles && sees(key0, page0);
+            const int32_t later = min(t + 2, tiles - 1);
+            if (((t + 2) & 63) == 0 && t + 2 < tiles) fetch_pages(t + 2);
+            const int32_t page2 = page_at(later), key2 = first_key(later);
+            const From f = from_page(key2, page2);
+            sync(!second);
+            // (one place for each: variants of both together cost copies of the sums between them)
+            if (saw) values_of(t - 1, f);
+            if (now) multiply(t, t + 2, f, of_keys);
+            else if (t < tiles) copy_tile(t + 2, f);
+            sync(second);
+            if (now) softmax(key0);
+            saw = now;
+            key0 = key1, page0 = page1, key1 = key2, page1 = page2;
         }
-        if (now) multiply(t, f, Number<1>{});
-        else if (t < tiles) copy_tile(t + 2, f);
-        sync(second);
-        if (now) softmax(key0);
-        saw = now;
-        key0 = key1, page0 = page1, key1 = key2, page1 = page2;
+        if (!second) lds_barrier();
+    } else {
+        // A tile after the other; the CU's other work-group multiplies meanwhile.
+#pragma unroll 1
+        for (int32_t t = 0; t < tiles; ++t) {
+            const bool now = sees(key0, page0);
+            if (((t + 1) & 63) == 0 && t + 1 < tiles) fetch_pages(t + 1);
+            const int32_t later = min(t + 1, tiles - 1), page = page_at(later), key = first_key(later);
+            const From f = from_page(key, page);
+            wait_barrier<0>();  // (this tile is there, and nobody reads the last one)
+            if (now) {
+                multiply(t, t + 1, f, of_keys);
+                softmax(key0);
+                values_of(t, f);
+            } else {
+                copy_tile(t + 1, f);
+            }
+            key0 = key, page0 = page;
+        }
     }
-    if (!second) lds_barrier();
     wait_copies<0>();
     __syncthreads();  // the tiles' memory is free
     if constexpr (!CAREFUL) {
@@ -450,44 +476,49 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
 }
 
 // (A call, so that its registers are not the common form's.)
-template <class T, int MODE>
-__device__ __attribute__((noinline)) void careful_block(AttendParams p, BlocksLds* lds) {
+template <class T, int MODE, int WAVES>
+__device__ __attribute__((noinline)) void careful_block(AttendParams p, BlocksLds<WAVES>* lds) {
     BlocksWork work;
-    if (find_work(p, work)) blocks_part<T, MODE, true>(p, work, *lds);
+    if (find_work<WAVES>(p, work)) blocks_part<T, MODE, WAVES, true>(p, work, *lds);
 }
 
-template <class T, int MODE>
-__global__ __launch_bounds__(64 * kWaves, 2) void blocks_kernel(AttendParams p) {
+template <class T, int MODE, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void blocks_kernel(AttendParams p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
-    auto& lds = *reinterpret_cast<BlocksLds*>(lds_raw);
+    auto& lds = *reinterpret_cast<BlocksLds<WAVES>*>(lds_raw);
     BlocksWork work;
-    if (!find_work(p, work)) return;
+    if (!find_work<WAVES>(p, work)) return;
     // (the same for the work-group, and in scalar registers from here on)
     for (int32_t* x : {&work.request, &work.kv, &work.block, &work.part, &work.parts}) *x = __builtin_amdgcn_readfirstlane(*x);
     if (p.parents) find_tree(p, work.w, lds.tree);
-    if (__builtin_expect(blocks_part<T, MODE, false>(p, work, lds), 0)) careful_block<T, MODE>(p, &lds);
+    if (__builtin_expect(blocks_part<T, MODE, WAVES, false>(p, work, lds), 0)) careful_block<T, MODE, WAVES>(p, &lds);
 }
 
-template <class T, int MODE>
+template <class T, int MODE, int WAVES>
 int launch(const AttendParams& p, int64_t groups, hipStream_t st) {
     static OncePerDevice once;
-    const auto kernel = blocks_kernel<T, MODE>;
-    const int rc = allow_lds(once, reinterpret_cast<const void*>(kernel), sizeof(BlocksLds), "paged_attend: LDS");
+    const auto kernel = blocks_kernel<T, MODE, WAVES>;
+    const int rc = allow_lds(once, reinterpret_cast<const void*>(kernel), sizeof(BlocksLds<WAVES>), "paged_attend: LDS");
     if (rc != V1_OK) return rc;
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)groups), dim3(64 * kWaves), sizeof(BlocksLds), st, p);
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)groups), dim3(64 * WAVES), sizeof(BlocksLds<WAVES>), st, p);
     return V1_LAUNCHED("paged_attend: blocks");
 }
 
-template <class T>
+template <class T, int WAVES>
 int launch(int mode, const AttendParams& p, int64_t groups, hipStream_t st) {
-    return mode == kPlain ? launch<T, kPlain>(p, groups, st) : mode == kCapped ? launch<T, kCapped>(p, groups, st)
-         : mode == kBiased ? launch<T, kBiased>(p, groups, st) : launch<T, kBoth>(p, groups, st);
+    return mode == kPlain ? launch<T, kPlain, WAVES>(p, groups, st) : mode == kCapped ? launch<T, kCapped, WAVES>(p, groups, st)
+         : mode == kBiased ? launch<T, kBiased, WAVES>(p, groups, st) : launch<T, kBoth, WAVES>(p, groups, st);
+}
+
+template <class T>
+int launch(int columns, int mode, const AttendParams& p, int64_t groups, hipStream_t st) {
+    return columns == 4 * kRows ? launch<T, 4>(mode, p, groups, st) : launch<T, 8>(mode, p, groups, st);
 }
 
 }  // namespace
 
-int paged::launch_blocks(bool fp16, int mode, const AttendParams& p, int64_t groups, hipStream_t st) {
-    return fp16 ? launch<_Float16>(mode, p, groups, st) : launch<__bf16>(mode, p, groups, st);
+int paged::launch_blocks(bool fp16, int columns, int mode, const AttendParams& p, int64_t groups, hipStream_t st) {
+    return fp16 ? launch<_Float16>(columns, mode, p, groups, st) : launch<__bf16>(columns, mode, p, groups, st);
 }
 
 }  // namespace v1

@@ -458,6 +458,11 @@ inline int32_t reach_of(int32_t window, int32_t max_q) {
     return window > 0 ? (int32_t)std::min<int64_t>((int64_t)window + max_q + kTileKeys, INT32_MAX) : 0;
 }
 
+// Whether work-groups of 128 columns are better than ones of 256, of which there would be `groups` without parts, over at
+// most `tiles` tiles of keys.  Two of them share a CU, so that one's first and last steps pass beside the other's products;
+// those of 256 have the longer turns of products and exponentials.
+inline bool small_blocks(int64_t groups, int64_t tiles) { return groups < device_cus() / 2 || (tiles <= 128 && groups <= 4 * device_cus()); }
+
 struct Shape {
     int32_t cols, blocks, together, reach;  // cols: of a block; 256: the kernel of many queries
     int32_t slots, units, xcds;
@@ -473,7 +478,8 @@ inline Shape shape_of(const int32_t* lens, int32_t tokens, int32_t requests, int
     s.reach = reach_of(window, max_q);
     const int64_t columns = (int64_t)max_q * group;
     const bool few = columns <= kFewColumns;
-    s.cols = !few ? kBlockColumns : columns <= 16 ? 16 : 32;
+    const bool small = !few && small_blocks(requests * cdiv(columns, kBlockColumns) * kv_heads, cdiv(s.reach > 0 ? std::min(keys, s.reach) : keys, kTileKeys));
+    s.cols = !few ? (small ? kSmallBlockColumns : kBlockColumns) : columns <= 16 ? 16 : 32;
     s.blocks = (int32_t)cdiv(columns, s.cols);
     s.together = !few ? 1 : kv_heads % 4 == 0 ? 4 : kv_heads % 2 == 0 ? 2 : 1;
     s.slots = s.units = 0, s.xcds = 1;
@@ -543,10 +549,10 @@ int launch_rows(int mode, const AttendParams& p, int64_t groups, hipStream_t st)
 template <class T>
 int attend(AttendParams& p, const Shape& s, int mode, hipStream_t st) {
     int rc;
-    if (s.cols == kBlockColumns) {
+    if (s.cols >= kSmallBlockColumns) {
         const int64_t groups = cdiv(s.items * p.kv_heads, s.xcds) * s.xcds * s.blocks;
         V1_REQUIRE(launchable(groups, 512) && s.items * p.kv_heads <= INT32_MAX, "paged_attend: too many requests, queries and heads for a launch");
-        rc = launch_blocks(__is_same(T, _Float16), mode, p, groups, st);
+        rc = launch_blocks(__is_same(T, _Float16), s.cols, mode, p, groups, st);
     } else {
         const int64_t sets = (int64_t)p.kv_heads / s.together * s.blocks;
         const int64_t spread = s.plan.chunk > 0 ? cdiv(s.items * sets, 8) : cdiv(s.items, 8) * sets;
