@@ -489,11 +489,11 @@ inline Shape shape_of(const int32_t* lens, int32_t tokens, int32_t requests, int
     // Parts at most, and tiles of a part at least.  Few queries: as many as run at once; where the requests alone are half that
     // many, two for each of the longer ones, unless a window makes them alike: 130 requests of 1000 to 20000 tokens, 32 heads
     // of 8 KV heads, 1013 us in one part each and 625 so; 250 of 8000, 4 KV heads, 685 and 694; 128 of 500, which parts of
-    // less than 32 tiles would cut, 46 and 59.  Many queries: enough for two work-groups a CU (32 trees of 64 drafts over
-    // 4K-64K tokens 1110 us, three a CU 1056, four 1085; 8 such trees 282, 303, 313), or for twice the requests where that is
+    // less than 32 tiles would cut, 46 and 59.  Many queries: enough for two work-groups of 256 columns a CU (32 trees of 64 drafts over
+    // 4K-64K tokens 1110 us, three a CU 1056, four 1085; 8 such trees 282, 303, 313), or for twice several requests where that is
     // four a CU or less (8 chunks of 512 behind 1000 to 32000 tokens, 32 heads: 1250 us in one part each, 706 so).
     const bool crowded = few && 2ll * requests > running;
-    const int64_t most = !few ? std::max<int64_t>({1, 2 * device_cus() / sets, std::min<int64_t>(4 * device_cus() / sets, 2ll * requests)})
+    const int64_t most = !few ? std::max<int64_t>({1, 2 * device_cus() / sets, requests > 1 ? std::min<int64_t>(4 * device_cus() / sets, 2ll * requests) : 0})
                        : crowded && s.reach == 0 ? std::max<int64_t>(running, std::min<int64_t>(4 * running, 2ll * requests)) : running;
     s.plan = Plan{lens, requests, keys, 0, 0, (int32_t)most, !few ? 4 : crowded ? (int32_t)(32 * streams) : 1};
     // (a request of few tiles is one work-group's: the join would take longer than its tiles)
