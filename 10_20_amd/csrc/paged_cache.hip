@@ -14,6 +14,11 @@ using namespace paged;
 // time; the table's row of the token's angles is loaded once for all of them.  Pairs
 // (d, d + R/2) meet through a lane permute, neighbours lie in one lane.  Products and
 // sums are fp32, rounded to the row's type once.
+//
+// Bound by memory, or by the call: 14 thousand tokens of 32 query and 8 KV heads 70 us, 367
+// MB at 5.2 TB/s, a copy's rate (78 with loads that leave the tokens, which nobody reads
+// again, in the caches; two, three and six rows in flight 1 us or 3 more).  128 requests of a
+// token 4.8 us, a wave for every four rows: offsets, start, page entry one after the other.
 struct AppendParams {
     const uint16_t* x[3];  // q, k, v
     int64_t x_token[3], x_head[3];
@@ -73,7 +78,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendParams p) {
             const int32_t w = row < p.heads ? 0 : row < p.heads + p.kv_heads ? 1 : 2;
             const int32_t h = row - (w == 0 ? 0 : w == 1 ? p.heads : p.heads + p.kv_heads);
             x[i] = u32x4{0, 0, 0, 0};
-            if (row < rows) x[i] = *reinterpret_cast<const u32x4*>(p.x[w] + t * p.x_token[w] + h * p.x_head[w] + 8 * ch);
+            if (row < rows) x[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p.x[w] + t * p.x_token[w] + h * p.x_head[w] + 8 * ch));
         }
 #pragma unroll
         for (int i = 0; i < kRowsAhead; ++i) {
@@ -109,7 +114,8 @@ __global__ __launch_bounds__(256) void append_kernel(AppendParams p) {
 // -------------------------------------------------------------------- keep
 // A work-group moves a request's rows of one head of K or V, 64 rows at a time: all of
 // them are read before any is written.  A row comes from its own index or a later one,
-// so that the next 64 were not written to by those before them.
+// so that the next 64 were not written to by those before them.  Bound by latency, five
+// dependent loads: 8 requests of five rows and a head 3.2 us, 128 of nine and 8 heads 4.9.
 struct KeepParams {
     uint16_t* pool[2];
     int64_t page[2], token[2], head[2];
