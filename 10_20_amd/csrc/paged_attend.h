@@ -278,8 +278,8 @@ __device__ __forceinline__ float capped(float t, float cap2) {
 
 // capped(d scale / cap) - sub of a tile's scores: where all of them are small, as those of
 // a model trained with a cap far above them are, by the shorter of two polynomials in
-// d^2, whose coefficients have the scale and the cap in them.  (4096 queries over 32K
-// keys, a cap of 50: 1.7 us a tile of 256 columns of `capped` alone, 1.2 so.)
+// d^2, whose coefficients have the scale and the cap in them: five operations a score
+// where `capped` takes fifteen and two of the quarter-rate ones.
 // `far`: the largest |d| of the lane's; each(f): d := f(d) for all of them.
 template <class Each>
 __device__ __forceinline__ void cap_scores(const Cap& cap, float cap_in, float cap2, float far, Each each) {

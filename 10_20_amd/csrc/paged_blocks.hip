@@ -1,5 +1,31 @@
-// Attention of many queries of each request over K / V pages of 16-bit numbers (the
-// same sums as those of few queries, with the keys' tiles shared by 256 columns).
+// Attention of many queries of each request over K / V pages of 16-bit numbers: the
+// sums of paged_rows.hip, with the tiles of keys shared by the waves of a work-group.
+//
+// A work-group takes 256 columns (queries times the heads of a KV head, so that heads
+// that share keys share their tiles too) or 128, a wave 32 of them, as columns of
+// v_mfma_f32_32x32x16:
+//   scores  S^T = K Q^T, a page of 64 keys at a time from LDS;
+//   output  O^T = V^T P^T: a lane's scores are already the probabilities of its B
+//           fragment (the key order inside 16 keys is chosen so), rounded to the pages'
+//           type once, half a step of each, as the output is (1.3-1.4 times the error of a
+//           rounded exact result; a second number for the rest would be 16 products
+//           more beside a tile's 32); values come transposed from LDS.
+// Scores, maxima and sums are fp32, exponentials base 2.  Rows are laid with their
+// 16-byte chunks XORed by the row so that the fragments' reads meet different banks.
+// Tiles are those that some column of the block sees: the prefix's pages, then from the
+// first key of the window or document on.
+//
+// Bound by vector issue where scores are capped, by products and their fragments else:
+// 4096 queries of 32 heads, 8 KV heads, over 32768 keys, us (TFLOP/s):
+//   plain 1835-1900 (1124-1085; an 8192^3 library product 1404 on the same card), a cap
+//   of 50 2200-2270, distances 1930-2050, both 2570-2650, a cap of 2 (scores past it) 3590.
+//   Matrix units are busy 40% of the time, vector units 58%, of a capped tile; the matrix part of
+//   a step alone takes 796 ns of 973, the vector part 610 and, capped, 1080.
+// On the way there (capped): fragments' reads left to the compiler, which waits for each
+// one, 2657; copies whose addresses are made between the products 2700; capped scores by
+// one polynomial of degree 5 2690, by the shorter where they are small 2394, and maxima
+// looked for only where the largest magnitude may pass the subtracted one 2205.  Keys from
+// the last one back where distances count, so that the first maximum stays: 2350 -> 2050.
 #include "paged_attend.h"
 
 namespace v1 {

@@ -1,7 +1,31 @@
 // Attention of a few queries of each request over K / V pages of 16-bit numbers:
 //   S[m, j] = scale q_m . k_j, capped and biased, O[m] = sum_j softmax_j(S[m, :]) v_j
-// for the columns m of a request (its queries times the heads of a KV head) and the
-// keys j that column m sees.
+// for the columns m of a request (its queries times the heads of a KV head), at most 32
+// of them, and the keys j that column m sees; and the host's side of both kernels.
+//
+// A work-group attends one, two or four KV heads of a request over one part of its
+// pages, a wave each; waves of one head take the part's pages in turn, each with its own
+// running maximum, and join through LDS.  A page is a tile of 64 keys.
+//   scores  S^T = K Q^T (v_mfma_f32_16x16x32): keys come straight into registers, 64
+//           bytes of 16 rows an instruction; column c of a fragment is column c of 16.
+//   output  O^T = V^T P^T: values go memory -> LDS and come back transposed
+//           (ds_read_b64_tr_b16); the lane's own scores are its B fragment's
+//           probabilities, each in two numbers of the pages' type, so that the output's
+//           rounding is all that is left (error against 64 bits 1.0 times a rounded exact
+//           result's).
+// Whether a tile is seen whole is known for the wave; else each column's 64 bits of it
+// are made once.  A masked key's probability is zero, which an infinite or NaN value
+// would turn into NaN: sums that end up not finite are found again by a careful form
+// (CAREFUL), which counts the infinities that each column sees.
+//
+// Bound by memory: 48 contexts of 4096 to 65536 tokens, 4 KV heads of 8 query heads,
+// 383 us for 2.18 GB, 5.7 TB/s (a copy of 512 MiB moves 5.3); 128 requests of which a
+// window leaves 4096 tokens, 8 KV heads, 316 us for 1.8 GB.  Few keys are bound by latency: 8
+// requests of 1500 to 16384 tokens, one KV head, 10.5 us and 4.5 for the join, of which a
+// work-group's own chain is lengths and plan 1.6, table and keys 2.7, a tile 1.5, the
+// join of its waves 1.8.
+// Loads of keys that pass the caches gain 5% at 2 GB (363 us) and lose 5-13% where the
+// keys fit the last cache (128 contexts of 45 to 500 tokens, 8 KV heads, 32 and 37 us).
 #include "paged_attend.h"
 
 namespace v1 {
@@ -458,9 +482,16 @@ inline int32_t reach_of(int32_t window, int32_t max_q) {
     return window > 0 ? (int32_t)std::min<int64_t>((int64_t)window + max_q + kTileKeys, INT32_MAX) : 0;
 }
 
-// Whether work-groups of 128 columns are better than ones of 256, of which there would be `groups` without parts, over at
-// most `tiles` tiles of keys.  Two of them share a CU, so that one's first and last steps pass beside the other's products;
-// those of 256 have the longer turns of products and exponentials.
+// Whether work-groups of 128 columns are better than ones of 256, of which there would
+// be `groups` without parts, over at most `tiles` tiles of keys.  Two of them share a CU,
+// so that one's first and last steps (12 us of a work-group) pass beside the other's
+// products; those of 256 read the keys half as often and overlap products and
+// exponentials by their turns.  256 and 128 columns, us:
+//   four prompts of 1193-3434, 16 heads, distances  188, 160    nine of 1-1500, 16 heads        26, 21
+//   one of 4096, 32 heads, 8 KV heads               198, 163    16 of 300, the same heads       63, 48
+//   8 chunks of 500 behind 4000, the same           327, 290    8 trees of 16 drafts, 4 heads   28, 24
+//   32 chunks of 64 behind 4000, the same           189, 210    four prompts of 4096, 32 heads 597, 627
+//   4096 queries over 32768 keys, the same         1856, 1945   32 trees of 64, 32 heads      1090, 1139
 inline bool small_blocks(int64_t groups, int64_t tiles) { return groups < device_cus() / 2 || (tiles <= 128 && groups <= 4 * device_cus()); }
 
 struct Shape {
@@ -470,7 +501,10 @@ struct Shape {
     Plan plan;
 };
 
-constexpr int kFewColumns = 32;  // the most that the kernel of few queries takes
+// The most columns that the kernel of few queries takes.  64 of them in two blocks of 32 (in one block of 64 a wave's
+// registers spill: 8 trees of 16 drafts, 4 heads, 33 us in place of 24) and by the kernel of many queries: 32 trees of 8 drafts, 8 heads a
+// KV head, 379 and 354 us; 128 trees of 16 drafts, 4 heads a KV head, 412 and 303; 8 trees of 16, 26.6 and 24.
+constexpr int kFewColumns = 32;
 
 inline Shape shape_of(const int32_t* lens, int32_t tokens, int32_t requests, int32_t kv_heads, int32_t group, int32_t max_q, int32_t keys,
                       int32_t window) {
