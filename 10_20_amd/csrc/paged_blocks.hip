@@ -17,10 +17,10 @@
 //
 // Bound by vector issue where scores are capped, by products and their fragments else:
 // 4096 queries of 32 heads, 8 KV heads, over 32768 keys, us (TFLOP/s):
-//   plain 1835-1900 (1124-1085; an 8192^3 library product 1404 on the same card), a cap
-//   of 50 2200-2270, distances 1930-2050, both 2570-2650, a cap of 2 (scores past it) 3590.
-//   Matrix units are busy 40% of the time, vector units 58%, of a capped tile; the matrix part of
-//   a step alone takes 796 ns of 973, the vector part 610 and, capped, 1080.
+//   plain 1813-1900 (1137-1085; an 8192^3 library product 1404 on such a card), a cap of 50
+//   2173-2270, distances 1887-2050, both 2570-2650, a cap of 2 (scores past it) 3590.
+//   Matrix units are busy 40% of the time and vector units 58% when capped; without
+//   probabilities a copy takes 1614, without products 1251 plain and 1761 capped.
 // On the way there (capped): fragments' reads left to the compiler, which waits for each
 // one, 2657; copies whose addresses are made between the products 2700; capped scores by
 // one polynomial of degree 5 2690, by the shorter where they are small 2394, and maxima

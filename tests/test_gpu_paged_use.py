@@ -151,11 +151,12 @@ def test_captured_steps_with_lengths_that_change(drafts, group):
 def test_two_graphs_replayed_side_by_side():
     """Their workspaces are their own."""
     g = gen(32)
-    graphs, outs, wants = [], [], []
+    graphs, outs, wants, inputs = [], [], [], []
     for i in range(2):
         (kp, vp), table = make(g, [3000 + 500 * i, 100], 1, BF16)
         q = torch.randn((2, 8, 128), device=DEV, generator=g).to(BF16)
         lens = i32([3000 + 500 * i, 100])
+        inputs.append((q, kp, vp, table, lens))  # (a graph reads them where they were: they stay for its replays)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             outs.append(PG.attend(q, kp, vp, table, lens))
@@ -318,3 +319,25 @@ def test_the_same_bits_again():
         want = call()
         for _ in range(5):
             assert all(torch.equal(a, b) for a, b in zip(call(), want))
+
+
+@gpu
+@pytest.mark.parametrize("nq,group", [(1, 4), (90, 2)])
+def test_subnormal_numbers(nq, group):
+    """fp16 keys and values below its normal numbers: the products keep them (an output is then off by half of
+    the smallest number, 2^-25, beside the bound)."""
+    g, n = gen(55), 300
+    (kp, vp), table = make(g, [n], 1, F16)
+    for pool, by in ((kp, 2.0 ** -18), (vp, 2.0 ** -20)):
+        pool.copy_(pool.float() * by)
+    q = torch.randn((nq, group, 128), device=DEV, generator=g).to(F16)
+    out, lse = PG.attend(q, kp, vp, table, i32([n]), offsets([nq]), softmax_scale=2.0 ** 14, return_lse=True)
+    k, v = rows_of(kp, table[0], n).double(), rows_of(vp, table[0], n).double()
+    seen, _ = seen_and_distance(nq, n)
+    s = 2.0 ** 14 * torch.einsum("qhd,kd->qhk", q.double(), k[:, 0]).masked_fill(~seen[:, None], -math.inf)
+    d = (128 + 8) * 2.0 ** -24 * 2.0 ** 14 * torch.einsum("qhd,kd->qhk", q.double().abs(), k[:, 0].abs()).amax(-1)
+    want_lse = torch.logsumexp(s, -1)
+    p = torch.exp(s - want_lse[..., None])
+    want, mag, u = p @ v[:, 0], p @ v[:, 0].abs(), 2.0 ** -11
+    assert bool(((out.double() - want).abs() <= u * (want.abs() + mag) * (1 + u) + 2 * d[..., None] * mag + 2.0 ** -25 + n * 2.0 ** -31 * v.abs().amax()).all())
+    assert bool(((lse.double() - want_lse).abs() <= d + 2.0 ** -21 * (1 + want_lse.abs() + s.masked_fill(~seen[:, None], 0).abs().amax(-1))).all())
