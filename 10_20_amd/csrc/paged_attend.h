@@ -31,14 +31,15 @@ __device__ __forceinline__ f32x4 mfma16(const Frag& a, const Frag& b, f32x4 c) {
     }
 }
 
-// tanh(t) / t in t^2 for |t| up to 0.33 and up to 0.75, and the same polynomials of
+// tanh(t) / t in t^2 for |t| up to 0.16, 0.33 and 0.75, and the same polynomials of
 // cap log2(e) tanh(d scale / cap) / d in d^2 for |d| up to so much.
+constexpr float kCapLeast[3] = {0.9999999721658054f, -0.3333137411469761f, 0.1312851958668552f}, kCapLeastMost = 0.16f;
 constexpr float kCapNear[4] = {0.9999999780542091f, -0.3333268647142513f, 0.1330338186573907f, -0.04948183016008989f}, kCapNearMost = 0.33f;
 constexpr float kCapFar[6] = {0.9999999710131235f, -0.33332958872695295f, 0.13325405922016131f, -0.053344425407917576f,
                               0.019582898606222813f, -0.0047162504597644895f}, kCapFarMost = 0.75f;
 struct Cap {
-    float near[4], far[6];
-    float near_most, far_most;
+    float least[3], near[4], far[6];
+    float least_most, near_most, far_most;
 };
 
 inline Cap cap_of(float scale, float softcap) {
@@ -47,11 +48,13 @@ inline Cap cap_of(float scale, float softcap) {
     const double in = (double)scale / softcap;
     double by = (double)scale * kLog2e;
     for (int i = 0; i < 6; ++i, by *= in * in) {
+        if (i < 3) c.least[i] = (float)(kCapLeast[i] * by);
         if (i < 4) c.near[i] = (float)(kCapNear[i] * by);
         c.far[i] = (float)(kCapFar[i] * by);
     }
-    // (a cap so far from the scale that the coefficients would not be normal numbers: neither polynomial)
+    // (a cap so far from the scale that the coefficients would not be normal numbers: no polynomial)
     const bool normal = in >= 0x1p-12 && in <= 0x1p12;
+    c.least_most = normal ? (float)(kCapLeastMost / in) : -1.f;
     c.near_most = normal ? (float)(kCapNearMost / in) : -1.f, c.far_most = normal ? (float)(kCapFarMost / in) : -1.f;
     return c;
 }
@@ -277,13 +280,18 @@ __device__ __forceinline__ float capped(float t, float cap2) {
 }
 
 // capped(d scale / cap) - sub of a tile's scores: where all of them are small, as those of
-// a model trained with a cap far above them are, by the shorter of two polynomials in
-// d^2, whose coefficients have the scale and the cap in them: five operations a score
+// a model trained with a cap far above them are, by the shortest of three polynomials in
+// d^2, whose coefficients have the scale and the cap in them: four operations a score
 // where `capped` takes fifteen and two of the quarter-rate ones.
 // `far`: the largest |d| of the lane's; each(f): d := f(d) for all of them.
 template <class Each>
 __device__ __forceinline__ void cap_scores(const Cap& cap, float cap_in, float cap2, float far, Each each) {
-    if (__ballot(far > cap.near_most) == 0) {
+    if (__ballot(far > cap.least_most) == 0) {
+        each([&](float d, float sub) __attribute__((always_inline)) {
+            const float z = d * d;
+            return fmaf(d, fmaf(fmaf(cap.least[2], z, cap.least[1]), z, cap.least[0]), -sub);
+        });
+    } else if (__ballot(far > cap.near_most) == 0) {
         each([&](float d, float sub) __attribute__((always_inline)) {
             const float z = d * d;
             return fmaf(d, fmaf(fmaf(fmaf(cap.near[3], z, cap.near[2]), z, cap.near[1]), z, cap.near[0]), -sub);

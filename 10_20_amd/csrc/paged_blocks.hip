@@ -293,7 +293,7 @@ __device__ __forceinline__ bool blocks_part(const AttendParams& p, const BlocksW
     Cap cap = p.cap;
     if constexpr (MODE == kCapped) {  // (in registers of the loop's own: there are too few scalar ones)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(cap.near[i]));
+        for (int i = 0; i < 3; ++i) asm volatile("" : "+v"(cap.least[i]));
     }
     uint64_t seen = ~0ull;  // bit 32u + 8 a + i: key 32u + 8a + 4h + i of the tile in `pf`
     auto softmax = [&](int32_t k0) __attribute__((always_inline)) {
