@@ -18,14 +18,14 @@
 // Bound by vector issue where scores are capped, by products and their fragments else:
 // 4096 queries of 32 heads, 8 KV heads, over 32768 keys, us (TFLOP/s):
 //   plain 1813-1900 (1137-1085; an 8192^3 library product 1404 on such a card), a cap of 50
-//   2173-2270, distances 1887-2050, both 2570-2650, a cap of 2 (scores past it) 3590.
+//   2148-2230, distances 1887-2050, both 2470-2570, a cap of 2 (scores past it) 3590.
 //   Matrix units are busy 40% of the time and vector units 58% when capped; without
-//   probabilities a copy takes 1614, without products 1251 plain and 1761 capped.
+//   probabilities a copy takes 1614, without products 1251 plain and 1761 capped (with the polynomial of three steps).
 // On the way there (capped): fragments' reads left to the compiler, which waits for each
 // one, 2657; copies whose addresses are made between the products 2700; capped scores by
 // one polynomial of degree 5 2690, by the shorter where they are small 2394, and maxima
-// looked for only where the largest magnitude may pass the subtracted one 2205.  Keys from
-// the last one back where distances count, so that the first maximum stays: 2350 -> 2050.
+// looked for only where the largest magnitude may pass the subtracted one 2205; by a
+// still shorter one below 0.16 of the cap 2148.  Keys from the last one back where distances count, so that the first maximum stays: 2350 -> 2050.
 #include "paged_attend.h"
 
 namespace v1 {
