@@ -25,7 +25,8 @@
 // one, 2657; copies whose addresses are made between the products 2700; capped scores by
 // one polynomial of degree 5 2690, by the shorter where they are small 2394, and maxima
 // looked for only where the largest magnitude may pass the subtracted one 2205; by a
-// still shorter one below 0.16 of the cap 2148.  Keys from the last one back where distances count, so that the first maximum stays: 2350 -> 2050.
+// still shorter one below 0.16 of the cap 2148.  Keys from the last one back where
+// distances count, so that the first maximum stays: 2350 -> 2050.
 #include "paged_attend.h"
 
 namespace v1 {

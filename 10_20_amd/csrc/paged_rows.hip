@@ -492,7 +492,7 @@ inline int32_t reach_of(int32_t window, int32_t max_q) {
 //   8 chunks of 500 behind 4000, the same           327, 290    8 trees of 16 drafts, 4 heads   28, 24
 //   32 chunks of 64 behind 4000, the same           189, 210    four prompts of 4096, 32 heads 597, 627
 //   4096 queries over 32768 keys, the same         1856, 1945   32 trees of 64, 32 heads      1090, 1139
-inline bool small_blocks(int64_t groups, int64_t tiles) { return groups < device_cus() / 2 || (tiles <= 128 && groups <= 4 * device_cus()); }
+inline bool small_blocks(double groups, int64_t tiles) { return groups < device_cus() / 2 || (tiles <= 128 && groups <= 4 * device_cus()); }
 
 struct Shape {
     int32_t cols, blocks, together, reach;  // cols: of a block; 256: the kernel of many queries
@@ -505,6 +505,7 @@ struct Shape {
 // registers spill: 8 trees of 16 drafts, 4 heads, 33 us in place of 24) and by the kernel of many queries: 32 trees of 8 drafts, 8 heads a
 // KV head, 379 and 354 us; 128 trees of 16 drafts, 4 heads a KV head, 412 and 303; 8 trees of 16, 26.6 and 24.
 constexpr int kFewColumns = 32;
+constexpr int32_t kMostRequests = 1 << 24;  // (so many and one head are past the grid of either kernel)
 
 inline Shape shape_of(const int32_t* lens, int32_t tokens, int32_t requests, int32_t kv_heads, int32_t group, int32_t max_q, int32_t keys,
                       int32_t window) {
@@ -512,7 +513,8 @@ inline Shape shape_of(const int32_t* lens, int32_t tokens, int32_t requests, int
     s.reach = reach_of(window, max_q);
     const int64_t columns = (int64_t)max_q * group;
     const bool few = columns <= kFewColumns;
-    const bool small = !few && small_blocks(requests * cdiv(columns, kBlockColumns) * kv_heads, cdiv(s.reach > 0 ? std::min(keys, s.reach) : keys, kTileKeys));
+    const double groups = (double)requests * cdiv(columns, kBlockColumns) * kv_heads;  // (the largest sizes: past 64 bits)
+    const bool small = !few && small_blocks(groups, cdiv(s.reach > 0 ? std::min(keys, s.reach) : keys, kTileKeys));
     s.cols = !few ? (small ? kSmallBlockColumns : kBlockColumns) : columns <= 16 ? 16 : 32;
     s.blocks = (int32_t)cdiv(columns, s.cols);
     s.together = !few ? 1 : kv_heads % 4 == 0 ? 4 : kv_heads % 2 == 0 ? 2 : 1;
@@ -540,7 +542,7 @@ inline Shape shape_of(const int32_t* lens, int32_t tokens, int32_t requests, int
         // Every request gets as many blocks as the longest can have, unless the blocks that the queries can need are
         // less than a third of those.
         const int64_t slots = (int64_t)tokens * group / s.cols + requests;
-        if (max_q > 1 && ((int64_t)requests * s.blocks > 3 * slots || !launchable(((int64_t)s.items * kv_heads + 7) * s.blocks, 512))) {
+        if (max_q > 1 && ((int64_t)requests * s.blocks > 3 * slots || (double)(s.items * kv_heads + 7) * s.blocks >= 0x1p32 / 512)) {
             s.slots = (int32_t)slots, s.blocks = 1, s.items = slots;
             s.plan.chunk = (int32_t)std::max<int64_t>(1, tiles);
         }
@@ -608,6 +610,9 @@ using namespace v1;
 extern "C" int64_t v1_paged_attend_workspace(int32_t tokens, int32_t requests, int32_t kv_heads, int32_t group, int32_t max_q,
                                              int32_t keys, int32_t window) {
     if (tokens <= 0 || requests <= 0 || kv_heads <= 0 || group <= 0 || max_q <= 0 || keys <= 0) return 0;
+    if ((int64_t)kv_heads * group >= 1 << 15 || (int64_t)tokens * group > kMostKeys || keys > kMostKeys || requests >= kMostRequests)
+        return 0;  // (refused by the entry)
+    max_q = std::min(max_q, tokens);
     return workspace_of(shape_of(nullptr, tokens, requests, kv_heads, group, max_q, keys, window), kv_heads);
 }
 
@@ -616,11 +621,12 @@ extern "C" int v1_paged_attend(const v1_paged_attend_args* a, void* stream) {
     auto [q, q_token, q_head, k_pool, kp_page, kp_token, kp_head, v_pool, vp_page, vp_token, vp_head, pages, table,
           table_stride, lens, cu_q, prefix, document, parents, slopes, out, o_token, o_head, lse, workspace,
           workspace_bytes, table_len, tokens, requests, max_q, kv_heads, group, window, fp16, scale, softcap] = *a;
-    if (!cu_q) max_q = 1;
+    max_q = cu_q ? std::min(max_q, tokens) : 1;
     V1_REQUIRE(tokens >= 0 && requests >= 0 && max_q >= 0 && kv_heads > 0 && group > 0 && pages >= 0 && table_len >= 0 &&
                    window >= 0 && (int64_t)kv_heads * group < 1 << 15,
                "paged_attend: bad shape");
     V1_REQUIRE((int64_t)table_len * kTileKeys <= kMostKeys && (int64_t)tokens * group <= kMostKeys, "paged_attend: too many keys or queries");
+    V1_REQUIRE(requests < kMostRequests, "paged_attend: too many requests for a launch");
     V1_REQUIRE(cu_q != nullptr || tokens == requests, "paged_attend: one query for each request");
     V1_REQUIRE(parents == nullptr || (max_q <= kMostDrafts && document == nullptr && prefix == nullptr),
                "paged_attend: at most %d drafted tokens of a request", kMostDrafts);

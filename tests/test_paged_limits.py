@@ -50,6 +50,8 @@ def refused(name, **fields):
     ("v1_paged_attend", ATTEND, dict(tl=1 << 25), "too many keys"), ("v1_paged_attend", ATTEND, dict(tokens=1 << 30, group=4), "too many keys"),
     ("v1_paged_attend", ATTEND, dict(cu=0), "one query"), ("v1_paged_attend", ATTEND, dict(parents=256, max_q=257, tokens=300), "256 drafted"),
     ("v1_paged_attend", ATTEND, dict(parents=256, prefix=256), "drafted"), ("v1_paged_attend", ATTEND, dict(parents=256, document=256), "drafted"),
+    ("v1_paged_attend", ATTEND, dict(tokens=(1 << 31) - 5000, group=1, requests=(1 << 31) - 1, max_q=(1 << 31) - 1, qh=128), "for a launch"),
+    ("v1_paged_attend", ATTEND, dict(tokens=1 << 24, requests=1 << 24, cu=0, kv_heads=64, group=8), "for a launch"),
     ("v1_paged_attend", ATTEND, dict(tl=1000, requests=3), "workspace"),
     ("v1_paged_attend", ATTEND, dict(tl=1000, requests=3, max_q=100, tokens=300), "workspace")])
 def test_refused_by_the_library(name, base, change, text):
@@ -67,6 +69,12 @@ def test_workspace_is_host_arithmetic():
     for sizes in ((0, 0, 1, 1, 1, 64, 0), (5, 5, 1, 4, 1, 0, 0), (5, 5, 1, 4, 1, 64, 0)):
         assert h.v1_paged_attend_workspace(*sizes) == 0, sizes
     assert h.v1_paged_attend_workspace(8, 8, 1, 4, 1, 16384, 0) >= 8 * 16 * 130 * 4
+    # sizes that the entry refuses, and a max_q past the tokens
+    most = (1 << 31) - 1
+    for sizes in ((most, 1, 1, 2, most, 64, 0), (5, 5, 1, 1 << 15, 5, 64, 0), (5, 5, 1 << 14, 2, 5, 64, 0), (5, 5, 1, 4, 5, most, 0)):
+        assert h.v1_paged_attend_workspace(*sizes) == 0, sizes
+    assert h.v1_paged_attend_workspace(100, 3, 1, 4, most, 16384, 0) == h.v1_paged_attend_workspace(100, 3, 1, 4, 100, 16384, 0) > 0
+    assert h.v1_paged_attend_workspace(most // 2, most, 1, 1, most, 64, 0) == 0  # (a grid that no launch holds)
     # a window leaves a few tiles of a long context
     assert h.v1_paged_attend_workspace(8, 8, 1, 4, 1, 1 << 20, 100) == 0
 
