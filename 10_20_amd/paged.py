@@ -109,8 +109,9 @@ def append(q, k, v, k_pool, v_pool, table, starts, cu_tokens, rotations, positio
 
     x, y -> x cos - y sin, y cos + x sin in fp32, rounded once.  Tokens outside the
     requests, or whose row of `rotations` is not there, are skipped: neither stored
-    nor written to `out`.  Positions below zero or past the table and pages outside
-    the pool are not written to.  Two tokens of a call have positions of their own."""
+    nor written to `out`.  A request that starts below zero is not stored, none of its
+    tokens, and positions past the table and pages outside the pool are not written to.
+    Two tokens of a call have positions of their own."""
     _lib.require_gpu(q, k, v, k_pool, v_pool, table, starts, cu_tokens, rotations, positions, out)
     dtype, pages, kv_heads, pools = _pools(k_pool, v_pool)
     ks = _rows("k", k, dtype, None, kv_heads)
@@ -146,9 +147,9 @@ def keep(k_pool, v_pool, table, starts, ids, cu_ids):
     """Moves rows of K and V within requests: position starts[r] + i takes what position
     starts[r] + ids[cu_ids[r] + i] held before the call, for i < cu_ids[r + 1] - cu_ids[r].
     The ids of a request ascend (accepted drafts, numbered from the first one behind
-    the context): each is at least its own index, others are not moved.  Positions
-    below zero or past the table and pages outside the pool are skipped; pages that
-    rows move in belong to one request.
+    the context): each is at least its own index, others are not moved.  Requests that
+    start below zero, positions past the table and pages outside the pool are skipped;
+    pages that rows move in belong to one request.
 
     table: [requests, entries] int32, starts: [requests], ids: [count], cu_ids:
     [requests + 1] int32."""

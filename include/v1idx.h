@@ -745,8 +745,9 @@ int64_t v1_kv8_attend_workspace(int32_t rows, int32_t kv_heads, int32_t group, i
  * angle's rotated / 2 pairs; pair i is numbers i and i + rotated / 2, or
  * (interleaved) 2i and 2i + 1; numbers from `rotated` (16, 32, .. 128) on are
  * copied.  A token's angle is its position, or positions[t] (NULL: none).  Tokens of
- * no request or with an angle outside the table are skipped; positions below zero or
- * past the table and pages outside the pool are not written to.
+ * no request or with an angle outside the table are skipped; a request with a start
+ * below zero is not stored, and positions past the table and pages outside the pool are
+ * not written to.
  * ---------------------------------------------------------------------- */
 typedef struct {
     const void* q;
@@ -774,8 +775,8 @@ typedef struct {
 int v1_paged_append(const v1_paged_append_args* a, void* stream);
 /* Row starts[r] + i of request r := row starts[r] + ids[cu_ids[r] + i], K and V, for
  * all i at once; ids of a request ascend from zero or above (an id below its own
- * index is not moved).  Positions past the table and pages outside the pool are
- * skipped. */
+ * index is not moved).  Requests with a start below zero, positions past the table
+ * and pages outside the pool are skipped. */
 typedef struct {
     void* k_pool;
     int64_t kp_page, kp_token, kp_head;
