@@ -182,16 +182,16 @@ __device__ __forceinline__ void cut(Item& it) {
     it.tiles = min(each, tiles - it.first);
 }
 
-// The planned parts of up to 64 R rows, R rows a lane (row R lane + i), of
-// keys_of_row(row) keys each; returns the number of parts before the lane's first row.
-template <int R, class Keys>
-__device__ __forceinline__ int32_t plan_parts(const Plan& p, int32_t (&keys)[R], int32_t (&parts)[R], Keys keys_of_row) {
+// The planned parts of up to 64 R rows, R rows a lane (row R lane + i); returns the
+// number of parts before the lane's first row.
+template <int R>
+__device__ __forceinline__ int32_t plan_parts(const Plan& p, int32_t (&keys)[R], int32_t (&parts)[R]) {
     const int32_t lane = (int32_t)threadIdx.x % kWave;
     int32_t tiles = 0;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         const int32_t r = R * lane + i;
-        keys[i] = keys_of_row(min(r, p.rows - 1));
+        keys[i] = keys_of(p, min(r, p.rows - 1));
         if (r >= p.rows) keys[i] = 0;
         tiles += tiles_of(keys[i]);
     }
@@ -223,11 +223,11 @@ __device__ __forceinline__ int32_t plan_parts(const Plan& p, int32_t (&keys)[R],
 }
 
 // Row, part, keys and parts of planned item `index`; false: there is none.
-template <int R, class Keys>
-__device__ __forceinline__ bool planned_item(const Plan& p, int32_t index, Item& it, Keys keys_of_row) {
+template <int R>
+__device__ __forceinline__ bool planned_item(const Plan& p, int32_t index, Item& it) {
     int32_t keys[R], parts[R];
     const int32_t lane = (int32_t)threadIdx.x % kWave;
-    int32_t at = plan_parts<R>(p, keys, parts, keys_of_row);
+    int32_t at = plan_parts<R>(p, keys, parts);
     int32_t row = -1, part = 0, n = 0, of = 0;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
@@ -250,18 +250,16 @@ __device__ __forceinline__ bool planned_item(const Plan& p, int32_t index, Item&
 }
 
 // Work item `index`; false: there is none.  (Every wave finds it by itself.)
-template <class Keys>
-__device__ __forceinline__ bool find_item(const Plan& p, int32_t index, Item& it, Keys keys_of_row) {
+__device__ __forceinline__ bool find_item(const Plan& p, int32_t index, Item& it) {
     if (p.chunk > 0) {
         it.parts = max(1, (tiles_of(p.keys) + p.chunk - 1) / p.chunk);
         it.row = index / it.parts;
         it.part = index - it.row * it.parts;
         if (it.row >= p.rows) return false;
-        it.keys = keys_of_row(it.row);
+        it.keys = keys_of(p, it.row);
     } else {
         // (a row a lane where that does: the search takes a quarter of the operations, 1.5 us less of a work-group)
-        if (!(p.rows <= kWave ? planned_item<1>(p, index, it, keys_of_row) : planned_item<kPlanRows / kWave>(p, index, it, keys_of_row)))
-            return false;
+        if (!(p.rows <= kWave ? planned_item<1>(p, index, it) : planned_item<kPlanRows / kWave>(p, index, it))) return false;
     }
     it.row = __builtin_amdgcn_readfirstlane(it.row);
     it.part = __builtin_amdgcn_readfirstlane(it.part);
@@ -269,10 +267,6 @@ __device__ __forceinline__ bool find_item(const Plan& p, int32_t index, Item& it
     it.parts = __builtin_amdgcn_readfirstlane(it.parts);
     cut(it);
     return true;
-}
-
-__device__ __forceinline__ bool find_item(const Plan& p, int32_t index, Item& it) {
-    return find_item(p, index, it, [&](int32_t row) __attribute__((always_inline)) { return keys_of(p, row); });
 }
 
 // Whether the device's lengths may decide: few rows, and their tiles can be added in 32 bits.

@@ -85,8 +85,7 @@ struct AttendParams {
     uint16_t* out;
     int64_t o_token, o_head;
     float* lse;
-    Plan plan;                // of the requests
-    int32_t reach;            // 0: a request's keys are all read; else its prefix and so many at its end
+    Plan plan;                // of the requests, by their keys or those that a window leaves (a prefix is not counted)
     int32_t blocks;           // of a request's columns
     // few queries: together: KV heads of a work-group, spread: work-groups of an XCD;
     // blocks: units (items or slots, times KV heads) and those that an XCD takes together
@@ -120,14 +119,6 @@ __device__ __forceinline__ Request request_at(const AttendParams& p, int32_t r) 
     w.len = __builtin_amdgcn_readfirstlane(w.len), w.before = __builtin_amdgcn_readfirstlane(w.before);
     w.pre = __builtin_amdgcn_readfirstlane(w.pre);
     return w;
-}
-
-// A request's keys by the plan: those of its prefix and its reach.
-__device__ __forceinline__ int32_t planned_keys(const AttendParams& p, int32_t r) {
-    const int32_t len = min(max(p.lens[r], 0), p.plan.keys);
-    if (p.reach == 0) return len;
-    const int32_t pre = p.prefix ? min(max(p.prefix[r], 0), len) : 0;
-    return min(len, pre + min(p.reach, len - pre));
 }
 
 // Drafted tokens of a request: which of them each one sees, itself and its ancestors

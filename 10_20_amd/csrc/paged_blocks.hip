@@ -128,7 +128,7 @@ __device__ __forceinline__ bool find_work(const AttendParams& p, BlocksWork& wor
     } else {
         Item it;
         const int32_t index = unit / p.kv_heads;
-        if (!find_item(p.plan, index, it, [&](int32_t r) __attribute__((always_inline)) { return planned_keys(p, r); })) return false;
+        if (!find_item(p.plan, index, it)) return false;
         work.block = p.blocks - 1 - rank;
         work.request = it.row, work.part = it.part, work.parts = it.parts;
         work.unit = ((int64_t)index * p.kv_heads + work.kv) * p.blocks + work.block;

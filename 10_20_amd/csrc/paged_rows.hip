@@ -392,7 +392,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void rows_kernel(AttendParams p) {
     const int32_t which = p.plan.chunk > 0 ? (xcd * p.spread + turn) % sets : turn % sets;
     work.index = p.plan.chunk > 0 ? (xcd * p.spread + turn) / sets : turn / sets * 8 + xcd;
     work.block = which % p.blocks, work.set = which / p.blocks;
-    if (!find_item(p.plan, work.index, work.item, [&](int32_t r) __attribute__((always_inline)) { return planned_keys(p, r); })) return;
+    if (!find_item(p.plan, work.index, work.item)) return;
     if (p.plan.chunk == 0 && work.item.part == 0 && which == 0 && threadIdx.x == 0)
         p.parts.of_row[work.item.row] = i32x2{work.index, work.item.parts};
     work.w = request_at(p, work.item.row);
@@ -477,7 +477,8 @@ int launch_join(const AttendParams& p, int32_t cols, hipStream_t st) {
 }
 
 // -------------------------------------------------------------- the host's side
-// Keys at the end of a request that a window leaves, with the rest of their first tile.
+// Keys at the end of a request that a window leaves, with the rest of their first tile.  The parts are planned for
+// these alone: a prefix beside a window, usually a few positions, is read by as few work-groups, however long it is.
 inline int32_t reach_of(int32_t window, int32_t max_q) {
     return window > 0 ? (int32_t)std::min<int64_t>((int64_t)window + max_q + kTileKeys, INT32_MAX) : 0;
 }
@@ -654,7 +655,7 @@ extern "C" int v1_paged_attend(const v1_paged_attend_args* a, void* stream) {
                    {kp_token, vp_token}, {kp_head, vp_head}, pages, table, table_stride, lens, cu_q, prefix, document,
                    parents, slopes, table_len, tokens, requests, max_q, kv_heads, group, small_div_magic((uint32_t)group),
                    window, scale * kLog2e, in, softcap * kLog2e, cap_of(scale, softcap),
-                   static_cast<uint16_t*>(out), o_token, o_head, lse, s.plan, s.reach, s.blocks, 0, s.together,
+                   static_cast<uint16_t*>(out), o_token, o_head, lse, s.plan, s.blocks, 0, s.together,
                    s.units, s.xcds, s.slots, parts_of(workspace, s, kv_heads)};
     return fp16 ? attend<_Float16>(p, s, mode, as_stream(stream)) : attend<__bf16>(p, s, mode, as_stream(stream));
 }
