@@ -32,11 +32,14 @@ __device__ __forceinline__ f32x4 mfma16(const Frag& a, const Frag& b, f32x4 c) {
 }
 
 // tanh(t) / t in t^2 for |t| up to 0.16, 0.33 and 0.75, and the same polynomials of
-// cap log2(e) tanh(d scale / cap) / d in d^2 for |d| up to so much.
-constexpr float kCapLeast[3] = {0.9999999721658054f, -0.3333137411469761f, 0.1312851958668552f}, kCapLeastMost = 0.16f;
-constexpr float kCapNear[4] = {0.9999999780542091f, -0.3333268647142513f, 0.1330338186573907f, -0.04948183016008989f}, kCapNearMost = 0.33f;
-constexpr float kCapFar[6] = {0.9999999710131235f, -0.33332958872695295f, 0.13325405922016131f, -0.053344425407917576f,
-                              0.019582898606222813f, -0.0047162504597644895f}, kCapFarMost = 0.75f;
+// cap log2(e) tanh(d scale / cap) / d in d^2 for |d| up to so much.  The fits are off by 3e-8
+// of the value at most; they are held in 64 bits, so that a coefficient is rounded once,
+// with the scale and the cap in it (by 1e-7 of the value then).
+constexpr double kCapLeast[3] = {0.9999999721658054, -0.3333137411469761, 0.1312851958668552};
+constexpr double kCapNear[4] = {0.9999999780542091, -0.3333268647142513, 0.1330338186573907, -0.04948183016008989};
+constexpr double kCapFar[6] = {0.9999999710131235, -0.33332958872695295, 0.13325405922016131, -0.053344425407917576,
+                               0.019582898606222813, -0.0047162504597644895};
+constexpr float kCapLeastMost = 0.16f, kCapNearMost = 0.33f, kCapFarMost = 0.75f;
 struct Cap {
     float least[3], near[4], far[6];
     float least_most, near_most, far_most;
@@ -46,7 +49,7 @@ inline Cap cap_of(float scale, float softcap) {
     Cap c{};
     if (softcap <= 0.f) return c;
     const double in = (double)scale / softcap;
-    double by = (double)scale * kLog2e;
+    double by = scale * 1.4426950408889634;  // (log2(e))
     for (int i = 0; i < 6; ++i, by *= in * in) {
         if (i < 3) c.least[i] = (float)(kCapLeast[i] * by);
         if (i < 4) c.near[i] = (float)(kCapNear[i] * by);
@@ -257,14 +260,14 @@ __device__ __forceinline__ float if_seen_or_least(uint32_t mask, float x) {
 
 // ------------------------------------------------------------------ capped scores
 // cap tanh(x / cap), base 2, of a product d = q . k, t = d scale / cap: past |t| = 0.75
-// cap (1 - 2 / (e^2t + 1)), below it t G(t^2) with a polynomial G fitted to tanh(t) / t
-// (off by 3e-8 of the value at most, half a step of fp32; the other form there is off by
-// as much of the cap).
+// cap (1 - 2 / (e^2t + 1)), below it t G(t^2) with a polynomial G fitted to tanh(t) / t, its
+// coefficients in fp32 (off by 7e-8 of the value, a step of fp32, beside the roundings of its
+// evaluation; the other form there is off by as much of the cap, many times a small value).
 __device__ __forceinline__ float capped(float t, float cap2) {
     const float z = t * t;
-    float g = kCapFar[5];
+    float g = (float)kCapFar[5];
 #pragma unroll
-    for (int i = 4; i >= 0; --i) g = fmaf(g, z, kCapFar[i]);
+    for (int i = 4; i >= 0; --i) g = fmaf(g, z, (float)kCapFar[i]);
     const float e = __builtin_amdgcn_exp2f(2.f * kLog2e * t);
     const float past = fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(e + 1.f), cap2);
     return fabsf(t) <= kCapFarMost ? t * cap2 * g : past;
