@@ -15,10 +15,12 @@ using namespace paged;
 // (d, d + R/2) meet through a lane permute, neighbours lie in one lane.  Products and
 // sums are fp32, rounded to the row's type once.
 //
-// Bound by memory, or by the call: 14 thousand tokens of 32 query and 8 KV heads 70 us, 367
-// MB at 5.2 TB/s, a copy's rate (78 with loads that leave the tokens, which nobody reads
-// again, in the caches; two, three and six rows in flight 1 us or 3 more).  128 requests of a
-// token 4.8 us, a wave for every four rows: offsets, start, page entry one after the other.
+// Bound by memory, or by the call: 14 thousand tokens of 32 query and 8 KV heads 69-70 us, 367
+// MB at 5.3 TB/s, a copy's rate, and up to 77 between passes that move other memory.  Loads
+// that leave the tokens, which nobody reads again, in the caches take 78 in turn with it, on
+// the same inputs again and on five in turn; two, three and six rows in flight 1 us or 3 more.
+// 128 requests of a token 4.8 us, a wave for every four rows: offsets, start, page entry one
+// after the other.
 struct AppendParams {
     const uint16_t* x[3];  // q, k, v
     int64_t x_token[3], x_head[3];

@@ -478,21 +478,32 @@ int launch_join(const AttendParams& p, int32_t cols, hipStream_t st) {
 
 // -------------------------------------------------------------- the host's side
 // Keys at the end of a request that a window leaves, with the rest of their first tile.  The parts are planned for
-// these alone: a prefix beside a window, usually a few positions, is read by as few work-groups, however long it is.
+// these alone: a prefix beside a window, usually a few positions, is read by as few work-groups, however long it is
+// (8 single tokens, one KV head, a window of 64: 15 us with a prefix of 4, 50 of 4096, 646 of 60000).
 inline int32_t reach_of(int32_t window, int32_t max_q) {
     return window > 0 ? (int32_t)std::min<int64_t>((int64_t)window + max_q + kTileKeys, INT32_MAX) : 0;
 }
 
 // Whether work-groups of 128 columns are better than ones of 256, of which there would
-// be `groups` without parts, over at most `tiles` tiles of keys.  Two of them share a CU,
-// so that one's first and last steps (12 us of a work-group) pass beside the other's
-// products; those of 256 read the keys half as often and overlap products and
-// exponentials by their turns.  256 and 128 columns, us:
-//   four prompts of 1193-3434, 16 heads, distances  188, 160    nine of 1-1500, 16 heads        26, 21
-//   one of 4096, 32 heads, 8 KV heads               198, 163    16 of 300, the same heads       63, 48
-//   8 chunks of 500 behind 4000, the same           327, 290    8 trees of 16 drafts, 4 heads   28, 24
-//   32 chunks of 64 behind 4000, the same           189, 210    four prompts of 4096, 32 heads 597, 627
-//   4096 queries over 32768 keys, the same         1856, 1945   32 trees of 64, 32 heads      1090, 1139
+// be `groups` without parts, over at most `tiles` tiles of keys (those of the table's width
+// or of a window: the lengths are on the device).  Two of 128 share a CU, so that one's
+// first and last steps (12 us of a work-group) pass beside the other's products; those of
+// 256 read the keys half as often and overlap products and exponentials by their turns.
+// 256 and 128 columns, us, 32 heads of 8 KV heads unless said:
+//   fewer than half of the CUs
+//     8 trees of 16 drafts, 4 heads         29, 24
+//   up to four a CU, up to 128 tiles
+//     nine prompts of 1-1500, 16 heads      27, 22     one of 2000                       78, 60
+//     four of 1193-3434, 16, distances     200, 166    16 of 300                         64, 47
+//     8 chunks of 500 behind 4000          336, 289    32 chunks of 100 behind 4000     335, 290
+//   where that is the slower side
+//     one prompt of 4096                   148, 161    two of 4096                      287, 291
+//     32 chunks of 64 behind 4000          175, 198    behind 8000                      340, 403
+//     32 chunks of 40 behind 4000          160, 190    64 of 64 behind 4000             388, 400
+//   past both
+//     four prompts of 4096                 572, 573    32 trees of 64, 4 KV heads      1081, 1163
+//   the second list in tables for 128K positions, which take 256 columns for it: 16
+//   prompts of 300 67 us (48 in tables of their own width), 8 chunks of 500 341 (295)
 inline bool small_blocks(double groups, int64_t tiles) { return groups < device_cus() / 2 || (tiles <= 128 && groups <= 4 * device_cus()); }
 
 struct Shape {
@@ -541,7 +552,8 @@ inline Shape shape_of(const int32_t* lens, int32_t tokens, int32_t requests, int
     s.items = items_at_most(s.plan);
     if (!few) {
         // Every request gets as many blocks as the longest can have, unless the blocks that the queries can need are
-        // less than a third of those.
+        // less than a third of those.  Contexts are not cut then: a chunk of 512 tokens and 16 single ones, 32 heads of 8
+        // KV heads over 64K each, 1590 us, as two calls 590 and 715.
         const int64_t slots = (int64_t)tokens * group / s.cols + requests;
         if (max_q > 1 && ((int64_t)requests * s.blocks > 3 * slots || (double)(s.items * kv_heads + 7) * s.blocks >= 0x1p32 / 512)) {
             s.slots = (int32_t)slots, s.blocks = 1, s.items = slots;
